@@ -14,6 +14,8 @@ Entry points mirror the reference's launch surfaces:
   spmspm_hm         gather_meta_kernel argument set (spmspm/spmspm.cu:256-319)
   spmspm            the same product on the padded rows layout
   gemm_diag         gemm_diag_kernel argument set (gemm_diag/gemm_diag.cu:119-131)
+Products with a block of vectors (spmm, spmm_backward) have no counterpart
+there: its products take one vector.
 """
 from __future__ import annotations
 
@@ -90,6 +92,16 @@ def lib():
                      "dia_dist_destroy", "dia_dist_create_timeout", "dia_dist_abort",
                      "dia_spmv_rows_peer", "dia_dist_peer_setup",
                      "dia_dist_spmv_fused", "dia_dist_set_timeout", "dia_dist_status"):
+            getattr(L, name).restype = i
+        L.dia_spmm_plan_create.argtypes = [i64, i64, i, p, p]
+        L.dia_spmm_plan_destroy.argtypes = [p]
+        L.dia_spmm.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i, p, i64, p, i64, p, i64, p]
+        L.dia_spmm_backward_workspace.argtypes = [p, i, i64, i64, i]
+        L.dia_spmm_backward_workspace.restype = i64
+        L.dia_spmm_backward.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i64, i, p, i64, p,
+                                        i64, p, p, p, i64, p]
+        for name in ("dia_spmm_plan_create", "dia_spmm_plan_destroy", "dia_spmm",
+                     "dia_spmm_backward"):
             getattr(L, name).restype = i
         L.dia_device_status.argtypes = [p, i]
         L.dia_device_status.restype = i
@@ -697,6 +709,193 @@ def spmspm(A: DiaRows, B: DiaRows, C_out: DiaRows | None = None, *, b_lo=None, b
                                 _dptr(C_out.d_offsets), C_out.K, A.vrow0, A.vrow0,
                                 A.vrow0 + A.nrows, _stream(stream)))
     return C_out
+
+
+# ------------------------------------------------------ block-vector product
+
+_SPMM_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_SPMM_ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+class SpmmPlan:
+    """Shape and offsets of an operator that multiplies blocks of vectors
+    (dia_spmm_plan_create): distinct host offsets in the order of the rows of
+    `vals`.  Calls on several streams and captured graphs may share a plan; it
+    has to outlive them."""
+
+    def __init__(self, n_rows, n_cols, offsets, *, device="cuda"):
+        self._h = C.c_void_p()
+        self.n_rows, self.n_cols = int(n_rows), int(n_cols)
+        off = np.asarray(offsets)
+        self.offsets = np.ascontiguousarray(off, np.int32)
+        if off.ndim != 1 or not np.array_equal(self.offsets, off):
+            raise DiaError(DIA_ERR_INVALID, "SpmmPlan: offsets must be a list of 32-bit integers")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise DiaError(DIA_ERR_INVALID, "SpmmPlan: device must be a CUDA device")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        with torch.cuda.device(self.device):
+            check(lib().dia_spmm_plan_create(self.n_rows, self.n_cols, self.K,
+                                             self.offsets.ctypes.data_as(C.c_void_p),
+                                             C.byref(self._h)))
+
+    @property
+    def K(self):
+        return len(self.offsets)
+
+    def __del__(self):
+        if getattr(self, "_h", None) and self._h.value and _lib is not None:
+            _lib.dia_spmm_plan_destroy(self._h)
+            self._h = C.c_void_p()
+
+
+def _spmm_block(who, name, t, plan, dtype, rows, width):
+    """(pointer, row stride) of a [rows, width] block with adjacent features."""
+    if t is None:
+        return None, width
+    if t.dtype != dtype or t.device != plan.device or t.dim() != 2:
+        raise DiaError(DIA_ERR_INVALID, f"{who}: {name} must be a 2-D {dtype} tensor on "
+                                        f"{plan.device}")
+    if tuple(t.shape) != (rows, width):
+        raise DiaError(DIA_ERR_INVALID,
+                       f"{who}: {name} has shape {tuple(t.shape)}, not {(rows, width)}")
+    if width > 1 and t.stride(1) != 1:
+        raise DiaError(DIA_ERR_INVALID, f"{who}: features of {name} must be adjacent in memory")
+    return C.c_void_p(t.data_ptr()), t.stride(0) if rows > 1 else width
+
+
+def _spmm_operator(who, plan, vals, x, seg):
+    """(dtype code, number of experts, stride) after checking x, vals and seg."""
+    if x.dtype not in _SPMM_TYPES:
+        raise DiaError(DIA_ERR_INVALID, f"{who}: {x.dtype} is not float32, float16 or bfloat16")
+    want = 2 if seg is None else 3
+    if vals.dim() != want or vals.shape[-2] != plan.K:
+        raise DiaError(DIA_ERR_INVALID, f"{who}: vals must be "
+                       + ("[K, stride]" if seg is None else "[experts, K, stride]"))
+    if vals.dtype != x.dtype or vals.device != plan.device or not vals.is_contiguous():
+        raise DiaError(DIA_ERR_INVALID,
+                       f"{who}: vals must be a contiguous {x.dtype} tensor on {plan.device}")
+    E = 1
+    if seg is not None:
+        E = vals.shape[0]
+        if (seg.dtype != torch.int64 or seg.device != plan.device or not seg.is_contiguous()
+                or tuple(seg.shape) != (E + 1,)):
+            raise DiaError(DIA_ERR_INVALID, f"{who}: seg must be a contiguous int64 tensor of "
+                                            f"{E + 1} elements on {plan.device}")
+    return _SPMM_TYPES[x.dtype], E, vals.shape[-1]
+
+
+def _spmm_vector(who, name, t, plan, dtype, shape):
+    if t is None:
+        return None
+    if (t.dtype != dtype or t.device != plan.device or tuple(t.shape) != shape
+            or not t.is_contiguous()):
+        raise DiaError(DIA_ERR_INVALID, f"{who}: {name} must be a contiguous {dtype} tensor of "
+                                        f"shape {shape} on {plan.device}")
+    return C.c_void_p(t.data_ptr())
+
+
+def _spmm_act(who, act):
+    if act not in _SPMM_ACTS:
+        raise DiaError(DIA_ERR_INVALID, f"{who}: act must be one of {sorted(_SPMM_ACTS)}")
+    return _SPMM_ACTS[act]
+
+
+def _spmm_made(stream, *made):
+    """Tensors allocated here and used on a stream that is not the current one
+    stay allocated until that stream has passed this point."""
+    if stream is not None:
+        for t in made:
+            if t is not None:
+                t.record_stream(stream)
+
+
+def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=None,
+         save_z=False, out=None, z=None, stream=None):
+    """act(x A^T + bias) + residual for a block x [M, n_cols] of vectors, one
+    per row (dia_spmm); float32, float16 or bfloat16, all of one type.
+
+    vals [K, stride] is the operator in the rows layout (round_stride).  With
+    seg (device int64 [E + 1]) vals is [E, K, stride], bias [E, n_rows], and
+    rows [seg[e], seg[e + 1]) of the block meet expert e; rows outside every
+    expert are left as they were (unset in a new out).  act: "none", "relu",
+    "silu", "gelu", "gelu_tanh".  Returns out [M, n_rows], or (out, z) with
+    save_z or a given z: the pre-activation that spmm_backward takes."""
+    who = "spmm"
+    code = _spmm_act(who, act)
+    dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
+    M, n = x.shape[0], plan.n_rows
+    xp, ldx = _spmm_block(who, "x", x, plan, x.dtype, M, plan.n_cols)
+    bp = _spmm_vector(who, "bias", bias, plan, x.dtype, (n,) if seg is None else (E, n))
+    rp, ldr = _spmm_block(who, "residual", residual, plan, x.dtype, M, n)
+    new_out, new_z = out is None, z is None and save_z
+    with torch.cuda.device(plan.device):
+        if new_out:
+            out = torch.empty((M, n), dtype=x.dtype, device=plan.device)
+        if new_z:
+            z = torch.empty((M, n), dtype=x.dtype, device=plan.device)
+        yp, ldy = _spmm_block(who, "out", out, plan, x.dtype, M, n)
+        zp, ldz = _spmm_block(who, "z", z, plan, x.dtype, M, n)
+        _spmm_made(stream, out if new_out else None, z if new_z else None)
+        check(lib().dia_spmm(plan._h, dt, M, E, _dptr(seg), xp, ldx, C.c_void_p(vals.data_ptr()),
+                             stride, bp, code, rp, ldr, zp, ldz, yp, ldy, _stream(stream)))
+    return (out, z) if z is not None else out
+
+
+def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, bias_grad=False,
+                  dx=None, dvals=None, dbias=None, work=None, stream=None):
+    """Gradients (dx, dvals, dbias) of spmm for dy, the gradient of its result
+    (dia_spmm_backward); that of the residual is dy.  z is what spmm saved, not
+    wanted for act "none".  dvals has the shape of vals, with zeros outside the
+    matrix; dbias is None unless bias_grad or given.  work: uint8 buffer of
+    spmm_backward_workspace bytes, for callers that allocate nothing."""
+    who = "spmm_backward"
+    code = _spmm_act(who, act)
+    dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
+    M, n = x.shape[0], plan.n_rows
+    xp, ldx = _spmm_block(who, "x", x, plan, x.dtype, M, plan.n_cols)
+    if dy is None or (code and z is None):
+        raise DiaError(DIA_ERR_INVALID, f"{who}: dy, and z for an activation, must be given")
+    gp, lddy = _spmm_block(who, "dy", dy, plan, x.dtype, M, n)
+    zp, ldz = _spmm_block(who, "z", z, plan, x.dtype, M, n) if code else (None, n)
+    bshape = (n,) if seg is None else (E, n)
+    with torch.cuda.device(plan.device):
+        made = []
+
+        def new(shape, dtype=x.dtype):
+            made.append(torch.empty(shape, dtype=dtype, device=plan.device))
+            return made[-1]
+
+        dx = new((M, plan.n_cols)) if dx is None else dx
+        dvals = new(tuple(vals.shape)) if dvals is None else dvals
+        if dbias is None and bias_grad:
+            dbias = new(bshape)
+        ws = spmm_backward_workspace(plan, vals, M, act)
+        if work is None:
+            work = new((max(ws, 1),), torch.uint8)
+        elif (work.dtype != torch.uint8 or work.device != plan.device
+              or not work.is_contiguous()):
+            raise DiaError(DIA_ERR_INVALID, f"{who}: work must be a contiguous uint8 tensor on "
+                                            f"{plan.device}")
+        dxp, lddx = _spmm_block(who, "dx", dx, plan, x.dtype, M, plan.n_cols)
+        dvp = _spmm_vector(who, "dvals", dvals, plan, x.dtype, tuple(vals.shape))
+        dbp = _spmm_vector(who, "dbias", dbias, plan, x.dtype, bshape)
+        _spmm_made(stream, *made)
+        check(lib().dia_spmm_backward(plan._h, dt, M, E, _dptr(seg), xp, ldx,
+                                      C.c_void_p(vals.data_ptr()), stride, gp, lddy, code, zp,
+                                      ldz, dxp, lddx, dvp, dbp, C.c_void_p(work.data_ptr()),
+                                      work.numel(), _stream(stream)))
+    return dx, dvals, dbias
+
+
+def spmm_backward_workspace(plan: SpmmPlan, vals, M, act="none"):
+    """Bytes of the work buffer of spmm_backward for a block of M vectors."""
+    ws = lib().dia_spmm_backward_workspace(plan._h, _SPMM_TYPES[vals.dtype], int(M),
+                                           vals.shape[-1], _spmm_act("spmm_backward", act))
+    if ws < 0:
+        raise DiaError(DIA_ERR_INVALID, "spmm_backward_workspace: bad size")
+    return ws
 
 
 # ---------------------------------------------------------------- gemm_diag

@@ -1,0 +1,699 @@
+/*
+ * spmm.cu -- a DIA operator times a block of vectors, with an epilogue, its
+ * gradients, and the same product grouped by expert.
+ *
+ *     z[t, i]    = bias[i] + sum_k vals[k, i] * x[t, i + d_k]
+ *     y[t, i]    = act(z[t, i]) + residual[t, i]
+ *     dz         = dy * act'(z)
+ *     dx[t, j]   = sum_k vals[k, j - d_k] * dz[t, j - d_k]
+ *     dvals[k,i] = sum_t dz[t, i] * x[t, i + d_k]
+ *     dbias[i]   = sum_t dz[t, i]
+ *
+ * The block holds one vector per row, so neighbouring lanes read neighbouring
+ * features and every diagonal value is read once for several vectors instead
+ * of once per vector, which is what a loop of SpMVs would do.  All sums are
+ * held in fp32, in ascending order of the offsets, and rounded once to the
+ * block's type.  Grouped: the rows are sorted by expert, rows [seg[e],
+ * seg[e+1]) use the diagonals vals[e].
+ */
+#include <algorithm>
+#include <climits>
+#include <cstring>
+#include <new>
+#include <numeric>
+#include <vector>
+
+#include "dia_core.cuh"
+#include "spmm.cuh"
+
+namespace dia {
+
+constexpr int kMmWarps = 8;
+constexpr int kMmThreads = kMmWarps * 32;
+constexpr int kMmFeat = 128;   /* features of a warp: four per lane */
+
+/* elements c .. c+3 of a row of n elements, zero outside */
+template <typename T, bool VEC>
+__device__ __forceinline__ float4 row4(const T* row, int c, int n)
+{
+    if (VEC && c >= 0 && c + 4 <= n) return load4<T>(row + c);
+    float4 v;
+    v.x = (unsigned)c < (unsigned)n ? to_f(row[c]) : 0.0f;
+    v.y = (unsigned)(c + 1) < (unsigned)n ? to_f(row[c + 1]) : 0.0f;
+    v.z = (unsigned)(c + 2) < (unsigned)n ? to_f(row[c + 2]) : 0.0f;
+    v.w = (unsigned)(c + 3) < (unsigned)n ? to_f(row[c + 3]) : 0.0f;
+    return v;
+}
+
+/* One warp: 128 features (four consecutive ones a lane), TT rows.  A quad's
+ * up to four diagonals read the window of seven inputs from two aligned
+ * chunks of four, so a run of consecutive offsets costs one chunk per four
+ * diagonals; a weight is read once for TT rows.  The CTA's warps split the
+ * quads `ks` ways (few rows: there are too few warps otherwise) and add up
+ * in shared memory in a fixed order; the other 8 / ks take other features. */
+template <typename T, bool TRANS, int TT, bool VEC>
+__global__ void __launch_bounds__(kMmThreads)
+spmm_kernel(ProdArgs a, int ks, int ftiles, long long ngroups, bool rows_first)
+{
+    __shared__ float s_sum[kMmWarps][TT * 4][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int part = warp % ks, sub = warp / ks, fper = kMmWarps / ks;
+    const int fblocks = (ftiles + fper - 1) / fper;
+    const long long b = blockIdx.x;
+    const long long g = rows_first ? b % ngroups : b / fblocks;
+    const int fb = (int)(rows_first ? b / ngroups : b % fblocks);
+    const RowGroup rg = row_group(a.seg, a.E, a.M, TT, g, false);
+    const int i = (fb * fper + sub) * kMmFeat + lane * 4;
+
+    float acc[TT][4];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[t][r] = 0.0f;
+
+    if (rg.e >= 0 && i < a.n_out) {
+        const T* vals = (const T*)a.vals + rg.e * a.estride;
+        const T* in = (const T*)a.in + (long long)rg.r0 * a.ldi;
+        const int nt = rg.r1 - rg.r0;
+        const int q0 = (int)((long long)a.dir.nquads * part / ks);
+        const int q1 = (int)((long long)a.dir.nquads * (part + 1) / ks);
+        for (int q = q0; q < q1; ++q) {
+            const int4 h = __ldg((const int4*)&a.dir.quads[q]);
+            const int k3 = __ldg(&a.dir.quads[q].k[3]);
+            const int kk[4] = {h.y, h.z, h.w, k3};
+            const int c = i + h.x;
+            if (c + 7 <= 0 || c >= a.n_in) continue;
+            float w[4][4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                if (kk[s] < 0) continue;
+                const T* vp = vals + (long long)kk[s] * a.stride;
+                if (TRANS) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = c + s + r;
+                        w[s][r] = ((unsigned)j < (unsigned)a.n_in && i + r < a.n_out)
+                                      ? to_f(vp[j]) : 0.0f;
+                    }
+                } else {
+                    const float4 v = load4<T>(vp + i);
+                    w[s][0] = v.x;
+                    w[s][1] = v.y;
+                    w[s][2] = v.z;
+                    w[s][3] = v.w;
+                    if (c < 0 || c + 7 > a.n_in) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if ((unsigned)(c + s + r) >= (unsigned)a.n_in) w[s][r] = 0.0f;
+                    }
+                }
+            }
+            float xs[TT][8];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                if (t < nt) {
+                    const T* row = in + t * a.ldi;
+                    const float4 u = row4<T, VEC>(row, c, a.n_in);
+                    const float4 v = row4<T, VEC>(row, c + 4, a.n_in);
+                    xs[t][0] = u.x; xs[t][1] = u.y; xs[t][2] = u.z; xs[t][3] = u.w;
+                    xs[t][4] = v.x; xs[t][5] = v.y; xs[t][6] = v.z; xs[t][7] = v.w;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) xs[t][r] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                if (kk[s] < 0) continue;
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        acc[t][r] = fmaf(w[s][r], xs[t][s + r], acc[t][r]);
+            }
+        }
+    }
+    if (ks > 1) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s_sum[warp][t * 4 + r][lane] = acc[t][r];
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = acc[t][r];
+                for (int p = 1; p < ks; ++p) v += s_sum[warp + p][t * 4 + r][lane];
+                acc[t][r] = v;
+            }
+    }
+    if (rg.e < 0 || i >= a.n_out) return;
+    const T* bias = a.bias ? (const T*)a.bias + (long long)rg.e * a.n_out : nullptr;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        const long long row = (long long)rg.r0 + t;
+        if (row >= rg.r1) break;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (i + r >= a.n_out) break;
+            float z = acc[t][r];
+            if (bias) z += to_f(bias[i + r]);
+            if (a.z) ((T*)a.z)[row * a.ldz + i + r] = from_f<T>(z);
+            float y = act_any(a.act, z);
+            if (a.res) y += to_f(((const T*)a.res)[row * a.ldr + i + r]);
+            ((T*)a.out)[row * a.ldo + i + r] = from_f<T>(y);
+        }
+    }
+}
+
+/* One CTA: 128 features, one quad, one part of an expert's rows; its warps
+ * take every eighth row and add up in shared memory in a fixed order.  Sums
+ * of an expert with one part go out at once, others to `part`. */
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kMmThreads)
+spmm_grad_kernel(GradArgs a, int ftiles)
+{
+    __shared__ float s_sum[kMmWarps][20][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int nq = max(a.dir.nquads, 1);
+    const long long b = blockIdx.x;
+    const int f = (int)(b % ftiles), q = (int)((b / ftiles) % nq);
+    const RowGroup rg = row_group(a.seg, a.E, a.M, a.per, b / ftiles / nq, true);
+    if (rg.e < 0 || (rg.nparts > 1 && rg.slot + rg.part >= a.slots)) return;
+    const int i = f * kMmFeat + lane * 4;
+    const bool on = i < a.n_rows;
+    int kk[4] = {-1, -1, -1, -1}, base = 0;
+    if (q < a.dir.nquads && a.dvals) {
+        base = a.dir.quads[q].base;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) kk[s] = a.dir.quads[q].k[s];
+    }
+    const int c = i + base;
+    float acc[4][4], sb[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[s][r] = 0.0f;
+    if (on) {
+        for (int t = rg.r0 + warp; t < rg.r1; t += kMmWarps) {
+            const float4 d = row4<T, VEC>((const T*)a.dz + t * a.lddz, i, a.n_rows);
+            const T* row = (const T*)a.x + t * a.ldx;
+            const float4 u = row4<T, VEC>(row, c, a.n_cols);
+            const float4 v = row4<T, VEC>(row, c + 4, a.n_cols);
+            const float dd[4] = {d.x, d.y, d.z, d.w};
+            const float xs[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (kk[s] >= 0)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[s][r] = fmaf(dd[r], xs[s + r], acc[s][r]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sb[r] += dd[r];
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_sum[warp][s * 4 + r][lane] = acc[s][r];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s_sum[warp][16 + r][lane] = sb[r];
+    __syncthreads();
+    /* output s * 128 + f: slot s (4: dbias) of feature f */
+    for (int o = threadIdx.x; o < 5 * kMmFeat; o += kMmThreads) {
+        const int s = o / kMmFeat, fi = o % kMmFeat, col = f * kMmFeat + fi;
+        if (col >= a.stride) continue;
+        float v = 0.0f;
+        for (int w = 0; w < kMmWarps; ++w) v += s_sum[w][s * 4 + (fi & 3)][fi >> 2];
+        if (s == 4) {
+            if (q != 0 || !a.dbias || col >= a.n_rows) continue;
+            if (rg.nparts > 1)
+                a.part[((long long)(rg.slot + rg.part) * (a.K + 1) + a.K) * a.stride + col] = v;
+            else
+                ((T*)a.dbias)[(long long)rg.e * a.n_rows + col] = from_f<T>(v);
+        } else if (kk[s] >= 0) {
+            /* an entry outside the matrix has no gradient */
+            if (col >= a.n_rows || (unsigned)(col + base + s) >= (unsigned)a.n_cols) v = 0.0f;
+            if (rg.nparts > 1)
+                a.part[((long long)(rg.slot + rg.part) * (a.K + 1) + kk[s]) * a.stride + col] = v;
+            else
+                ((T*)a.dvals)[rg.e * a.estride + (long long)kk[s] * a.stride + col] = from_f<T>(v);
+        }
+    }
+}
+
+/* Sums the parts of experts that have several, in the parts' order. */
+template <typename T>
+__global__ void __launch_bounds__(256) spmm_join_kernel(GradArgs a, int cblocks)
+{
+    const int k = (int)(blockIdx.x / cblocks) % (a.K + 1);
+    const int e = (int)(blockIdx.x / cblocks / (a.K + 1));
+    const int col = (int)(blockIdx.x % cblocks) * 256 + threadIdx.x;
+    int nparts, slot = 0;
+    if (a.seg) {
+        int mine = 0;
+        for (int j = threadIdx.x & 31; j <= e; j += 32) {
+            int lo, hi;
+            expert_rows(a.seg, j, a.M, lo, hi);
+            const int c = (hi - lo + a.per - 1) / a.per;
+            if (j < e) slot += c > 1 ? c : 0;
+            if (j == e) mine = c;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            slot += __shfl_xor_sync(0xffffffffu, slot, d);
+            mine += __shfl_xor_sync(0xffffffffu, mine, d);
+        }
+        nparts = mine;
+    } else {
+        nparts = (a.M + a.per - 1) / a.per;
+    }
+    if (nparts <= 1 || col >= a.stride || slot + nparts > a.slots) return;
+    if (k == a.K ? (!a.dbias || col >= a.n_rows) : !a.dvals) return;
+    const float* p = a.part + ((long long)slot * (a.K + 1) + k) * a.stride + col;
+    const long long step = (long long)(a.K + 1) * a.stride;
+    float v = 0.0f;
+    for (int s = 0; s < nparts; ++s) v += p[s * step];
+    if (k == a.K)
+        ((T*)a.dbias)[(long long)e * a.n_rows + col] = from_f<T>(v);
+    else
+        ((T*)a.dvals)[e * a.estride + (long long)k * a.stride + col] = from_f<T>(v);
+}
+
+/* dz = dy * act'(z), rounded to the block's type: both gradients read it as
+ * a matrix operand of that type, and one rounding of half a step is no more
+ * than the ones dy and z already carry. */
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256)
+spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z, long long ldz,
+               T* __restrict__ dz, long long lddz, int M, int n)
+{
+    const long long per = (n + 3) / 4;
+    const long long total = per * M;
+    for (long long p = blockIdx.x * 256ll + threadIdx.x; p < total; p += gridDim.x * 256ll) {
+        const long long t = p / per;
+        const int i = (int)(p % per) * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (i + r < n)
+                dz[t * lddz + i + r] = from_f<T>(to_f(dy[t * lddy + i + r]) *
+                                                 dact_of<ACT>(to_f(z[t * ldz + i + r])));
+    }
+}
+
+/* ---------------------------------------------------------------- host */
+
+static size_t elem_size(int dtype) { return dtype == DIA_F32 ? 4 : 2; }
+
+static bool vec4(const void* p, long long ld, int dtype)
+{
+    return (uintptr_t)p % (4 * elem_size(dtype)) == 0 && ld % 4 == 0;
+}
+
+template <typename T, bool TRANS, int TT>
+static int launch_product_tt(const ProdArgs& a, int dtype, cudaStream_t stream)
+{
+    const int ftiles = (a.n_out + kMmFeat - 1) / kMmFeat;
+    const long long ngroups =
+        a.seg ? a.M / TT + std::min(a.E, a.M) : (a.M + TT - 1) / TT;
+    /* warps that share a tile: enough to give every SM a few */
+    int ks = 1;
+    while (ks < kMmWarps && (long long)ftiles * ngroups * ks < 8ll * num_sms() &&
+           a.dir.nquads > 2 * ks)
+        ks *= 2;
+    const int fper = kMmWarps / ks;
+    const long long grid = ngroups * ((ftiles + fper - 1) / fper);
+    if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: block too large");
+    /* the larger of block and operator is streamed once, the other stays in L2 */
+    const bool rows_first = (long long)a.M * a.n_in < a.stride * 4 * a.dir.nquads;
+    if (vec4(a.in, a.ldi, dtype))
+        spmm_kernel<T, TRANS, TT, true>
+            <<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ks, ftiles, ngroups, rows_first);
+    else
+        spmm_kernel<T, TRANS, TT, false>
+            <<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ks, ftiles, ngroups, rows_first);
+    DIA_TRY_CUDA(cudaGetLastError());
+    return DIA_OK;
+}
+
+template <typename T>
+static int launch_product(const ProdArgs& a, int dtype, cudaStream_t stream)
+{
+    if (a.M == 0 || a.n_out == 0) return DIA_OK;
+    const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
+    if (a.trans)
+        return per >= 4 ? launch_product_tt<T, true, 4>(a, dtype, stream)
+                        : launch_product_tt<T, true, 1>(a, dtype, stream);
+    return per >= 4 ? launch_product_tt<T, false, 4>(a, dtype, stream)
+                    : launch_product_tt<T, false, 1>(a, dtype, stream);
+}
+
+template <typename T, int ACT>
+static void launch_dz_act(const void* dy, long long lddy, const void* z, long long ldz, void* dz,
+                          long long lddz, int M, int n, cudaStream_t stream)
+{
+    const long long work = (long long)M * ((n + 3) / 4);
+    const int grid = (int)std::min<long long>((work + 255) / 256, 16ll * num_sms());
+    spmm_dz_kernel<T, ACT><<<grid, 256, 0, stream>>>((const T*)dy, lddy, (const T*)z, ldz, (T*)dz,
+                                                     lddz, M, n);
+}
+
+template <typename T>
+static int launch_dz(int act, const void* dy, long long lddy, const void* z, long long ldz,
+                     void* dz, long long lddz, int M, int n, cudaStream_t stream)
+{
+    if (M == 0 || n == 0) return DIA_OK;
+    switch (act) {
+        case DIA_ACT_RELU:
+            launch_dz_act<T, DIA_ACT_RELU>(dy, lddy, z, ldz, dz, lddz, M, n, stream);
+            break;
+        case DIA_ACT_SILU:
+            launch_dz_act<T, DIA_ACT_SILU>(dy, lddy, z, ldz, dz, lddz, M, n, stream);
+            break;
+        case DIA_ACT_GELU:
+            launch_dz_act<T, DIA_ACT_GELU>(dy, lddy, z, ldz, dz, lddz, M, n, stream);
+            break;
+        default:
+            launch_dz_act<T, DIA_ACT_GELU_TANH>(dy, lddy, z, ldz, dz, lddz, M, n, stream);
+    }
+    DIA_TRY_CUDA(cudaGetLastError());
+    return DIA_OK;
+}
+
+/* rows of a part of the gradient's sum: enough parts to fill the GPU, none
+ * so short that writing and joining its sums costs more than it saves */
+static int grad_part_rows(const DiaSpmmPlan* p, long long M, long long stride)
+{
+    const long long tiles = std::max<long long>(1, (stride + kMmFeat - 1) / kMmFeat) *
+                            std::max(1, p->fwd.nquads);
+    const long long want = std::max<long long>(1, 4ll * num_sms() / tiles);
+    const long long per = std::max<long long>(256, (M + want - 1) / want);
+    return (int)std::min<long long>(per, INT_MAX / 2);
+}
+
+/* parts of experts that have several: at most two a `per` rows */
+static long long grad_slots(long long M, long long per) { return M > per ? 2 * (M / per) + 1 : 0; }
+
+template <typename T>
+static int launch_grad(const GradArgs& a, int dtype, cudaStream_t stream)
+{
+    const int ftiles = (int)((a.stride + kMmFeat - 1) / kMmFeat);
+    const long long parts = a.seg ? a.M / a.per + a.E : std::max(1, (a.M + a.per - 1) / a.per);
+    const long long grid = parts * ftiles * std::max(a.dir.nquads, 1);
+    const int cblocks = (int)((a.stride + 255) / 256);
+    const long long jgrid = (long long)a.E * (a.K + 1) * cblocks;
+    if (grid > INT_MAX || jgrid > INT_MAX)
+        return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
+    if (vec4(a.dz, a.lddz, dtype) && vec4(a.x, a.ldx, dtype))
+        spmm_grad_kernel<T, true><<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ftiles);
+    else
+        spmm_grad_kernel<T, false><<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ftiles);
+    DIA_TRY_CUDA(cudaGetLastError());
+    if (a.M > a.per) {
+        spmm_join_kernel<T><<<(unsigned)jgrid, 256, 0, stream>>>(a, cblocks);
+        DIA_TRY_CUDA(cudaGetLastError());
+    }
+    return DIA_OK;
+}
+
+static std::vector<Quad> build_quads(const std::vector<int>& off)
+{
+    std::vector<int> order(off.size());
+    std::iota(order.begin(), order.end(), 0);
+    std::sort(order.begin(), order.end(), [&](int a, int b) { return off[a] < off[b]; });
+    std::vector<Quad> quads;
+    for (int k : order) {
+        const int base = off[k] & ~3;   /* floor to a multiple of four */
+        if (quads.empty() || quads.back().base != base) {
+            Quad q;
+            std::memset(&q, 0, sizeof(q));
+            q.base = base;
+            q.k[0] = q.k[1] = q.k[2] = q.k[3] = -1;
+            quads.push_back(q);
+        }
+        quads.back().k[off[k] - base] = k;
+    }
+    return quads;
+}
+
+/* arguments both directions share; DIA_OK or the error */
+static int check_common(const char* who, const DiaSpmmPlan* p, int dtype, int64_t M, int E,
+                        const int64_t* seg, int act, int64_t stride, const void* vals)
+{
+    const std::string w = std::string(who) + ": ";
+    if (dtype != DIA_F32 && dtype != DIA_F16 && dtype != DIA_BF16)
+        return fail(DIA_ERR_INVALID, w + "unknown dtype");
+    if (act < DIA_ACT_NONE || act > DIA_ACT_GELU_TANH)
+        return fail(DIA_ERR_INVALID, w + "unknown activation");
+    if (M < 0 || M > INT_MAX / 2) return fail(DIA_ERR_INVALID, w + "bad number of rows");
+    if (E < 1 || E > (1 << 20)) return fail(DIA_ERR_INVALID, w + "bad number of experts");
+    if (E > 1 && !seg) return fail(DIA_ERR_INVALID, w + "experts without seg");
+    if (!p) return fail(DIA_ERR_INVALID, w + "null plan");
+    int dev = -1;
+    DIA_TRY_CUDA(cudaGetDevice(&dev));
+    if (dev != p->device)
+        return fail(DIA_ERR_INVALID, w + "the plan belongs to another device");
+    if (stride < p->n_rows || stride % 32 != 0)
+        return fail(DIA_ERR_INVALID, w + "stride must be a multiple of 32, at least n_rows");
+    if (stride > INT_MAX / 2) return fail(DIA_ERR_UNSUPPORTED, w + "stride too large");
+    if (p->K > 0 && p->n_rows > 0 && !vals) return fail(DIA_ERR_INVALID, w + "null values");
+    if ((uintptr_t)vals % 16) return fail(DIA_ERR_INVALID, w + "values must be 16-byte aligned");
+    return DIA_OK;
+}
+
+/* a block of M rows of n elements: pointer, row stride and element alignment */
+static int check_block(const char* who, const char* name, const void* ptr, int64_t ld, int64_t M,
+                       int n, int dtype)
+{
+    const std::string w = std::string(who) + ": " + name;
+    if (M == 0 || n == 0) return DIA_OK;
+    if (!ptr) return fail(DIA_ERR_INVALID, w + " is null");
+    if (M > 1 && ld < n) return fail(DIA_ERR_INVALID, w + " has rows shorter than its width");
+    if ((uintptr_t)ptr % elem_size(dtype)) return fail(DIA_ERR_INVALID, w + " is misaligned");
+    return DIA_OK;
+}
+
+template <typename F>
+static int by_type(int dtype, F f)
+{
+    if (dtype == DIA_F32) return f((float*)nullptr);
+    if (dtype == DIA_F16) return f((__half*)nullptr);
+    return f((__nv_bfloat16*)nullptr);
+}
+
+static long long align256(long long b) { return (b + 255) / 256 * 256; }
+
+/* the gradient's workspace: dz (where the activation makes one), then sums
+ * of parts (where there are several) */
+struct GradPlan {
+    int per;
+    long long lddz, dz_bytes, part_bytes;
+};
+
+static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int64_t stride, int act)
+{
+    GradPlan g;
+    g.per = grad_part_rows(p, M, stride);
+    g.lddz = (p->n_rows + 7) / 8 * 8;
+    g.dz_bytes = act == DIA_ACT_NONE ? 0 : align256(M * g.lddz * (long long)elem_size(dtype));
+    g.part_bytes = align256(grad_slots(M, g.per) * (p->K + 1) * stride * 4);
+    return g;
+}
+
+}  // namespace dia
+
+using namespace dia;
+
+extern "C" int dia_spmm_plan_create(int64_t n_rows, int64_t n_cols, int num_diags,
+                                    const int* h_offsets, DiaSpmmPlan** plan)
+{
+    if (!plan) return fail(DIA_ERR_INVALID, "dia_spmm_plan_create: null plan");
+    *plan = nullptr;
+    if (n_rows < 0 || n_cols < 0 || num_diags < 0)
+        return fail(DIA_ERR_INVALID, "dia_spmm_plan_create: negative size");
+    if (num_diags > 0 && !h_offsets)
+        return fail(DIA_ERR_INVALID, "dia_spmm_plan_create: null offsets");
+    /* every i + d of a stored entry, and a tile beyond, stays a 32-bit int */
+    if (n_rows + n_cols > INT_MAX / 2 || num_diags > (1 << 20))
+        return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_plan_create: operator too large");
+    try {
+        std::vector<int> fwd(h_offsets, h_offsets + num_diags);
+        std::vector<int> sorted = fwd;
+        std::sort(sorted.begin(), sorted.end());
+        if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+            return fail(DIA_ERR_INVALID, "dia_spmm_plan_create: an offset occurs twice");
+        /* a diagonal outside the matrix has no entries: its place in the
+         * tables is any offset out of reach, one for each */
+        int out = (int)n_cols;
+        for (int& d : fwd)
+            if (d <= -n_rows || d >= n_cols) d = out++;
+        std::vector<int> trn(fwd.size());
+        for (size_t k = 0; k < fwd.size(); ++k) trn[k] = -fwd[k];
+        const std::vector<Quad> qf = build_quads(fwd), qt = build_quads(trn);
+        DiaSpmmPlan* p = new DiaSpmmPlan();
+        p->n_rows = (int)n_rows;
+        p->n_cols = (int)n_cols;
+        p->K = num_diags;
+        const size_t bytes = (qf.size() + qt.size()) * sizeof(Quad);
+        cudaError_t e = cudaGetDevice(&p->device);
+        if (e == cudaSuccess && bytes) e = cudaMalloc(&p->blob, bytes);
+        if (e == cudaSuccess && bytes) {
+            std::vector<Quad> all(qf);
+            all.insert(all.end(), qt.begin(), qt.end());
+            e = cudaMemcpy(p->blob, all.data(), bytes, cudaMemcpyHostToDevice);
+        }
+        if (e != cudaSuccess) {
+            if (p->blob) cudaFree(p->blob);
+            delete p;
+            return cuda_fail(e, "dia_spmm_plan_create");
+        }
+        p->fwd = SpmmDir{(const Quad*)p->blob, (int)qf.size()};
+        p->trn = SpmmDir{(const Quad*)p->blob + qf.size(), (int)qt.size()};
+        *plan = p;
+        return DIA_OK;
+    } catch (const std::bad_alloc&) {
+        return fail(DIA_ERR_CAPACITY, "dia_spmm_plan_create: out of host memory");
+    }
+}
+
+extern "C" int dia_spmm_plan_destroy(DiaSpmmPlan* plan)
+{
+    if (!plan) return DIA_OK;
+    if (plan->blob) cudaFree(plan->blob);
+    delete plan;
+    return DIA_OK;
+}
+
+extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
+                        const int64_t* d_seg, const void* d_x, int64_t ldx, const void* d_vals,
+                        int64_t stride, const void* d_bias, int act, const void* d_res,
+                        int64_t ldr, void* d_z, int64_t ldz, void* d_y, int64_t ldy,
+                        cudaStream_t stream)
+{
+    const char* who = "dia_spmm";
+    int rc = check_common(who, plan, dtype, M, num_experts, d_seg, act, stride, d_vals);
+    if (rc == DIA_OK && plan->K > 0)
+        rc = check_block(who, "x", d_x, ldx, M, plan->n_cols, dtype);
+    if (rc == DIA_OK) rc = check_block(who, "y", d_y, ldy, M, plan->n_rows, dtype);
+    if (rc == DIA_OK && d_res) rc = check_block(who, "residual", d_res, ldr, M, plan->n_rows, dtype);
+    if (rc == DIA_OK && d_z) rc = check_block(who, "z", d_z, ldz, M, plan->n_rows, dtype);
+    if (rc != DIA_OK) return rc;
+    ProdArgs a{};
+    a.in = d_x;
+    a.vals = d_vals;
+    a.bias = d_bias;
+    a.res = d_res;
+    a.z = d_z;
+    a.out = d_y;
+    a.seg = (const long long*)d_seg;
+    a.ldi = ldx;
+    a.ldr = ldr;
+    a.ldz = ldz;
+    a.ldo = ldy;
+    a.stride = stride;
+    a.estride = stride * plan->K;
+    a.M = (int)M;
+    a.E = num_experts;
+    a.n_in = plan->n_cols;
+    a.n_out = plan->n_rows;
+    a.act = act;
+    a.dir = plan->fwd;
+    a.trans = false;
+    return by_type(dtype, [&](auto* t) {
+        return launch_product<std::remove_pointer_t<decltype(t)>>(a, dtype, stream);
+    });
+}
+
+extern "C" int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
+                                               int64_t stride, int act)
+{
+    if (!plan || M < 0 || M > INT_MAX / 2 || stride < 0) return -1;
+    const GradPlan g = grad_plan(plan, dtype, M, stride, act);
+    return g.dz_bytes + g.part_bytes;
+}
+
+extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
+                                 const int64_t* d_seg, const void* d_x, int64_t ldx,
+                                 const void* d_vals, int64_t stride, const void* d_dy,
+                                 int64_t lddy, int act, const void* d_z, int64_t ldz, void* d_dx,
+                                 int64_t lddx, void* d_dvals, void* d_dbias, void* d_work,
+                                 int64_t work_bytes, cudaStream_t stream)
+{
+    const char* who = "dia_spmm_backward";
+    int rc = check_common(who, plan, dtype, M, num_experts, d_seg, act, stride,
+                          d_dx ? d_vals : (const void*)16);
+    if (rc == DIA_OK && d_dvals && plan->K > 0)
+        rc = check_block(who, "x", d_x, ldx, M, plan->n_cols, dtype);
+    if (rc == DIA_OK) rc = check_block(who, "dy", d_dy, lddy, M, plan->n_rows, dtype);
+    if (rc == DIA_OK && act != DIA_ACT_NONE)
+        rc = check_block(who, "z", d_z, ldz, M, plan->n_rows, dtype);
+    if (rc == DIA_OK && d_dx) rc = check_block(who, "dx", d_dx, lddx, M, plan->n_cols, dtype);
+    if (rc != DIA_OK) return rc;
+    const GradPlan g = grad_plan(plan, dtype, M, stride, act);
+    if (g.dz_bytes + g.part_bytes > work_bytes)
+        return fail(DIA_ERR_CAPACITY, "dia_spmm_backward: workspace too small");
+    if (g.dz_bytes + g.part_bytes > 0 && (!d_work || (uintptr_t)d_work % 256))
+        return fail(DIA_ERR_INVALID, "dia_spmm_backward: workspace must be 256-byte aligned");
+
+    return by_type(dtype, [&](auto* t) -> int {
+        using T = std::remove_pointer_t<decltype(t)>;
+        const void* dz = d_dy;
+        long long lddz = lddy;
+        if (act != DIA_ACT_NONE) {
+            dz = d_work;
+            lddz = g.lddz;
+            const int r = launch_dz<T>(act, d_dy, lddy, d_z, ldz, d_work, lddz, (int)M,
+                                       plan->n_rows, stream);
+            if (r != DIA_OK) return r;
+        }
+        if (d_dvals || d_dbias) {
+            GradArgs a{};
+            a.dz = dz;
+            a.x = d_x;
+            a.dvals = plan->K > 0 ? d_dvals : nullptr;
+            a.dbias = d_dbias;
+            a.part = (float*)((char*)d_work + g.dz_bytes);
+            a.seg = (const long long*)d_seg;
+            a.lddz = lddz;
+            a.ldx = ldx;
+            a.stride = stride;
+            a.estride = stride * plan->K;
+            a.M = (int)M;
+            a.E = num_experts;
+            a.n_rows = plan->n_rows;
+            a.n_cols = plan->n_cols;
+            a.K = plan->K;
+            a.per = g.per;
+            a.slots = grad_slots(M, g.per);
+            a.dir = plan->fwd;
+            if (!a.dvals) {   /* dbias alone: x is not looked at */
+                a.dir.nquads = 0;
+                a.n_cols = 0;
+            }
+            if (stride > 0) {
+                const int r = launch_grad<T>(a, dtype, stream);
+                if (r != DIA_OK) return r;
+            }
+        }
+        if (d_dx) {
+            ProdArgs a{};
+            a.in = dz;
+            a.vals = d_vals;
+            a.out = d_dx;
+            a.seg = (const long long*)d_seg;
+            a.ldi = lddz;
+            a.ldo = lddx;
+            a.stride = stride;
+            a.estride = stride * plan->K;
+            a.M = (int)M;
+            a.E = num_experts;
+            a.n_in = plan->n_rows;
+            a.n_out = plan->n_cols;
+            a.dir = plan->trn;
+            a.trans = true;
+            return launch_product<T>(a, dtype, stream);
+        }
+        return DIA_OK;
+    });
+}

@@ -1,0 +1,255 @@
+/*
+ * spmm.cuh -- what the two translation units of the block-vector product
+ * (spmm.cu: CUDA-core kernels, plan and C entry points; spmm_tc.cu: tcgen05
+ * kernels) share: the plan, argument blocks, activations, expert lookup.
+ */
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <stdint.h>
+
+#include <vector>
+
+#include "../../include/diagpu_b200.h"
+
+namespace dia {
+
+/* Up to four diagonals whose offsets share a multiple of four: slot s holds
+ * the storage index of offset base + s, or -1. */
+struct __align__(32) Quad {
+    int base;
+    int k[4];
+    int pad[3];
+};
+
+/* One direction of a plan.  Forward: out[i] = sum_k vals[k*stride + i] *
+ * in[i + off_k].  Transposed (the gradient with respect to the input): out[j]
+ * = sum_k vals[k*stride + j + o_k] * in[j + o_k] with o_k = -off_k.  Both are
+ * lists of offsets o_k; only the weight's address differs. */
+struct SpmmDir {
+    const Quad* quads;   /* device */
+    int nquads;
+};
+
+}  // namespace dia
+
+struct DiaSpmmPlan {
+    int n_rows, n_cols, K;
+    int device;
+    void* blob;          /* device: every table of the plan */
+    dia::SpmmDir fwd, trn;
+};
+
+namespace dia {
+
+/* rows [r0, r1) of expert e; e < 0: nothing to do */
+struct RowGroup {
+    int e;
+    int r0, r1;
+    int part, nparts;    /* of the expert's parts */
+    int slot;            /* index of its first part among experts of several parts */
+};
+
+/* seg is the caller's device memory: entries are clamped to [0, M] and a
+ * decreasing pair is an empty expert, so no value of it leads out of the
+ * block (rows that two experts claim are computed by both). */
+__device__ __forceinline__ void expert_rows(const long long* seg, int e, int M, int& lo, int& hi)
+{
+    const long long a = seg[e], b = seg[e + 1];
+    lo = (int)(a < 0 ? 0 : (a > M ? M : a));
+    hi = (int)(b < 0 ? 0 : (b > M ? M : b));
+    if (hi < lo) hi = lo;
+}
+
+/* The g-th group of at most `per` consecutive rows of one expert, experts in
+ * order; an expert without rows has one empty group where `empties` is set,
+ * else none.  All 32 lanes call it and get the same answer.  Without seg the
+ * block is one expert. */
+__device__ __forceinline__ RowGroup row_group(const long long* seg, int E, int M, int per,
+                                              long long g, bool empties)
+{
+    RowGroup r;
+    if (!seg) {
+        const int cnt = max((M + per - 1) / per, empties ? 1 : 0);
+        r.e = g < cnt ? 0 : -1;
+        r.r0 = (int)min((long long)M, g * per);
+        r.r1 = (int)min((long long)M, (g + 1) * per);
+        r.part = (int)g;
+        r.nparts = cnt;
+        r.slot = 0;
+        return r;
+    }
+    const int lane = threadIdx.x & 31;
+    int slot0 = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+        const int e = e0 + lane;
+        int lo = 0, hi = 0, cnt = 0;
+        if (e < E) {
+            expert_rows(seg, e, M, lo, hi);
+            cnt = max((hi - lo + per - 1) / per, empties ? 1 : 0);
+        }
+        int inc = cnt, sl = cnt > 1 ? cnt : 0;
+        int sinc = sl;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, d);
+            const int v = __shfl_up_sync(0xffffffffu, sinc, d);
+            if (lane >= d) {
+                inc += u;
+                sinc += v;
+            }
+        }
+        const int total = __shfl_sync(0xffffffffu, inc, 31);
+        if (g < total) {
+            const unsigned hit = __ballot_sync(0xffffffffu, g < inc);
+            const int src = __ffs(hit) - 1;
+            const int part = (int)g - __shfl_sync(0xffffffffu, inc - cnt, src);
+            lo = __shfl_sync(0xffffffffu, lo, src);
+            hi = __shfl_sync(0xffffffffu, hi, src);
+            r.e = e0 + src;
+            r.r0 = (int)min((long long)hi, lo + (long long)part * per);
+            r.r1 = (int)min((long long)hi, (long long)r.r0 + per);
+            r.part = part;
+            r.nparts = __shfl_sync(0xffffffffu, cnt, src);
+            r.slot = slot0 + __shfl_sync(0xffffffffu, sinc - sl, src);
+            return r;
+        }
+        g -= total;
+        slot0 += __shfl_sync(0xffffffffu, sinc, 31);
+    }
+    r.e = -1;
+    r.r0 = r.r1 = r.part = r.nparts = r.slot = 0;
+    return r;
+}
+
+/* ------------------------------------------------------------ activations */
+
+template <int ACT>
+__device__ __forceinline__ float act_of(float z)
+{
+    if (ACT == DIA_ACT_RELU) return z < 0.0f ? 0.0f : z;          /* NaN stays NaN */
+    if (ACT == DIA_ACT_SILU) return z / (1.0f + __expf(-z));
+    if (ACT == DIA_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    if (ACT == DIA_ACT_GELU_TANH)
+        return 0.5f * z * (1.0f + tanhf(0.79788456f * (z + 0.044715f * z * z * z)));
+    return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float dact_of(float z)
+{
+    if (ACT == DIA_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
+    if (ACT == DIA_ACT_SILU) {
+        const float s = 1.0f / (1.0f + __expf(-z));
+        return s * (1.0f + z * (1.0f - s));
+    }
+    if (ACT == DIA_ACT_GELU)
+        return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+    if (ACT == DIA_ACT_GELU_TANH) {
+        const float u = tanhf(0.79788456f * (z + 0.044715f * z * z * z));
+        return 0.5f * (1.0f + u) +
+               0.5f * z * (1.0f - u * u) * 0.79788456f * (1.0f + 0.134145f * z * z);
+    }
+    return 1.0f;
+}
+
+__device__ __forceinline__ float act_any(int act, float z)
+{
+    switch (act) {
+        case DIA_ACT_RELU: return act_of<DIA_ACT_RELU>(z);
+        case DIA_ACT_SILU: return act_of<DIA_ACT_SILU>(z);
+        case DIA_ACT_GELU: return act_of<DIA_ACT_GELU>(z);
+        case DIA_ACT_GELU_TANH: return act_of<DIA_ACT_GELU_TANH>(z);
+        default: return z;
+    }
+}
+
+__device__ __forceinline__ float dact_any(int act, float z)
+{
+    switch (act) {
+        case DIA_ACT_RELU: return dact_of<DIA_ACT_RELU>(z);
+        case DIA_ACT_SILU: return dact_of<DIA_ACT_SILU>(z);
+        case DIA_ACT_GELU: return dact_of<DIA_ACT_GELU>(z);
+        case DIA_ACT_GELU_TANH: return dact_of<DIA_ACT_GELU_TANH>(z);
+        default: return 1.0f;
+    }
+}
+
+/* --------------------------------------------------------------- elements */
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v)
+{
+    return __float2bfloat16_rn(v);
+}
+
+/* four consecutive elements, p aligned to four elements */
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p);
+template <>
+__device__ __forceinline__ float4 load4<float>(const float* p)
+{
+    return __ldg((const float4*)p);
+}
+template <>
+__device__ __forceinline__ float4 load4<__half>(const __half* p)
+{
+    const uint2 u = __ldg((const uint2*)p);
+    const float2 a = __half22float2(*(const __half2*)&u.x);
+    const float2 b = __half22float2(*(const __half2*)&u.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+template <>
+__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p)
+{
+    const uint2 u = __ldg((const uint2*)p);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
+                       __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+}
+
+/* ------------------------------------------------------------- arguments */
+
+/* out = act(in * A + bias) + res of one direction, z kept where given */
+struct ProdArgs {
+    const void* in;
+    const void* vals;
+    const void* bias;
+    const void* res;
+    void* z;
+    void* out;
+    const long long* seg;
+    long long ldi, ldr, ldz, ldo, stride, estride;
+    int M, E, n_in, n_out;
+    int act;
+    SpmmDir dir;
+    bool trans;
+};
+
+/* dvals[k, i] = sum_t dz[t, i] x[t, i + off_k], dbias[i] = sum_t dz[t, i] */
+struct GradArgs {
+    const void* dz;
+    const void* x;
+    void* dvals;          /* may be null */
+    void* dbias;          /* may be null */
+    float* part;          /* [slots][K + 1][stride] sums of experts with several parts */
+    const long long* seg;
+    long long lddz, ldx, stride, estride;
+    int M, E, n_rows, n_cols, K;
+    int per;              /* rows a part */
+    long long slots;      /* parts that `part` holds */
+    SpmmDir dir;          /* forward */
+};
+
+}  // namespace dia

@@ -166,6 +166,69 @@ int dia_spmspm_plan_execute(const DiaSpmspmPlan* plan, const float* d_A_vals,
                             int64_t row_hi, int use_tiles, cudaStream_t stream);
 int dia_spmspm_plan_destroy(DiaSpmspmPlan* plan);
 
+/* ------------------------------------------------- block-vector product
+ *
+ * A DIA operator times a block of M vectors (tokens, states), one vector per
+ * row, and its gradients.  No counterpart in the reference, whose products
+ * take one vector.  Element t of feature i of a block p is p[t*ld + i], ld >=
+ * the block's width (any value where M <= 1), rows may not overlap.  vals is
+ * the rows layout in the block's type: vals[(e*K + k)*stride + i] = A_e[i, i +
+ * off[k]], stride a multiple of 32 and >= n_rows, 16-byte aligned; entries
+ * outside the matrix and the padding are not read as values (any bits).
+ * Blocks whose address and row strides are multiples of 16 bytes are the
+ * fastest; any element-aligned ones are taken.  Sums are fp32; results are
+ * rounded once to the block's type, the same bits on every run. */
+enum { DIA_F32 = 0, DIA_F16 = 1, DIA_BF16 = 2 };
+enum {
+    DIA_ACT_NONE = 0,
+    DIA_ACT_RELU = 1,
+    DIA_ACT_SILU = 2,
+    DIA_ACT_GELU = 3,      /* z Phi(z) */
+    DIA_ACT_GELU_TANH = 4  /* its tanh form */
+};
+
+/* Fixes an operator's shape and (distinct, any order) offsets on the current
+ * device; calls on other devices fail with DIA_ERR_INVALID.  Holds only
+ * constant tables, so calls and captured graphs may share a plan.  The plan
+ * outlives every call and graph that uses it. */
+typedef struct DiaSpmmPlan DiaSpmmPlan;
+int dia_spmm_plan_create(int64_t n_rows, int64_t n_cols, int num_diags, const int* h_offsets,
+                         DiaSpmmPlan** plan);
+int dia_spmm_plan_destroy(DiaSpmmPlan* plan);
+
+/* z[t,i] = bias[e,i] + sum_k vals[e,k,i] x[t, i + off[k]],
+ * y[t,i] = act(z[t,i]) + res[t,i].
+ * bias [num_experts, n_rows], res and z may be NULL (z receives the
+ * pre-activation that dia_spmm_backward wants).  Without d_seg num_experts
+ * is 1 and e = 0.  With it (num_experts + 1 int64 on the device, not read
+ * before the kernel runs) rows [seg[e], seg[e+1]) belong to expert e; seg
+ * does not decrease and lies in [0, M], experts may have no rows.  Rows
+ * before seg[0] and from seg[num_experts] on are left as they were.  y and z
+ * must not overlap inputs, except that y may be res itself (same address and
+ * stride).  Allocates nothing and does not synchronise. */
+int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
+             const int64_t* d_seg, const void* d_x, int64_t ldx, const void* d_vals,
+             int64_t stride, const void* d_bias, int act, const void* d_res, int64_t ldr,
+             void* d_z, int64_t ldz, void* d_y, int64_t ldy, cudaStream_t stream);
+
+/* Gradients of dia_spmm for dy = the gradient of y (that of the residual is
+ * dy itself).  With dz = dy act'(z), rounded to the block's type:
+ *   dx[t,j] = sum_k vals[e,k,j-off[k]] dz[t,j-off[k]],
+ *   dvals[e,k,i] = sum_t dz[t,i] x[t,i+off[k]]  (whole stride: 0 outside the
+ *   matrix and in the padding; 0 for an expert without rows),
+ *   dbias[e,i] = sum_t dz[t,i].
+ * dx, dvals and dbias may each be NULL; act DIA_ACT_NONE takes no z.  Outputs
+ * are overwritten, rows of dx outside [seg[0], seg[num_experts]) left as they
+ * were.  work: dia_spmm_backward_workspace bytes, 256-byte aligned, not shared
+ * by calls that may run at the same time. */
+int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
+                                    int64_t stride, int act);
+int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
+                      const int64_t* d_seg, const void* d_x, int64_t ldx, const void* d_vals,
+                      int64_t stride, const void* d_dy, int64_t lddy, int act, const void* d_z,
+                      int64_t ldz, void* d_dx, int64_t lddx, void* d_dvals, void* d_dbias,
+                      void* d_work, int64_t work_bytes, cudaStream_t stream);
+
 /* Lanczos on a symmetric DIA operator (whole matrix, rows layout, stride
  * >= n), m steps without host synchronisation: d_alpha[0..m) and
  * d_beta[0..max(m,1)) (fp64, device) receive the tridiagonal T_m whose

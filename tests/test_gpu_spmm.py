@@ -1,0 +1,548 @@
+"""A DIA operator times a block of vectors (spmm, spmm_backward) against its
+definition in 64 bits on the CPU.
+
+Tolerances are elementwise bounds.  u is half a step of the block's type, a an
+fp32 sum's unit (2^-24; 2^-22 for 16-bit types, whose sums may run on tensor
+cores, which align products before adding and cut rather than round).  With S
+the sum of |terms| of one output, a sum of K terms is off by at most (K+4) a S
+in any order.  An activation and its derivative are evaluated to within e|z|
+and e (e = 2^-18; 2^-13 for 16-bit types, a quarter of fp16's half step), and
+change by at most 1.13 times a change of z.  dz is rounded to the block's
+type.  Storing rounds once more (fp16 also flushes to steps of 2^-24)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import diagpu_b200 as dg
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+ACTS = ["none", "relu", "silu", "gelu", "gelu_tanh"]
+
+
+def unit(t):
+    return torch.finfo(t).eps / 2
+
+
+def sum_unit(t):
+    return 2.0 ** -24 if t == torch.float32 else 2.0 ** -22
+
+
+def act_err(t):
+    return 2.0 ** -18 if t == torch.float32 else 2.0 ** -13
+
+
+def tiny(t):
+    return 2.0 ** -24 if t == torch.float16 else 1e-37
+
+
+def act64(z, act):
+    if act == "relu":
+        return z.clamp(min=0)
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    if act == "gelu":
+        return 0.5 * z * torch.special.erfc(-z * math.sqrt(0.5))
+    if act == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    return z
+
+
+def dact64(z, act):
+    if act == "relu":
+        return (z > 0).double()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return s * (1 + z * (1 - s))
+    if act == "gelu":
+        return (0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+                + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi))
+    if act == "gelu_tanh":
+        c = math.sqrt(2 / math.pi)
+        t = torch.tanh(c * (z + 0.044715 * z ** 3))
+        return 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
+    return torch.ones_like(z)
+
+
+def spans(off, n, m):
+    for k, d in enumerate(off):
+        lo, hi = max(0, -d), min(n, m - d)
+        if hi > lo:
+            yield k, d, lo, hi
+
+
+def product64(off, n, m, vals, x, parts, bias=None):
+    """z and the sum of |terms|."""
+    z = torch.zeros(x.shape[0], n, dtype=torch.float64)
+    S = torch.zeros_like(z)
+    for e, a, b in parts:
+        for k, d, lo, hi in spans(off, n, m):
+            p = vals[e, k, lo:hi] * x[a:b, lo + d:hi + d]
+            z[a:b, lo:hi] += p
+            S[a:b, lo:hi] += p.abs()
+        if bias is not None:
+            z[a:b] += bias[e]
+            S[a:b] += bias[e].abs()
+    return z, S
+
+
+def gradient64(off, n, m, vals, x, dz, parts):
+    dx, dv = torch.zeros_like(x), torch.zeros_like(vals)
+    db = torch.zeros(vals.shape[0], n, dtype=torch.float64)
+    for e, a, b in parts:
+        db[e] = dz[a:b].sum(0)
+        for k, d, lo, hi in spans(off, n, m):
+            dx[a:b, lo + d:hi + d] += vals[e, k, lo:hi] * dz[a:b, lo:hi]
+            dv[e, k, lo:hi] = (dz[a:b, lo:hi] * x[a:b, lo + d:hi + d]).sum(0)
+    return dx, dv, db
+
+
+def near(got, want, tol, what):
+    got = got.double().cpu()
+    bad = ~((got - want).abs() <= tol)
+    assert not bool(bad.any()), (what, int(bad.sum()), (got - want).abs()[bad][:4].tolist(),
+                                 tol[bad][:4].tolist(), bad.nonzero()[:4].tolist())
+
+
+class Case:
+    """Inputs on the GPU and, exactly the same values, in 64 bits on the CPU."""
+
+    def __init__(self, t, M, n, m, off, *, seed=0, seg=None, ld=None, shift=0, junk=None,
+                 mult=True):
+        g = torch.Generator().manual_seed(seed)
+        self.t, self.M, self.n, self.m, self.off, self.seg = t, M, n, m, list(off), seg
+        self.E = 1 if seg is None else len(seg) - 1
+        K = len(self.off)
+        stride = max(32, (n + 31) // 32 * 32)
+        v = torch.zeros(self.E, K, stride, dtype=torch.float64)
+        if junk is not None:
+            v += junk
+        for k, d, lo, hi in spans(self.off, n, m):
+            v[:, k, lo:hi] = torch.randn(self.E, hi - lo, generator=g, dtype=torch.float64)
+        self.vals = v.to(t).cuda()
+        self.ld, self.shift = ld, shift
+        self.x = self.block(torch.randn(M, m, generator=g))
+        self.dy = self.block(torch.randn(M, n, generator=g))
+        self.zin = self.block(torch.randn(M, n, generator=g) * 2)
+        self.res = self.block(torch.randn(M, n, generator=g))
+        self.bias = torch.randn(self.E, n, generator=g).to(t).cuda()
+        if seg is None:
+            self.parts = [(0, 0, M)]
+            self.dseg = None
+        else:
+            self.parts = [(e, seg[e], seg[e + 1]) for e in range(self.E)]
+            self.dseg = torch.tensor(seg, dtype=torch.int64).cuda()
+        self.plan = dg.SpmmPlan(n, m, np.array(self.off, np.int32))
+
+    def block(self, v):
+        """v on the GPU in rows of ld elements (None: adjacent), `shift` elements
+        past an aligned address."""
+        M, w = v.shape
+        ld = w if self.ld is None else w + self.ld
+        buf = torch.full((M * ld + self.shift + 8,), 7.0, dtype=self.t, device="cuda")
+        b = buf[self.shift:self.shift + M * ld].view(M, ld)[:, :w]
+        b.copy_(v)
+        return b
+
+    def v(self, a):
+        return a.double().cpu()
+
+    def pv(self):
+        return self.vals if self.seg is not None else self.vals[0]
+
+    def rows(self):
+        r = torch.zeros(self.M, dtype=torch.bool)
+        for _, a, b in self.parts:
+            r[a:b] = True
+        return r
+
+    def product(self, act="none", bias=False, res=False, z=False):
+        out = self.block(torch.full((self.M, self.n), 3.0))
+        zb = self.block(torch.full((self.M, self.n), 5.0)) if z else None
+        b = None if not bias else (self.bias if self.seg is not None else self.bias[0])
+        r = dg.spmm(self.plan, self.pv(), self.x, bias=b, act=act,
+                    residual=self.res if res else None, seg=self.dseg, out=out, z=zb)
+        y = r[0] if z else r
+        t, K, u = self.t, len(self.off), unit(self.t)
+        z64, S = product64(self.off, self.n, self.m, self.v(self.vals), self.v(self.x),
+                           self.parts, self.v(self.bias) if bias else None)
+        ez = (K + 4) * sum_unit(t) * S
+        f = act64(z64, act)
+        want = f + (self.v(self.res) if res else 0)
+        tol = 1.13 * ez + (act_err(t) * z64.abs() if act not in ("none", "relu") else 0)
+        tol = tol + 2.0 ** -23 * (f.abs() + want.abs())
+        on = self.rows()
+        near(y[on], want[on], (tol + u * (want.abs() + tol) + tiny(t))[on], "y")
+        assert bool((y[~on].cpu() == 3).all())
+        if z:
+            near(r[1][on], z64[on], (ez + u * (z64.abs() + ez) + tiny(t))[on], "z")
+            assert bool((r[1][~on].cpu() == 5).all())
+        return y
+
+    def gradient(self, act="none", bias=True):
+        t, K, u, n, m = self.t, len(self.off), unit(self.t), self.n, self.m
+        dx = self.block(torch.full((self.M, m), 3.0))
+        dv = torch.full_like(self.vals, 9.0)
+        db = torch.full_like(self.bias, 9.0) if bias else None
+        z = self.zin if act != "none" else None
+        sq = (lambda a: a) if self.seg is not None else (lambda a: a[0])
+        dg.spmm_backward(self.plan, self.pv(), self.x, self.dy, z=z, act=act, seg=self.dseg,
+                         dx=dx, dvals=sq(dv), dbias=sq(db) if bias else None)
+        dy, x, vals = self.v(self.dy), self.v(self.x), self.v(self.vals)
+        dz = dy if act == "none" else dy * dact64(self.v(self.zin), act)
+        ed = torch.zeros_like(dz)
+        if act != "none":
+            ed = 1.01 * u * dz.abs() + tiny(t)
+            if act != "relu":
+                ed += 1.01 * act_err(t) * dy.abs()
+        gx, gv, gb = gradient64(self.off, n, m, vals, x, dz, self.parts)
+        sx, sv, sb = gradient64(self.off, n, m, vals.abs(), x.abs(), dz.abs(), self.parts)
+        tx, tv, tb = gradient64(self.off, n, m, vals.abs(), x.abs(), ed, self.parts)
+        on = self.rows()
+        long = max([b - a for _, a, b in self.parts], default=0)
+        for got, want, S, T, terms, what in ((dx[on], gx[on], sx[on], tx[on], K, "dx"),
+                                             (dv, gv, sv, tv, long, "dvals"),
+                                             (db, gb, sb, tb, long, "dbias")):
+            if got is None:
+                continue
+            e = T + (terms + 4) * sum_unit(t) * (S + T)
+            near(got, want, e + u * (want.abs() + e) + tiny(t), what)
+        assert bool((dx[~on].cpu() == 3).all())
+        return dx, dv, db
+
+
+def band(w):
+    return list(range(-w, w + 1))
+
+
+# name: (M, n_rows, n_cols, offsets)
+SHAPES = {
+    "one": (1, 1, 1, [0]),
+    "one row": (1, 128, 128, band(3)),
+    "odd": (5, 37, 37, band(4)),
+    "unsorted": (9, 64, 64, [5, -3, 0, 1, 40, -63]),
+    "no diagonal": (3, 40, 40, []),
+    "outside": (4, 40, 33, [0, 33, 100, -40, -39, 2 ** 30, -2 ** 31]),
+    "wide": (7, 100, 260, [0, 1, 2, 100, 159, 259, -99]),
+    "tall": (66, 260, 100, [0, -1, -159, 99, -259, -160, -161]),
+    "tile": (128, 128, 128, band(64)),
+    "tile+1": (129, 129, 136, band(64)),
+    "wide band": (200, 328, 328, band(130)),
+    "scattered": (130, 640, 640, [-512, -377, -200, -111, -64, -7, 0, 1, 13, 90, 255, 511]),
+    "stencil": (257, 512, 512, [i + 8 * j + 64 * k for i in (-1, 0, 1) for j in (-1, 0, 1)
+                                for k in (-1, 0, 1)]),
+    "long": (700, 264, 264, band(20)),
+}
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_product(shape, t):
+    Case(t, *SHAPES[shape], seed=1).product(bias=True)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gradient(shape, t):
+    Case(t, *SHAPES[shape], seed=2).gradient(act="silu")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M", [2, 150])
+def test_epilogue(M, act, t):
+    c = Case(t, M, 200, 200, band(9), seed=3)
+    c.product(act=act, bias=True, res=True, z=True)
+    c.product(act=act, z=True)
+    c.product(act=act, res=True)
+    c.gradient(act=act)
+    c.gradient(act=act, bias=False)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("ld,shift", [(8, 0), (1, 0), (None, 1), (24, 8), (3, 3), (64, 2)])
+def test_strides_and_alignment(ld, shift, t):
+    c = Case(t, 140, 136, 144, band(12), seed=4, ld=ld, shift=shift)
+    c.product(act="gelu", bias=True, res=True, z=True)
+    c.gradient(act="gelu")
+
+
+SEGS = {
+    "one expert": [0, 150],
+    "empty ones": [0, 0, 1, 1, 64, 64, 64, 150, 150],
+    "rows around": [3, 40, 140],
+    "no rows": [0, 0, 0],
+    "none at the end": [10, 10],
+    "many": list(range(0, 151)),
+    "ragged": [0, 2, 7, 8, 71, 149, 149, 150],
+}
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("name", SEGS)
+def test_experts(name, t):
+    c = Case(t, 150, 136, 136, band(10), seed=5, seg=SEGS[name])
+    c.product(act="silu", bias=True, res=True, z=True)
+    c.gradient(act="silu")
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_experts_long_and_short(t):
+    c = Case(t, 1500, 72, 72, band(3), seed=6, seg=[0, 1100, 1101, 1101, 1500])
+    c.product(act="gelu", bias=True)
+    c.gradient(act="gelu")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M", [3, 140])
+def test_unread_values(M, t):
+    """Bits outside the matrix, in the padding and in rows outside every expert
+    do not reach a result."""
+    nan = float("nan")
+    c = Case(t, M, 130, 120, band(20), seed=7, junk=nan, seg=[1, 2, M - 1])
+    for b in (c.x, c.dy, c.zin, c.res):
+        b[0] = nan
+        b[M - 1] = nan
+    c.product(act="gelu", bias=True, res=True)
+    outside = c.vals.isnan()
+    dx = torch.zeros(M, 120, dtype=t, device="cuda")
+    dv = torch.full_like(c.vals, 9.0)
+    db = torch.full_like(c.bias, 9.0)
+    dg.spmm_backward(c.plan, c.vals, c.x, c.dy, z=c.zin, act="gelu", seg=c.dseg, dx=dx, dvals=dv,
+                     dbias=db)
+    assert bool(dx.isfinite().all() and dv.isfinite().all() and db.isfinite().all())
+    assert bool((dv[outside] == 0).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_infinite_values_stay_where_they_belong(value, M, t):
+    """An infinite or undefined feature reaches exactly the outputs that a
+    diagonal joins to it; the rest keep their values."""
+    n, off = 200, [-33, -2, 0, 5, 6, 70]
+    c = Case(t, M, n, n, off, seed=8)
+    x0, dy0 = c.x.clone(), c.dy.clone()
+    y0 = dg.spmm(c.plan, c.vals[0], c.x)
+    dx0, dv0, _ = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy)
+    c.x[1, 100] = value
+    y = dg.spmm(c.plan, c.vals[0], c.x)
+    hit = torch.zeros(M, n, dtype=torch.bool, device="cuda")
+    hit[1, [100 - d for d in off]] = True
+    assert bool((~y[hit].isfinite()).all())
+    assert torch.equal(y[~hit], y0[~hit])
+    if not math.isnan(value):      # one infinite term: the sum is that infinity
+        sign = torch.stack([c.vals[0, k, 100 - d] for k, d in enumerate(off)]).sign() * value
+        assert torch.equal(torch.stack([y[1, 100 - d] for d in off]), sign)
+    _, dv, _ = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy)
+    hit = torch.zeros(len(off), 224, dtype=torch.bool, device="cuda")
+    for k, d in enumerate(off):
+        hit[k, 100 - d] = True
+    assert bool((~dv[hit].isfinite()).all())
+    assert torch.equal(dv[~hit], dv0[~hit])
+    c.x.copy_(x0)
+    c.dy[2, 90] = value
+    dx, dv, _ = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy)
+    hit = torch.zeros(M, n, dtype=torch.bool, device="cuda")
+    hit[2, [90 + d for d in off]] = True
+    assert bool((~dx[hit].isfinite()).all())
+    assert torch.equal(dx[~hit], dx0[~hit])
+    assert bool((~dv[:, 90].isfinite()).all())
+    keep = torch.ones(224, dtype=torch.bool, device="cuda")
+    keep[90] = False
+    assert torch.equal(dv[:, keep], dv0[:, keep])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("seg", [[0, 90, 20, 200], [-5, 50, 100, 10 ** 12], [200, 0, 200, 0],
+                                 [0, 200, 0, 200]])
+def test_bad_segments_stay_inside(seg, t):
+    """A seg that decreases or leaves the block gives some result, without a
+    read or write outside the buffers."""
+    c = Case(t, 200, 136, 136, band(6), seed=9, seg=[0, 50, 100, 200])
+    s = torch.tensor(seg, dtype=torch.int64).cuda()
+    guard = torch.full((3, 200, 136), 3.0, dtype=t, device="cuda")
+    dg.spmm(c.plan, c.vals, c.x, seg=s, out=guard[1])
+    dg.spmm_backward(c.plan, c.vals, c.x, c.dy, seg=s, dx=guard[1])
+    torch.cuda.synchronize()
+    assert bool((guard[0] == 3).all() and (guard[2] == 3).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M", [1, 600])
+def test_same_bits_every_time(M, t):
+    c = Case(t, M, 264, 264, band(30), seed=10)
+    a = dg.spmm(c.plan, c.vals[0], c.x, act="gelu")
+    ga = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=c.zin, act="gelu", bias_grad=True)
+    for _ in range(3):
+        assert torch.equal(a, dg.spmm(c.plan, c.vals[0], c.x, act="gelu"))
+        gb = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=c.zin, act="gelu", bias_grad=True)
+        assert all(torch.equal(p, q) for p, q in zip(ga, gb))
+
+
+def test_result_over_the_residual():
+    c = Case(torch.bfloat16, 140, 136, 136, band(6), seed=11)
+    want = dg.spmm(c.plan, c.vals[0], c.x, act="silu", residual=c.res)
+    r = c.res.clone()
+    dg.spmm(c.plan, c.vals[0], c.x, act="silu", residual=r, out=r)
+    assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_streams_and_graphs(t):
+    """Two streams at once with one plan; then forward and backward captured
+    into a graph and replayed on new inputs, beside a second graph of the same
+    plan with buffers of its own."""
+    a, b = (Case(t, 300, 200, 200, band(12), seed=s) for s in (12, 13))
+    want = []
+    for c in (a, b):
+        y, z = dg.spmm(c.plan, c.vals[0], c.x, act="gelu", save_z=True)
+        want.append((y, *dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=z, act="gelu",
+                                          bias_grad=True)))
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        got = []
+        for c, s in zip((a, b), side):
+            y, z = dg.spmm(a.plan, c.vals[0], c.x, act="gelu", save_z=True, stream=s)
+            got.append((y, *dg.spmm_backward(a.plan, c.vals[0], c.x, c.dy, z=z, act="gelu",
+                                             bias_grad=True, stream=s)))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(g, w))
+    graphs, outs = [], []
+    for c in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y, z = dg.spmm(a.plan, c.vals[0], c.x, act="gelu", save_z=True)
+            outs.append((y, *dg.spmm_backward(a.plan, c.vals[0], c.x, c.dy, z=z, act="gelu",
+                                              bias_grad=True)))
+        graphs.append(g)
+    x = a.x.clone()
+    a.x.copy_(b.x)
+    for s, g in zip(side, graphs):
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(outs[1], want[1]))
+    a.x.copy_(x)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(outs[0], want[0]))
+
+
+class Layer(torch.autograd.Function):
+    """How a program trains such a layer."""
+
+    @staticmethod
+    def forward(ctx, plan, act, seg, x, vals, bias, residual):
+        y, z = dg.spmm(plan, vals, x, bias=bias, act=act, residual=residual, seg=seg, save_z=True)
+        ctx.plan, ctx.act = plan, act
+        ctx.save_for_backward(x, vals, z, *([seg] if seg is not None else []))
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, vals, z, *seg = ctx.saved_tensors
+        dx, dvals, dbias = dg.spmm_backward(ctx.plan, vals, x, dy.contiguous(), z=z, act=ctx.act,
+                                            seg=seg[0] if seg else None, bias_grad=True)
+        return None, None, None, dx, dvals, dbias, dy
+
+
+@pytest.mark.parametrize("grouped", [False, True])
+def test_layers_trained_together(grouped):
+    """Two layers with a residual, as a model runs them: the loss's derivative
+    along random directions against differences of the same loss in 64 bits.
+    The step h = 1e-5 leaves about h^2 and 1e-16 / h of the loss's size, and the
+    fp32 gradients K * 2^-24 of theirs: 1e-4 of the gradients' norm covers all."""
+    M, n, m = 40, 96, 80
+    seg = [0, 11, 11, 40] if grouped else None
+    up = Case(torch.float32, M, n, m, band(5), seed=14, seg=seg)
+    down = Case(torch.float32, M, m, n, band(7), seed=15, seg=seg)
+    sq = (lambda a: a) if grouped else (lambda a: a[0])
+    theta = [up.x.clone(), sq(up.vals).clone(), sq(up.bias).clone(), sq(down.vals).clone(),
+             sq(down.bias).clone()]
+    theta = [p.requires_grad_() for p in theta]
+    x, v1, b1, v2, b2 = theta
+    target = torch.randn(M, m, generator=torch.Generator().manual_seed(3)).cuda()
+    h = Layer.apply(up.plan, "gelu", up.dseg, x, v1, b1, torch.zeros(M, n, device="cuda"))
+    y = Layer.apply(down.plan, "none", down.dseg, h, v2, b2, x)
+    ((y - target) ** 2).sum().backward()
+
+    def loss(p):
+        x, v1, b1, v2, b2 = p
+        f = lambda a, dims: a if a.dim() == dims else a[None]
+        z, _ = product64(up.off, n, m, f(v1, 3), x, up.parts, f(b1, 2))
+        z2, _ = product64(down.off, m, n, f(v2, 3), act64(z, "gelu"), down.parts, f(b2, 2))
+        return float(((z2 + x - target.double().cpu()) ** 2).sum())
+
+    base = [p.detach().double().cpu() for p in theta]
+    g = torch.Generator().manual_seed(16)
+    for j in range(len(base)):
+        d = torch.randn(base[j].shape, generator=g, dtype=torch.float64)
+        d /= d.norm()
+        step = 1e-5
+        lo = loss([b - step * d if i == j else b for i, b in enumerate(base)])
+        hi = loss([b + step * d if i == j else b for i, b in enumerate(base)])
+        grad = theta[j].grad.double().cpu()
+        assert abs((hi - lo) / (2 * step) - float((grad * d).sum())) <= 1e-4 * float(grad.norm())
+
+
+def test_matches_spmv():
+    """One fp32 vector: the same operator through spmv."""
+    n, off = 5000, [-70, -1, 0, 1, 70]
+    A = dg.DiaRows.synth(n, n, np.array(off, np.int32), seed=1)
+    x = dg.synth_vector(n, seed=2)
+    y = dg.spmm(dg.SpmmPlan(n, n, off), A.vals, x[None])
+    ref = dg.spmv(A, x)[:n]
+    S = product64(off, n, n, A.vals.double().cpu()[None], x.double().cpu()[None],
+                  [(0, 0, 1)])[1][0]
+    near(y[0], ref.double().cpu(), 2 * 9 * 2.0 ** -24 * S, "spmv")
+
+
+def test_offsets_past_32_bits():
+    """Rows whose element offsets pass 2^31: views far apart in one buffer."""
+    n, M, off = 64, 3, band(2)
+    ld = (1 << 30) + 8
+    buf = torch.empty(2 * ld + n, dtype=torch.bfloat16, device="cuda")
+    x = buf.as_strided((M, n), (ld, 1))
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x.copy_(torch.randn(M, n, generator=g, device="cuda"))
+    v = torch.randn(5, 64, generator=g, device="cuda").bfloat16()
+    plan = dg.SpmmPlan(n, n, off)
+    assert torch.equal(dg.spmm(plan, v, x), dg.spmm(plan, v, x.contiguous()))
+    a = dg.spmm_backward(plan, v, x, x, bias_grad=True)
+    b = dg.spmm_backward(plan, v, x.contiguous(), x.contiguous(), bias_grad=True)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_refusals_on_the_device():
+    c = Case(torch.bfloat16, 20, 64, 64, band(2), seed=17)
+    plan, v, x = c.plan, c.vals[0], c.x
+
+    def refused(code, f, *a, **k):
+        with pytest.raises(dg.DiaError) as e:
+            f(*a, **k)
+        assert e.value.code == code
+
+    refused(dg.DIA_ERR_INVALID, dg.spmm, plan, v, x.cpu())
+    refused(dg.DIA_ERR_INVALID, dg.spmm, plan, v.cpu(), x)
+    refused(dg.DIA_ERR_INVALID, dg.spmm, plan, torch.zeros(5, 48, dtype=x.dtype, device="cuda"), x)
+    refused(dg.DIA_ERR_INVALID, dg.spmm, plan, torch.zeros(5, 32, dtype=x.dtype, device="cuda"), x)
+    odd = torch.zeros(5 * 64 + 1, dtype=x.dtype, device="cuda")[1:].view(5, 64)
+    refused(dg.DIA_ERR_INVALID, dg.spmm, plan, odd, x)
+    refused(dg.DIA_ERR_INVALID, dg.spmm, plan, v, x[:1].expand(20, 64))
+    refused(dg.DIA_ERR_INVALID, dg.spmm, plan, v, x, out=torch.zeros(20, 63, dtype=x.dtype,
+                                                                      device="cuda"))
+    ws = dg.spmm_backward_workspace(plan, v, 20, "silu")
+    assert ws > 0
+    work = torch.empty(ws - 1, dtype=torch.uint8, device="cuda")
+    refused(dg.DIA_ERR_CAPACITY, dg.spmm_backward, plan, v, x, c.dy, z=c.zin, act="silu",
+            work=work)
+    work = torch.empty(ws + 1, dtype=torch.uint8, device="cuda")[1:]
+    refused(dg.DIA_ERR_INVALID, dg.spmm_backward, plan, v, x, c.dy, z=c.zin, act="silu",
+            work=work)
