@@ -96,12 +96,13 @@ def lib():
         L.dia_spmm_plan_create.argtypes = [i64, i64, i, p, p]
         L.dia_spmm_plan_destroy.argtypes = [p]
         L.dia_spmm.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i, p, i64, p, i64, p, i64, p]
-        L.dia_spmm_backward_workspace.argtypes = [p, i, i64, i64, i]
+        L.dia_spmm_backward_workspace.argtypes = [p, i, i64, i, i64, i]
         L.dia_spmm_backward_workspace.restype = i64
         L.dia_spmm_backward.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i64, i, p, i64, p,
                                         i64, p, p, p, i64, p]
+        L.dia_test_spmm_form.argtypes = [i]
         for name in ("dia_spmm_plan_create", "dia_spmm_plan_destroy", "dia_spmm",
-                     "dia_spmm_backward"):
+                     "dia_spmm_backward", "dia_test_spmm_form"):
             getattr(L, name).restype = i
         L.dia_device_status.argtypes = [p, i]
         L.dia_device_status.restype = i
@@ -892,6 +893,7 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
 def spmm_backward_workspace(plan: SpmmPlan, vals, M, act="none"):
     """Bytes of the work buffer of spmm_backward for a block of M vectors."""
     ws = lib().dia_spmm_backward_workspace(plan._h, _SPMM_TYPES[vals.dtype], int(M),
+                                           vals.shape[0] if vals.dim() == 3 else 1,
                                            vals.shape[-1], _spmm_act("spmm_backward", act))
     if ws < 0:
         raise DiaError(DIA_ERR_INVALID, "spmm_backward_workspace: bad size")

@@ -44,6 +44,8 @@
 
 #include "../../include/diagpu_b200.h"
 #include "dia_core.cuh"
+#include "spmm.cuh"
+#include "tcgen05.cuh"
 
 namespace dia {
 
@@ -78,10 +80,6 @@ struct TcArgs {
     int ntiles, beta;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p)
-{
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
 
 
 /* byte offset of element (r, k) in a K-major operand slice of 32 K-columns
@@ -94,19 +92,6 @@ __device__ __forceinline__ uint32_t kmajor_off(int r, int k)
 {
     return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((((k >> 2) ^ r) & 7) << 4) +
                       (k & 3) * 4);
-}
-
-/* UMMA shared-memory descriptor, K-major with 128-byte swizzle: SBO = 1024
- * bytes between 8-row atoms, LBO unused (1), sm_100 descriptor version 1. */
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr)
-{
-    uint64_t d = 0;
-    d |= (uint64_t)((addr >> 4) & 0x3FFF);
-    d |= (uint64_t)1 << 16;                          /* LBO (unused when swizzled) */
-    d |= (uint64_t)((1024u >> 4) & 0x3FFF) << 32;   /* SBO */
-    d |= (uint64_t)1 << 46;                          /* descriptor version */
-    d |= (uint64_t)2 << 61;                          /* SWIZZLE_128B */
-    return d;
 }
 
 /* one 4-byte cp.async into shared memory when `store`; `val` false copies
@@ -469,26 +454,6 @@ struct WsBars {
     unsigned long long win_free[kMaxWin];
 };
 
-__device__ __forceinline__ unsigned long long global_ns()
-{
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 /* Waits for the phase of `bar` with parity `parity`; false if another role
  * aborted or the wait ran past its time limit (then this one aborts). */
 __device__ bool ws_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag)
@@ -522,23 +487,6 @@ __device__ void ws_drain(uint32_t bar, uint32_t parity)
             atomicOr(&g_device_status, (unsigned)DIA_TC_TIMEOUT);
             return;
         }
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar)
-{
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
-                                            uint32_t bar, uint32_t bytes)
-{
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                 ::"r"(bar), "r"(bytes) : "memory");
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"((unsigned long long)map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8])
@@ -968,29 +916,6 @@ int gemm_diag_tc_supported(const int* h_off_A, int P, const int* h_off_B, int Q,
     return DIA_OK;
 }
 
-/* cuTensorMapEncodeTiled from the driver, fetched through the runtime so
- * the library needs no link against libcuda */
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_tiled()
-{
-    static EncodeTiledFn fn = nullptr;
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (EncodeTiledFn)p;
-    }
-    return fn;
-}
-
 /* rows x diags fp32 matrix stored diagonal-major with row stride n; box of
  * box_rows x diags */
 static bool make_map(CUtensorMap* map, const float* base, int n, int diags, int box_rows)
@@ -1094,7 +1019,10 @@ int gemm_diag_tc_launch(const float* d_DA, const float* d_DB, const int* h_off_A
 extern "C" int dia_device_status(unsigned int* flags, int clear)
 {
     if (!flags) return dia::fail(DIA_ERR_INVALID, "dia_device_status: null pointer");
+    unsigned int mm = 0;
+    DIA_TRY_CUDA(dia::spmm_tc_status(&mm, clear != 0));
     DIA_TRY_CUDA(cudaMemcpyFromSymbol(flags, dia::g_device_status, sizeof(unsigned int)));
+    *flags |= mm;
     if (clear) {
         const unsigned int z = 0;
         DIA_TRY_CUDA(cudaMemcpyToSymbol(dia::g_device_status, &z, sizeof(unsigned int)));

@@ -17,6 +17,7 @@
  * seg[e+1]) use the diagonals vals[e].
  */
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstring>
 #include <new>
@@ -304,6 +305,18 @@ spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z
 
 /* ---------------------------------------------------------------- host */
 
+/* test hook (dia_test_spmm_form): 0 the rule, 1 CUDA cores, 2 tensor cores
+ * wherever they can run */
+static std::atomic<int> g_form{0};
+
+static bool tensor_form(int dtype, long long M, int E, const SpmmDir& d)
+{
+    const int form = g_form.load(std::memory_order_relaxed);
+    if (dtype == DIA_F32 || d.nboxes == 0 || form == 1) return false;
+    if (form == 2) return true;
+    return M / std::max(E, 1) >= 64;
+}
+
 static size_t elem_size(int dtype) { return dtype == DIA_F32 ? 4 : 2; }
 
 static bool vec4(const void* p, long long ld, int dtype)
@@ -341,6 +354,8 @@ template <typename T>
 static int launch_product(const ProdArgs& a, int dtype, cudaStream_t stream)
 {
     if (a.M == 0 || a.n_out == 0) return DIA_OK;
+    if (tensor_form(dtype, a.M, a.E, a.dir) && a.n_in > 0 && spmm_tc_block(a.in, a.ldi))
+        return spmm_tc_product(a, dtype, stream);
     const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
     if (a.trans)
         return per >= 4 ? launch_product_tt<T, true, 4>(a, dtype, stream)
@@ -383,8 +398,16 @@ static int launch_dz(int act, const void* dy, long long lddy, const void* z, lon
 
 /* rows of a part of the gradient's sum: enough parts to fill the GPU, none
  * so short that writing and joining its sums costs more than it saves */
-static int grad_part_rows(const DiaSpmmPlan* p, long long M, long long stride)
+static int grad_part_rows(const DiaSpmmPlan* p, int dtype, long long M, int E, long long stride)
 {
+    if (tensor_form(dtype, M, E, p->fwd)) {
+        /* one CTA an SM */
+        const long long tiles = std::max<long long>(1, (stride + 127) / 128) *
+                                ((p->fwd.nboxes + 3) / 4);
+        const long long want = std::max<long long>(1, num_sms() / tiles);
+        const long long per = std::max<long long>(256, (M + want - 1) / want);
+        return (int)((per + 63) / 64 * 64);
+    }
     const long long tiles = std::max<long long>(1, (stride + kMmFeat - 1) / kMmFeat) *
                             std::max(1, p->fwd.nquads);
     const long long want = std::max<long long>(1, 4ll * num_sms() / tiles);
@@ -398,12 +421,23 @@ static long long grad_slots(long long M, long long per) { return M > per ? 2 * (
 template <typename T>
 static int launch_grad(const GradArgs& a, int dtype, cudaStream_t stream)
 {
+    const int cblocks = (int)((a.stride + 255) / 256);
+    const long long jgrid = (long long)a.E * (a.K + 1) * cblocks;
+    if (jgrid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
+    if (tensor_form(dtype, a.M, a.E, a.dir) && a.M > 0 && a.n_cols > 0 && a.n_rows > 0 &&
+        a.dvals && spmm_tc_block(a.dz, a.lddz) && spmm_tc_block(a.x, a.ldx)) {
+        const int r = spmm_tc_gradient(a, dtype, stream);
+        if (r != DIA_OK) return r;
+        if (a.M > a.per) {
+            spmm_join_kernel<T><<<(unsigned)jgrid, 256, 0, stream>>>(a, cblocks);
+            DIA_TRY_CUDA(cudaGetLastError());
+        }
+        return DIA_OK;
+    }
     const int ftiles = (int)((a.stride + kMmFeat - 1) / kMmFeat);
     const long long parts = a.seg ? a.M / a.per + a.E : std::max(1, (a.M + a.per - 1) / a.per);
     const long long grid = parts * ftiles * std::max(a.dir.nquads, 1);
-    const int cblocks = (int)((a.stride + 255) / 256);
-    const long long jgrid = (long long)a.E * (a.K + 1) * cblocks;
-    if (grid > INT_MAX || jgrid > INT_MAX)
+    if (grid > INT_MAX)
         return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
     if (vec4(a.dz, a.lddz, dtype) && vec4(a.x, a.ldx, dtype))
         spmm_grad_kernel<T, true><<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ftiles);
@@ -417,14 +451,38 @@ static int launch_grad(const GradArgs& a, int dtype, cudaStream_t stream)
     return DIA_OK;
 }
 
-static std::vector<Quad> build_quads(const std::vector<int>& off)
+/* (offset, storage index) in ascending order */
+static std::vector<int2> sorted_offsets(const std::vector<int>& off)
 {
-    std::vector<int> order(off.size());
-    std::iota(order.begin(), order.end(), 0);
-    std::sort(order.begin(), order.end(), [&](int a, int b) { return off[a] < off[b]; });
+    std::vector<int2> s(off.size());
+    for (size_t k = 0; k < off.size(); ++k) s[k] = make_int2(off[k], (int)k);
+    std::sort(s.begin(), s.end(), [](int2 a, int2 b) { return a.x < b.x; });
+    return s;
+}
+
+static std::vector<Box> build_boxes(const std::vector<int2>& s)
+{
+    std::vector<Box> boxes;
+    int end = INT_MIN;   /* inputs below this are covered */
+    for (const int2& o : s)
+        for (end = std::max(end, o.x & ~7); end < o.x + 128; end += 64) {
+            Box b{end, 0, 0, 0};
+            auto first = [&](int d) {
+                return (int)(std::lower_bound(s.begin(), s.end(), d,
+                                              [](int2 a, int v) { return a.x < v; }) - s.begin());
+            };
+            b.k0 = first(end - 127);
+            b.k1 = first(end + 64);
+            boxes.push_back(b);
+        }
+    return boxes;
+}
+
+static std::vector<Quad> build_quads(const std::vector<int2>& s)
+{
     std::vector<Quad> quads;
-    for (int k : order) {
-        const int base = off[k] & ~3;   /* floor to a multiple of four */
+    for (const int2& o : s) {
+        const int base = o.x & ~3;   /* floor to a multiple of four */
         if (quads.empty() || quads.back().base != base) {
             Quad q;
             std::memset(&q, 0, sizeof(q));
@@ -432,9 +490,46 @@ static std::vector<Quad> build_quads(const std::vector<int>& off)
             q.k[0] = q.k[1] = q.k[2] = q.k[3] = -1;
             quads.push_back(q);
         }
-        quads.back().k[off[k] - base] = k;
+        quads.back().k[o.x - base] = o.y;
     }
     return quads;
+}
+
+/* One direction's tables appended to `blob`; offsets into it, made pointers
+ * once the blob is on the device. */
+struct DirTables {
+    size_t quads, boxes, offs;
+    int nquads, nboxes;
+};
+
+template <typename T>
+static size_t append(std::vector<char>& blob, const std::vector<T>& v)
+{
+    const size_t at = (blob.size() + 31) / 32 * 32;
+    blob.resize(at + v.size() * sizeof(T));
+    if (!v.empty()) std::memcpy(blob.data() + at, v.data(), v.size() * sizeof(T));
+    return at;
+}
+
+static DirTables append_dir(std::vector<char>& blob, const std::vector<int>& off)
+{
+    const std::vector<int2> s = sorted_offsets(off);
+    const std::vector<Quad> q = build_quads(s);
+    const std::vector<Box> b = build_boxes(s);
+    DirTables t;
+    t.nquads = (int)q.size();
+    t.nboxes = (int)b.size();
+    t.quads = append(blob, q);
+    t.boxes = append(blob, b);
+    t.offs = append(blob, s);
+    return t;
+}
+
+static SpmmDir dir_on_device(const void* blob, const DirTables& t)
+{
+    const char* p = (const char*)blob;
+    return SpmmDir{(const Quad*)(p + t.quads), (const Box*)(p + t.boxes),
+                   (const int2*)(p + t.offs), t.nquads, t.nboxes};
 }
 
 /* arguments both directions share; DIA_OK or the error */
@@ -491,10 +586,11 @@ struct GradPlan {
     long long lddz, dz_bytes, part_bytes;
 };
 
-static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int64_t stride, int act)
+static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int E, int64_t stride,
+                          int act)
 {
     GradPlan g;
-    g.per = grad_part_rows(p, M, stride);
+    g.per = grad_part_rows(p, dtype, M, E, stride);
     g.lddz = (p->n_rows + 7) / 8 * 8;
     g.dz_bytes = act == DIA_ACT_NONE ? 0 : align256(M * g.lddz * (long long)elem_size(dtype));
     g.part_bytes = align256(grad_slots(M, g.per) * (p->K + 1) * stride * 4);
@@ -530,26 +626,23 @@ extern "C" int dia_spmm_plan_create(int64_t n_rows, int64_t n_cols, int num_diag
             if (d <= -n_rows || d >= n_cols) d = out++;
         std::vector<int> trn(fwd.size());
         for (size_t k = 0; k < fwd.size(); ++k) trn[k] = -fwd[k];
-        const std::vector<Quad> qf = build_quads(fwd), qt = build_quads(trn);
+        std::vector<char> blob;
+        const DirTables tf = append_dir(blob, fwd), tt = append_dir(blob, trn);
         DiaSpmmPlan* p = new DiaSpmmPlan();
         p->n_rows = (int)n_rows;
         p->n_cols = (int)n_cols;
         p->K = num_diags;
-        const size_t bytes = (qf.size() + qt.size()) * sizeof(Quad);
         cudaError_t e = cudaGetDevice(&p->device);
-        if (e == cudaSuccess && bytes) e = cudaMalloc(&p->blob, bytes);
-        if (e == cudaSuccess && bytes) {
-            std::vector<Quad> all(qf);
-            all.insert(all.end(), qt.begin(), qt.end());
-            e = cudaMemcpy(p->blob, all.data(), bytes, cudaMemcpyHostToDevice);
-        }
+        if (e == cudaSuccess && !blob.empty()) e = cudaMalloc(&p->blob, blob.size());
+        if (e == cudaSuccess && !blob.empty())
+            e = cudaMemcpy(p->blob, blob.data(), blob.size(), cudaMemcpyHostToDevice);
         if (e != cudaSuccess) {
             if (p->blob) cudaFree(p->blob);
             delete p;
             return cuda_fail(e, "dia_spmm_plan_create");
         }
-        p->fwd = SpmmDir{(const Quad*)p->blob, (int)qf.size()};
-        p->trn = SpmmDir{(const Quad*)p->blob + qf.size(), (int)qt.size()};
+        p->fwd = dir_on_device(p->blob, tf);
+        p->trn = dir_on_device(p->blob, tt);
         *plan = p;
         return DIA_OK;
     } catch (const std::bad_alloc&) {
@@ -597,6 +690,7 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
     a.E = num_experts;
     a.n_in = plan->n_cols;
     a.n_out = plan->n_rows;
+    a.K = plan->K;
     a.act = act;
     a.dir = plan->fwd;
     a.trans = false;
@@ -606,10 +700,10 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
 }
 
 extern "C" int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
-                                               int64_t stride, int act)
+                                               int num_experts, int64_t stride, int act)
 {
-    if (!plan || M < 0 || M > INT_MAX / 2 || stride < 0) return -1;
-    const GradPlan g = grad_plan(plan, dtype, M, stride, act);
+    if (!plan || M < 0 || M > INT_MAX / 2 || stride < 0 || num_experts < 1) return -1;
+    const GradPlan g = grad_plan(plan, dtype, M, num_experts, stride, act);
     return g.dz_bytes + g.part_bytes;
 }
 
@@ -630,7 +724,7 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
         rc = check_block(who, "z", d_z, ldz, M, plan->n_rows, dtype);
     if (rc == DIA_OK && d_dx) rc = check_block(who, "dx", d_dx, lddx, M, plan->n_cols, dtype);
     if (rc != DIA_OK) return rc;
-    const GradPlan g = grad_plan(plan, dtype, M, stride, act);
+    const GradPlan g = grad_plan(plan, dtype, M, num_experts, stride, act);
     if (g.dz_bytes + g.part_bytes > work_bytes)
         return fail(DIA_ERR_CAPACITY, "dia_spmm_backward: workspace too small");
     if (g.dz_bytes + g.part_bytes > 0 && (!d_work || (uintptr_t)d_work % 256))
@@ -690,10 +784,18 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
             a.E = num_experts;
             a.n_in = plan->n_rows;
             a.n_out = plan->n_cols;
+            a.K = plan->K;
             a.dir = plan->trn;
             a.trans = true;
             return launch_product<T>(a, dtype, stream);
         }
         return DIA_OK;
     });
+}
+
+extern "C" int dia_test_spmm_form(int form)
+{
+    if (form < 0 || form > 2) return fail(DIA_ERR_INVALID, "dia_test_spmm_form: 0, 1 or 2");
+    g_form.store(form);
+    return DIA_OK;
 }

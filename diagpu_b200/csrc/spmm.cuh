@@ -29,9 +29,22 @@ struct __align__(32) Quad {
  * in[i + off_k].  Transposed (the gradient with respect to the input): out[j]
  * = sum_k vals[k*stride + j + o_k] * in[j + o_k] with o_k = -off_k.  Both are
  * lists of offsets o_k; only the weight's address differs. */
+/* A tile of 128 outputs from i0 reads, for diagonal d, inputs i0+d ..
+ * i0+d+127.  Boxes are the 64-wide pieces of input, disjoint and in ascending
+ * order, that cover all of these: inputs i0+col .. i0+col+63, col a multiple
+ * of 8 (16 bytes: where a TMA copy may start).  Diagonals [k0, k1) of the
+ * sorted list meet it. */
+struct __align__(16) Box {
+    int col;
+    int k0, k1;
+    int pad;
+};
+
 struct SpmmDir {
     const Quad* quads;   /* device */
-    int nquads;
+    const Box* boxes;    /* device */
+    const int2* offs;    /* device: (offset, storage index), ascending */
+    int nquads, nboxes;
 };
 
 }  // namespace dia
@@ -49,6 +62,7 @@ namespace dia {
 struct RowGroup {
     int e;
     int r0, r1;
+    int hi;              /* end of the expert's rows */
     int part, nparts;    /* of the expert's parts */
     int slot;            /* index of its first part among experts of several parts */
 };
@@ -77,6 +91,7 @@ __device__ __forceinline__ RowGroup row_group(const long long* seg, int E, int M
         r.e = g < cnt ? 0 : -1;
         r.r0 = (int)min((long long)M, g * per);
         r.r1 = (int)min((long long)M, (g + 1) * per);
+        r.hi = M;
         r.part = (int)g;
         r.nparts = cnt;
         r.slot = 0;
@@ -112,6 +127,7 @@ __device__ __forceinline__ RowGroup row_group(const long long* seg, int E, int M
             r.e = e0 + src;
             r.r0 = (int)min((long long)hi, lo + (long long)part * per);
             r.r1 = (int)min((long long)hi, (long long)r.r0 + per);
+            r.hi = hi;
             r.part = part;
             r.nparts = __shfl_sync(0xffffffffu, cnt, src);
             r.slot = slot0 + __shfl_sync(0xffffffffu, sinc - sl, src);
@@ -121,8 +137,23 @@ __device__ __forceinline__ RowGroup row_group(const long long* seg, int E, int M
         slot0 += __shfl_sync(0xffffffffu, sinc, 31);
     }
     r.e = -1;
-    r.r0 = r.r1 = r.part = r.nparts = r.slot = 0;
+    r.r0 = r.r1 = r.hi = r.part = r.nparts = r.slot = 0;
     return r;
+}
+
+/* how many such groups there are (whole warp) */
+__device__ __forceinline__ long long row_groups(const long long* seg, int E, int M, int per)
+{
+    if (!seg) return (M + per - 1) / per;
+    long long n = 0;
+    for (int e = threadIdx.x & 31; e < E; e += 32) {
+        int lo, hi;
+        expert_rows(seg, e, M, lo, hi);
+        n += (hi - lo + per - 1) / per;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+    return n;
 }
 
 /* ------------------------------------------------------------ activations */
@@ -231,7 +262,7 @@ struct ProdArgs {
     void* out;
     const long long* seg;
     long long ldi, ldr, ldz, ldo, stride, estride;
-    int M, E, n_in, n_out;
+    int M, E, n_in, n_out, K;
     int act;
     SpmmDir dir;
     bool trans;
@@ -251,5 +282,12 @@ struct GradArgs {
     long long slots;      /* parts that `part` holds */
     SpmmDir dir;          /* forward */
 };
+
+/* Tensor-core forms for 16-bit blocks (spmm_tc.cu).  spmm_tc_block: address
+ * and row stride are ones TMA takes. */
+bool spmm_tc_block(const void* p, long long ld);
+int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream);
+int spmm_tc_gradient(const GradArgs& a, int dtype, cudaStream_t stream);
+cudaError_t spmm_tc_status(unsigned int* flags, bool clear);
 
 }  // namespace dia

@@ -222,12 +222,16 @@ int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
  * were.  work: dia_spmm_backward_workspace bytes, 256-byte aligned, not shared
  * by calls that may run at the same time. */
 int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
-                                    int64_t stride, int act);
+                                    int num_experts, int64_t stride, int act);
 int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
                       const int64_t* d_seg, const void* d_x, int64_t ldx, const void* d_vals,
                       int64_t stride, const void* d_dy, int64_t lddy, int act, const void* d_z,
                       int64_t ldz, void* d_dx, int64_t lddx, void* d_dvals, void* d_dbias,
                       void* d_work, int64_t work_bytes, cudaStream_t stream);
+/* Test hook: 1 makes later calls of this process use the CUDA-core form, 2 the
+ * tensor-core form wherever it can run (16-bit blocks on 16-byte boundaries),
+ * 0 the library's rule.  Workspace sizes follow it. */
+int dia_test_spmm_form(int form);
 
 /* Lanczos on a symmetric DIA operator (whole matrix, rows layout, stride
  * >= n), m steps without host synchronisation: d_alpha[0..m) and

@@ -103,4 +103,5 @@ def test_c_abi_before_cuda():
                           (dict(E=2), "seg"), (dict(), "null plan")):
             assert f(**bad) == dg.DIA_ERR_INVALID
             assert word in L.dia_last_error().decode(), bad
-    assert L.dia_spmm_backward_workspace(None, 0, 4, 32, 0) == -1
+    assert L.dia_spmm_backward_workspace(None, 0, 4, 1, 32, 0) == -1
+    assert L.dia_test_spmm_form(3) == dg.DIA_ERR_INVALID
