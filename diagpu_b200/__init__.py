@@ -95,7 +95,10 @@ def lib():
             getattr(L, name).restype = i
         L.dia_spmm_plan_create.argtypes = [i64, i64, i, p, p]
         L.dia_spmm_plan_destroy.argtypes = [p]
-        L.dia_spmm.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i, p, i64, p, i64, p, i64, p]
+        L.dia_spmm_workspace.argtypes = [p, i, i64, i]
+        L.dia_spmm_workspace.restype = i64
+        L.dia_spmm.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i, p, i64, p, i64, p, i64, p,
+                               i64, p]
         L.dia_spmm_backward_workspace.argtypes = [p, i, i64, i, i64, i]
         L.dia_spmm_backward_workspace.restype = i64
         L.dia_spmm_backward.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i64, i, p, i64, p,
@@ -803,6 +806,19 @@ def _spmm_act(who, act):
     return _SPMM_ACTS[act]
 
 
+def _spmm_work(who, work, need, plan):
+    """(pointer, bytes, buffer made here or None)"""
+    if work is None:
+        if need <= 0:
+            return None, 0, None
+        made = torch.empty(need, dtype=torch.uint8, device=plan.device)
+        return C.c_void_p(made.data_ptr()), need, made
+    if work.dtype != torch.uint8 or work.device != plan.device or not work.is_contiguous():
+        raise DiaError(DIA_ERR_INVALID, f"{who}: work must be a contiguous uint8 tensor on "
+                                        f"{plan.device}")
+    return C.c_void_p(work.data_ptr()), work.numel(), None
+
+
 def _spmm_made(stream, *made):
     """Tensors allocated here and used on a stream that is not the current one
     stay allocated until that stream has passed this point."""
@@ -813,7 +829,7 @@ def _spmm_made(stream, *made):
 
 
 def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=None,
-         save_z=False, out=None, z=None, stream=None):
+         save_z=False, out=None, z=None, work=None, stream=None):
     """act(x A^T + bias) + residual for a block x [M, n_cols] of vectors, one
     per row (dia_spmm); float32, float16 or bfloat16, all of one type.
 
@@ -822,7 +838,8 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
     rows [seg[e], seg[e + 1]) of the block meet expert e; rows outside every
     expert are left as they were (unset in a new out).  act: "none", "relu",
     "silu", "gelu", "gelu_tanh".  Returns out [M, n_rows], or (out, z) with
-    save_z or a given z: the pre-activation that spmm_backward takes."""
+    save_z or a given z: the pre-activation that spmm_backward takes.  work:
+    uint8 buffer of spmm_workspace bytes, for callers that allocate nothing."""
     who = "spmm"
     code = _spmm_act(who, act)
     dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
@@ -838,9 +855,11 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
             z = torch.empty((M, n), dtype=x.dtype, device=plan.device)
         yp, ldy = _spmm_block(who, "out", out, plan, x.dtype, M, n)
         zp, ldz = _spmm_block(who, "z", z, plan, x.dtype, M, n)
-        _spmm_made(stream, out if new_out else None, z if new_z else None)
+        wp, wbytes, made = _spmm_work(who, work, lib().dia_spmm_workspace(plan._h, dt, M, E), plan)
+        _spmm_made(stream, out if new_out else None, z if new_z else None, made)
         check(lib().dia_spmm(plan._h, dt, M, E, _dptr(seg), xp, ldx, C.c_void_p(vals.data_ptr()),
-                             stride, bp, code, rp, ldr, zp, ldz, yp, ldy, _stream(stream)))
+                             stride, bp, code, rp, ldr, zp, ldz, yp, ldy, wp, wbytes,
+                             _stream(stream)))
     return (out, z) if z is not None else out
 
 
@@ -872,22 +891,25 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
         dvals = new(tuple(vals.shape)) if dvals is None else dvals
         if dbias is None and bias_grad:
             dbias = new(bshape)
-        ws = spmm_backward_workspace(plan, vals, M, act)
-        if work is None:
-            work = new((max(ws, 1),), torch.uint8)
-        elif (work.dtype != torch.uint8 or work.device != plan.device
-              or not work.is_contiguous()):
-            raise DiaError(DIA_ERR_INVALID, f"{who}: work must be a contiguous uint8 tensor on "
-                                            f"{plan.device}")
+        wp, wbytes, wmade = _spmm_work(who, work, spmm_backward_workspace(plan, vals, M, act), plan)
+        made.append(wmade)
         dxp, lddx = _spmm_block(who, "dx", dx, plan, x.dtype, M, plan.n_cols)
         dvp = _spmm_vector(who, "dvals", dvals, plan, x.dtype, tuple(vals.shape))
         dbp = _spmm_vector(who, "dbias", dbias, plan, x.dtype, bshape)
         _spmm_made(stream, *made)
         check(lib().dia_spmm_backward(plan._h, dt, M, E, _dptr(seg), xp, ldx,
                                       C.c_void_p(vals.data_ptr()), stride, gp, lddy, code, zp,
-                                      ldz, dxp, lddx, dvp, dbp, C.c_void_p(work.data_ptr()),
-                                      work.numel(), _stream(stream)))
+                                      ldz, dxp, lddx, dvp, dbp, wp, wbytes, _stream(stream)))
     return dx, dvals, dbias
+
+
+def spmm_workspace(plan: SpmmPlan, vals, M):
+    """Bytes of the work buffer of spmm for a block of M vectors."""
+    ws = lib().dia_spmm_workspace(plan._h, _SPMM_TYPES[vals.dtype], int(M),
+                                  vals.shape[0] if vals.dim() == 3 else 1)
+    if ws < 0:
+        raise DiaError(DIA_ERR_INVALID, "spmm_workspace: bad size")
+    return ws
 
 
 def spmm_backward_workspace(plan: SpmmPlan, vals, M, act="none"):

@@ -284,22 +284,42 @@ __global__ void __launch_bounds__(256) spmm_join_kernel(GradArgs a, int cblocks)
 
 /* dz = dy * act'(z), rounded to the block's type: both gradients read it as
  * a matrix operand of that type, and one rounding of half a step is no more
- * than the ones dy and z already carry. */
-template <typename T, int ACT>
+ * than the ones dy and z already carry.  Eight elements a thread. */
+template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256)
 spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z, long long ldz,
                T* __restrict__ dz, long long lddz, int M, int n)
 {
-    const long long per = (n + 3) / 4;
-    const long long total = per * M;
+    const int per = (n + 7) / 8;
+    const long long total = (long long)per * M;
     for (long long p = blockIdx.x * 256ll + threadIdx.x; p < total; p += gridDim.x * 256ll) {
         const long long t = p / per;
-        const int i = (int)(p % per) * 4;
+        const int i = (int)(p - t * per) * 8;
+        const T* g = dy + t * lddy + i;
+        const T* y = z + t * ldz + i;
+        T* o = dz + t * lddz + i;
+        if (VEC && i + 8 <= n) {
+            float a[8], b[8];
+            *(float4*)a = load4<T>(g);
+            *(float4*)(a + 4) = load4<T>(g + 4);
+            *(float4*)b = load4<T>(y);
+            *(float4*)(b + 4) = load4<T>(y + 4);
+            __align__(16) T r[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (i + r < n)
-                dz[t * lddz + i + r] = from_f<T>(to_f(dy[t * lddy + i + r]) *
-                                                 dact_of<ACT>(to_f(z[t * ldz + i + r])));
+            for (int c = 0; c < 8; c += 2) {
+                const float2 d = sizeof(T) == 2
+                                     ? dact2<ACT>(make_float2(b[c], b[c + 1]))
+                                     : make_float2(dact_of<ACT>(b[c]), dact_of<ACT>(b[c + 1]));
+                r[c] = from_f<T>(a[c] * d.x);
+                r[c + 1] = from_f<T>(a[c + 1] * d.y);
+            }
+#pragma unroll
+            for (int c = 0; c < (int)(8 * sizeof(T)); c += 16)
+                *(uint4*)((char*)o + c) = *(const uint4*)((const char*)r + c);
+        } else {
+            for (int c = 0; c < 8 && i + c < n; ++c)
+                o[c] = from_f<T>(to_f(g[c]) * dact_of<ACT>(to_f(y[c])));
+        }
     }
 }
 
@@ -368,10 +388,15 @@ template <typename T, int ACT>
 static void launch_dz_act(const void* dy, long long lddy, const void* z, long long ldz, void* dz,
                           long long lddz, int M, int n, cudaStream_t stream)
 {
-    const long long work = (long long)M * ((n + 3) / 4);
-    const int grid = (int)std::min<long long>((work + 255) / 256, 16ll * num_sms());
-    spmm_dz_kernel<T, ACT><<<grid, 256, 0, stream>>>((const T*)dy, lddy, (const T*)z, ldz, (T*)dz,
-                                                     lddz, M, n);
+    const long long work = (long long)M * ((n + 7) / 8);
+    const int grid = (int)std::min<long long>((work + 255) / 256, 8ll * num_sms());
+    const int dtype = sizeof(T) == 4 ? DIA_F32 : DIA_F16;
+    if (vec4(dy, lddy, dtype) && vec4(z, ldz, dtype))
+        spmm_dz_kernel<T, ACT, true><<<grid, 256, 0, stream>>>(
+            (const T*)dy, lddy, (const T*)z, ldz, (T*)dz, lddz, M, n);
+    else
+        spmm_dz_kernel<T, ACT, false><<<grid, 256, 0, stream>>>(
+            (const T*)dy, lddy, (const T*)z, ldz, (T*)dz, lddz, M, n);
 }
 
 template <typename T>
@@ -579,11 +604,18 @@ static int by_type(int dtype, F f)
 
 static long long align256(long long b) { return (b + 255) / 256 * 256; }
 
+/* the operator in tensor-core form */
+static long long pack_bytes(const SpmmDir& d, int dtype, int64_t M, int E, int n_out)
+{
+    return M > 0 && tensor_form(dtype, M, E, d) ? spmm_tc_pack_bytes(n_out, d.nboxes, E) : 0;
+}
+
 /* the gradient's workspace: dz (where the activation makes one), then sums
- * of parts (where there are several) */
+ * of parts (where there are several), then the operator's boxes */
 struct GradPlan {
     int per;
-    long long lddz, dz_bytes, part_bytes;
+    long long lddz, dz_bytes, part_bytes, pack_bytes;
+    long long bytes() const { return dz_bytes + part_bytes + pack_bytes; }
 };
 
 static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int E, int64_t stride,
@@ -594,6 +626,7 @@ static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int E, int
     g.lddz = (p->n_rows + 7) / 8 * 8;
     g.dz_bytes = act == DIA_ACT_NONE ? 0 : align256(M * g.lddz * (long long)elem_size(dtype));
     g.part_bytes = align256(grad_slots(M, g.per) * (p->K + 1) * stride * 4);
+    g.pack_bytes = pack_bytes(p->trn, dtype, M, E, p->n_cols);
     return g;
 }
 
@@ -662,7 +695,7 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
                         const int64_t* d_seg, const void* d_x, int64_t ldx, const void* d_vals,
                         int64_t stride, const void* d_bias, int act, const void* d_res,
                         int64_t ldr, void* d_z, int64_t ldz, void* d_y, int64_t ldy,
-                        cudaStream_t stream)
+                        void* d_work, int64_t work_bytes, cudaStream_t stream)
 {
     const char* who = "dia_spmm";
     int rc = check_common(who, plan, dtype, M, num_experts, d_seg, act, stride, d_vals);
@@ -672,7 +705,12 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
     if (rc == DIA_OK && d_res) rc = check_block(who, "residual", d_res, ldr, M, plan->n_rows, dtype);
     if (rc == DIA_OK && d_z) rc = check_block(who, "z", d_z, ldz, M, plan->n_rows, dtype);
     if (rc != DIA_OK) return rc;
+    const long long need = pack_bytes(plan->fwd, dtype, M, num_experts, plan->n_rows);
+    if (need > work_bytes) return fail(DIA_ERR_CAPACITY, "dia_spmm: workspace too small");
+    if (need > 0 && (!d_work || (uintptr_t)d_work % 256))
+        return fail(DIA_ERR_INVALID, "dia_spmm: workspace must be 256-byte aligned");
     ProdArgs a{};
+    a.pack = d_work;
     a.in = d_x;
     a.vals = d_vals;
     a.bias = d_bias;
@@ -699,12 +737,19 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
     });
 }
 
+extern "C" int64_t dia_spmm_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
+                                      int num_experts)
+{
+    if (!plan || M < 0 || M > INT_MAX / 2 || num_experts < 1) return -1;
+    return pack_bytes(plan->fwd, dtype, M, num_experts, plan->n_rows);
+}
+
 extern "C" int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
                                                int num_experts, int64_t stride, int act)
 {
     if (!plan || M < 0 || M > INT_MAX / 2 || stride < 0 || num_experts < 1) return -1;
     const GradPlan g = grad_plan(plan, dtype, M, num_experts, stride, act);
-    return g.dz_bytes + g.part_bytes;
+    return g.bytes();
 }
 
 extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
@@ -725,9 +770,9 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
     if (rc == DIA_OK && d_dx) rc = check_block(who, "dx", d_dx, lddx, M, plan->n_cols, dtype);
     if (rc != DIA_OK) return rc;
     const GradPlan g = grad_plan(plan, dtype, M, num_experts, stride, act);
-    if (g.dz_bytes + g.part_bytes > work_bytes)
+    if (g.bytes() > work_bytes)
         return fail(DIA_ERR_CAPACITY, "dia_spmm_backward: workspace too small");
-    if (g.dz_bytes + g.part_bytes > 0 && (!d_work || (uintptr_t)d_work % 256))
+    if (g.bytes() > 0 && (!d_work || (uintptr_t)d_work % 256))
         return fail(DIA_ERR_INVALID, "dia_spmm_backward: workspace must be 256-byte aligned");
 
     return by_type(dtype, [&](auto* t) -> int {
@@ -775,6 +820,7 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
             a.in = dz;
             a.vals = d_vals;
             a.out = d_dx;
+            a.pack = (char*)d_work + g.dz_bytes + g.part_bytes;
             a.seg = (const long long*)d_seg;
             a.ldi = lddz;
             a.ldo = lddx;

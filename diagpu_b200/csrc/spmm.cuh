@@ -158,14 +158,15 @@ __device__ __forceinline__ long long row_groups(const long long* seg, int E, int
 
 /* ------------------------------------------------------------ activations */
 
+/* fp32 blocks: CUDA's functions. */
 template <int ACT>
 __device__ __forceinline__ float act_of(float z)
 {
     if (ACT == DIA_ACT_RELU) return z < 0.0f ? 0.0f : z;          /* NaN stays NaN */
-    if (ACT == DIA_ACT_SILU) return z / (1.0f + __expf(-z));
+    if (ACT == DIA_ACT_SILU) return z / (1.0f + expf(-z));
     if (ACT == DIA_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
     if (ACT == DIA_ACT_GELU_TANH)
-        return 0.5f * z * (1.0f + tanhf(0.79788456f * (z + 0.044715f * z * z * z)));
+        return 0.5f * z * (1.0f + tanhf(0.79788456f * z * fmaf(0.044715f * z, z, 1.0f)));
     return z;
 }
 
@@ -174,15 +175,15 @@ __device__ __forceinline__ float dact_of(float z)
 {
     if (ACT == DIA_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
     if (ACT == DIA_ACT_SILU) {
-        const float s = 1.0f / (1.0f + __expf(-z));
-        return s * (1.0f + z * (1.0f - s));
+        const float s = 1.0f / (1.0f + expf(-z));
+        return s * fmaf(z, 1.0f - s, 1.0f);
     }
     if (ACT == DIA_ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+        return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
     if (ACT == DIA_ACT_GELU_TANH) {
-        const float u = tanhf(0.79788456f * (z + 0.044715f * z * z * z));
-        return 0.5f * (1.0f + u) +
-               0.5f * z * (1.0f - u * u) * 0.79788456f * (1.0f + 0.134145f * z * z);
+        const float t = tanhf(0.79788456f * z * fmaf(0.044715f * z, z, 1.0f));
+        return 0.5f * (1.0f + t) +
+               0.5f * z * (1.0f - t * t) * 0.79788456f * fmaf(0.134145f * z, z, 1.0f);
     }
     return 1.0f;
 }
@@ -198,15 +199,119 @@ __device__ __forceinline__ float act_any(int act, float z)
     }
 }
 
-__device__ __forceinline__ float dact_any(int act, float z)
+/* 16-bit blocks: two elements at a time, with the two-element fp32
+ * instructions and the hardware's approximations of 2^x and 1/x (relative
+ * errors of a few 2^-23).  They are within 2^-19 |z| of the function, far
+ * below half a step of the result:
+ *   z Phi(z) by Abramowitz and Stegun's 7.1.26 (their bound 1.5e-7 on erf):
+ *     Phi(-x) = (a1 t + .. + a5 t^5) exp(-x^2 / 2) / 2, t = 1 / (1 + p x / sqrt 2);
+ *   tanh u = 2 s - 1 with the logistic function s of 2 u. */
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 {
-    switch (act) {
-        case DIA_ACT_RELU: return dact_of<DIA_ACT_RELU>(z);
-        case DIA_ACT_SILU: return dact_of<DIA_ACT_SILU>(z);
-        case DIA_ACT_GELU: return dact_of<DIA_ACT_GELU>(z);
-        case DIA_ACT_GELU_TANH: return dact_of<DIA_ACT_GELU_TANH>(z);
-        default: return 1.0f;
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 exp2_2(float2 z)
+{
+    float2 d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d.x) : "f"(z.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d.y) : "f"(z.y));
+    return d;
+}
+__device__ __forceinline__ float2 rcp2(float2 z)
+{
+    float2 d;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d.x) : "f"(z.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d.y) : "f"(z.y));
+    return d;
+}
+
+/* 1 / (1 + 2^(c z)) for c = -log2 e times a factor */
+__device__ __forceinline__ float2 logistic2(float2 z, float c)
+{
+    return rcp2(add2(exp2_2(mul2(z, both(c))), both(1.0f)));
+}
+
+/* Phi(z), and e = exp(-z^2 / 2) */
+__device__ __forceinline__ float2 normal_cdf2(float2 z, float2& e)
+{
+    const float2 x = make_float2(fabsf(z.x), fabsf(z.y));
+    const float2 t = rcp2(fma2(x, both(0.2316419f), both(1.0f)));
+    e = exp2_2(mul2(mul2(z, z), both(-0.72134752f)));
+    float2 p = fma2(t, both(0.5307027145f), both(-0.7265760135f));
+    p = fma2(p, t, both(0.7107068705f));
+    p = fma2(p, t, both(-0.142248368f));
+    p = fma2(p, t, both(0.127414796f));
+    p = mul2(p, mul2(t, e));
+    const float2 q = fma2(p, both(-1.0f), both(1.0f));
+    return make_float2(z.x < 0.0f ? p.x : q.x, z.y < 0.0f ? p.y : q.y);
+}
+
+template <int ACT>
+__device__ __forceinline__ float2 act2(float2 z)
+{
+    if (ACT == DIA_ACT_RELU)
+        return make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
+    if (ACT == DIA_ACT_SILU) return mul2(z, logistic2(z, -1.44269504f));
+    if (ACT == DIA_ACT_GELU) {
+        float2 e;
+        return mul2(z, normal_cdf2(z, e));
     }
+    if (ACT == DIA_ACT_GELU_TANH) {
+        const float2 u = mul2(z, fma2(mul2(z, both(0.044715f)), z, both(1.0f)));
+        return mul2(z, logistic2(u, -2.0f * 0.79788456f * 1.44269504f));
+    }
+    return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float2 dact2(float2 z)
+{
+    if (ACT == DIA_ACT_RELU) return make_float2(dact_of<ACT>(z.x), dact_of<ACT>(z.y));
+    if (ACT == DIA_ACT_SILU) {
+        const float2 s = logistic2(z, -1.44269504f);
+        return mul2(s, fma2(z, fma2(s, both(-1.0f), both(1.0f)), both(1.0f)));
+    }
+    if (ACT == DIA_ACT_GELU) {
+        float2 e;
+        const float2 c = normal_cdf2(z, e);
+        return fma2(mul2(z, both(0.39894228f)), e, c);
+    }
+    if (ACT == DIA_ACT_GELU_TANH) {
+        const float2 w = mul2(z, both(0.044715f));
+        const float2 u = mul2(z, fma2(w, z, both(1.0f)));
+        const float2 s = logistic2(u, -2.0f * 0.79788456f * 1.44269504f);
+        /* s + 2 z s (1 - s) u', u' = sqrt(2 / pi) (1 + 3 * 0.044715 z^2) */
+        const float2 du = fma2(mul2(w, both(3.0f)), z, both(1.0f));
+        const float2 k = mul2(mul2(mul2(z, both(2.0f * 0.79788456f)), du),
+                              fma2(s, both(-1.0f), both(1.0f)));
+        return fma2(k, s, s);
+    }
+    return both(1.0f);
 }
 
 /* --------------------------------------------------------------- elements */
@@ -260,6 +365,7 @@ struct ProdArgs {
     const void* res;
     void* z;
     void* out;
+    void* pack;           /* tensor-core form: spmm_tc_pack_bytes, 256-byte aligned */
     const long long* seg;
     long long ldi, ldr, ldz, ldo, stride, estride;
     int M, E, n_in, n_out, K;
@@ -286,6 +392,7 @@ struct GradArgs {
 /* Tensor-core forms for 16-bit blocks (spmm_tc.cu).  spmm_tc_block: address
  * and row stride are ones TMA takes. */
 bool spmm_tc_block(const void* p, long long ld);
+long long spmm_tc_pack_bytes(int n_out, int nboxes, int E);
 int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream);
 int spmm_tc_gradient(const GradArgs& a, int dtype, cudaStream_t stream);
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear);

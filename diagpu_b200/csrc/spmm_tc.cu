@@ -10,12 +10,12 @@
  * a box that a few diagonals cross is already cheaper there; a band fills its
  * boxes by half or more.
  *
- * spmm_tc_kernel: the operator's boxes of a feature tile are laid out once in
- * shared memory (K-major, 128-byte swizzle) by four warps and kept while the
- * CTA walks along the rows of the block, whose boxes arrive by TMA; one thread
- * issues the MMAs (D = 128 rows x 128 features, fp32, tensor memory, four
- * accumulators), eight warps run the epilogue of one tile under the MMAs of
- * the next.  An operator of more boxes than shared memory holds is laid out
+ * spmm_pack_kernel writes the boxes of the operator as the tensor cores read
+ * them.  spmm_tc_kernel keeps a feature tile's boxes in shared memory while
+ * the CTA walks along the rows of the block, whose boxes arrive by TMA; one
+ * thread issues the MMAs (D = 128 rows x 128 features, fp32, tensor memory,
+ * four accumulators), sixteen warps run the epilogue of one tile under the MMAs
+ * of the next.  An operator of more boxes than shared memory holds is read
  * again for every four tiles.
  *
  * Zeros of a box meet inputs that no diagonal joins to its features; where
@@ -43,11 +43,13 @@ constexpr int kTN = 128;             /* features of a tile */
 constexpr int kBoxCols = 64;         /* one 128-byte swizzle row */
 constexpr int kBoxBytes = 128 * kBoxCols * 2;
 constexpr int kWSlots = 6;           /* operator boxes in shared memory */
-constexpr int kXStages = 6;          /* block boxes in flight */
+constexpr int kXStages = 5;          /* block boxes in flight */
 constexpr int kAccs = 4;             /* accumulators of 128 columns */
-constexpr int kBuildWarp0 = 2, kEpiWarp0t = 6, kTcWarps = 14;
-constexpr int kEpiThreads = 256;
-constexpr int kTcSmem = (kWSlots + kXStages) * kBoxBytes + 1024;
+constexpr int kEpiWarp0t = 4, kEpiWarpsT = 16, kTcWarps = kEpiWarp0t + kEpiWarpsT;
+constexpr int kOffs = 512;           /* offsets kept in shared memory */
+constexpr int kEpiThreads = kEpiWarpsT * 32;
+constexpr int kEpiBuf = 32 * 64;     /* a warp's 32 rows of 32 features */
+constexpr int kTcSmem = (kWSlots + kXStages) * kBoxBytes + kEpiWarpsT * kEpiBuf + 1024;
 
 struct MmBars {
     unsigned long long xfull[kXStages], xempty[kXStages];
@@ -77,19 +79,14 @@ __device__ __noinline__ bool mm_wait_long(uint32_t bar, uint32_t parity, volatil
     }
 }
 
-__device__ __forceinline__ bool mm_wait(unsigned long long& b, uint32_t parity,
-                                        volatile int* abort_flag)
+__device__ __forceinline__ bool mm_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag)
 {
-    const uint32_t bar = smem_u32(&b);
-    for (int it = 0; it < 64; ++it)
-        if (mbar_try(bar, parity)) return true;
-    return mm_wait_long(bar, parity, abort_flag);
+    return mbar_try(bar, parity) || mm_wait_long(bar, parity, abort_flag);
 }
 
 /* without regard to the abort flag: copies and MMAs already issued land */
-__device__ void mm_drain(unsigned long long& b, uint32_t parity)
+__device__ void mm_drain(uint32_t bar, uint32_t parity)
 {
-    const uint32_t bar = smem_u32(&b);
     const unsigned long long t0 = global_ns();
     while (!mbar_try(bar, parity))
         if (global_ns() - t0 > kMmWaitNs) {
@@ -98,11 +95,36 @@ __device__ void mm_drain(unsigned long long& b, uint32_t parity)
         }
 }
 
-__device__ __forceinline__ void mm_commit(unsigned long long& b)
+__device__ __forceinline__ void mm_commit(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                 ::"r"(smem_u32(&b)) : "memory");
+                 ::"r"(bar) : "memory");
 }
+
+/* the same one lane of the warp wherever it is asked; unlike lane == 0 it
+ * leaves the warp's control flow uniform */
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+/* a ring of N stages: the stage and the parity of its current round */
+template <int N>
+struct Ring {
+    uint32_t s = 0, round = 0;
+    __device__ __forceinline__ void next()
+    {
+        if (++s == N) {
+            s = 0;
+            round ^= 1;
+        }
+    }
+    /* address of the stage's barrier in an array of them */
+    __device__ __forceinline__ uint32_t bar(uint32_t base) const { return base + 8 * s; }
+};
 
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc,
                                         bool accumulate)
@@ -160,7 +182,7 @@ __device__ __forceinline__ float tmem_ld1(uint32_t addr)
     return v;
 }
 
-/* ------------------------------------------------- 16 elements of a row */
+/* ------------------------------------------------------ pairs of elements */
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -189,44 +211,90 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u)
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
-/* `wide`: p is 32-byte aligned and all 16 elements exist (one full sector a
- * lane); else the first n elements one by one */
-template <typename T>
-__device__ __forceinline__ void store16(T* p, const float (&v)[16], bool wide, int n)
+/* waits for the launches before this one (programmatic dependent launch) */
+__device__ __forceinline__ void dependency_wait()
 {
-    if (wide) {
-        uint32_t u[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) u[c] = pack2<T>(v[2 * c], v[2 * c + 1]);
-        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                     ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
-                       "r"(u[6]), "r"(u[7]) : "memory");
-    } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-            if (c < n) p[c] = from_f<T>(v[c]);
-    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ void load16(const T* p, float (&v)[16], bool wide, int n)
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint32_t bar)
 {
-    if (wide) {
-        uint32_t u[8];
-        asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
-                       "=r"(u[6]), "=r"(u[7])
-                     : "l"(p));
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const float2 f = unpack2<T>(u[c]);
-            v[2 * c] = f.x;
-            v[2 * c + 1] = f.y;
-        }
-    } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) v[c] = c < n ? to_f(p[c]) : 0.0f;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                 ::"r"(bar), "r"(bytes) : "memory");
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+        ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+/* The operator as the tensor cores read it: for every expert, feature tile and
+ * box a dense 128 x 64 matrix, K-major with the 128-byte swizzle.  One CTA
+ * makes one box.  It copies the pieces of the diagonals that cross the box to
+ * shared memory (each 128 consecutive features, all copies in flight at
+ * once), then a thread gathers eight columns of a feature at a time: their
+ * offsets are consecutive, a table gives their rows. */
+constexpr int kPackRows = 191;                      /* offsets that can cross a box */
+constexpr int kPackPitch = 136;                     /* 128 features, up to 7 before them */
+constexpr int kPackSmem = kBoxBytes + kPackRows * kPackPitch * 2;
+
+template <bool TRANS>
+__global__ void __launch_bounds__(256) spmm_pack_kernel(const __grid_constant__ ProdArgs a)
+{
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ int16_t s_row[kPackRows + 1];
+    __shared__ int2 s_off[kPackRows + 1];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int tid = threadIdx.x;
+    unsigned char* box = smem_raw;
+    uint16_t* slab = (uint16_t*)(smem_raw + kBoxBytes);
+    const int nb = a.dir.nboxes, nfb = (a.n_out + kTN - 1) / kTN;
+    const int b = blockIdx.x % nb, fb = blockIdx.x / nb % nfb, e = blockIdx.x / nb / nfb;
+    if (a.seg) {
+        int lo, hi;
+        expert_rows(a.seg, e, a.M, lo, hi);
+        if (lo == hi) return;   /* nobody reads them */
     }
+    const Box bx = a.dir.boxes[b];
+    const int nk = bx.k1 - bx.k0, i0 = fb * kTN;
+    for (int d = tid; d < kPackRows; d += 256) s_row[d] = -1;
+    if (tid < nk) s_off[tid] = a.dir.offs[bx.k0 + tid];
+    __syncthreads();
+    if (tid < nk) s_row[s_off[tid].x - (bx.col - 127)] = (int16_t)tid;
+    const uint16_t* vals = (const uint16_t*)a.vals + e * a.estride;
+    /* rows of 17 pieces of eight elements, from the aligned element at or
+     * before the first; elements outside [0, stride) are not read */
+    for (int o = tid; o < nk * 17; o += 256) {
+        const int k = o / 17, c = o - k * 17;
+        const int first = (TRANS ? i0 + s_off[k].x : i0) & ~7;
+        const int x = first + c * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (x >= 0 && x < a.stride) v = __ldg((const uint4*)(vals + s_off[k].y * a.stride + x));
+        *(uint4*)(slab + k * kPackPitch + c * 8) = v;
+    }
+    __syncthreads();
+    /* element (f, c) is offset col + c - f; lanes take consecutive features */
+    const int f = tid & 127, i = i0 + f;
+#pragma unroll
+    for (int q = tid >> 7; q < 8; q += 2) {
+        uint32_t u[4] = {0, 0, 0, 0};
+        if (i < a.n_out) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const int t = 8 * q + c - f + 127;            /* index into s_row */
+                const int d = t + bx.col - 127;
+                const int k = s_row[t];
+                if (k >= 0 && (unsigned)(i + d) < (unsigned)a.n_in) {
+                    const int shift = TRANS ? (i0 + d) & 7 : 0;
+                    const uint32_t v = slab[k * kPackPitch + f + shift];
+                    u[c >> 1] |= c & 1 ? v << 16 : v;
+                }
+            }
+        }
+        *(uint4*)(box + f * 128 + ((q ^ (f & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    __syncthreads();
+    uint4* dst = (uint4*)((char*)a.pack + (long long)blockIdx.x * kBoxBytes);
+#pragma unroll
+    for (int o = 0; o < kBoxBytes / 16; o += 256) dst[o + tid] = ((const uint4*)box)[o + tid];
 }
 
 /* the sum of one output's own terms, in ascending order of the offsets */
@@ -243,6 +311,26 @@ __device__ __noinline__ float product_terms(const ProdArgs& a, int K, int e, lon
             s = fmaf(to_f(vals[ok.y * a.stride + (TRANS ? j : i)]), to_f(in[j]), s);
     }
     return s;
+}
+
+/* The results of a row whose sums were not finite (bits of `which`, from
+ * feature i on), from their own terms, into the row's pieces in shared memory:
+ * row points to piece 0, pieces are spread by `spread`. */
+template <typename T, bool TRANS, int ACT>
+__device__ __noinline__ void sum_again(const ProdArgs& a, int K, int e, long long row_, int i,
+                                       uint32_t which, uint4* row, int spread, bool res)
+{
+    unsigned char* base = (unsigned char*)row - (spread << 4);
+    for (; which; which &= which - 1) {
+        const int c = __ffs(which) - 1;
+        float v = product_terms<T, TRANS>(a, K, e, row_, i + c);
+        if (!TRANS) {
+            if (a.bias) v += to_f(((const T*)a.bias)[(long long)e * a.n_out + i + c]);
+            v = act_of<ACT>(v);
+            if (res && a.res) v += to_f(((const T*)a.res)[row_ * a.ldr + i + c]);
+        }
+        *(T*)(base + (((c >> 3) ^ spread) << 4) + (c & 7) * 2) = from_f<T>(v);
+    }
 }
 
 /* A run of tiles of one feature block and one expert. */
@@ -287,11 +375,10 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     __shared__ __align__(8) MmBars bars;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ float s_bias[kTN];
+    __shared__ __align__(16) float s_bias[kTN];
     volatile int* abort_flag = &s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    unsigned char* wslot = smem;
-    unsigned char* xstage = smem + kWSlots * kBoxBytes;
+    const uint32_t wst = smem_u32(smem), xst = wst + kWSlots * kBoxBytes;
 
     if (tid == 0) {
         s_abort = 0;
@@ -300,12 +387,12 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             mbar_init(bars.xempty[s], 1);
         }
         for (int s = 0; s < kWSlots; ++s) {
-            mbar_init(bars.wfull[s], 4);
+            mbar_init(bars.wfull[s], 1);
             mbar_init(bars.wempty[s], 1);
         }
         for (int s = 0; s < kAccs; ++s) {
             mbar_init(bars.afull[s], 1);
-            mbar_init(bars.aempty[s], 8);
+            mbar_init(bars.aempty[s], kEpiWarpsT);
         }
         mbar_init(bars.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -329,143 +416,158 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     const int NB = a.dir.nboxes;
     Run r;
 
+    const uint32_t xfull = smem_u32(bars.xfull), xempty = smem_u32(bars.xempty);
+    const uint32_t wfull = smem_u32(bars.wfull), wempty = smem_u32(bars.wempty);
+    const uint32_t afull = smem_u32(bars.afull), aempty = smem_u32(bars.aempty);
     if (warp == 0) {
         /* ---------------- TMA: the block's boxes */
-        int g = 0;
+        Ring<kXStages> x;
+        int issued = 0;
         bool ok = true;
+        const bool leader = elect_one();
         while (ok && next_run(a, nt, w, w1, r)) {
             const int i0 = r.fb * kTN;
             const int used = used_boxes(a.dir, i0, a.n_in);
             const int group = used <= kWSlots ? 1 : kAccs;
-            if (lane == 0) {
-                for (int j0 = 0; j0 < r.ntiles && ok; j0 += group)
-                    for (int b = 0; b < NB && ok; ++b) {
-                        const Box bx = a.dir.boxes[b];
-                        if (!(box_used(bx, i0, a.n_in) || (used == 0 && b == 0))) continue;
-                        for (int j = j0; j < min(j0 + group, r.ntiles); ++j, ++g) {
-                            const int s = g % kXStages;
-                            ok = mm_wait(bars.xempty[s], ((g / kXStages) & 1) ^ 1, abort_flag);
-                            if (!ok) break;
-                            tma_load_2d(smem_u32(xstage + s * kBoxBytes), &tmX, i0 + bx.col,
-                                        r.r0 + j * kTM, smem_u32(&bars.xfull[s]), kBoxBytes);
-                        }
-                    }
-            }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-        }
-        /* no copy may still be landing when the CTA exits */
-        if (lane == 0)
-            for (int i = max(0, g - kXStages); i < g; ++i)
-                mm_drain(bars.xfull[i % kXStages], (i / kXStages) & 1);
-    } else if (warp == 1) {
-        /* ---------------- MMA issue */
-        const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-        const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) |
-                               ((uint32_t)(kTN >> 3) << 17) | ((uint32_t)(kTM >> 4) << 24);
-        int g = 0, q = 0, tc = 0;
-        bool ok = true;
-        while (ok && next_run(a, nt, w, w1, r)) {
-            const int i0 = r.fb * kTN;
-            const int used = max(1, used_boxes(a.dir, i0, a.n_in));
-            const bool keep = used <= kWSlots;
-            const int group = keep ? 1 : kAccs;
-            if (lane == 0) {
-                for (int j0 = 0; j0 < r.ntiles && ok; j0 += group) {
-                    const int j1 = min(j0 + group, r.ntiles);
-                    const bool last_use = !keep || j1 == r.ntiles;
-                    for (int u = 0; u < used && ok; ++u) {
-                        const int qs = q + u, slot = qs % kWSlots;
-                        if (!keep || j0 == 0)
-                            ok = mm_wait(bars.wfull[slot], (qs / kWSlots) & 1, abort_flag);
-                        const uint32_t wb = smem_u32(wslot + slot * kBoxBytes);
-                        for (int j = j0; j < j1 && ok; ++j, ++g) {
-                            const int t = tc + j - j0, acc = t % kAccs;
-                            if (u == 0)
-                                ok = mm_wait(bars.aempty[acc], ((t / kAccs) & 1) ^ 1, abort_flag);
-                            const int s = g % kXStages;
-                            ok = ok && mm_wait(bars.xfull[s], (g / kXStages) & 1, abort_flag);
-                            if (!ok) break;
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                            const uint32_t xb = smem_u32(xstage + s * kBoxBytes);
-#pragma unroll
-                            for (int kk = 0; kk < kBoxCols / 16; ++kk)
-                                mma_f16(tmem + (uint32_t)(acc * kTN), smem_desc(xb + 32u * kk),
-                                        smem_desc(wb + 32u * kk), idesc, u > 0 || kk > 0);
-                            mm_commit(bars.xempty[s]);
-                            if (u == used - 1) mm_commit(bars.afull[acc]);
-                        }
-                        if (ok && last_use) mm_commit(bars.wempty[slot]);
-                    }
-                    tc += j1 - j0;
-                    if (!keep) q += used;
-                }
-                if (keep) q += used;
-            }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-        }
-        if (lane == 0) {
-            /* every MMA issued has completed before tensor memory is freed */
-            mm_commit(bars.drain);
-            mm_drain(bars.drain, 0);
-        }
-    } else if (warp < kEpiWarp0t) {
-        /* ---------------- operator boxes: one feature a thread */
-        const int f = (warp - kBuildWarp0) * 32 + lane;
-        const uint16_t* vals0 = (const uint16_t*)a.vals;
-        int q = 0;
-        bool ok = true;
-        while (ok && next_run(a, nt, w, w1, r)) {
-            const int i0 = r.fb * kTN, i = i0 + f;
-            const int used = used_boxes(a.dir, i0, a.n_in);
-            const int reps = used <= kWSlots ? 1 : (r.ntiles + kAccs - 1) / kAccs;
-            const uint16_t* vals = vals0 + r.e * a.estride;
-            for (int rep = 0; rep < reps && ok; ++rep)
+            for (int j0 = 0; j0 < r.ntiles && ok; j0 += group)
                 for (int b = 0; b < NB && ok; ++b) {
                     const Box bx = a.dir.boxes[b];
                     if (!(box_used(bx, i0, a.n_in) || (used == 0 && b == 0))) continue;
-                    const int slot = q % kWSlots;
-                    ok = mm_wait(bars.wempty[slot], ((q / kWSlots) & 1) ^ 1, abort_flag);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    const uint32_t row = smem_u32(wslot + slot * kBoxBytes) + f * 128;
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) sts128(row + ((c ^ (f & 7)) << 4), 0);
-                    for (int k0 = bx.k0; k0 < bx.k1; k0 += 8) {
-                        uint16_t v[8];
-                        int col[8];
-#pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            col[u] = -1;
-                            if (k0 + u < bx.k1) {
-                                const int2 ok2 = __ldg(&a.dir.offs[k0 + u]);
-                                const int c = ok2.x + f - bx.col, j = i + ok2.x;
-                                if ((unsigned)c < (unsigned)kBoxCols && i < a.n_out &&
-                                    (unsigned)j < (unsigned)a.n_in) {
-                                    col[u] = c;
-                                    v[u] = __ldg(vals + ok2.y * a.stride + (TRANS ? j : i));
-                                }
-                            }
-                        }
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            if (col[u] >= 0)
-                                sts16(row + (((col[u] >> 3) ^ (f & 7)) << 4) + (col[u] & 7) * 2,
-                                      v[u]);
+                    for (int j = j0; j < min(j0 + group, r.ntiles); ++j) {
+                        ok = mm_wait(x.bar(xempty), x.round ^ 1, abort_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (leader)
+                            tma_load_2d(xst + x.s * kBoxBytes, &tmX, i0 + bx.col, r.r0 + j * kTM,
+                                        x.bar(xfull), kBoxBytes);
+                        x.next();
+                        ++issued;
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&bars.wfull[slot]));
-                    ++q;
                 }
         }
-    } else {
-        /* ---------------- epilogue: a lane is a row, a warp 64 features */
-        const int half = (warp - kEpiWarp0t) >> 2;
+        /* no copy may still be landing when the CTA exits: each stage's last */
+        for (int n = min(issued, kXStages); n < kXStages; ++n) x.next();
+        for (int n = 0; n < min(issued, kXStages); ++n, x.next())
+            mm_drain(x.bar(xfull), x.round ^ 1);
+    } else if (warp == 1) {
+        /* ---------------- MMA issue */
+        const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+        const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) |
+                               ((uint32_t)(kTN >> 3) << 17) | ((uint32_t)(kTM >> 4) << 24);
+        const bool leader = elect_one();
+        const uint64_t xdesc = smem_desc(xst), wdesc = smem_desc(wst);
+        Ring<kXStages> x;
+        Ring<kWSlots> wq;
+        Ring<kAccs> ac;
+        bool ok = true;
+        /* one box of one tile; the stage goes back to the TMA */
+        auto box = [&](uint32_t wslot, uint32_t acc, bool first) {
+            ok = mm_wait(x.bar(xfull), x.round, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (leader) {
+                const uint64_t xd = xdesc + x.s * (kBoxBytes >> 4);
+                const uint64_t wd = wdesc + wslot * (kBoxBytes >> 4);
+                const uint32_t d = tmem + acc * kTN;
+#pragma unroll
+                for (int kk = 0; kk < kBoxCols / 16; ++kk)
+                    mma_f16(d, xd + 2 * kk, wd + 2 * kk, idesc, !first || kk > 0);
+                mm_commit(x.bar(xempty));
+            }
+            x.next();
+        };
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            ok = mm_wait(bar, parity, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            return ok;
+        };
+        while (ok && next_run(a, nt, w, w1, r)) {
+            const int used = max(1, used_boxes(a.dir, r.fb * kTN, a.n_in));
+            if (used <= kWSlots) {
+                /* the boxes stay for the whole run */
+                for (int j = 0; j < r.ntiles && ok; ++j) {
+                    if (!wait(ac.bar(aempty), ac.round ^ 1)) break;
+                    Ring<kWSlots> q = wq;
+                    for (int u = 0; u < used && ok; ++u, q.next()) {
+                        if (j == 0 && !wait(q.bar(wfull), q.round)) break;
+                        box(q.s, ac.s, u == 0);
+                        if (ok && j == r.ntiles - 1 && leader) mm_commit(q.bar(wempty));
+                    }
+                    if (ok && leader) mm_commit(ac.bar(afull));
+                    ac.next();
+                    if (j == r.ntiles - 1) wq = q;
+                }
+            } else {
+                for (int j0 = 0; j0 < r.ntiles && ok; j0 += kAccs) {
+                    const int n = min(kAccs, r.ntiles - j0);
+                    Ring<kAccs> t = ac;
+                    for (int j = 0; j < n && ok; ++j, t.next()) wait(t.bar(aempty), t.round ^ 1);
+                    for (int u = 0; u < used && ok; ++u, wq.next()) {
+                        if (!wait(wq.bar(wfull), wq.round)) break;
+                        t = ac;
+                        for (int j = 0; j < n && ok; ++j, t.next()) {
+                            box(wq.s, t.s, u == 0);
+                            if (ok && u == used - 1 && leader) mm_commit(t.bar(afull));
+                        }
+                        if (ok && leader) mm_commit(wq.bar(wempty));
+                    }
+                    ac = t;
+                }
+            }
+        }
+        /* every MMA issued has completed before tensor memory is freed */
+        if (leader) mm_commit(smem_u32(&bars.drain));
+        mm_drain(smem_u32(&bars.drain), 0);
+    } else if (warp == 2) {
+        /* ---------------- the operator's boxes, as spmm_pack_kernel left them */
+        dependency_wait();
+        Ring<kWSlots> q;
+        int issued = 0;
+        bool ok = true;
+        const bool leader = elect_one();
+        while (ok && next_run(a, nt, w, w1, r)) {
+            const int i0 = r.fb * kTN;
+            const int used = used_boxes(a.dir, i0, a.n_in);
+            const int reps = used <= kWSlots ? 1 : (r.ntiles + kAccs - 1) / kAccs;
+            const char* src = (const char*)a.pack +
+                              ((long long)r.e * ((a.n_out + kTN - 1) / kTN) + r.fb) * NB * kBoxBytes;
+            for (int rep = 0; rep < reps && ok; ++rep)
+                for (int b = 0; b < NB; ++b) {
+                    if (!(box_used(a.dir.boxes[b], i0, a.n_in) || (used == 0 && b == 0))) continue;
+                    ok = mm_wait(q.bar(wempty), q.round ^ 1, abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (leader)
+                        bulk_load(wst + q.s * kBoxBytes, src + (long long)b * kBoxBytes, kBoxBytes,
+                                  q.bar(wfull));
+                    q.next();
+                    ++issued;
+                }
+        }
+        for (int n = min(issued, kWSlots); n < kWSlots; ++n) q.next();
+        for (int n = 0; n < min(issued, kWSlots); ++n, q.next())
+            mm_drain(q.bar(wfull), q.round ^ 1);
+    } else if (warp >= kEpiWarp0t) {
+        /* ---------------- epilogue: a warp's 32 rows of 32 features.  The
+         * accumulators come a row a lane; memory is read and written eight
+         * rows of 64 bytes at a time, by way of the warp's own 2 KB of shared
+         * memory (a lane that wrote its own row's 32-byte sectors to memory
+         * kept the L1 busy four times as long).  The residual is read while
+         * the tile's MMAs run. */
+        const int ew = warp - kEpiWarp0t;
+        const int fw = (ew >> 2) * 32;
         const uint32_t tq = (uint32_t)(warp & 3);
-        const bool al = ((uintptr_t)a.out % 32 == 0) && (a.ldo % 16 == 0);
-        const bool alz = ((uintptr_t)a.z % 32 == 0) && (a.ldz % 16 == 0);
-        const bool alr = ((uintptr_t)a.res % 32 == 0) && (a.ldr % 16 == 0);
-        int tc = 0;
+        unsigned char* buf = smem + (kWSlots + kXStages) * kBoxBytes + ew * kEpiBuf;
+        /* a row's four 16-byte pieces, spread over the banks */
+        auto piece = [&](int row, int c) {
+            return (uint4*)(buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+        };
+        const int crow = lane >> 2, cpc = lane & 3;   /* of memory accesses */
+        const bool al = ((uintptr_t)a.out % 16 == 0) && (a.ldo % 8 == 0);
+        const bool alz = ((uintptr_t)a.z % 16 == 0) && (a.ldz % 8 == 0);
+        const bool alr = ((uintptr_t)a.res % 16 == 0) && (a.ldr % 8 == 0);
+        Ring<kAccs> ac;
         bool ok = true;
         while (ok && next_run(a, nt, w, w1, r)) {
             const int i0 = r.fb * kTN;
@@ -478,56 +580,133 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                                     : 0.0f;
                 asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
             }
-            for (int j = 0; j < r.ntiles && ok; ++j, ++tc) {
-                const int acc = tc % kAccs;
-                ok = mm_wait(bars.afull[acc], (tc / kAccs) & 1, abort_flag);
+            const int ic = i0 + fw + 8 * cpc;              /* of this lane's pieces */
+            const int nc = min(8, a.n_out - ic);
+            /* the warp's 32 x 32 block out of shared memory */
+            auto copy_out = [&](void* p, long long ld, int row0, bool vec) {
+                __syncwarp();
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const int rr = 8 * it + crow;
+                    const long long row = (long long)row0 + rr;
+                    const uint4 u = *piece(rr, cpc);
+                    if (row < r.hi && nc > 0) {
+                        T* q = (T*)p + row * ld + ic;
+                        if (vec && nc == 8)
+                            *(uint4*)q = u;
+                        else {
+                            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                            for (int c = 0; c < nc; ++c) {
+                                const uint16_t h = (uint16_t)(x[c >> 1] >> (16 * (c & 1)));
+                                ((uint16_t*)q)[c] = h;
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+            };
+            for (int j = 0; j < r.ntiles && ok; ++j, ac.next()) {
+                const int row0 = r.r0 + j * kTM + 32 * (int)tq;
+                const bool live = row0 + lane < r.hi;
+                if (!TRANS && a.res) {
+                    uint4 rr[4];
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) {
+                        const long long row = (long long)row0 + 8 * it + crow;
+                        const T* q = (const T*)a.res + row * a.ldr + ic;
+                        rr[it] = make_uint4(0, 0, 0, 0);
+                        if (row < r.hi && nc > 0) {
+                            if (alr && nc == 8)
+                                rr[it] = *(const uint4*)q;
+                            else {
+                                uint32_t x[4] = {0, 0, 0, 0};
+#pragma unroll
+                                for (int c = 0; c < 8; ++c)
+                                    if (c < nc)
+                                        x[c >> 1] |= (uint32_t)((const uint16_t*)q)[c] << (16 * (c & 1));
+                                rr[it] = make_uint4(x[0], x[1], x[2], x[3]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) *piece(8 * it + crow, cpc) = rr[it];
+                    __syncwarp();
+                }
+                ok = mm_wait(ac.bar(afull), ac.round, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const long long row = (long long)r.r0 + j * kTM + 32 * (int)tq + lane;
-                const bool live = row < r.hi;
-                const uint32_t ta = tmem + ((tq * 32) << 16) + (uint32_t)(acc * kTN + 64 * half);
+                uint32_t y[16], again = 0;
+                const uint32_t ta = tmem + ((tq * 32) << 16) + (uint32_t)(ac.s * kTN + fw);
 #pragma unroll
-                for (int cc = 0; cc < 4; ++cc) {
+                for (int cc = 0; cc < 2; ++cc) {
                     float v[16];
                     tmem_ld16(ta + 16u * cc, v);
-                    if (cc == 3) {
+                    if (cc == 1) {
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&bars.aempty[acc]));
+                        if (lane == 0) mbar_arrive(ac.bar(aempty));
                     }
-                    const int fo = 64 * half + 16 * cc, i = i0 + fo;
-                    const int n = a.n_out - i;
-                    if (live && n > 0) {
-                        float chk = 0.0f;
-    #pragma unroll
-                        for (int c = 0; c < 16; ++c) chk = fmaf(v[c], 0.0f, chk);
-                        if (chk != 0.0f) {   /* some sum is not finite */
-    #pragma unroll
-                            for (int c = 0; c < 16; ++c)
-                                if (c < n && !isfinite(v[c]))
-                                    v[c] = product_terms<T, TRANS>(a, K, r.e, row, i + c);
-                        }
-                        if (!TRANS) {
-    #pragma unroll
-                            for (int c = 0; c < 16; ++c) v[c] += s_bias[fo + c];
-                            if (a.z)
-                                store16<T>((T*)a.z + row * a.ldz + i, v, alz && n >= 16, n);
-                            if (ACT != DIA_ACT_NONE) {
-    #pragma unroll
-                                for (int c = 0; c < 16; ++c) v[c] = act_of<ACT>(v[c]);
-                            }
-                            if (a.res) {
-                                float u[16];
-                                load16<T>((const T*)a.res + row * a.ldr + i, u, alr && n >= 16, n);
-    #pragma unroll
-                                for (int c = 0; c < 16; ++c) v[c] += u[c];
-                            }
-                        }
-                        store16<T>((T*)a.out + row * a.ldo + i, v, al && n >= 16, n);
+                    const int fo = fw + 16 * cc;
+                    uint32_t res[8];
+                    float2 chk = both(0.0f);
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2)
+                        chk = fma2(make_float2(v[c], v[c + 1]), both(0.0f), chk);
+                    if (chk.x + chk.y != 0.0f && live) {   /* some sum is not finite */
+#pragma unroll
+                        for (int c = 0; c < 16; ++c)
+                            if (!isfinite(v[c]) && i0 + fo + c < a.n_out) again |= 1u << (16 * cc + c);
                     }
                     __syncwarp();
+                    if (!TRANS) {
+#pragma unroll
+                        for (int c = 0; c < 16; c += 4) {
+                            const float4 b = *(const float4*)&s_bias[fo + c];
+                            const float2 p = add2(make_float2(v[c], v[c + 1]), make_float2(b.x, b.y));
+                            const float2 q = add2(make_float2(v[c + 2], v[c + 3]), make_float2(b.z, b.w));
+                            v[c] = p.x;
+                            v[c + 1] = p.y;
+                            v[c + 2] = q.x;
+                            v[c + 3] = q.y;
+                        }
+                        /* the row's residual makes room for its z */
+                        if (a.res) {
+                            const uint4 u = *piece(lane, 2 * cc), w4 = *piece(lane, 2 * cc + 1);
+                            res[0] = u.x; res[1] = u.y; res[2] = u.z; res[3] = u.w;
+                            res[4] = w4.x; res[5] = w4.y; res[6] = w4.z; res[7] = w4.w;
+                        }
+                        if (a.z) {
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                *piece(lane, 2 * cc + c) = make_uint4(
+                                    pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
+                                    pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        float2 u = make_float2(v[2 * c], v[2 * c + 1]);
+                        if (!TRANS) {
+                            u = act2<ACT>(u);
+                            if (a.res) u = add2(u, unpack2<T>(res[c]));
+                        }
+                        y[8 * cc + c] = pack2<T>(u.x, u.y);
+                    }
                 }
+                if (!TRANS && a.z) {
+                    if (again)
+                        sum_again<T, TRANS, DIA_ACT_NONE>(a, K, r.e, row0 + lane, i0 + fw, again,
+                                                          piece(lane, 0), (lane >> 1) & 3, false);
+                    copy_out(a.z, a.ldz, row0, alz);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *piece(lane, c) = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+                if (again)
+                    sum_again<T, TRANS, ACT>(a, K, r.e, row0 + lane, i0 + fw, again,
+                                             piece(lane, 0), (lane >> 1) & 3, true);
+                copy_out(a.out, a.ldo, row0, al);
             }
         }
     }
@@ -591,6 +770,8 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     __shared__ __align__(8) unsigned long long xfull[kGStages], xempty[kGStages], done;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
+    __shared__ Box s_box[kGBoxes];
+    __shared__ int2 s_offs[kOffs];
     volatile int* abort_flag = &s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long b = blockIdx.x;
@@ -605,6 +786,8 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     const int nst = i0 < a.n_rows ? (rg.r1 - rg.r0 + kGRows - 1) / kGRows : 0;
     unsigned char* ones = smem + kGStages * kGStageBytes;
 
+    for (int k = tid; k < min(a.K, kOffs); k += kGWarps * 32) s_offs[k] = a.dir.offs[k];
+    if (tid < nb) s_box[tid] = a.dir.boxes[b0 + tid];
     if (tid == 0) {
         s_abort = 0;
         for (int s = 0; s < kGStages; ++s) {
@@ -636,7 +819,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
             int g = 0;
             for (; g < nst; ++g) {
                 const int s = g % kGStages, r = rg.r0 + g * kGRows;
-                ok = mm_wait(xempty[s], ((g / kGStages) & 1) ^ 1, abort_flag);
+                ok = mm_wait(smem_u32(&xempty[s]), ((g / kGStages) & 1) ^ 1, abort_flag);
                 if (!ok) break;
                 const uint32_t st = smem_u32(smem + s * kGStageBytes), bar = smem_u32(&xfull[s]);
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
@@ -644,10 +827,10 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                 tma_box(st, &tmD, i0, r, bar);
                 tma_box(st + kGBoxBytes, &tmD, i0 + 64, r, bar);
                 for (int c = 0; c < nb; ++c)
-                    tma_box(st + (2 + c) * kGBoxBytes, &tmX, i0 + a.dir.boxes[b0 + c].col, r, bar);
+                    tma_box(st + (2 + c) * kGBoxBytes, &tmX, i0 + s_box[c].col, r, bar);
             }
             for (int i = max(0, g - kGStages); i < g; ++i)
-                mm_drain(xfull[i % kGStages], (i / kGStages) & 1);
+                mm_drain(smem_u32(&xfull[i % kGStages]), (i / kGStages) & 1);
         }
     } else if (warp == 1) {
         const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -657,7 +840,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         const uint32_t ido = id0 | ((uint32_t)(kBoxCols >> 3) << 17);
         for (int g = 0; g < nst; ++g) {
             const int s = g % kGStages, left = rg.r1 - rg.r0 - g * kGRows;
-            ok = mm_wait(xfull[s], (g / kGStages) & 1, abort_flag);
+            ok = mm_wait(smem_u32(&xfull[s]), (g / kGStages) & 1, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             unsigned char* st = smem + s * kGStageBytes;
@@ -687,13 +870,13 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                         mma_f16(tmem + 256, mn_desc(sa + 2048u * kk), mn_desc(so), ido,
                                 g > 0 || kk > 0);
                 }
-                mm_commit(xempty[s]);
+                mm_commit(smem_u32(&xempty[s]));
             }
             __syncwarp();
         }
         if (lane == 0) {
-            mm_commit(done);
-            mm_drain(done, 0);
+            mm_commit(smem_u32(&done));
+            mm_drain(smem_u32(&done), 0);
         }
     }
     /* the results: every MMA has completed (the stages are free) */
@@ -734,26 +917,35 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
             ((T*)a.dbias)[(long long)rg.e * a.n_rows + i0 + tid] = from_f<T>(0.0f);
     }
     if (!a.dvals) return;
-    for (int c = 0; c < nb; ++c) {
-        const Box bx = a.dir.boxes[b0 + c];
-        for (int k = bx.k0 + warp; k < bx.k1; k += kGWarps) {
-            const int2 ok2 = a.dir.offs[k];
+    /* a diagonal's 128 entries: consecutive features, consecutive columns of
+     * one or two boxes; what lies in other CTAs' boxes is theirs */
+    const int k_lo = nb > 0 ? s_box[0].k0 : 0, k_hi = nb > 0 ? s_box[nb - 1].k1 : 0;
+    const float* tf = tile + lane * kGPitch;
+#pragma unroll 2
+    for (int k = k_lo + warp; k < k_hi; k += kGWarps) {
+        const int2 o = a.K <= kOffs ? s_offs[k] : a.dir.offs[k];
+        const long long at = rg.nparts > 1
+            ? ((long long)(rg.slot + rg.part) * (a.K + 1) + o.y) * a.stride + i0
+            : rg.e * a.estride + o.y * a.stride + i0;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int f = 32 * s + lane, i = i0 + f, p = ok2.x + f - bx.col;
-                if ((unsigned)p >= (unsigned)kBoxCols || i >= a.stride) continue;
-                const int j = i + ok2.x;
-                float v = 0.0f;
-                /* an entry outside the matrix, or in the padding, has no gradient */
-                if (nst > 0 && i < a.n_rows && (unsigned)j < (unsigned)a.n_cols) {
-                    v = tile[f * kGPitch + c * kBoxCols + p];
-                    if (!isfinite(v)) v = gradient_terms<T>(a, rg.r0, rg.r1, i, j);
-                }
-                if (rg.nparts > 1)
-                    a.part[((long long)(rg.slot + rg.part) * (a.K + 1) + ok2.y) * a.stride + i] = v;
-                else
-                    ((T*)a.dvals)[rg.e * a.estride + ok2.y * a.stride + i] = from_f<T>(v);
+        for (int s = 0; s < 4; ++s) {
+            const int f = 32 * s + lane, i = i0 + f, p = o.x + f;
+            int col = -1;
+            for (int c = 0; c < nb; ++c)
+                if ((unsigned)(p - s_box[c].col) < (unsigned)kBoxCols)
+                    col = c * kBoxCols + p - s_box[c].col;
+            if (col < 0 || i >= a.stride) continue;
+            const int j = i + o.x;
+            float v = 0.0f;
+            /* an entry outside the matrix, or in the padding, has no gradient */
+            if (nst > 0 && i < a.n_rows && (unsigned)j < (unsigned)a.n_cols) {
+                v = tf[32 * s * kGPitch + col];
+                if (!isfinite(v)) v = gradient_terms<T>(a, rg.r0, rg.r1, i, j);
             }
+            if (rg.nparts > 1)
+                a.part[at + f] = v;
+            else
+                ((T*)a.dvals)[at + f] = from_f<T>(v);
         }
     }
 }
@@ -782,6 +974,30 @@ static bool block_map(CUtensorMap* map, const void* base, int dtype, int width, 
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+/* kernel launch that may begin while the launch before it ends; the kernel
+ * waits for it where it reads its results */
+template <typename... P, typename... A>
+static cudaError_t launch_dependent(void (*kernel)(P...), int grid, int block, int smem,
+                                    cudaStream_t stream, A... args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+long long spmm_tc_pack_bytes(int n_out, int nboxes, int E)
+{
+    return (long long)E * ((n_out + kTN - 1) / kTN) * nboxes * kBoxBytes;
+}
+
 template <typename T, bool TRANS, int ACT>
 static int launch_tc(const CUtensorMap& map, const ProdArgs& a, int K, cudaStream_t stream)
 {
@@ -790,8 +1006,8 @@ static int launch_tc(const CUtensorMap& map, const ProdArgs& a, int K, cudaStrea
     const int grid = (int)std::min<long long>(items, num_sms());
     DIA_TRY_CUDA(cudaFuncSetAttribute(spmm_tc_kernel<T, TRANS, ACT>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem));
-    spmm_tc_kernel<T, TRANS, ACT><<<grid, kTcWarps * 32, kTcSmem, stream>>>(map, a, K);
-    DIA_TRY_CUDA(cudaGetLastError());
+    DIA_TRY_CUDA(launch_dependent(spmm_tc_kernel<T, TRANS, ACT>, grid, kTcWarps * 32, kTcSmem,
+                                  stream, map, a, K));
     return DIA_OK;
 }
 
@@ -813,6 +1029,13 @@ int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream)
     CUtensorMap map;
     if (!block_map(&map, a.in, dtype, a.n_in, a.M, a.ldi, kTM))
         return fail(DIA_ERR_CUDA, "dia_spmm: cuTensorMapEncodeTiled failed");
+    const long long boxes = spmm_tc_pack_bytes(a.n_out, a.dir.nboxes, a.E) / kBoxBytes;
+    if (boxes > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: operator too large");
+    const auto pack = a.trans ? spmm_pack_kernel<true> : spmm_pack_kernel<false>;
+    DIA_TRY_CUDA(cudaFuncSetAttribute(pack, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kPackSmem));
+    pack<<<(unsigned)boxes, 256, kPackSmem, stream>>>(a);
+    DIA_TRY_CUDA(cudaGetLastError());
     return dtype == DIA_F16 ? launch_tc_type<__half>(map, a, a.K, stream)
                             : launch_tc_type<__nv_bfloat16>(map, a, a.K, stream);
 }

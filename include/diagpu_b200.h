@@ -205,11 +205,15 @@ int dia_spmm_plan_destroy(DiaSpmmPlan* plan);
  * does not decrease and lies in [0, M], experts may have no rows.  Rows
  * before seg[0] and from seg[num_experts] on are left as they were.  y and z
  * must not overlap inputs, except that y may be res itself (same address and
- * stride).  Allocates nothing and does not synchronise. */
+ * stride).  Allocates nothing and does not synchronise.  work:
+ * dia_spmm_workspace bytes (0 where the CUDA cores do the work), 256-byte
+ * aligned, not shared by calls that may run at the same time. */
+int64_t dia_spmm_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts);
 int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
              const int64_t* d_seg, const void* d_x, int64_t ldx, const void* d_vals,
              int64_t stride, const void* d_bias, int act, const void* d_res, int64_t ldr,
-             void* d_z, int64_t ldz, void* d_y, int64_t ldy, cudaStream_t stream);
+             void* d_z, int64_t ldz, void* d_y, int64_t ldy, void* d_work,
+             int64_t work_bytes, cudaStream_t stream);
 
 /* Gradients of dia_spmm for dy = the gradient of y (that of the residual is
  * dy itself).  With dz = dy act'(z), rounded to the block's type:

@@ -90,7 +90,7 @@ def test_c_abi_before_cuda():
 
     def fwd(dtype=0, M=4, E=1, seg=None, act=0):
         return L.dia_spmm(None, dtype, M, E, seg, None, 8, None, 32, None, act, None, 8, None, 8,
-                          None, 8, None)
+                          None, 8, None, 0, None)
 
     def bwd(dtype=0, M=4, E=1, seg=None, act=0):
         return L.dia_spmm_backward(None, dtype, M, E, seg, None, 8, None, 32, None, 8, act, None,
@@ -103,5 +103,6 @@ def test_c_abi_before_cuda():
                           (dict(E=2), "seg"), (dict(), "null plan")):
             assert f(**bad) == dg.DIA_ERR_INVALID
             assert word in L.dia_last_error().decode(), bad
+    assert L.dia_spmm_workspace(None, 0, 4, 1) == -1
     assert L.dia_spmm_backward_workspace(None, 0, 4, 1, 32, 0) == -1
     assert L.dia_test_spmm_form(3) == dg.DIA_ERR_INVALID
