@@ -244,13 +244,14 @@ spmm_grad_kernel(GradArgs a, int ftiles)
     }
 }
 
-/* Sums the parts of experts that have several, in the parts' order. */
+/* Sums the parts of experts that have several, in the parts' order; four
+ * columns a thread. */
 template <typename T>
-__global__ void __launch_bounds__(256) spmm_join_kernel(GradArgs a, int cblocks)
+__global__ void __launch_bounds__(128) spmm_join_kernel(GradArgs a, int cblocks)
 {
     const int k = (int)(blockIdx.x / cblocks) % (a.K + 1);
     const int e = (int)(blockIdx.x / cblocks / (a.K + 1));
-    const int col = (int)(blockIdx.x % cblocks) * 256 + threadIdx.x;
+    const int col = ((int)(blockIdx.x % cblocks) * 128 + threadIdx.x) * 4;
     int nparts, slot = 0;
     if (a.seg) {
         int mine = 0;
@@ -270,57 +271,94 @@ __global__ void __launch_bounds__(256) spmm_join_kernel(GradArgs a, int cblocks)
     } else {
         nparts = (a.M + a.per - 1) / a.per;
     }
+    dependency_wait();
     if (nparts <= 1 || col >= a.stride || slot + nparts > a.slots) return;
-    if (k == a.K ? (!a.dbias || col >= a.n_rows) : !a.dvals) return;
+    if (k == a.K ? !a.dbias : !a.dvals) return;
     const float* p = a.part + ((long long)slot * (a.K + 1) + k) * a.stride + col;
     const long long step = (long long)(a.K + 1) * a.stride;
-    float v = 0.0f;
-    for (int s = 0; s < nparts; ++s) v += p[s * step];
-    if (k == a.K)
-        ((T*)a.dbias)[(long long)e * a.n_rows + col] = from_f<T>(v);
-    else
-        ((T*)a.dvals)[e * a.estride + (long long)k * a.stride + col] = from_f<T>(v);
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int s = 0; s < nparts; ++s) {
+        const float4 u = *(const float4*)(p + s * step);
+        v.x += u.x;
+        v.y += u.y;
+        v.z += u.z;
+        v.w += u.w;
+    }
+    const float o[4] = {v.x, v.y, v.z, v.w};
+    T* dst = k == a.K ? (T*)a.dbias + (long long)e * a.n_rows + col
+                      : (T*)a.dvals + e * a.estride + (long long)k * a.stride + col;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (k < a.K || col + c < a.n_rows) dst[c] = from_f<T>(o[c]);
+}
+
+/* eight elements, p aligned to 16 bytes */
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8])
+{
+    if (sizeof(T) == 4) {
+        *(float4*)v = __ldg((const float4*)p);
+        *(float4*)(v + 4) = __ldg((const float4*)p + 1);
+    } else {
+        __align__(16) T h[8];
+        *(uint4*)h = __ldg((const uint4*)p);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = to_f(h[c]);
+    }
 }
 
 /* dz = dy * act'(z), rounded to the block's type: both gradients read it as
  * a matrix operand of that type, and one rounding of half a step is no more
- * than the ones dy and z already carry.  Eight elements a thread. */
+ * than the ones dy and z already carry.  Eight elements a thread at a time,
+ * two of them in flight. */
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256)
 spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z, long long ldz,
                T* __restrict__ dz, long long lddz, int M, int n)
 {
+    dependents_begin();
     const int per = (n + 7) / 8;
-    const long long total = (long long)per * M;
-    for (long long p = blockIdx.x * 256ll + threadIdx.x; p < total; p += gridDim.x * 256ll) {
-        const long long t = p / per;
-        const int i = (int)(p - t * per) * 8;
-        const T* g = dy + t * lddy + i;
-        const T* y = z + t * ldz + i;
-        T* o = dz + t * lddz + i;
-        if (VEC && i + 8 <= n) {
-            float a[8], b[8];
-            *(float4*)a = load4<T>(g);
-            *(float4*)(a + 4) = load4<T>(g + 4);
-            *(float4*)b = load4<T>(y);
-            *(float4*)(b + 4) = load4<T>(y + 4);
+    const long long total = (long long)per * M, step = gridDim.x * 256ll;
+    for (long long p0 = blockIdx.x * 256ll + threadIdx.x; p0 < total; p0 += 2 * step) {
+        float a[2][8], b[2][8];
+        long long at[2];
+        bool wide[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const long long p = p0 + h * step;
+            const long long t = p < total ? p / per : 0;
+            const int i = (int)(p - t * per) * 8;
+            at[h] = p < total ? t * lddz + i : -1;
+            wide[h] = VEC && i + 8 <= n;
+            if (at[h] < 0) continue;
+            if (wide[h]) {
+                load8<T>(dy + t * lddy + i, a[h]);
+                load8<T>(z + t * ldz + i, b[h]);
+            } else {
+                for (int c = 0; c < 8 && i + c < n; ++c)
+                    dz[at[h] + c] = from_f<T>(to_f(dy[t * lddy + i + c]) *
+                                              dact_of<ACT>(to_f(z[t * ldz + i + c])));
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (at[h] < 0 || !wide[h]) continue;
             __align__(16) T r[8];
 #pragma unroll
             for (int c = 0; c < 8; c += 2) {
                 const float2 d = sizeof(T) == 2
-                                     ? dact2<ACT>(make_float2(b[c], b[c + 1]))
-                                     : make_float2(dact_of<ACT>(b[c]), dact_of<ACT>(b[c + 1]));
-                r[c] = from_f<T>(a[c] * d.x);
-                r[c + 1] = from_f<T>(a[c + 1] * d.y);
+                                     ? dact2<ACT>(make_float2(b[h][c], b[h][c + 1]))
+                                     : make_float2(dact_of<ACT>(b[h][c]), dact_of<ACT>(b[h][c + 1]));
+                r[c] = from_f<T>(a[h][c] * d.x);
+                r[c + 1] = from_f<T>(a[h][c + 1] * d.y);
             }
 #pragma unroll
             for (int c = 0; c < (int)(8 * sizeof(T)); c += 16)
-                *(uint4*)((char*)o + c) = *(const uint4*)((const char*)r + c);
-        } else {
-            for (int c = 0; c < 8 && i + c < n; ++c)
-                o[c] = from_f<T>(to_f(g[c]) * dact_of<ACT>(to_f(y[c])));
+                *(uint4*)((char*)(dz + at[h]) + c) = *(const uint4*)((const char*)r + c);
         }
     }
+    dependency_wait();
 }
 
 /* ---------------------------------------------------------------- host */
@@ -370,12 +408,18 @@ static int launch_product_tt(const ProdArgs& a, int dtype, cudaStream_t stream)
     return DIA_OK;
 }
 
+/* the tensor-core form it is (its operator has to be packed first) */
+static bool product_on_tc(const ProdArgs& a, int dtype)
+{
+    return a.M > 0 && a.n_out > 0 && a.n_in > 0 && tensor_form(dtype, a.M, a.E, a.dir) &&
+           spmm_tc_block(a.in, a.ldi);
+}
+
 template <typename T>
 static int launch_product(const ProdArgs& a, int dtype, cudaStream_t stream)
 {
     if (a.M == 0 || a.n_out == 0) return DIA_OK;
-    if (tensor_form(dtype, a.M, a.E, a.dir) && a.n_in > 0 && spmm_tc_block(a.in, a.ldi))
-        return spmm_tc_product(a, dtype, stream);
+    if (product_on_tc(a, dtype)) return spmm_tc_product(a, dtype, stream);
     const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
     if (a.trans)
         return per >= 4 ? launch_product_tt<T, true, 4>(a, dtype, stream)
@@ -384,40 +428,39 @@ static int launch_product(const ProdArgs& a, int dtype, cudaStream_t stream)
                     : launch_product_tt<T, false, 1>(a, dtype, stream);
 }
 
+static bool vec16(const void* p, long long ld, int dtype)
+{
+    return (uintptr_t)p % 16 == 0 && ld * (long long)elem_size(dtype) % 16 == 0;
+}
+
 template <typename T, int ACT>
-static void launch_dz_act(const void* dy, long long lddy, const void* z, long long ldz, void* dz,
-                          long long lddz, int M, int n, cudaStream_t stream)
+static cudaError_t launch_dz_act(const void* dy, long long lddy, const void* z, long long ldz,
+                                 void* dz, long long lddz, int M, int n, bool dependent,
+                                 cudaStream_t stream)
 {
     const long long work = (long long)M * ((n + 7) / 8);
-    const int grid = (int)std::min<long long>((work + 255) / 256, 8ll * num_sms());
+    const int grid = (int)std::min<long long>((work + 511) / 512, 8ll * num_sms());
     const int dtype = sizeof(T) == 4 ? DIA_F32 : DIA_F16;
-    if (vec4(dy, lddy, dtype) && vec4(z, ldz, dtype))
-        spmm_dz_kernel<T, ACT, true><<<grid, 256, 0, stream>>>(
-            (const T*)dy, lddy, (const T*)z, ldz, (T*)dz, lddz, M, n);
-    else
-        spmm_dz_kernel<T, ACT, false><<<grid, 256, 0, stream>>>(
-            (const T*)dy, lddy, (const T*)z, ldz, (T*)dz, lddz, M, n);
+    const auto kernel = vec16(dy, lddy, dtype) && vec16(z, ldz, dtype)
+                            ? spmm_dz_kernel<T, ACT, true>
+                            : spmm_dz_kernel<T, ACT, false>;
+    if (dependent)
+        return launch_dependent(kernel, grid, 256, 0, stream, (const T*)dy, lddy, (const T*)z, ldz,
+                                (T*)dz, lddz, M, n);
+    kernel<<<grid, 256, 0, stream>>>((const T*)dy, lddy, (const T*)z, ldz, (T*)dz, lddz, M, n);
+    return cudaGetLastError();
 }
 
 template <typename T>
 static int launch_dz(int act, const void* dy, long long lddy, const void* z, long long ldz,
-                     void* dz, long long lddz, int M, int n, cudaStream_t stream)
+                     void* dz, long long lddz, int M, int n, bool dependent, cudaStream_t stream)
 {
     if (M == 0 || n == 0) return DIA_OK;
-    switch (act) {
-        case DIA_ACT_RELU:
-            launch_dz_act<T, DIA_ACT_RELU>(dy, lddy, z, ldz, dz, lddz, M, n, stream);
-            break;
-        case DIA_ACT_SILU:
-            launch_dz_act<T, DIA_ACT_SILU>(dy, lddy, z, ldz, dz, lddz, M, n, stream);
-            break;
-        case DIA_ACT_GELU:
-            launch_dz_act<T, DIA_ACT_GELU>(dy, lddy, z, ldz, dz, lddz, M, n, stream);
-            break;
-        default:
-            launch_dz_act<T, DIA_ACT_GELU_TANH>(dy, lddy, z, ldz, dz, lddz, M, n, stream);
-    }
-    DIA_TRY_CUDA(cudaGetLastError());
+    const auto launch = act == DIA_ACT_RELU   ? launch_dz_act<T, DIA_ACT_RELU>
+                        : act == DIA_ACT_SILU ? launch_dz_act<T, DIA_ACT_SILU>
+                        : act == DIA_ACT_GELU ? launch_dz_act<T, DIA_ACT_GELU>
+                                              : launch_dz_act<T, DIA_ACT_GELU_TANH>;
+    DIA_TRY_CUDA(launch(dy, lddy, z, ldz, dz, lddz, M, n, dependent, stream));
     return DIA_OK;
 }
 
@@ -443,36 +486,36 @@ static int grad_part_rows(const DiaSpmmPlan* p, int dtype, long long M, int E, l
 /* parts of experts that have several: at most two a `per` rows */
 static long long grad_slots(long long M, long long per) { return M > per ? 2 * (M / per) + 1 : 0; }
 
+static bool grad_on_tc(const GradArgs& a, int dtype)
+{
+    return tensor_form(dtype, a.M, a.E, a.dir) && a.M > 0 && a.n_cols > 0 && a.n_rows > 0 &&
+           a.dvals && spmm_tc_block(a.dz, a.lddz) && spmm_tc_block(a.x, a.ldx);
+}
+
 template <typename T>
 static int launch_grad(const GradArgs& a, int dtype, cudaStream_t stream)
 {
-    const int cblocks = (int)((a.stride + 255) / 256);
-    const long long jgrid = (long long)a.E * (a.K + 1) * cblocks;
-    if (jgrid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
-    if (tensor_form(dtype, a.M, a.E, a.dir) && a.M > 0 && a.n_cols > 0 && a.n_rows > 0 &&
-        a.dvals && spmm_tc_block(a.dz, a.lddz) && spmm_tc_block(a.x, a.ldx)) {
-        const int r = spmm_tc_gradient(a, dtype, stream);
-        if (r != DIA_OK) return r;
-        if (a.M > a.per) {
-            spmm_join_kernel<T><<<(unsigned)jgrid, 256, 0, stream>>>(a, cblocks);
-            DIA_TRY_CUDA(cudaGetLastError());
-        }
-        return DIA_OK;
-    }
+    if (grad_on_tc(a, dtype)) return spmm_tc_gradient(a, dtype, stream);
     const int ftiles = (int)((a.stride + kMmFeat - 1) / kMmFeat);
     const long long parts = a.seg ? a.M / a.per + a.E : std::max(1, (a.M + a.per - 1) / a.per);
     const long long grid = parts * ftiles * std::max(a.dir.nquads, 1);
-    if (grid > INT_MAX)
-        return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
+    if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
     if (vec4(a.dz, a.lddz, dtype) && vec4(a.x, a.ldx, dtype))
         spmm_grad_kernel<T, true><<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ftiles);
     else
         spmm_grad_kernel<T, false><<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ftiles);
     DIA_TRY_CUDA(cudaGetLastError());
-    if (a.M > a.per) {
-        spmm_join_kernel<T><<<(unsigned)jgrid, 256, 0, stream>>>(a, cblocks);
-        DIA_TRY_CUDA(cudaGetLastError());
-    }
+    return DIA_OK;
+}
+
+template <typename T>
+static int launch_join(const GradArgs& a, cudaStream_t stream)
+{
+    if (a.M <= a.per) return DIA_OK;   /* no expert has several parts */
+    const int cblocks = (int)((a.stride + 511) / 512);
+    const long long grid = (long long)a.E * (a.K + 1) * cblocks;
+    if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
+    DIA_TRY_CUDA(launch_dependent(spmm_join_kernel<T>, (int)grid, 128, 0, stream, a, cblocks));
     return DIA_OK;
 }
 
@@ -732,6 +775,10 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
     a.act = act;
     a.dir = plan->fwd;
     a.trans = false;
+    if (product_on_tc(a, dtype)) {
+        rc = spmm_tc_pack(a, stream);
+        if (rc != DIA_OK) return rc;
+    }
     return by_type(dtype, [&](auto* t) {
         return launch_product<std::remove_pointer_t<decltype(t)>>(a, dtype, stream);
     });
@@ -777,65 +824,63 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
 
     return by_type(dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        const void* dz = d_dy;
-        long long lddz = lddy;
-        if (act != DIA_ACT_NONE) {
-            dz = d_work;
-            lddz = g.lddz;
-            const int r = launch_dz<T>(act, d_dy, lddy, d_z, ldz, d_work, lddz, (int)M,
-                                       plan->n_rows, stream);
-            if (r != DIA_OK) return r;
+        const bool made = act != DIA_ACT_NONE;
+        ProdArgs p{};
+        p.in = made ? d_work : d_dy;
+        p.vals = d_vals;
+        p.out = d_dx;
+        p.pack = (char*)d_work + g.dz_bytes + g.part_bytes;
+        p.seg = (const long long*)d_seg;
+        p.ldi = made ? g.lddz : lddy;
+        p.ldo = lddx;
+        p.stride = stride;
+        p.estride = stride * plan->K;
+        p.M = (int)M;
+        p.E = num_experts;
+        p.n_in = plan->n_rows;
+        p.n_out = plan->n_cols;
+        p.K = plan->K;
+        p.dir = plan->trn;
+        p.trans = true;
+        GradArgs a{};
+        a.dz = p.in;
+        a.x = d_x;
+        a.dvals = plan->K > 0 ? d_dvals : nullptr;
+        a.dbias = d_dbias;
+        a.part = (float*)((char*)d_work + g.dz_bytes);
+        a.seg = p.seg;
+        a.lddz = p.ldi;
+        a.ldx = ldx;
+        a.stride = stride;
+        a.estride = p.estride;
+        a.M = p.M;
+        a.E = num_experts;
+        a.n_rows = plan->n_rows;
+        a.n_cols = plan->n_cols;
+        a.K = plan->K;
+        a.per = g.per;
+        a.slots = grad_slots(M, g.per);
+        a.dir = plan->fwd;
+        if (!a.dvals) {   /* dbias alone: x is not looked at */
+            a.dir.nquads = 0;
+            a.n_cols = 0;
         }
-        if (d_dvals || d_dbias) {
-            GradArgs a{};
-            a.dz = dz;
-            a.x = d_x;
-            a.dvals = plan->K > 0 ? d_dvals : nullptr;
-            a.dbias = d_dbias;
-            a.part = (float*)((char*)d_work + g.dz_bytes);
-            a.seg = (const long long*)d_seg;
-            a.lddz = lddz;
-            a.ldx = ldx;
-            a.stride = stride;
-            a.estride = stride * plan->K;
-            a.M = (int)M;
-            a.E = num_experts;
-            a.n_rows = plan->n_rows;
-            a.n_cols = plan->n_cols;
-            a.K = plan->K;
-            a.per = g.per;
-            a.slots = grad_slots(M, g.per);
-            a.dir = plan->fwd;
-            if (!a.dvals) {   /* dbias alone: x is not looked at */
-                a.dir.nquads = 0;
-                a.n_cols = 0;
-            }
-            if (stride > 0) {
-                const int r = launch_grad<T>(a, dtype, stream);
-                if (r != DIA_OK) return r;
-            }
+        const bool grad = (a.dvals || a.dbias) && stride > 0;
+        /* launches overlap where each is of the tensor-core form: operator
+         * packed, dz, gradient of the diagonals, dx, parts joined */
+        const bool tc = d_dx && product_on_tc(p, dtype);
+        int r = DIA_OK;
+        if (tc) r = spmm_tc_pack(p, stream);
+        if (r == DIA_OK && made)
+            r = launch_dz<T>(act, d_dy, lddy, d_z, ldz, d_work, p.ldi, p.M, p.n_in, tc, stream);
+        if (r == DIA_OK && grad) {
+            const bool overlap = tc && grad_on_tc(a, dtype);
+            r = launch_grad<T>(a, dtype, stream);
+            p.early = overlap;
         }
-        if (d_dx) {
-            ProdArgs a{};
-            a.in = dz;
-            a.vals = d_vals;
-            a.out = d_dx;
-            a.pack = (char*)d_work + g.dz_bytes + g.part_bytes;
-            a.seg = (const long long*)d_seg;
-            a.ldi = lddz;
-            a.ldo = lddx;
-            a.stride = stride;
-            a.estride = stride * plan->K;
-            a.M = (int)M;
-            a.E = num_experts;
-            a.n_in = plan->n_rows;
-            a.n_out = plan->n_cols;
-            a.K = plan->K;
-            a.dir = plan->trn;
-            a.trans = true;
-            return launch_product<T>(a, dtype, stream);
-        }
-        return DIA_OK;
+        if (r == DIA_OK && d_dx) r = launch_product<T>(p, dtype, stream);
+        if (r == DIA_OK && grad) r = launch_join<T>(a, stream);
+        return r;
     });
 }
 

@@ -372,6 +372,7 @@ struct ProdArgs {
     int act;
     SpmmDir dir;
     bool trans;
+    bool early;           /* tensor-core form: inputs are complete when the kernel may begin */
 };
 
 /* dvals[k, i] = sum_t dz[t, i] x[t, i + off_k], dbias[i] = sum_t dz[t, i] */
@@ -389,10 +390,45 @@ struct GradArgs {
     SpmmDir dir;          /* forward */
 };
 
+/* ------------------------------------------------------- dependent launches
+ *
+ * The launches of one call overlap (programmatic dependent launch): a kernel
+ * may begin once every CTA of the one before has said dependents_begin() or
+ * ended, and dependency_wait() returns when that one has completed.  The
+ * first launch of a call is an ordinary one, and every later one waits before
+ * it ends, so that its own completion means that of all before. */
+__device__ __forceinline__ void dependency_wait()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+__device__ __forceinline__ void dependents_begin()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+static cudaError_t launch_dependent(void (*kernel)(P...), int grid, int block, int smem,
+                                    cudaStream_t stream, A... args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 /* Tensor-core forms for 16-bit blocks (spmm_tc.cu).  spmm_tc_block: address
  * and row stride are ones TMA takes. */
 bool spmm_tc_block(const void* p, long long ld);
 long long spmm_tc_pack_bytes(int n_out, int nboxes, int E);
+int spmm_tc_pack(const ProdArgs& a, cudaStream_t stream);   /* an ordinary launch */
 int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream);
 int spmm_tc_gradient(const GradArgs& a, int dtype, cudaStream_t stream);
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear);

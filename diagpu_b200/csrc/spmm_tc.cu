@@ -211,12 +211,6 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u)
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
-/* waits for the launches before this one (programmatic dependent launch) */
-__device__ __forceinline__ void dependency_wait()
-{
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint32_t bar)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
@@ -242,7 +236,7 @@ __global__ void __launch_bounds__(256) spmm_pack_kernel(const __grid_constant__ 
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ int16_t s_row[kPackRows + 1];
     __shared__ int2 s_off[kPackRows + 1];
-    asm volatile("griddepcontrol.launch_dependents;");
+    dependents_begin();
     const int tid = threadIdx.x;
     unsigned char* box = smem_raw;
     uint16_t* slab = (uint16_t*)(smem_raw + kBoxBytes);
@@ -421,6 +415,8 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     const uint32_t afull = smem_u32(bars.afull), aempty = smem_u32(bars.aempty);
     if (warp == 0) {
         /* ---------------- TMA: the block's boxes */
+        /* dx: the block is dz, which the launch before may still be making */
+        if (TRANS && !a.early) dependency_wait();
         Ring<kXStages> x;
         int issued = 0;
         bool ok = true;
@@ -521,7 +517,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         mm_drain(smem_u32(&bars.drain), 0);
     } else if (warp == 2) {
         /* ---------------- the operator's boxes, as spmm_pack_kernel left them */
-        dependency_wait();
+        if (!a.early) dependency_wait();
         Ring<kWSlots> q;
         int issued = 0;
         bool ok = true;
@@ -548,6 +544,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         for (int n = min(issued, kWSlots); n < kWSlots; ++n) q.next();
         for (int n = 0; n < min(issued, kWSlots); ++n, q.next())
             mm_drain(q.bar(wfull), q.round ^ 1);
+        if (a.early) dependency_wait();
     } else if (warp >= kEpiWarp0t) {
         /* ---------------- epilogue: a warp's 32 rows of 32 features.  The
          * accumulators come a row a lane; memory is read and written eight
@@ -735,7 +732,7 @@ constexpr int kGStageBytes = (2 + kGBoxes) * kGBoxBytes;
 constexpr int kGStages = 4;
 constexpr int kGOnesBytes = 16 * 128;
 constexpr int kGSmem = kGStages * kGStageBytes + kGOnesBytes + 1024;
-constexpr int kGWarps = 10;                    /* TMA, MMA, eight for the results */
+constexpr int kGWarps = 18;                    /* TMA, MMA, sixteen for the results */
 constexpr int kGPitch = kGBoxes * kBoxCols + 1;
 
 /* MN-major operand with the 128-byte swizzle: groups of 64 elements kGBoxBytes
@@ -777,7 +774,10 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     const long long b = blockIdx.x;
     const int fb = (int)(b % nfb), ch = (int)(b / nfb % nch);
     const RowGroup rg = row_group(a.seg, a.E, a.M, a.per, b / nfb / nch, true);
-    if (rg.e < 0 || (rg.nparts > 1 && rg.slot + rg.part >= a.slots)) return;   /* whole CTA */
+    if (rg.e < 0 || (rg.nparts > 1 && rg.slot + rg.part >= a.slots)) {
+        dependency_wait();
+        return;   /* whole CTA */
+    }
     const int i0 = fb * 128;
     /* boxes in nch nearly equal shares */
     const int b0 = (int)((long long)a.dir.nboxes * ch / nch);
@@ -813,15 +813,23 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
     bool ok = true;
+    /* dz is the launch before this one's; the product that follows needs
+     * nothing of this kernel's and may begin */
+    dependency_wait();
+    dependents_begin();
 
+    const uint32_t st0 = smem_u32(smem), full0 = smem_u32(xfull), empty0 = smem_u32(xempty);
     if (warp == 0) {
-        if (lane == 0) {
-            int g = 0;
-            for (; g < nst; ++g) {
-                const int s = g % kGStages, r = rg.r0 + g * kGRows;
-                ok = mm_wait(smem_u32(&xempty[s]), ((g / kGStages) & 1) ^ 1, abort_flag);
-                if (!ok) break;
-                const uint32_t st = smem_u32(smem + s * kGStageBytes), bar = smem_u32(&xfull[s]);
+        const bool leader = elect_one();
+        Ring<kGStages> x;
+        int g = 0;
+        for (; g < nst; ++g, x.next()) {
+            ok = mm_wait(x.bar(empty0), x.round ^ 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (leader) {
+                const int r = rg.r0 + g * kGRows;
+                const uint32_t st = st0 + x.s * kGStageBytes, bar = x.bar(full0);
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
                              ::"r"(bar), "r"((2 + nb) * kGBoxBytes) : "memory");
                 tma_box(st, &tmD, i0, r, bar);
@@ -829,55 +837,54 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                 for (int c = 0; c < nb; ++c)
                     tma_box(st + (2 + c) * kGBoxBytes, &tmX, i0 + s_box[c].col, r, bar);
             }
-            for (int i = max(0, g - kGStages); i < g; ++i)
-                mm_drain(smem_u32(&xfull[i % kGStages]), (i / kGStages) & 1);
         }
+        for (int n = min(g, kGStages); n < kGStages; ++n) x.next();
+        for (int n = 0; n < min(g, kGStages); ++n, x.next())
+            mm_drain(x.bar(full0), x.round ^ 1);
     } else if (warp == 1) {
         const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
         const uint32_t id0 = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) |
                              ((uint32_t)(128 >> 4) << 24);
         const uint32_t idx = id0 | ((uint32_t)(nb * kBoxCols >> 3) << 17);
         const uint32_t ido = id0 | ((uint32_t)(kBoxCols >> 3) << 17);
-        for (int g = 0; g < nst; ++g) {
-            const int s = g % kGStages, left = rg.r1 - rg.r0 - g * kGRows;
-            ok = mm_wait(smem_u32(&xfull[s]), (g / kGStages) & 1, abort_flag);
+        const bool leader = elect_one();
+        const uint64_t desc0 = mn_desc(st0), odesc = mn_desc(smem_u32(ones));
+        Ring<kGStages> x;
+        for (int g = 0; g < nst; ++g, x.next()) {
+            const int left = rg.r1 - rg.r0 - g * kGRows;
+            ok = mm_wait(x.bar(full0), x.round, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            unsigned char* st = smem + s * kGStageBytes;
             if (left < kGRows) {
                 /* rows past the part: another expert's, or nobody's */
+                const uint32_t st = st0 + x.s * kGStageBytes;
                 const int per = (kGRows - left) * 8;
                 for (int o = lane; o < per * (2 + nb); o += 32)
-                    sts128(smem_u32(st) + o / per * kGBoxBytes + left * 128 + o % per * 16, 0);
+                    sts128(st + o / per * kGBoxBytes + left * 128 + o % per * 16, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
-            if (lane == 0) {
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t sa = smem_u32(st), so = smem_u32(ones);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (leader) {
+                const uint64_t ad = desc0 + x.s * (kGStageBytes >> 4);
+                const uint64_t bd = ad + (2 * kGBoxBytes >> 4);
+                if (nb > 0) {
 #pragma unroll
-                for (int kk = 0; kk < kGRows / 16; ++kk) {
-                    const uint64_t ad = mn_desc(sa + 2048u * kk);
-                    if (nb > 0)
-                        mma_f16(tmem, ad, mn_desc(sa + 2 * kGBoxBytes + 2048u * kk), idx,
-                                g > 0 || kk > 0);
+                    for (int kk = 0; kk < kGRows / 16; ++kk)
+                        mma_f16(tmem, ad + 128 * kk, bd + 128 * kk, idx, g > 0 || kk > 0);
                 }
                 /* a loop of its own: alternating the two accumulators' MMAs in
                  * one unrolled loop gave undefined sums in the second (nvcc 12.9) */
                 if (bias) {
 #pragma unroll
                     for (int kk = 0; kk < kGRows / 16; ++kk)
-                        mma_f16(tmem + 256, mn_desc(sa + 2048u * kk), mn_desc(so), ido,
-                                g > 0 || kk > 0);
+                        mma_f16(tmem + 256, ad + 128 * kk, odesc, ido, g > 0 || kk > 0);
                 }
-                mm_commit(smem_u32(&xempty[s]));
+                mm_commit(x.bar(empty0));
             }
-            __syncwarp();
         }
-        if (lane == 0) {
-            mm_commit(smem_u32(&done));
-            mm_drain(smem_u32(&done), 0);
-        }
+        if (leader) mm_commit(smem_u32(&done));
+        mm_drain(smem_u32(&done), 0);
     }
     /* the results: every MMA has completed (the stages are free) */
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -886,14 +893,14 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     float* tile = (float*)smem;
     if (ok && warp >= 2 && nst > 0) {
         const uint32_t tq = (uint32_t)(warp & 3);
-        const int half = (warp - 2) >> 2, f = 32 * (int)tq + lane;
-        for (int c0 = half * 16; c0 < nb * kBoxCols; c0 += 32) {
+        const int grp = (warp - 2) >> 2, f = 32 * (int)tq + lane;
+        for (int c0 = grp * 16; c0 < nb * kBoxCols; c0 += 64) {
             float v[16];
             tmem_ld16(tmem + ((tq * 32) << 16) + (uint32_t)c0, v);
 #pragma unroll
             for (int c = 0; c < 16; ++c) tile[f * kGPitch + c0 + c] = v[c];
         }
-        if (bias && half == 0) {
+        if (bias && grp == 0) {
             const float v = tmem_ld1(tmem + ((tq * 32) << 16) + 256u);
             const int i = i0 + f;
             if (i < a.n_rows) {
@@ -918,34 +925,34 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     }
     if (!a.dvals) return;
     /* a diagonal's 128 entries: consecutive features, consecutive columns of
-     * one or two boxes; what lies in other CTAs' boxes is theirs */
+     * one box or more; what lies in other CTAs' boxes is theirs */
     const int k_lo = nb > 0 ? s_box[0].k0 : 0, k_hi = nb > 0 ? s_box[nb - 1].k1 : 0;
-    const float* tf = tile + lane * kGPitch;
-#pragma unroll 2
+    const int f_end = (int)min(128ll, a.stride - i0);
     for (int k = k_lo + warp; k < k_hi; k += kGWarps) {
         const int2 o = a.K <= kOffs ? s_offs[k] : a.dir.offs[k];
-        const long long at = rg.nparts > 1
+        const bool parts = rg.nparts > 1;
+        const long long at = parts
             ? ((long long)(rg.slot + rg.part) * (a.K + 1) + o.y) * a.stride + i0
             : rg.e * a.estride + o.y * a.stride + i0;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int f = 32 * s + lane, i = i0 + f, p = o.x + f;
-            int col = -1;
-            for (int c = 0; c < nb; ++c)
-                if ((unsigned)(p - s_box[c].col) < (unsigned)kBoxCols)
-                    col = c * kBoxCols + p - s_box[c].col;
-            if (col < 0 || i >= a.stride) continue;
-            const int j = i + o.x;
-            float v = 0.0f;
-            /* an entry outside the matrix, or in the padding, has no gradient */
-            if (nst > 0 && i < a.n_rows && (unsigned)j < (unsigned)a.n_cols) {
-                v = tf[32 * s * kGPitch + col];
-                if (!isfinite(v)) v = gradient_terms<T>(a, rg.r0, rg.r1, i, j);
+        /* features whose entry lies in the matrix; outside, and in the
+         * padding, there is no gradient */
+        const int in_lo = max(0, -(i0 + o.x));
+        const int in_hi = nst > 0 ? min(a.n_rows - i0, a.n_cols - i0 - o.x) : 0;
+        for (int c = 0; c < nb; ++c) {
+            const int rel = o.x - s_box[c].col;    /* column of feature 0 */
+            const int f1 = min(f_end, kBoxCols - rel);
+            const float* src = tile + c * kBoxCols + rel;
+            for (int f = max(0, -rel) + lane; f < f1; f += 32) {
+                float v = 0.0f;
+                if (f >= in_lo && f < in_hi) {
+                    v = src[f * (kGPitch + 1)];
+                    if (!isfinite(v)) v = gradient_terms<T>(a, rg.r0, rg.r1, i0 + f, i0 + f + o.x);
+                }
+                if (parts)
+                    a.part[at + f] = v;
+                else
+                    ((T*)a.dvals)[at + f] = from_f<T>(v);
             }
-            if (rg.nparts > 1)
-                a.part[at + f] = v;
-            else
-                ((T*)a.dvals)[at + f] = from_f<T>(v);
         }
     }
 }
@@ -972,25 +979,6 @@ static bool block_map(CUtensorMap* map, const void* base, int dtype, int width, 
               2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-/* kernel launch that may begin while the launch before it ends; the kernel
- * waits for it where it reads its results */
-template <typename... P, typename... A>
-static cudaError_t launch_dependent(void (*kernel)(P...), int grid, int block, int smem,
-                                    cudaStream_t stream, A... args)
-{
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3((unsigned)block);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 long long spmm_tc_pack_bytes(int n_out, int nboxes, int E)
@@ -1024,11 +1012,8 @@ static int launch_tc_type(const CUtensorMap& map, const ProdArgs& a, int K, cuda
     }
 }
 
-int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream)
+int spmm_tc_pack(const ProdArgs& a, cudaStream_t stream)
 {
-    CUtensorMap map;
-    if (!block_map(&map, a.in, dtype, a.n_in, a.M, a.ldi, kTM))
-        return fail(DIA_ERR_CUDA, "dia_spmm: cuTensorMapEncodeTiled failed");
     const long long boxes = spmm_tc_pack_bytes(a.n_out, a.dir.nboxes, a.E) / kBoxBytes;
     if (boxes > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: operator too large");
     const auto pack = a.trans ? spmm_pack_kernel<true> : spmm_pack_kernel<false>;
@@ -1036,6 +1021,14 @@ int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream)
                                       kPackSmem));
     pack<<<(unsigned)boxes, 256, kPackSmem, stream>>>(a);
     DIA_TRY_CUDA(cudaGetLastError());
+    return DIA_OK;
+}
+
+int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream)
+{
+    CUtensorMap map;
+    if (!block_map(&map, a.in, dtype, a.n_in, a.M, a.ldi, kTM))
+        return fail(DIA_ERR_CUDA, "dia_spmm: cuTensorMapEncodeTiled failed");
     return dtype == DIA_F16 ? launch_tc_type<__half>(map, a, a.K, stream)
                             : launch_tc_type<__nv_bfloat16>(map, a, a.K, stream);
 }
@@ -1051,8 +1044,8 @@ static int launch_grad_tc(const CUtensorMap& md, const CUtensorMap& mx, const Gr
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
     DIA_TRY_CUDA(cudaFuncSetAttribute(spmm_grad_tc_kernel<T>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kGSmem));
-    spmm_grad_tc_kernel<T><<<(unsigned)grid, kGWarps * 32, kGSmem, stream>>>(md, mx, a, nfb, nch);
-    DIA_TRY_CUDA(cudaGetLastError());
+    DIA_TRY_CUDA(launch_dependent(spmm_grad_tc_kernel<T>, (int)grid, kGWarps * 32, kGSmem, stream,
+                                  md, mx, a, nfb, nch));
     return DIA_OK;
 }
 
