@@ -469,10 +469,10 @@ static int launch_dz(int act, const void* dy, long long lddy, const void* z, lon
 static int grad_part_rows(const DiaSpmmPlan* p, int dtype, long long M, int E, long long stride)
 {
     if (tensor_form(dtype, M, E, p->fwd)) {
-        /* one CTA an SM */
+        /* one CTA an SM, of which every expert takes one a tile */
         const long long tiles = std::max<long long>(1, (stride + 127) / 128) *
                                 ((p->fwd.nboxes + 3) / 4);
-        const long long want = std::max<long long>(1, num_sms() / tiles);
+        const long long want = std::max<long long>(1, num_sms() / tiles - (E - 1));
         const long long per = std::max<long long>(256, (M + want - 1) / want);
         return (int)((per + 63) / 64 * 64);
     }

@@ -43,13 +43,13 @@ constexpr int kTN = 128;             /* features of a tile */
 constexpr int kBoxCols = 64;         /* one 128-byte swizzle row */
 constexpr int kBoxBytes = 128 * kBoxCols * 2;
 constexpr int kWSlots = 6;           /* operator boxes in shared memory */
-constexpr int kXStages = 5;          /* block boxes in flight */
+constexpr int kXStages = 4;          /* block boxes in flight */
 constexpr int kAccs = 4;             /* accumulators of 128 columns */
 constexpr int kEpiWarp0t = 4, kEpiWarpsT = 16, kTcWarps = kEpiWarp0t + kEpiWarpsT;
 constexpr int kOffs = 512;           /* offsets kept in shared memory */
 constexpr int kEpiThreads = kEpiWarpsT * 32;
 constexpr int kEpiBuf = 32 * 64;     /* a warp's 32 rows of 32 features */
-constexpr int kTcSmem = (kWSlots + kXStages) * kBoxBytes + kEpiWarpsT * kEpiBuf + 1024;
+constexpr int kTcSmem = (kWSlots + kXStages) * kBoxBytes + 2 * kEpiWarpsT * kEpiBuf + 1024;
 
 struct MmBars {
     unsigned long long xfull[kXStages], xempty[kXStages];
@@ -142,6 +142,11 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t v)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};"
+                 ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 __device__ __forceinline__ void sts16(uint32_t addr, uint16_t v)
 {
     asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
@@ -168,6 +173,24 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16])
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
           "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
           "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(addr)
+        : "memory");
+}
+
+/* 32 columns */
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+          "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]),
+          "=f"(v[31])
         : "r"(addr)
         : "memory");
 }
@@ -308,13 +331,12 @@ __device__ __noinline__ float product_terms(const ProdArgs& a, int K, int e, lon
 }
 
 /* The results of a row whose sums were not finite (bits of `which`, from
- * feature i on), from their own terms, into the row's pieces in shared memory:
- * row points to piece 0, pieces are spread by `spread`. */
+ * feature i on), from their own terms, into the row in shared memory (four
+ * 16-byte pieces, piece c at c ^ spread). */
 template <typename T, bool TRANS, int ACT>
 __device__ __noinline__ void sum_again(const ProdArgs& a, int K, int e, long long row_, int i,
-                                       uint32_t which, uint4* row, int spread, bool res)
+                                       uint32_t which, uint32_t row, uint32_t spread, bool res)
 {
-    unsigned char* base = (unsigned char*)row - (spread << 4);
     for (; which; which &= which - 1) {
         const int c = __ffs(which) - 1;
         float v = product_terms<T, TRANS>(a, K, e, row_, i + c);
@@ -323,7 +345,8 @@ __device__ __noinline__ void sum_again(const ProdArgs& a, int K, int e, long lon
             v = act_of<ACT>(v);
             if (res && a.res) v += to_f(((const T*)a.res)[row_ * a.ldr + i + c]);
         }
-        *(T*)(base + (((c >> 3) ^ spread) << 4) + (c & 7) * 2) = from_f<T>(v);
+        const T h = from_f<T>(v);
+        sts16(row + (((c >> 3) ^ spread) << 4) + (c & 7) * 2, *(const uint16_t*)&h);
     }
 }
 
@@ -548,164 +571,180 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     } else if (warp >= kEpiWarp0t) {
         /* ---------------- epilogue: a warp's 32 rows of 32 features.  The
          * accumulators come a row a lane; memory is read and written eight
-         * rows of 64 bytes at a time, by way of the warp's own 2 KB of shared
-         * memory (a lane that wrote its own row's 32-byte sectors to memory
-         * kept the L1 busy four times as long).  The residual is read while
-         * the tile's MMAs run. */
+         * rows of 64 bytes at a time, by way of the warp's own shared memory
+         * (a lane that wrote its own row's 32-byte sectors to memory kept the
+         * L1 busy four times as long).  A tile's residual is copied there
+         * while the tile before is worked on: two buffers a warp. */
         const int ew = warp - kEpiWarp0t;
         const int fw = (ew >> 2) * 32;
         const uint32_t tq = (uint32_t)(warp & 3);
-        unsigned char* buf = smem + (kWSlots + kXStages) * kBoxBytes + ew * kEpiBuf;
-        /* a row's four 16-byte pieces, spread over the banks */
-        auto piece = [&](int row, int c) {
-            return (uint4*)(buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
-        };
-        const int crow = lane >> 2, cpc = lane & 3;   /* of memory accesses */
+        const bool has_res = !TRANS && a.res, has_z = !TRANS && a.z;
         const bool al = ((uintptr_t)a.out % 16 == 0) && (a.ldo % 8 == 0);
         const bool alz = ((uintptr_t)a.z % 16 == 0) && (a.ldz % 8 == 0);
         const bool alr = ((uintptr_t)a.res % 16 == 0) && (a.ldr % 8 == 0);
+        const uint32_t buf0 = smem_u32(smem) + (kWSlots + kXStages) * kBoxBytes + 2 * ew * kEpiBuf;
+        /* a row's four 16-byte pieces are spread over the banks: this lane's
+         * own row, and its piece of rows lane / 4, + 8, + 16, + 24 */
+        const uint32_t own = lane * 64, spread = (lane >> 1) & 3;
+        const int crow = lane >> 2;
+        const uint32_t mine = crow * 64 + (((lane & 3) ^ ((crow >> 1) & 3)) << 4);
+        const int cfeat = fw + 8 * (lane & 3);
+        uint32_t flip = 0;                        /* the buffer in use, 0 or kEpiBuf */
+
+        /* a tile's 32 x 32 block out of the buffer; rows left of the expert */
+        auto copy_out = [&](T* p, long long ld, int i, int row0, int left, bool vec) {
+            __syncwarp();
+            const uint32_t src = buf0 + flip + mine;
+            const int nc = a.n_out - i;           /* of this lane's eight features */
+            T* q = p + (row0 + crow) * ld + i;
+#pragma unroll
+            for (int it = 0; it < 4; ++it, q += 8 * ld) {
+                uint32_t x[4];
+                asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                             : "r"(src + it * 512));
+                if (crow + 8 * it < left) {
+                    if (vec && nc >= 8)
+                        *(uint4*)q = make_uint4(x[0], x[1], x[2], x[3]);
+                    else
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            if (c < nc) ((uint16_t*)q)[c] = (uint16_t)(x[c >> 1] >> (16 * (c & 1)));
+                }
+            }
+            __syncwarp();
+        };
+        /* a tile's residual into the other buffer */
+        auto fetch = [&](int i, int row0, int left, uint32_t to) {
+            const int nc = a.n_out - i;
+            const T* q = (const T*)a.res + (row0 + crow) * a.ldr + i;
+#pragma unroll
+            for (int it = 0; it < 4; ++it, q += 8 * a.ldr) {
+                if (crow + 8 * it < left) {
+                    if (alr && nc >= 8)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                     ::"r"(buf0 + to + mine + it * 512), "l"(q) : "memory");
+                    else
+                        for (int c = 0; c < nc && c < 8; ++c)
+                            sts16(buf0 + to + mine + it * 512 + 2 * c, ((const uint16_t*)q)[c]);
+                }
+            }
+        };
         Ring<kAccs> ac;
         bool ok = true;
+        /* the tile whose residual is fetched next: one ahead */
+        long long pw = w;
+        Run pr;
+        int pleft = 0, prow = 0, pi = 0, phi = 0;   /* tiles left of its run, row, feature, end */
+        auto next_fetch = [&]() {
+            if (pleft == 0 && next_run(a, nt, pw, w1, pr)) {
+                pleft = pr.ntiles;
+                prow = pr.r0 + 32 * (int)tq;
+                pi = pr.fb * kTN + cfeat;
+                phi = pr.hi;
+            }
+            if (pleft > 0) {
+                --pleft;
+                return true;
+            }
+            return false;
+        };
+        if (has_res) {
+            if (next_fetch()) fetch(pi, prow, phi - prow, 0);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
         while (ok && next_run(a, nt, w, w1, r)) {
-            const int i0 = r.fb * kTN;
+            const int i0 = r.fb * kTN, hi = r.hi, e = r.e;
             if (!TRANS) {
                 asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
                 const int f = tid - kEpiWarp0t * 32;
                 if (f < kTN)
                     s_bias[f] = a.bias && i0 + f < a.n_out
-                                    ? to_f(((const T*)a.bias)[(long long)r.e * a.n_out + i0 + f])
+                                    ? to_f(((const T*)a.bias)[(long long)e * a.n_out + i0 + f])
                                     : 0.0f;
                 asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
             }
-            const int ic = i0 + fw + 8 * cpc;              /* of this lane's pieces */
-            const int nc = min(8, a.n_out - ic);
-            /* the warp's 32 x 32 block out of shared memory */
-            auto copy_out = [&](void* p, long long ld, int row0, bool vec) {
-                __syncwarp();
-#pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    const int rr = 8 * it + crow;
-                    const long long row = (long long)row0 + rr;
-                    const uint4 u = *piece(rr, cpc);
-                    if (row < r.hi && nc > 0) {
-                        T* q = (T*)p + row * ld + ic;
-                        if (vec && nc == 8)
-                            *(uint4*)q = u;
-                        else {
-                            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                            for (int c = 0; c < nc; ++c) {
-                                const uint16_t h = (uint16_t)(x[c >> 1] >> (16 * (c & 1)));
-                                ((uint16_t*)q)[c] = h;
-                            }
-                        }
-                    }
-                }
-                __syncwarp();
-            };
-            for (int j = 0; j < r.ntiles && ok; ++j, ac.next()) {
-                const int row0 = r.r0 + j * kTM + 32 * (int)tq;
-                const bool live = row0 + lane < r.hi;
-                if (!TRANS && a.res) {
-                    uint4 rr[4];
-#pragma unroll
-                    for (int it = 0; it < 4; ++it) {
-                        const long long row = (long long)row0 + 8 * it + crow;
-                        const T* q = (const T*)a.res + row * a.ldr + ic;
-                        rr[it] = make_uint4(0, 0, 0, 0);
-                        if (row < r.hi && nc > 0) {
-                            if (alr && nc == 8)
-                                rr[it] = *(const uint4*)q;
-                            else {
-                                uint32_t x[4] = {0, 0, 0, 0};
-#pragma unroll
-                                for (int c = 0; c < 8; ++c)
-                                    if (c < nc)
-                                        x[c >> 1] |= (uint32_t)((const uint16_t*)q)[c] << (16 * (c & 1));
-                                rr[it] = make_uint4(x[0], x[1], x[2], x[3]);
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int it = 0; it < 4; ++it) *piece(8 * it + crow, cpc) = rr[it];
-                    __syncwarp();
+            int row0 = r.r0 + 32 * (int)tq;
+            for (int j = r.ntiles; j > 0 && ok; --j, row0 += kTM, ac.next()) {
+                const int left = hi - row0;
+                if (has_res) {
+                    prow += kTM;
+                    if (next_fetch()) fetch(pi, prow, phi - prow, flip ^ kEpiBuf);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
                 }
                 ok = mm_wait(ac.bar(afull), ac.round, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t y[16], again = 0;
-                const uint32_t ta = tmem + ((tq * 32) << 16) + (uint32_t)(ac.s * kTN + fw);
+                float v[32];
+                tmem_ld32(tmem + ((tq * 32) << 16) + (uint32_t)(ac.s * kTN + fw), v);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ac.bar(aempty));
+                float2 chk = both(0.0f);
 #pragma unroll
-                for (int cc = 0; cc < 2; ++cc) {
-                    float v[16];
-                    tmem_ld16(ta + 16u * cc, v);
-                    if (cc == 1) {
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(ac.bar(aempty));
-                    }
-                    const int fo = fw + 16 * cc;
-                    uint32_t res[8];
-                    float2 chk = both(0.0f);
+                for (int c = 0; c < 32; c += 2)
+                    chk = fma2(make_float2(v[c], v[c + 1]), both(0.0f), chk);
+                uint32_t again = 0;
+                if (chk.x + chk.y != 0.0f && lane < left) {   /* some sum is not finite */
 #pragma unroll
-                    for (int c = 0; c < 16; c += 2)
-                        chk = fma2(make_float2(v[c], v[c + 1]), both(0.0f), chk);
-                    if (chk.x + chk.y != 0.0f && live) {   /* some sum is not finite */
-#pragma unroll
-                        for (int c = 0; c < 16; ++c)
-                            if (!isfinite(v[c]) && i0 + fo + c < a.n_out) again |= 1u << (16 * cc + c);
-                    }
-                    __syncwarp();
-                    if (!TRANS) {
-#pragma unroll
-                        for (int c = 0; c < 16; c += 4) {
-                            const float4 b = *(const float4*)&s_bias[fo + c];
-                            const float2 p = add2(make_float2(v[c], v[c + 1]), make_float2(b.x, b.y));
-                            const float2 q = add2(make_float2(v[c + 2], v[c + 3]), make_float2(b.z, b.w));
-                            v[c] = p.x;
-                            v[c + 1] = p.y;
-                            v[c + 2] = q.x;
-                            v[c + 3] = q.y;
-                        }
-                        /* the row's residual makes room for its z */
-                        if (a.res) {
-                            const uint4 u = *piece(lane, 2 * cc), w4 = *piece(lane, 2 * cc + 1);
-                            res[0] = u.x; res[1] = u.y; res[2] = u.z; res[3] = u.w;
-                            res[4] = w4.x; res[5] = w4.y; res[6] = w4.z; res[7] = w4.w;
-                        }
-                        if (a.z) {
-#pragma unroll
-                            for (int c = 0; c < 2; ++c)
-                                *piece(lane, 2 * cc + c) = make_uint4(
-                                    pack2<T>(v[8 * c], v[8 * c + 1]), pack2<T>(v[8 * c + 2], v[8 * c + 3]),
-                                    pack2<T>(v[8 * c + 4], v[8 * c + 5]), pack2<T>(v[8 * c + 6], v[8 * c + 7]));
-                        }
-                    }
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        float2 u = make_float2(v[2 * c], v[2 * c + 1]);
-                        if (!TRANS) {
-                            u = act2<ACT>(u);
-                            if (a.res) u = add2(u, unpack2<T>(res[c]));
-                        }
-                        y[8 * cc + c] = pack2<T>(u.x, u.y);
-                    }
+                    for (int c = 0; c < 32; ++c)
+                        if (!isfinite(v[c]) && i0 + fw + c < a.n_out) again |= 1u << c;
                 }
-                if (!TRANS && a.z) {
+                __syncwarp();
+                if (has_res) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    __syncwarp();
+                }
+                const uint32_t row = buf0 + flip + own;
+                uint32_t y[16];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {   /* eight features */
+                    const uint32_t at = row + ((c ^ spread) << 4);
+                    uint32_t res[4];
+                    if (has_res)
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(res[0]), "=r"(res[1]), "=r"(res[2]), "=r"(res[3])
+                                     : "r"(at));
+                    float2 u[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) u[h] = make_float2(v[8 * c + 2 * h], v[8 * c + 2 * h + 1]);
+                    if (!TRANS) {
+                        const float4* b = (const float4*)&s_bias[fw + 8 * c];
+                        u[0] = add2(u[0], make_float2(b[0].x, b[0].y));
+                        u[1] = add2(u[1], make_float2(b[0].z, b[0].w));
+                        u[2] = add2(u[2], make_float2(b[1].x, b[1].y));
+                        u[3] = add2(u[3], make_float2(b[1].z, b[1].w));
+                        /* the row's residual makes room for its z */
+                        if (has_z)
+                            sts128(at, pack2<T>(u[0].x, u[0].y), pack2<T>(u[1].x, u[1].y),
+                                   pack2<T>(u[2].x, u[2].y), pack2<T>(u[3].x, u[3].y));
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            u[h] = act2<ACT>(u[h]);
+                            if (has_res) u[h] = add2(u[h], unpack2<T>(res[h]));
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) y[4 * c + h] = pack2<T>(u[h].x, u[h].y);
+                }
+                if (has_z) {
                     if (again)
-                        sum_again<T, TRANS, DIA_ACT_NONE>(a, K, r.e, row0 + lane, i0 + fw, again,
-                                                          piece(lane, 0), (lane >> 1) & 3, false);
-                    copy_out(a.z, a.ldz, row0, alz);
+                        sum_again<T, TRANS, DIA_ACT_NONE>(a, K, e, row0 + lane, i0 + fw, again, row,
+                                                          spread, false);
+                    copy_out((T*)a.z, a.ldz, i0 + cfeat, row0, left, alz);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    *piece(lane, c) = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+                    sts128(row + ((c ^ spread) << 4), y[4 * c], y[4 * c + 1], y[4 * c + 2],
+                           y[4 * c + 3]);
                 if (again)
-                    sum_again<T, TRANS, ACT>(a, K, r.e, row0 + lane, i0 + fw, again,
-                                             piece(lane, 0), (lane >> 1) & 3, true);
-                copy_out(a.out, a.ldo, row0, al);
+                    sum_again<T, TRANS, ACT>(a, K, e, row0 + lane, i0 + fw, again, row, spread, true);
+                copy_out((T*)a.out, a.ldo, i0 + cfeat, row0, left, al);
+                if (has_res) flip ^= kEpiBuf;
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
 
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -730,7 +769,8 @@ constexpr int kGBoxBytes = kGRows * 128;
 constexpr int kGBoxes = 4;                     /* boxes of inputs of a CTA */
 constexpr int kGStageBytes = (2 + kGBoxes) * kGBoxBytes;
 constexpr int kGStages = 4;
-constexpr int kGOnesBytes = 16 * 128;
+constexpr int kGOnes = 16;                      /* columns of ones */
+constexpr int kGOnesBytes = kGOnes * 16 * 2;
 constexpr int kGSmem = kGStages * kGStageBytes + kGOnesBytes + 1024;
 constexpr int kGWarps = 18;                    /* TMA, MMA, sixteen for the results */
 constexpr int kGPitch = kGBoxes * kBoxCols + 1;
@@ -745,6 +785,18 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t addr)
     d |= (uint64_t)((1024u >> 4) & 0x3FFF) << 32;
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
+    return d;
+}
+
+/* MN-major operand without swizzle, 8 x 8 cells of 128 bytes: for the ones,
+ * of which any order is the same */
+__device__ __forceinline__ uint64_t ones_desc(uint32_t addr)
+{
+    uint64_t d = 0;
+    d |= (uint64_t)((addr >> 4) & 0x3FFF);
+    d |= (uint64_t)(128 >> 4) << 16;
+    d |= (uint64_t)(256 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
     return d;
 }
 
@@ -846,9 +898,9 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         const uint32_t id0 = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) |
                              ((uint32_t)(128 >> 4) << 24);
         const uint32_t idx = id0 | ((uint32_t)(nb * kBoxCols >> 3) << 17);
-        const uint32_t ido = id0 | ((uint32_t)(kBoxCols >> 3) << 17);
+        const uint32_t ido = id0 | ((uint32_t)(kGOnes >> 3) << 17);
         const bool leader = elect_one();
-        const uint64_t desc0 = mn_desc(st0), odesc = mn_desc(smem_u32(ones));
+        const uint64_t desc0 = mn_desc(st0), odesc = ones_desc(smem_u32(ones));
         Ring<kGStages> x;
         for (int g = 0; g < nst; ++g, x.next()) {
             const int left = rg.r1 - rg.r0 - g * kGRows;
@@ -927,32 +979,47 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     /* a diagonal's 128 entries: consecutive features, consecutive columns of
      * one box or more; what lies in other CTAs' boxes is theirs */
     const int k_lo = nb > 0 ? s_box[0].k0 : 0, k_hi = nb > 0 ? s_box[nb - 1].k1 : 0;
+    int col[kGBoxes];
+#pragma unroll
+    for (int c = 0; c < kGBoxes; ++c) col[c] = c < nb ? s_box[c].col : INT_MAX / 2;
+    const bool parts = rg.nparts > 1;
     const int f_end = (int)min(128ll, a.stride - i0);
+    float* part0 = a.part + (long long)(rg.slot + rg.part) * (a.K + 1) * a.stride + i0 + lane;
+    T* out0 = (T*)a.dvals + rg.e * a.estride + i0 + lane;
+    const float* row = tile + lane * kGPitch;
     for (int k = k_lo + warp; k < k_hi; k += kGWarps) {
         const int2 o = a.K <= kOffs ? s_offs[k] : a.dir.offs[k];
-        const bool parts = rg.nparts > 1;
-        const long long at = parts
-            ? ((long long)(rg.slot + rg.part) * (a.K + 1) + o.y) * a.stride + i0
-            : rg.e * a.estride + o.y * a.stride + i0;
         /* features whose entry lies in the matrix; outside, and in the
          * padding, there is no gradient */
         const int in_lo = max(0, -(i0 + o.x));
         const int in_hi = nst > 0 ? min(a.n_rows - i0, a.n_cols - i0 - o.x) : 0;
-        for (int c = 0; c < nb; ++c) {
-            const int rel = o.x - s_box[c].col;    /* column of feature 0 */
-            const int f1 = min(f_end, kBoxCols - rel);
-            const float* src = tile + c * kBoxCols + rel;
-            for (int f = max(0, -rel) + lane; f < f1; f += 32) {
-                float v = 0.0f;
-                if (f >= in_lo && f < in_hi) {
-                    v = src[f * (kGPitch + 1)];
-                    if (!isfinite(v)) v = gradient_terms<T>(a, rg.r0, rg.r1, i0 + f, i0 + f + o.x);
-                }
-                if (parts)
-                    a.part[at + f] = v;
-                else
-                    ((T*)a.dvals)[at + f] = from_f<T>(v);
+        float v[4];
+        bool on[4], bad = false;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int f = 32 * s + lane, p = o.x + f;
+            int at = -1;
+#pragma unroll
+            for (int c = 0; c < kGBoxes; ++c)
+                if ((unsigned)(p - col[c]) < (unsigned)kBoxCols) at = c * kBoxCols + p - col[c];
+            on[s] = at >= 0 && f < f_end;
+            v[s] = on[s] && f >= in_lo && f < in_hi ? row[32 * s * kGPitch + at] : 0.0f;
+            bad |= !isfinite(v[s]);
+        }
+        if (bad) {
+            for (int s = 0; s < 4; ++s) {
+                const int i = i0 + 32 * s + lane;
+                if (!isfinite(v[s])) v[s] = gradient_terms<T>(a, rg.r0, rg.r1, i, i + o.x);
             }
+        }
+        const long long at = (long long)o.y * a.stride;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (!on[s]) continue;
+            if (parts)
+                part0[at + 32 * s] = v[s];
+            else
+                out0[at + 32 * s] = from_f<T>(v[s]);
         }
     }
 }
