@@ -372,6 +372,7 @@ struct ProdArgs {
     int act;
     SpmmDir dir;
     bool trans;
+    int groups;           /* set by the tensor-core launch */
     bool early;           /* tensor-core form: inputs are complete when the kernel may begin */
 };
 
