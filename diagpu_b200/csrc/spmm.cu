@@ -29,219 +29,367 @@
 
 namespace dia {
 
-constexpr int kMmWarps = 8;
-constexpr int kMmThreads = kMmWarps * 32;
-constexpr int kMmFeat = 128;   /* features of a warp: four per lane */
+/* ------------------------------------------------- few rows, or any at all
+ *
+ * A lane is a feature; a diagonal value is read once for TT rows, an input
+ * straight from memory.  With few rows a call is as long as its chain of
+ * memory latencies, so the CTA's warps split the diagonals `ks` ways (four at
+ * a time in flight each) and add up in shared memory in a fixed order, and
+ * what the epilogue reads is fetched first.  The other 16 / ks warps take
+ * other features. */
+constexpr int kFewWarps = 16;
+constexpr int kFewOffs = 512;   /* offsets staged at once */
 
-/* elements c .. c+3 of a row of n elements, zero outside */
-template <typename T, bool VEC>
-__device__ __forceinline__ float4 row4(const T* row, int c, int n)
+template <typename T, bool TRANS, int TT>
+__global__ void __launch_bounds__(kFewWarps * 32)
+spmm_few_kernel(const __grid_constant__ ProdArgs a, int ks, int ftiles, long long ngroups,
+                bool rows_first)
 {
-    if (VEC && c >= 0 && c + 4 <= n) return load4<T>(row + c);
-    float4 v;
-    v.x = (unsigned)c < (unsigned)n ? to_f(row[c]) : 0.0f;
-    v.y = (unsigned)(c + 1) < (unsigned)n ? to_f(row[c + 1]) : 0.0f;
-    v.z = (unsigned)(c + 2) < (unsigned)n ? to_f(row[c + 2]) : 0.0f;
-    v.w = (unsigned)(c + 3) < (unsigned)n ? to_f(row[c + 3]) : 0.0f;
-    return v;
-}
-
-/* One warp: 128 features (four consecutive ones a lane), TT rows.  A quad's
- * up to four diagonals read the window of seven inputs from two aligned
- * chunks of four, so a run of consecutive offsets costs one chunk per four
- * diagonals; a weight is read once for TT rows.  The CTA's warps split the
- * quads `ks` ways (few rows: there are too few warps otherwise) and add up
- * in shared memory in a fixed order; the other 8 / ks take other features. */
-template <typename T, bool TRANS, int TT, bool VEC>
-__global__ void __launch_bounds__(kMmThreads)
-spmm_kernel(ProdArgs a, int ks, int ftiles, long long ngroups, bool rows_first)
-{
-    __shared__ float s_sum[kMmWarps][TT * 4][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int part = warp % ks, sub = warp / ks, fper = kMmWarps / ks;
+    __shared__ int2 s_off[kFewOffs];
+    __shared__ float s_sum[kFewWarps][TT][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int part = warp % ks, sub = warp / ks, fper = kFewWarps / ks;
     const int fblocks = (ftiles + fper - 1) / fper;
     const long long b = blockIdx.x;
     const long long g = rows_first ? b % ngroups : b / fblocks;
     const int fb = (int)(rows_first ? b / ngroups : b % fblocks);
+    for (int k = tid; k < min(a.K, kFewOffs); k += kFewWarps * 32) s_off[k] = a.dir.offs[k];
     const RowGroup rg = row_group(a.seg, a.E, a.M, TT, g, false);
-    const int i = (fb * fper + sub) * kMmFeat + lane * 4;
-
-    float acc[TT][4];
+    if (rg.e < 0) return;   /* whole CTA */
+    const int i = (fb * fper + sub) * 32 + lane;
+    const bool on = i < a.n_out;
+    const int nt = rg.r1 - rg.r0;
+    const T* vals = (const T*)a.vals + rg.e * a.estride;
+    const T* in = (const T*)a.in + rg.r0 * a.ldi;
+    float bias = 0.0f, res[TT];
 #pragma unroll
-    for (int t = 0; t < TT; ++t)
+    for (int t = 0; t < TT; ++t) res[t] = 0.0f;
+    if (!TRANS && part == 0 && on) {
+        if (a.bias) bias = to_f(((const T*)a.bias)[(long long)rg.e * a.n_out + i]);
+        if (a.res)
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+                if (t < nt) res[t] = to_f(((const T*)a.res)[(rg.r0 + t) * a.ldr + i]);
+    }
+    float acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = 0.0f;
+    for (int base = 0; base < a.K; base += kFewOffs) {
+        const int n = min(a.K - base, kFewOffs);
+        if (base > 0) {
+            __syncthreads();
+            for (int k = tid; k < n; k += kFewWarps * 32) s_off[k] = a.dir.offs[base + k];
+        }
+        __syncthreads();
+        const int k0 = n * part / ks, k1 = n * (part + 1) / ks;
+        constexpr int U = TT == 1 ? 8 : 4;
+        for (int k = k0; k < k1; k += U) {
+            float w[U], x[U][TT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int2 o = s_off[min(k + u, k1 - 1)];
+                const int j = i + o.x;
+                const bool ok = k + u < k1 && on && (unsigned)j < (unsigned)a.n_in;
+                w[u] = ok ? to_f(vals[o.y * a.stride + (TRANS ? j : i)]) : 0.0f;
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+                    x[u][t] = ok && t < nt ? to_f(in[t * a.ldi + j]) : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) acc[t] = fmaf(w[u], x[u][t], acc[t]);
+        }
+    }
+    if (ks > 1) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) s_sum[warp][t][lane] = acc[t];
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+            for (int p = 1; p < ks; ++p) acc[t] += s_sum[warp + p][t][lane];
+    }
+    if (!on) return;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        if (t >= nt) break;
+        const long long row = rg.r0 + t;
+        const float z = acc[t] + bias;
+        if (!TRANS && a.z) ((T*)a.z)[row * a.ldz + i] = from_f<T>(z);
+        ((T*)a.out)[row * a.ldo + i] = from_f<T>(TRANS ? z : act_any(a.act, z) + res[t]);
+    }
+}
+
+/* ----------------------------------------------------------- many rows
+ *
+ * A CTA takes a tile of features and copies the inputs it reads to
+ * shared memory; a warp takes 128 features of eight rows.  QUADS: a lane owns
+ * four consecutive features, and the up to four diagonals of a quad read
+ * seven consecutive inputs as two 16-byte pieces, of which the second is the
+ * next quad's first: for runs of consecutive offsets shared memory gives a
+ * piece per sixteen products.  Otherwise (fewer than three diagonals a quad)
+ * a lane owns features 32 apart and reads an input per product, without bank
+ * conflicts at any offset.  Shared memory's bandwidth bounds both. */
+constexpr int kTileWarps = 8;
+constexpr int kTileRows = 8;    /* rows of a warp */
+
+/* `rows` rows of the spans' inputs to shared memory, zero outside the block;
+ * pitch in elements */
+template <typename T, bool VEC>
+__device__ __forceinline__ void stage_spans(T* dst, int pitch, const InputSpan* spans, int s0, int s1,
+                                            const T* in, long long ld, int i0, int n_in, int rows,
+                                            int nt, int tid, int threads)
+{
+    constexpr int V = 16 / sizeof(T);
+    for (int s = s0; s < s1; ++s) {
+        const InputSpan sp = spans[s];
+        const int per = sp.len / V;
+        for (int o = tid; o < per * rows; o += threads) {
+            const int t = o / per, c = (o - t * per) * V;
+            T* d = dst + t * pitch + sp.at + c;
+            const int j = i0 + sp.from + c;
+            if (VEC && t < nt && j >= 0 && j + V <= n_in) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                             ::"r"((uint32_t)__cvta_generic_to_shared(d)), "l"(in + t * ld + j)
+                             : "memory");
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    d[v] = t < nt && (unsigned)(j + v) < (unsigned)n_in ? in[t * ld + j + v]
+                                                                        : from_f<T>(0.0f);
+            }
+        }
+    }
+}
+
+template <typename T, bool TRANS, bool VEC, bool QUADS>
+__global__ void __launch_bounds__(kTileWarps * 32)
+spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long long ngroups,
+                 bool rows_first)
+{
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    T* xs = (T*)smem_raw;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int F = kTileF[0] << shape, wf = F / 128;   /* warps side by side */
+    const int rows = kTileWarps / wf * kTileRows;
+    const long long b = blockIdx.x;
+    const long long g = rows_first ? b % ngroups : b / ftiles;
+    const int i0 = (int)(rows_first ? b / ngroups : b % ftiles) * F;
+    const RowGroup rg = row_group(a.seg, a.E, a.M, rows, g, false);
+    if (rg.e < 0) return;   /* whole CTA */
+    const int nt = rg.r1 - rg.r0, pitch = a.dir.width[shape];
+    stage_spans<T, VEC>(xs, pitch, a.dir.spans[shape], 0, a.dir.nspans[shape],
+                        (const T*)a.in + rg.r0 * a.ldi, a.ldi, i0, a.n_in, rows, nt, tid,
+                        kTileWarps * 32);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    const int t0 = warp / wf * kTileRows, f0 = warp % wf * 128;
+    if (t0 >= nt || i0 + f0 >= a.n_out) return;
+    const int live = min(nt - t0, kTileRows);
+    const T* vals = (const T*)a.vals + rg.e * a.estride;
+    const T* xw = xs + t0 * pitch;
+    float acc[kTileRows][4];
+#pragma unroll
+    for (int t = 0; t < kTileRows; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[t][r] = 0.0f;
 
-    if (rg.e >= 0 && i < a.n_out) {
-        const T* vals = (const T*)a.vals + rg.e * a.estride;
-        const T* in = (const T*)a.in + (long long)rg.r0 * a.ldi;
-        const int nt = rg.r1 - rg.r0;
-        const int q0 = (int)((long long)a.dir.nquads * part / ks);
-        const int q1 = (int)((long long)a.dir.nquads * (part + 1) / ks);
-        for (int q = q0; q < q1; ++q) {
-            const int4 h = __ldg((const int4*)&a.dir.quads[q]);
-            const int k3 = __ldg(&a.dir.quads[q].k[3]);
-            const int kk[4] = {h.y, h.z, h.w, k3};
+    constexpr int STEP = QUADS ? 1 : 32;             /* between a lane's features */
+    const int f = f0 + (QUADS ? 4 * lane : lane), i = i0 + f;
+    if (QUADS) {
+        const Quad* quads = a.dir.quads[shape];
+        float carry[kTileRows][4];
+        int next = INT_MIN;   /* base of the quad whose first piece `carry` holds */
+        for (int q = 0; q < a.dir.nquads; ++q) {
+            const int4 h = __ldg((const int4*)&quads[q]);
+            const int2 h2 = __ldg((const int2*)&quads[q].k[3]);
+            const int kk[4] = {h.y, h.z, h.w, h2.x};
             const int c = i + h.x;
-            if (c + 7 <= 0 || c >= a.n_in) continue;
             float w[4][4];
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 if (kk[s] < 0) continue;
                 const T* vp = vals + (long long)kk[s] * a.stride;
-                if (TRANS) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = c + s + r;
-                        w[s][r] = ((unsigned)j < (unsigned)a.n_in && i + r < a.n_out)
-                                      ? to_f(vp[j]) : 0.0f;
-                    }
-                } else {
-                    const float4 v = load4<T>(vp + i);
-                    w[s][0] = v.x;
-                    w[s][1] = v.y;
-                    w[s][2] = v.z;
-                    w[s][3] = v.w;
-                    if (c < 0 || c + 7 > a.n_in) {
+                for (int r = 0; r < 4; ++r) {
+                    const int j = c + s + r;
+                    w[s][r] = i + r < a.n_out && (unsigned)j < (unsigned)a.n_in
+                                  ? to_f(vp[TRANS ? j : i + r]) : 0.0f;
+                }
+            }
+            const T* p = xw + h2.y + f;
+            if (h.x != next) {
+#pragma unroll
+                for (int t = 0; t < kTileRows; ++t) *(float4*)carry[t] = load4<T>(p + t * pitch);
+            }
+            next = h.x + 4;
+#pragma unroll
+            for (int t = 0; t < kTileRows; ++t) {
+                float x[8];
+                *(float4*)x = *(float4*)carry[t];
+                *(float4*)(x + 4) = load4<T>(p + t * pitch + 4);
+                *(float4*)carry[t] = *(float4*)(x + 4);
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    if (kk[s] >= 0)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if ((unsigned)(c + s + r) >= (unsigned)a.n_in) w[s][r] = 0.0f;
-                    }
-                }
-            }
-            float xs[TT][8];
-#pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                if (t < nt) {
-                    const T* row = in + t * a.ldi;
-                    const float4 u = row4<T, VEC>(row, c, a.n_in);
-                    const float4 v = row4<T, VEC>(row, c + 4, a.n_in);
-                    xs[t][0] = u.x; xs[t][1] = u.y; xs[t][2] = u.z; xs[t][3] = u.w;
-                    xs[t][4] = v.x; xs[t][5] = v.y; xs[t][6] = v.z; xs[t][7] = v.w;
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) xs[t][r] = 0.0f;
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                if (kk[s] < 0) continue;
-#pragma unroll
-                for (int t = 0; t < TT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[t][r] = fmaf(w[s][r], xs[t][s + r], acc[t][r]);
+                            acc[t][r] = fmaf(w[s][r], x[s + r], acc[t][r]);
             }
         }
-    }
-    if (ks > 1) {
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s_sum[warp][t * 4 + r][lane] = acc[t][r];
-        __syncthreads();
-        if (part != 0) return;
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
+    } else {
+        const int* cols = a.dir.cols[shape];
+        /* the next diagonal's values are on their way while one is worked on */
+        auto fetch = [&](int k, float (&w)[4], int& col) {
+            const int2 o = __ldg(&a.dir.offs[k]);
+            col = __ldg(cols + k);
+            const T* vp = vals + (long long)o.y * a.stride;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float v = acc[t][r];
-                for (int p = 1; p < ks; ++p) v += s_sum[warp + p][t * 4 + r][lane];
-                acc[t][r] = v;
+                const int ir = i + 32 * r, j = ir + o.x;
+                w[r] = ir < a.n_out && (unsigned)j < (unsigned)a.n_in
+                           ? to_f(__ldg(vp + (TRANS ? j : ir))) : 0.0f;
             }
-    }
-    if (rg.e < 0 || i >= a.n_out) return;
-    const T* bias = a.bias ? (const T*)a.bias + (long long)rg.e * a.n_out : nullptr;
+        };
+        float w[4], wn[4];
+        int col = 0, cn = 0;
+        if (a.K > 0) fetch(0, w, col);
+#pragma unroll 2
+        for (int k = 0; k < a.K; ++k) {
+            if (k + 1 < a.K) fetch(k + 1, wn, cn);
+            const T* p = xw + col + f;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        const long long row = (long long)rg.r0 + t;
-        if (row >= rg.r1) break;
+            for (int t = 0; t < kTileRows; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[t][r] = fmaf(w[r], to_f(p[t * pitch + 32 * r]), acc[t][r]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[r] = wn[r];
+            col = cn;
+        }
+    }
+    float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!TRANS && a.bias)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (i + STEP * r < a.n_out)
+                bias[r] = to_f(((const T*)a.bias)[(long long)rg.e * a.n_out + i + STEP * r]);
+#pragma unroll
+    for (int t = 0; t < kTileRows; ++t) {
+        if (t >= live) break;
+        const long long row = (long long)rg.r0 + t0 + t;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            if (i + r >= a.n_out) break;
-            float z = acc[t][r];
-            if (bias) z += to_f(bias[i + r]);
-            if (a.z) ((T*)a.z)[row * a.ldz + i + r] = from_f<T>(z);
-            float y = act_any(a.act, z);
-            if (a.res) y += to_f(((const T*)a.res)[row * a.ldr + i + r]);
-            ((T*)a.out)[row * a.ldo + i + r] = from_f<T>(y);
+            const int ir = i + STEP * r;
+            if (ir >= a.n_out) continue;
+            const float z = acc[t][r] + bias[r];
+            float y = z;
+            if (!TRANS) {
+                if (a.z) ((T*)a.z)[row * a.ldz + ir] = from_f<T>(z);
+                y = act_any(a.act, z);
+                if (a.res) y += to_f(((const T*)a.res)[row * a.ldr + ir]);
+            }
+            ((T*)a.out)[row * a.ldo + ir] = from_f<T>(y);
         }
     }
 }
 
-/* One CTA: 128 features, one quad, one part of an expert's rows; its warps
- * take every eighth row and add up in shared memory in a fixed order.  Sums
- * of an expert with one part go out at once, others to `part`. */
+/* ------------------------------------------------- gradient of the diagonals
+ *
+ * A CTA takes 128 features, one window of diagonals (at most 64) and one part
+ * of an expert's rows, eight rows at a time by way of shared memory; a warp
+ * keeps the sums of its eight diagonals at its lanes' four features.  Sums of
+ * an expert with one part go out at once, others to `part`. */
+constexpr int kGradRows = 8;
+constexpr int kGradDiags = 8;   /* diagonals of a warp */
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kMmThreads)
-spmm_grad_kernel(GradArgs a, int ftiles)
+__global__ void __launch_bounds__(kTileWarps * 32)
+spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins)
 {
-    __shared__ float s_sum[kMmWarps][20][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int nq = max(a.dir.nquads, 1);
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long b = blockIdx.x;
-    const int f = (int)(b % ftiles), q = (int)((b / ftiles) % nq);
-    const RowGroup rg = row_group(a.seg, a.E, a.M, a.per, b / ftiles / nq, true);
+    const int f0 = (int)(b % ftiles) * 128, wi = (int)(b / ftiles % nwins);
+    const RowGroup rg = row_group(a.seg, a.E, a.M, a.per, b / ftiles / nwins, true);
     if (rg.e < 0 || (rg.nparts > 1 && rg.slot + rg.part >= a.slots)) return;
-    const int i = f * kMmFeat + lane * 4;
-    const bool on = i < a.n_rows;
-    int kk[4] = {-1, -1, -1, -1}, base = 0;
-    if (q < a.dir.nquads && a.dvals) {
-        base = a.dir.quads[q].base;
+    const bool diags = a.dvals && a.dir.nwins > 0;
+    GradWindow win{};
+    if (diags) win = a.dir.wins[wi];
+    const int pitch = diags ? a.dir.wwidth : 0;
+    T* xs = (T*)smem_raw;
+    T* ds = xs + kGradRows * pitch;                  /* [row][128] */
+    const InputSpan dspan{0, 128, 0, 0};
+    const int per = (win.k1 - win.k0 + kTileWarps - 1) / kTileWarps;
+    const int k0 = win.k0 + warp * per, nk = max(0, min(per, win.k1 - k0));
+    int col[kGradDiags];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) kk[s] = a.dir.quads[q].k[s];
-    }
-    const int c = i + base;
-    float acc[4][4], sb[4] = {0, 0, 0, 0};
+    for (int u = 0; u < kGradDiags; ++u) col[u] = u < nk ? a.dir.wcols[k0 + u] + lane : 0;
+    const bool bias = a.dbias && wi == 0 && warp == 0;
+    float acc[kGradDiags][4], sb[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int u = 0; u < kGradDiags; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[s][r] = 0.0f;
-    if (on) {
-        for (int t = rg.r0 + warp; t < rg.r1; t += kMmWarps) {
-            const float4 d = row4<T, VEC>((const T*)a.dz + t * a.lddz, i, a.n_rows);
-            const T* row = (const T*)a.x + t * a.ldx;
-            const float4 u = row4<T, VEC>(row, c, a.n_cols);
-            const float4 v = row4<T, VEC>(row, c + 4, a.n_cols);
-            const float dd[4] = {d.x, d.y, d.z, d.w};
-            const float xs[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        for (int r = 0; r < 4; ++r) acc[u][r] = 0.0f;
+    if (f0 < a.n_rows) {
+        for (int t0 = rg.r0; t0 < rg.r1; t0 += kGradRows) {
+            const int nt = min(rg.r1 - t0, kGradRows);
+            __syncthreads();
+            if (diags)
+                stage_spans<T, VEC>(xs, pitch, a.dir.wspans, win.s0, win.s1,
+                                    (const T*)a.x + t0 * a.ldx, a.ldx, f0, a.n_cols, kGradRows, nt,
+                                    tid, kTileWarps * 32);
+            stage_spans<T, VEC>(ds, 128, &dspan, 0, 1, (const T*)a.dz + t0 * a.lddz, a.lddz, f0,
+                                a.n_rows, kGradRows, nt, tid, kTileWarps * 32);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncthreads();
+#pragma unroll 2
+            for (int t = 0; t < kGradRows; ++t) {
+                float d[4];
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-                if (kk[s] >= 0)
+                for (int r = 0; r < 4; ++r) d[r] = to_f(ds[t * 128 + lane + 32 * r]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[s][r] = fmaf(dd[r], xs[s + r], acc[s][r]);
+                for (int u = 0; u < kGradDiags; ++u)
+                    if (u < nk)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sb[r] += dd[r];
+                        for (int r = 0; r < 4; ++r)
+                            acc[u][r] = fmaf(d[r], to_f(xs[t * pitch + col[u] + 32 * r]), acc[u][r]);
+                if (bias)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sb[r] += d[r];
+            }
         }
     }
+    const bool parts = rg.nparts > 1;
+    float* part = a.part + (long long)(rg.slot + rg.part) * (a.K + 1) * a.stride;
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int u = 0; u < kGradDiags; ++u) {
+        if (u >= nk) break;
+        const int2 o = a.dir.offs[k0 + u];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s_sum[warp][s * 4 + r][lane] = acc[s][r];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) s_sum[warp][16 + r][lane] = sb[r];
-    __syncthreads();
-    /* output s * 128 + f: slot s (4: dbias) of feature f */
-    for (int o = threadIdx.x; o < 5 * kMmFeat; o += kMmThreads) {
-        const int s = o / kMmFeat, fi = o % kMmFeat, col = f * kMmFeat + fi;
-        if (col >= a.stride) continue;
-        float v = 0.0f;
-        for (int w = 0; w < kMmWarps; ++w) v += s_sum[w][s * 4 + (fi & 3)][fi >> 2];
-        if (s == 4) {
-            if (q != 0 || !a.dbias || col >= a.n_rows) continue;
-            if (rg.nparts > 1)
-                a.part[((long long)(rg.slot + rg.part) * (a.K + 1) + a.K) * a.stride + col] = v;
+        for (int r = 0; r < 4; ++r) {
+            const int i = f0 + lane + 32 * r;
+            if (i >= a.stride) continue;
+            /* an entry outside the matrix, or in the padding, has no gradient */
+            const bool in = i < a.n_rows && (unsigned)(i + o.x) < (unsigned)a.n_cols;
+            const float v = in ? acc[u][r] : 0.0f;
+            if (parts)
+                part[o.y * a.stride + i] = v;
             else
-                ((T*)a.dbias)[(long long)rg.e * a.n_rows + col] = from_f<T>(v);
-        } else if (kk[s] >= 0) {
-            /* an entry outside the matrix has no gradient */
-            if (col >= a.n_rows || (unsigned)(col + base + s) >= (unsigned)a.n_cols) v = 0.0f;
-            if (rg.nparts > 1)
-                a.part[((long long)(rg.slot + rg.part) * (a.K + 1) + kk[s]) * a.stride + col] = v;
-            else
-                ((T*)a.dvals)[rg.e * a.estride + (long long)kk[s] * a.stride + col] = from_f<T>(v);
+                ((T*)a.dvals)[rg.e * a.estride + o.y * a.stride + i] = from_f<T>(v);
         }
     }
+    if (bias)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = f0 + lane + 32 * r;
+            if (i >= a.n_rows) continue;
+            if (parts)
+                part[a.K * a.stride + i] = sb[r];
+            else
+                ((T*)a.dbias)[(long long)rg.e * a.n_rows + i] = from_f<T>(sb[r]);
+        }
 }
 
 /* Sums the parts of experts that have several, in the parts' order; four
@@ -377,35 +525,79 @@ static bool tensor_form(int dtype, long long M, int E, const SpmmDir& d)
 
 static size_t elem_size(int dtype) { return dtype == DIA_F32 ? 4 : 2; }
 
-static bool vec4(const void* p, long long ld, int dtype)
+static bool vec16(const void* p, long long ld, int dtype)
 {
-    return (uintptr_t)p % (4 * elem_size(dtype)) == 0 && ld % 4 == 0;
+    return (uintptr_t)p % 16 == 0 && ld * (long long)elem_size(dtype) % 16 == 0;
 }
 
 template <typename T, bool TRANS, int TT>
-static int launch_product_tt(const ProdArgs& a, int dtype, cudaStream_t stream)
+static int launch_few(const ProdArgs& a, cudaStream_t stream)
 {
-    const int ftiles = (a.n_out + kMmFeat - 1) / kMmFeat;
-    const long long ngroups =
-        a.seg ? a.M / TT + std::min(a.E, a.M) : (a.M + TT - 1) / TT;
-    /* warps that share a tile: enough to give every SM a few */
+    const int ftiles = (a.n_out + 31) / 32;
+    const long long ngroups = a.seg ? a.M / TT + std::min(a.E, a.M) : (a.M + TT - 1) / TT;
+    /* warps that share a tile: until every SM has 16, or a warp four diagonals */
     int ks = 1;
-    while (ks < kMmWarps && (long long)ftiles * ngroups * ks < 8ll * num_sms() &&
-           a.dir.nquads > 2 * ks)
+    while (ks < kFewWarps && (long long)ftiles * ngroups * ks < 16ll * num_sms() && a.K > 4 * ks)
         ks *= 2;
-    const int fper = kMmWarps / ks;
+    const int fper = kFewWarps / ks;
     const long long grid = ngroups * ((ftiles + fper - 1) / fper);
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: block too large");
     /* the larger of block and operator is streamed once, the other stays in L2 */
-    const bool rows_first = (long long)a.M * a.n_in < a.stride * 4 * a.dir.nquads;
-    if (vec4(a.in, a.ldi, dtype))
-        spmm_kernel<T, TRANS, TT, true>
-            <<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ks, ftiles, ngroups, rows_first);
-    else
-        spmm_kernel<T, TRANS, TT, false>
-            <<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ks, ftiles, ngroups, rows_first);
+    const bool rows_first = (long long)a.M * a.n_in < a.stride * a.K;
+    spmm_few_kernel<T, TRANS, TT><<<(unsigned)grid, kFewWarps * 32, 0, stream>>>(
+        a, ks, ftiles, ngroups, rows_first);
     DIA_TRY_CUDA(cudaGetLastError());
     return DIA_OK;
+}
+
+template <typename T, bool TRANS, bool VEC, bool QUADS>
+static int launch_tile_as(const ProdArgs& a, int shape, int smem, cudaStream_t stream)
+{
+    const int F = kTileF[shape], rows = kTileWarps * kTileRows * 128 / F;
+    const int ftiles = (a.n_out + F - 1) / F;
+    const long long ngroups = a.seg ? a.M / rows + std::min(a.E, a.M) : (a.M + rows - 1) / rows;
+    if (ngroups * ftiles > INT_MAX)
+        return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: block too large");
+    const bool rows_first = (long long)a.M * a.n_in < a.stride * a.K;
+    const auto kernel = spmm_tile_kernel<T, TRANS, VEC, QUADS>;
+    DIA_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<(unsigned)(ngroups * ftiles), kTileWarps * 32, smem, stream>>>(a, shape, ftiles,
+                                                                            ngroups, rows_first);
+    DIA_TRY_CUDA(cudaGetLastError());
+    return DIA_OK;
+}
+
+constexpr int kTileSmem = 112 * 1024;   /* two CTAs an SM */
+
+static int tile_smem(const SpmmDir& d, int shape, size_t elem)
+{
+    return (int)std::min<long long>(INT_MAX, (long long)kTileWarps * kTileRows * 128 /
+                                                 kTileF[shape] * d.width[shape] * (long long)elem);
+}
+
+template <typename T, bool TRANS>
+static int launch_cores(const ProdArgs& a, int dtype, cudaStream_t stream)
+{
+    const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
+    if (per >= 8 && a.K > 0) {
+        /* the widest tile (an input is read again by fewer tiles) whose inputs
+         * fit and that leaves a CTA for every SM */
+        for (int shape = 2; shape >= 0; --shape) {
+            const int smem = tile_smem(a.dir, shape, sizeof(T));
+            const int rows = kTileWarps * kTileRows * 128 / kTileF[shape];
+            const long long ctas = (long long)((a.n_out + kTileF[shape] - 1) / kTileF[shape]) *
+                                   ((a.M + rows - 1) / rows);
+            if (smem > kTileSmem || (shape > 0 && ctas < num_sms())) continue;
+            const bool vec = vec16(a.in, a.ldi, dtype), quads = 3 * a.dir.nquads <= a.K;
+            if (vec)
+                return quads ? launch_tile_as<T, TRANS, true, true>(a, shape, smem, stream)
+                             : launch_tile_as<T, TRANS, true, false>(a, shape, smem, stream);
+            return quads ? launch_tile_as<T, TRANS, false, true>(a, shape, smem, stream)
+                         : launch_tile_as<T, TRANS, false, false>(a, shape, smem, stream);
+        }
+    }
+    if (per >= 5) return launch_few<T, TRANS, 8>(a, stream);
+    return per >= 2 ? launch_few<T, TRANS, 4>(a, stream) : launch_few<T, TRANS, 1>(a, stream);
 }
 
 /* the tensor-core form it is (its operator has to be packed first) */
@@ -420,17 +612,8 @@ static int launch_product(const ProdArgs& a, int dtype, cudaStream_t stream)
 {
     if (a.M == 0 || a.n_out == 0) return DIA_OK;
     if (product_on_tc(a, dtype)) return spmm_tc_product(a, dtype, stream);
-    const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
-    if (a.trans)
-        return per >= 4 ? launch_product_tt<T, true, 4>(a, dtype, stream)
-                        : launch_product_tt<T, true, 1>(a, dtype, stream);
-    return per >= 4 ? launch_product_tt<T, false, 4>(a, dtype, stream)
-                    : launch_product_tt<T, false, 1>(a, dtype, stream);
-}
-
-static bool vec16(const void* p, long long ld, int dtype)
-{
-    return (uintptr_t)p % 16 == 0 && ld * (long long)elem_size(dtype) % 16 == 0;
+    return a.trans ? launch_cores<T, true>(a, dtype, stream)
+                   : launch_cores<T, false>(a, dtype, stream);
 }
 
 template <typename T, int ACT>
@@ -476,11 +659,11 @@ static int grad_part_rows(const DiaSpmmPlan* p, int dtype, long long M, int E, l
         const long long per = std::max<long long>(256, (M + want - 1) / want);
         return (int)((per + 63) / 64 * 64);
     }
-    const long long tiles = std::max<long long>(1, (stride + kMmFeat - 1) / kMmFeat) *
-                            std::max(1, p->fwd.nquads);
-    const long long want = std::max<long long>(1, 4ll * num_sms() / tiles);
-    const long long per = std::max<long long>(256, (M + want - 1) / want);
-    return (int)std::min<long long>(per, INT_MAX / 2);
+    /* a few CTAs an SM */
+    const long long tiles = std::max<long long>(1, (stride + 127) / 128) * std::max(1, p->fwd.nwins);
+    const long long want = std::max<long long>(1, 4ll * num_sms() / tiles - (E - 1));
+    const long long per = std::max<long long>(64, (M + want - 1) / want);
+    return (int)((per + 7) / 8 * 8);
 }
 
 /* parts of experts that have several: at most two a `per` rows */
@@ -496,14 +679,16 @@ template <typename T>
 static int launch_grad(const GradArgs& a, int dtype, cudaStream_t stream)
 {
     if (grad_on_tc(a, dtype)) return spmm_tc_gradient(a, dtype, stream);
-    const int ftiles = (int)((a.stride + kMmFeat - 1) / kMmFeat);
+    const int ftiles = (int)((a.stride + 127) / 128);
+    const int nwins = a.dvals ? std::max(a.dir.nwins, 1) : 1;
     const long long parts = a.seg ? a.M / a.per + a.E : std::max(1, (a.M + a.per - 1) / a.per);
-    const long long grid = parts * ftiles * std::max(a.dir.nquads, 1);
+    const long long grid = parts * ftiles * nwins;
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
-    if (vec4(a.dz, a.lddz, dtype) && vec4(a.x, a.ldx, dtype))
-        spmm_grad_kernel<T, true><<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ftiles);
-    else
-        spmm_grad_kernel<T, false><<<(unsigned)grid, kMmThreads, 0, stream>>>(a, ftiles);
+    const int smem = kGradRows * ((a.dvals ? a.dir.wwidth : 0) + 128) * (int)sizeof(T);
+    const auto kernel = vec16(a.dz, a.lddz, dtype) && vec16(a.x, a.ldx, dtype)
+                            ? spmm_grad_kernel<T, true> : spmm_grad_kernel<T, false>;
+    DIA_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<(unsigned)grid, kTileWarps * 32, smem, stream>>>(a, ftiles, nwins);
     DIA_TRY_CUDA(cudaGetLastError());
     return DIA_OK;
 }
@@ -546,58 +731,137 @@ static std::vector<Box> build_boxes(const std::vector<int2>& s)
     return boxes;
 }
 
-static std::vector<Quad> build_quads(const std::vector<int2>& s)
+/* Windows of F features: spans for the sorted offsets [k0, k1), neighbouring
+ * ones in one span where the gap is below 32 inputs; the columns they take.
+ * cols[k - k0] becomes the column that input i0 + offset of diagonal k has. */
+static int build_spans(const std::vector<int2>& s, size_t k0, size_t k1, int F,
+                       std::vector<InputSpan>& spans, std::vector<int>& cols)
+{
+    const size_t first = spans.size();
+    long long at = 0;
+    for (size_t k = k0; k < k1; ++k) {
+        const int d = s[k].x, end = d + F;
+        if (spans.size() == first || d > spans.back().from + spans.back().len + 24) {
+            InputSpan sp{d & ~7, 0, 0, 0};
+            spans.push_back(sp);
+        }
+        spans.back().len = (end - spans.back().from + 15) / 8 * 8;   /* eight to spare */
+    }
+    for (size_t i = first; i < spans.size(); ++i) {
+        spans[i].at = (int)std::min<long long>(at, INT_MAX / 2);
+        at += spans[i].len;
+    }
+    size_t i = first;
+    for (size_t k = k0; k < k1; ++k) {
+        while (s[k].x >= spans[i].from + spans[i].len) ++i;
+        cols.push_back(spans[i].at + s[k].x - spans[i].from);
+    }
+    return (int)std::min<long long>(at, INT_MAX / 2);
+}
+
+static std::vector<Quad> build_quads(const std::vector<int2>& s, const std::vector<int>& cols)
 {
     std::vector<Quad> quads;
-    for (const int2& o : s) {
-        const int base = o.x & ~3;   /* floor to a multiple of four */
+    for (size_t k = 0; k < s.size(); ++k) {
+        const int base = s[k].x & ~3;   /* floor to a multiple of four */
         if (quads.empty() || quads.back().base != base) {
             Quad q;
             std::memset(&q, 0, sizeof(q));
             q.base = base;
             q.k[0] = q.k[1] = q.k[2] = q.k[3] = -1;
+            q.col = cols[k] - (s[k].x - base);   /* spans begin at multiples of eight */
             quads.push_back(q);
         }
-        quads.back().k[o.x - base] = o.y;
+        quads.back().k[s[k].x - base] = s[k].y;
     }
     return quads;
 }
 
-/* One direction's tables appended to `blob`; offsets into it, made pointers
- * once the blob is on the device. */
-struct DirTables {
-    size_t quads, boxes, offs;
-    int nquads, nboxes;
-};
-
+/* One direction's tables appended to `blob`: `dir` with offsets into it in
+ * place of pointers, which dir_on_device makes pointers. */
 template <typename T>
-static size_t append(std::vector<char>& blob, const std::vector<T>& v)
+static const T* append(std::vector<char>& blob, const std::vector<T>& v)
 {
     const size_t at = (blob.size() + 31) / 32 * 32;
     blob.resize(at + v.size() * sizeof(T));
     if (!v.empty()) std::memcpy(blob.data() + at, v.data(), v.size() * sizeof(T));
-    return at;
+    return (const T*)at;
 }
 
-static DirTables append_dir(std::vector<char>& blob, const std::vector<int>& off)
+constexpr int kWinCols = 2304;   /* columns of a gradient window: 72 KB of eight fp32 rows */
+
+static SpmmDir append_dir(std::vector<char>& blob, const std::vector<int>& off)
 {
     const std::vector<int2> s = sorted_offsets(off);
-    const std::vector<Quad> q = build_quads(s);
     const std::vector<Box> b = build_boxes(s);
-    DirTables t;
-    t.nquads = (int)q.size();
-    t.nboxes = (int)b.size();
-    t.quads = append(blob, q);
-    t.boxes = append(blob, b);
-    t.offs = append(blob, s);
-    return t;
+    SpmmDir d{};
+    d.nboxes = (int)b.size();
+    d.boxes = append(blob, b);
+    d.offs = append(blob, s);
+    for (int shape = 0; shape < 3; ++shape) {
+        std::vector<InputSpan> spans;
+        std::vector<int> cols;
+        d.width[shape] = build_spans(s, 0, s.size(), kTileF[shape], spans, cols);
+        const std::vector<Quad> q = build_quads(s, cols);
+        d.nquads = (int)q.size();
+        d.nspans[shape] = (int)spans.size();
+        d.quads[shape] = append(blob, q);
+        d.spans[shape] = append(blob, spans);
+        d.cols[shape] = append(blob, cols);
+    }
+    /* up to 64 diagonals a window, fewer where they lie apart (two always fit) */
+    std::vector<GradWindow> wins;
+    std::vector<InputSpan> wspans;
+    std::vector<int> wcols;
+    for (size_t k0 = 0; k0 < s.size();) {
+        size_t k1 = std::min(s.size(), k0 + kTileWarps * kGradDiags);
+        std::vector<InputSpan> spans;
+        std::vector<int> cols;
+        int width = build_spans(s, k0, k1, 128, spans, cols);
+        while (width > kWinCols) {
+            k1 = k0 + (k1 - k0 + 1) / 2;
+            spans.clear();
+            cols.clear();
+            width = build_spans(s, k0, k1, 128, spans, cols);
+        }
+        GradWindow w{};
+        w.k0 = (int)k0;
+        w.k1 = (int)k1;
+        w.s0 = (int)wspans.size();
+        w.s1 = w.s0 + (int)spans.size();
+        w.cols = width;
+        wins.push_back(w);
+        wspans.insert(wspans.end(), spans.begin(), spans.end());
+        wcols.insert(wcols.end(), cols.begin(), cols.end());
+        d.wwidth = std::max(d.wwidth, width);
+        k0 = k1;
+    }
+    d.nwins = (int)wins.size();
+    d.wins = append(blob, wins);
+    d.wspans = append(blob, wspans);
+    d.wcols = append(blob, wcols);
+    return d;
 }
 
-static SpmmDir dir_on_device(const void* blob, const DirTables& t)
+template <typename T>
+static void place(const T*& p, const void* blob)
 {
-    const char* p = (const char*)blob;
-    return SpmmDir{(const Quad*)(p + t.quads), (const Box*)(p + t.boxes),
-                   (const int2*)(p + t.offs), t.nquads, t.nboxes};
+    p = (const T*)((const char*)blob + (size_t)p);
+}
+
+static SpmmDir dir_on_device(const void* blob, SpmmDir d)
+{
+    place(d.boxes, blob);
+    place(d.offs, blob);
+    for (int shape = 0; shape < 3; ++shape) {
+        place(d.quads[shape], blob);
+        place(d.spans[shape], blob);
+        place(d.cols[shape], blob);
+    }
+    place(d.wins, blob);
+    place(d.wspans, blob);
+    place(d.wcols, blob);
+    return d;
 }
 
 /* arguments both directions share; DIA_OK or the error */
@@ -703,7 +967,7 @@ extern "C" int dia_spmm_plan_create(int64_t n_rows, int64_t n_cols, int num_diag
         std::vector<int> trn(fwd.size());
         for (size_t k = 0; k < fwd.size(); ++k) trn[k] = -fwd[k];
         std::vector<char> blob;
-        const DirTables tf = append_dir(blob, fwd), tt = append_dir(blob, trn);
+        const SpmmDir tf = append_dir(blob, fwd), tt = append_dir(blob, trn);
         DiaSpmmPlan* p = new DiaSpmmPlan();
         p->n_rows = (int)n_rows;
         p->n_cols = (int)n_cols;
@@ -861,10 +1125,6 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
         a.per = g.per;
         a.slots = grad_slots(M, g.per);
         a.dir = plan->fwd;
-        if (!a.dvals) {   /* dbias alone: x is not looked at */
-            a.dir.nquads = 0;
-            a.n_cols = 0;
-        }
         const bool grad = (a.dvals || a.dbias) && stride > 0;
         /* launches overlap where each is of the tensor-core form: operator
          * packed, dz, gradient of the diagonals, dx, parts joined */

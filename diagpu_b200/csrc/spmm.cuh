@@ -18,17 +18,28 @@
 namespace dia {
 
 /* Up to four diagonals whose offsets share a multiple of four: slot s holds
- * the storage index of offset base + s, or -1. */
+ * the storage index of offset base + s, or -1.  col: where input i0 + base of
+ * a window lies (Windows). */
 struct __align__(32) Quad {
     int base;
     int k[4];
-    int pad[3];
+    int col;
+    int pad[2];
 };
 
-/* One direction of a plan.  Forward: out[i] = sum_k vals[k*stride + i] *
- * in[i + off_k].  Transposed (the gradient with respect to the input): out[j]
- * = sum_k vals[k*stride + j + o_k] * in[j + o_k] with o_k = -off_k.  Both are
- * lists of offsets o_k; only the weight's address differs. */
+/* The inputs that a tile of outputs i0 .. i0+F-1 reads through diagonals
+ * [k0, k1) of the sorted list, side by side in shared memory: spans [k0, k1)
+ * of the span table, `cols` columns in all.  A span holds inputs i0 + from ..
+ * i0 + from + len - 1 from column `at` on; from, len and at are multiples of
+ * eight, and at least eight columns follow the last input that is read. */
+struct __align__(16) InputSpan {
+    int from, len, at, pad;
+};
+struct __align__(16) GradWindow {
+    int k0, k1, s0, s1;
+    int cols, pad[3];
+};
+
 /* A tile of 128 outputs from i0 reads, for diagonal d, inputs i0+d ..
  * i0+d+127.  Boxes are the 64-wide pieces of input, disjoint and in ascending
  * order, that cover all of these: inputs i0+col .. i0+col+63, col a multiple
@@ -40,11 +51,23 @@ struct __align__(16) Box {
     int pad;
 };
 
+constexpr int kTileF[3] = {256, 512, 1024};   /* feature tiles of spmm_tile_kernel */
+
 struct SpmmDir {
-    const Quad* quads;   /* device */
     const Box* boxes;    /* device */
     const int2* offs;    /* device: (offset, storage index), ascending */
-    int nquads, nboxes;
+    int nboxes;
+    /* CUDA-core form: per feature tile one window over all diagonals, its
+     * spans, and the column of each diagonal and of each quad */
+    const Quad* quads[3];
+    const InputSpan* spans[3];
+    const int* cols[3];
+    int nquads, nspans[3], width[3];
+    /* gradient of the diagonals, 128 features: windows over groups of diagonals */
+    const GradWindow* wins;
+    const InputSpan* wspans;
+    const int* wcols;
+    int nwins, wwidth, wdiags;
 };
 
 }  // namespace dia
@@ -331,18 +354,18 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v)
     return __float2bfloat16_rn(v);
 }
 
-/* four consecutive elements, p aligned to four elements */
+/* four consecutive elements, p aligned to four elements (global or shared) */
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p);
 template <>
 __device__ __forceinline__ float4 load4<float>(const float* p)
 {
-    return __ldg((const float4*)p);
+    return *(const float4*)p;
 }
 template <>
 __device__ __forceinline__ float4 load4<__half>(const __half* p)
 {
-    const uint2 u = __ldg((const uint2*)p);
+    const uint2 u = *(const uint2*)p;
     const float2 a = __half22float2(*(const __half2*)&u.x);
     const float2 b = __half22float2(*(const __half2*)&u.y);
     return make_float4(a.x, a.y, b.x, b.y);
@@ -350,7 +373,7 @@ __device__ __forceinline__ float4 load4<__half>(const __half* p)
 template <>
 __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p)
 {
-    const uint2 u = __ldg((const uint2*)p);
+    const uint2 u = *(const uint2*)p;
     return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
                        __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
 }
