@@ -20,6 +20,7 @@ there: its products take one vector.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from dataclasses import dataclass
 
@@ -746,7 +747,7 @@ class SpmmPlan:
 
     @property
     def K(self):
-        return len(self.offsets)
+        return self.offsets.shape[0]
 
     def __del__(self):
         if getattr(self, "_h", None) and self._h.value and _lib is not None:
@@ -761,73 +762,93 @@ def _spmm_block(who, name, t, plan, dtype, rows, width):
     if t.dtype != dtype or t.device != plan.device or t.dim() != 2:
         raise DiaError(DIA_ERR_INVALID, f"{who}: {name} must be a 2-D {dtype} tensor on "
                                         f"{plan.device}")
-    if tuple(t.shape) != (rows, width):
+    if t.shape != (rows, width):
         raise DiaError(DIA_ERR_INVALID,
                        f"{who}: {name} has shape {tuple(t.shape)}, not {(rows, width)}")
-    if width > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if step != 1 and width > 1:
         raise DiaError(DIA_ERR_INVALID, f"{who}: features of {name} must be adjacent in memory")
-    return C.c_void_p(t.data_ptr()), t.stride(0) if rows > 1 else width
+    return t.data_ptr(), ld if rows > 1 else width
 
 
 def _spmm_operator(who, plan, vals, x, seg):
     """(dtype code, number of experts, stride) after checking x, vals and seg."""
-    if x.dtype not in _SPMM_TYPES:
+    code = _SPMM_TYPES.get(x.dtype)
+    if code is None:
         raise DiaError(DIA_ERR_INVALID, f"{who}: {x.dtype} is not float32, float16 or bfloat16")
-    want = 2 if seg is None else 3
-    if vals.dim() != want or vals.shape[-2] != plan.K:
+    shape = vals.shape
+    if len(shape) != (2 if seg is None else 3) or shape[-2] != plan.K:
         raise DiaError(DIA_ERR_INVALID, f"{who}: vals must be "
                        + ("[K, stride]" if seg is None else "[experts, K, stride]"))
     if vals.dtype != x.dtype or vals.device != plan.device or not vals.is_contiguous():
         raise DiaError(DIA_ERR_INVALID,
                        f"{who}: vals must be a contiguous {x.dtype} tensor on {plan.device}")
-    E = 1
-    if seg is not None:
-        E = vals.shape[0]
-        if (seg.dtype != torch.int64 or seg.device != plan.device or not seg.is_contiguous()
-                or tuple(seg.shape) != (E + 1,)):
-            raise DiaError(DIA_ERR_INVALID, f"{who}: seg must be a contiguous int64 tensor of "
-                                            f"{E + 1} elements on {plan.device}")
-    return _SPMM_TYPES[x.dtype], E, vals.shape[-1]
+    if seg is None:
+        return code, 1, shape[1]
+    E = shape[0]
+    if (seg.dtype != torch.int64 or seg.device != plan.device or not seg.is_contiguous()
+            or seg.shape != (E + 1,)):
+        raise DiaError(DIA_ERR_INVALID, f"{who}: seg must be a contiguous int64 tensor of "
+                                        f"{E + 1} elements on {plan.device}")
+    return code, E, shape[2]
 
 
 def _spmm_vector(who, name, t, plan, dtype, shape):
     if t is None:
         return None
-    if (t.dtype != dtype or t.device != plan.device or tuple(t.shape) != shape
-            or not t.is_contiguous()):
+    if t.dtype != dtype or t.device != plan.device or t.shape != shape or not t.is_contiguous():
         raise DiaError(DIA_ERR_INVALID, f"{who}: {name} must be a contiguous {dtype} tensor of "
                                         f"shape {shape} on {plan.device}")
-    return C.c_void_p(t.data_ptr())
+    return t.data_ptr()
 
 
 def _spmm_act(who, act):
-    if act not in _SPMM_ACTS:
+    code = _SPMM_ACTS.get(act)
+    if code is None:
         raise DiaError(DIA_ERR_INVALID, f"{who}: act must be one of {sorted(_SPMM_ACTS)}")
-    return _SPMM_ACTS[act]
+    return code
 
 
-def _spmm_work(who, work, need, plan):
-    """(pointer, bytes, buffer made here or None)"""
+def _spmm_new(made, plan, shape, dtype):
+    made.append(torch.empty(shape, dtype=dtype, device=plan.device))
+    return made[-1]
+
+
+def _spmm_work(who, made, work, need, plan):
+    """(pointer, bytes) of the workspace, made here if need be."""
     if work is None:
         if need <= 0:
-            return None, 0, None
-        made = torch.empty(need, dtype=torch.uint8, device=plan.device)
-        return C.c_void_p(made.data_ptr()), need, made
+            return None, 0
+        return _spmm_new(made, plan, (need,), torch.uint8).data_ptr(), need
     if work.dtype != torch.uint8 or work.device != plan.device or not work.is_contiguous():
         raise DiaError(DIA_ERR_INVALID, f"{who}: work must be a contiguous uint8 tensor on "
                                         f"{plan.device}")
-    return C.c_void_p(work.data_ptr()), work.numel(), None
+    return work.data_ptr(), work.numel()
 
 
-def _spmm_made(stream, *made):
-    """Tensors allocated here and used on a stream that is not the current one
-    stay allocated until that stream has passed this point."""
-    if stream is not None:
-        for t in made:
-            if t is not None:
-                t.record_stream(stream)
+def _spmm_stream(plan, stream, made):
+    """The raw stream of a call.  Tensors that the call allocated come from the
+    current stream: on another one they stay allocated until it has passed the
+    call."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(plan.device.index)
+    for t in made:
+        t.record_stream(stream)
+    return stream.cuda_stream
 
 
+def _on_device(f):
+    """f(plan, ...) with the plan's device as the current one."""
+    @functools.wraps(f)
+    def call(plan, *args, **kwargs):
+        if plan.device.index is None or torch.cuda.current_device() == plan.device.index:
+            return f(plan, *args, **kwargs)
+        with torch.cuda.device(plan.device):
+            return f(plan, *args, **kwargs)
+    return call
+
+
+@_on_device
 def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=None,
          save_z=False, out=None, z=None, work=None, stream=None):
     """act(x A^T + bias) + residual for a block x [M, n_cols] of vectors, one
@@ -840,29 +861,30 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
     "silu", "gelu", "gelu_tanh".  Returns out [M, n_rows], or (out, z) with
     save_z or a given z: the pre-activation that spmm_backward takes.  work:
     uint8 buffer of spmm_workspace bytes, for callers that allocate nothing."""
-    who = "spmm"
+    who, made = "spmm", []
     code = _spmm_act(who, act)
     dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
-    M, n = x.shape[0], plan.n_rows
-    xp, ldx = _spmm_block(who, "x", x, plan, x.dtype, M, plan.n_cols)
-    bp = _spmm_vector(who, "bias", bias, plan, x.dtype, (n,) if seg is None else (E, n))
-    rp, ldr = _spmm_block(who, "residual", residual, plan, x.dtype, M, n)
-    new_out, new_z = out is None, z is None and save_z
-    with torch.cuda.device(plan.device):
-        if new_out:
-            out = torch.empty((M, n), dtype=x.dtype, device=plan.device)
-        if new_z:
-            z = torch.empty((M, n), dtype=x.dtype, device=plan.device)
-        yp, ldy = _spmm_block(who, "out", out, plan, x.dtype, M, n)
-        zp, ldz = _spmm_block(who, "z", z, plan, x.dtype, M, n)
-        wp, wbytes, made = _spmm_work(who, work, lib().dia_spmm_workspace(plan._h, dt, M, E), plan)
-        _spmm_made(stream, out if new_out else None, z if new_z else None, made)
-        check(lib().dia_spmm(plan._h, dt, M, E, _dptr(seg), xp, ldx, C.c_void_p(vals.data_ptr()),
-                             stride, bp, code, rp, ldr, zp, ldz, yp, ldy, wp, wbytes,
-                             _stream(stream)))
-    return (out, z) if z is not None else out
+    t, M, n = x.dtype, x.shape[0], plan.n_rows
+    xp, ldx = _spmm_block(who, "x", x, plan, t, M, plan.n_cols)
+    bp = _spmm_vector(who, "bias", bias, plan, t, (n,) if seg is None else (E, n))
+    rp, ldr = _spmm_block(who, "residual", residual, plan, t, M, n)
+    if out is None:
+        out = _spmm_new(made, plan, (M, n), t)
+    yp, ldy = _spmm_block(who, "out", out, plan, t, M, n)
+    if z is None and save_z:
+        z = _spmm_new(made, plan, (M, n), t)
+    zp, ldz = _spmm_block(who, "z", z, plan, t, M, n)
+    L = lib()
+    wp, wbytes = _spmm_work(who, made, work, L.dia_spmm_workspace(plan._h, dt, M, E), plan)
+    rc = L.dia_spmm(plan._h, dt, M, E, None if seg is None else seg.data_ptr(), xp, ldx,
+                    vals.data_ptr(), stride, bp, code, rp, ldr, zp, ldz, yp, ldy, wp, wbytes,
+                    _spmm_stream(plan, stream, made))
+    if rc:
+        check(rc)
+    return out if z is None else (out, z)
 
 
+@_on_device
 def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, bias_grad=False,
                   dx=None, dvals=None, dbias=None, work=None, stream=None):
     """Gradients (dx, dvals, dbias) of spmm for dy, the gradient of its result
@@ -870,36 +892,33 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
     wanted for act "none".  dvals has the shape of vals, with zeros outside the
     matrix; dbias is None unless bias_grad or given.  work: uint8 buffer of
     spmm_backward_workspace bytes, for callers that allocate nothing."""
-    who = "spmm_backward"
+    who, made = "spmm_backward", []
     code = _spmm_act(who, act)
     dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
-    M, n = x.shape[0], plan.n_rows
-    xp, ldx = _spmm_block(who, "x", x, plan, x.dtype, M, plan.n_cols)
+    t, M, n = x.dtype, x.shape[0], plan.n_rows
+    xp, ldx = _spmm_block(who, "x", x, plan, t, M, plan.n_cols)
     if dy is None or (code and z is None):
         raise DiaError(DIA_ERR_INVALID, f"{who}: dy, and z for an activation, must be given")
-    gp, lddy = _spmm_block(who, "dy", dy, plan, x.dtype, M, n)
-    zp, ldz = _spmm_block(who, "z", z, plan, x.dtype, M, n) if code else (None, n)
+    gp, lddy = _spmm_block(who, "dy", dy, plan, t, M, n)
+    zp, ldz = _spmm_block(who, "z", z, plan, t, M, n) if code else (None, n)
     bshape = (n,) if seg is None else (E, n)
-    with torch.cuda.device(plan.device):
-        made = []
-
-        def new(shape, dtype=x.dtype):
-            made.append(torch.empty(shape, dtype=dtype, device=plan.device))
-            return made[-1]
-
-        dx = new((M, plan.n_cols)) if dx is None else dx
-        dvals = new(tuple(vals.shape)) if dvals is None else dvals
-        if dbias is None and bias_grad:
-            dbias = new(bshape)
-        wp, wbytes, wmade = _spmm_work(who, work, spmm_backward_workspace(plan, vals, M, act), plan)
-        made.append(wmade)
-        dxp, lddx = _spmm_block(who, "dx", dx, plan, x.dtype, M, plan.n_cols)
-        dvp = _spmm_vector(who, "dvals", dvals, plan, x.dtype, tuple(vals.shape))
-        dbp = _spmm_vector(who, "dbias", dbias, plan, x.dtype, bshape)
-        _spmm_made(stream, *made)
-        check(lib().dia_spmm_backward(plan._h, dt, M, E, _dptr(seg), xp, ldx,
-                                      C.c_void_p(vals.data_ptr()), stride, gp, lddy, code, zp,
-                                      ldz, dxp, lddx, dvp, dbp, wp, wbytes, _stream(stream)))
+    if dx is None:
+        dx = _spmm_new(made, plan, (M, plan.n_cols), t)
+    if dvals is None:
+        dvals = _spmm_new(made, plan, vals.shape, t)
+    if dbias is None and bias_grad:
+        dbias = _spmm_new(made, plan, bshape, t)
+    dxp, lddx = _spmm_block(who, "dx", dx, plan, t, M, plan.n_cols)
+    dvp = _spmm_vector(who, "dvals", dvals, plan, t, vals.shape)
+    dbp = _spmm_vector(who, "dbias", dbias, plan, t, bshape)
+    L = lib()
+    need = L.dia_spmm_backward_workspace(plan._h, dt, M, E, stride, code)
+    wp, wbytes = _spmm_work(who, made, work, need, plan)
+    rc = L.dia_spmm_backward(plan._h, dt, M, E, None if seg is None else seg.data_ptr(), xp, ldx,
+                             vals.data_ptr(), stride, gp, lddy, code, zp, ldz, dxp, lddx, dvp,
+                             dbp, wp, wbytes, _spmm_stream(plan, stream, made))
+    if rc:
+        check(rc)
     return dx, dvals, dbias
 
 

@@ -133,31 +133,38 @@ spmm_few_kernel(const __grid_constant__ ProdArgs a, int ks, int ftiles, long lon
  * conflicts at any offset.  Shared memory's bandwidth bounds both. */
 constexpr int kTileWarps = 8;
 constexpr int kTileRows = 8;    /* rows of a warp */
+constexpr int kTileSmem = 112 * 1024;   /* two CTAs an SM */
 
-/* `rows` rows of the spans' inputs to shared memory, zero outside the block;
- * pitch in elements */
+/* `rows` rows of the spans' inputs to shared memory, zero outside the block
+ * and for rows from nt on; pitch in elements; a warp takes a row */
 template <typename T, bool VEC>
-__device__ __forceinline__ void stage_spans(T* dst, int pitch, const InputSpan* spans, int s0, int s1,
-                                            const T* in, long long ld, int i0, int n_in, int rows,
-                                            int nt, int tid, int threads)
+__device__ __forceinline__ void stage_spans(T* dst, int pitch, const InputSpan* spans, int s0,
+                                            int s1, const T* in, long long ld, int i0, int n_in,
+                                            int rows, int nt)
 {
     constexpr int V = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31;
     for (int s = s0; s < s1; ++s) {
-        const InputSpan sp = spans[s];
-        const int per = sp.len / V;
-        for (int o = tid; o < per * rows; o += threads) {
-            const int t = o / per, c = (o - t * per) * V;
-            T* d = dst + t * pitch + sp.at + c;
-            const int j = i0 + sp.from + c;
-            if (VEC && t < nt && j >= 0 && j + V <= n_in) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                             ::"r"((uint32_t)__cvta_generic_to_shared(d)), "l"(in + t * ld + j)
-                             : "memory");
-            } else {
+        const int4 sp = __ldg((const int4*)(spans + s));   /* from, len, at */
+        const int j0 = i0 + sp.x;
+        for (int t = threadIdx.x >> 5; t < rows; t += kTileWarps) {
+            T* d = dst + t * pitch + sp.z;
+            const T* p = in + t * ld + j0;
+            const int n = t < nt ? n_in : INT_MIN;     /* no input of the row is read */
+#pragma unroll 4
+            for (int c = lane * V; c < sp.y; c += 32 * V) {
+                if (VEC && j0 + c >= 0 && j0 + c + V <= n) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                 ::"r"((uint32_t)__cvta_generic_to_shared(d + c)), "l"(p + c)
+                                 : "memory");
+                } else {
+                    T v[V];
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    d[v] = t < nt && (unsigned)(j + v) < (unsigned)n_in ? in[t * ld + j + v]
-                                                                        : from_f<T>(0.0f);
+                    for (int u = 0; u < V; ++u)
+                        v[u] = j0 + c + u >= 0 && j0 + c + u < n ? p[c + u] : from_f<T>(0.0f);
+#pragma unroll
+                    for (int u = 0; u < V; ++u) d[c + u] = v[u];
+                }
             }
         }
     }
@@ -180,8 +187,7 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
     if (rg.e < 0) return;   /* whole CTA */
     const int nt = rg.r1 - rg.r0, pitch = a.dir.width[shape];
     stage_spans<T, VEC>(xs, pitch, a.dir.spans[shape], 0, a.dir.nspans[shape],
-                        (const T*)a.in + rg.r0 * a.ldi, a.ldi, i0, a.n_in, rows, nt, tid,
-                        kTileWarps * 32);
+                        (const T*)a.in + rg.r0 * a.ldi, a.ldi, i0, a.n_in, rows, nt);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     const int t0 = warp / wf * kTileRows, f0 = warp % wf * 128;
@@ -298,15 +304,16 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
 /* ------------------------------------------------- gradient of the diagonals
  *
  * A CTA takes 128 features, one window of diagonals (at most 64) and one part
- * of an expert's rows, eight rows at a time by way of shared memory; a warp
- * keeps the sums of its eight diagonals at its lanes' four features.  Sums of
- * an expert with one part go out at once, others to `part`. */
-constexpr int kGradRows = 8;
-constexpr int kGradDiags = 8;   /* diagonals of a warp */
+ * of an expert's rows, `rows` of them at a time by way of shared memory, the
+ * next ones on their way meanwhile; a warp keeps the sums of its eight
+ * diagonals at its lanes' four features.  Sums of an expert with one part go
+ * out at once, others to `part`. */
+constexpr int kGradDiags = 8;             /* diagonals of a warp */
+constexpr int kGradSmem = 160 * 1024;     /* two buffers of at least eight rows */
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, int ND>
 __global__ void __launch_bounds__(kTileWarps * 32)
-spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins)
+spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins, int rows)
 {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -318,53 +325,64 @@ spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins)
     GradWindow win{};
     if (diags) win = a.dir.wins[wi];
     const int pitch = diags ? a.dir.wwidth : 0;
-    T* xs = (T*)smem_raw;
-    T* ds = xs + kGradRows * pitch;                  /* [row][128] */
-    const InputSpan dspan{0, 128, 0, 0};
+    const int buf = rows * (pitch + 128);            /* x, then dz [row][128] */
     const int per = (win.k1 - win.k0 + kTileWarps - 1) / kTileWarps;
     const int k0 = win.k0 + warp * per, nk = max(0, min(per, win.k1 - k0));
-    int col[kGradDiags];
+    /* a warp with fewer than ND repeats its last (or column 0) and drops it */
+    int col[ND];
 #pragma unroll
-    for (int u = 0; u < kGradDiags; ++u) col[u] = u < nk ? a.dir.wcols[k0 + u] + lane : 0;
+    for (int u = 0; u < ND; ++u)
+        col[u] = (nk > 0 ? a.dir.wcols[k0 + min(u, nk - 1)] : 0) + lane;
     const bool bias = a.dbias && wi == 0 && warp == 0;
-    float acc[kGradDiags][4], sb[4] = {0, 0, 0, 0};
+    float acc[ND][4], sb[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int u = 0; u < kGradDiags; ++u)
+    for (int u = 0; u < ND; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[u][r] = 0.0f;
     if (f0 < a.n_rows) {
-        for (int t0 = rg.r0; t0 < rg.r1; t0 += kGradRows) {
-            const int nt = min(rg.r1 - t0, kGradRows);
+        auto fetch = [&](int t0, int which) {
+            const int nt = min(rg.r1 - t0, rows);
+            T* xs = (T*)smem_raw + which * buf;
+            if (nt > 0) {
+                if (diags)
+                    stage_spans<T, VEC>(xs, pitch, a.dir.wspans, win.s0, win.s1,
+                                        (const T*)a.x + t0 * a.ldx, a.ldx, f0, a.n_cols, nt, nt);
+                stage_spans<T, VEC>(xs + rows * pitch, 128, a.dir.tile_span, 0, 1,
+                                    (const T*)a.dz + t0 * a.lddz, a.lddz, f0, a.n_rows, nt, nt);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int which = 0;
+        fetch(rg.r0, 0);
+        for (int t0 = rg.r0; t0 < rg.r1; t0 += rows, which ^= 1) {
+            const int nt = min(rg.r1 - t0, rows);
+            fetch(t0 + rows, which ^ 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncthreads();
-            if (diags)
-                stage_spans<T, VEC>(xs, pitch, a.dir.wspans, win.s0, win.s1,
-                                    (const T*)a.x + t0 * a.ldx, a.ldx, f0, a.n_cols, kGradRows, nt,
-                                    tid, kTileWarps * 32);
-            stage_spans<T, VEC>(ds, 128, &dspan, 0, 1, (const T*)a.dz + t0 * a.lddz, a.lddz, f0,
-                                a.n_rows, kGradRows, nt, tid, kTileWarps * 32);
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            __syncthreads();
-#pragma unroll 2
-            for (int t = 0; t < kGradRows; ++t) {
-                float d[4];
+            const T* xs = (const T*)smem_raw + which * buf;
+            const T* ds = xs + rows * pitch;
+            if (nk > 0 || bias) {
+#pragma unroll 4
+                for (int t = 0; t < nt; ++t) {
+                    float d[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) d[r] = to_f(ds[t * 128 + lane + 32 * r]);
+                    for (int r = 0; r < 4; ++r) d[r] = to_f(ds[t * 128 + lane + 32 * r]);
 #pragma unroll
-                for (int u = 0; u < kGradDiags; ++u)
-                    if (u < nk)
+                    for (int u = 0; u < ND; ++u)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             acc[u][r] = fmaf(d[r], to_f(xs[t * pitch + col[u] + 32 * r]), acc[u][r]);
-                if (bias)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) sb[r] += d[r];
+                }
             }
+            __syncthreads();   /* the buffer is filled again */
         }
     }
     const bool parts = rg.nparts > 1;
     float* part = a.part + (long long)(rg.slot + rg.part) * (a.K + 1) * a.stride;
 #pragma unroll
-    for (int u = 0; u < kGradDiags; ++u) {
+    for (int u = 0; u < ND; ++u) {
         if (u >= nk) break;
         const int2 o = a.dir.offs[k0 + u];
 #pragma unroll
@@ -535,9 +553,9 @@ static int launch_few(const ProdArgs& a, cudaStream_t stream)
 {
     const int ftiles = (a.n_out + 31) / 32;
     const long long ngroups = a.seg ? a.M / TT + std::min(a.E, a.M) : (a.M + TT - 1) / TT;
-    /* warps that share a tile: until every SM has 16, or a warp four diagonals */
+    /* warps that share a tile: until every SM has 32, or a warp four diagonals */
     int ks = 1;
-    while (ks < kFewWarps && (long long)ftiles * ngroups * ks < 16ll * num_sms() && a.K > 4 * ks)
+    while (ks < kFewWarps && (long long)ftiles * ngroups * ks < 32ll * num_sms() && a.K > 4 * ks)
         ks *= 2;
     const int fper = kFewWarps / ks;
     const long long grid = ngroups * ((ftiles + fper - 1) / fper);
@@ -560,14 +578,13 @@ static int launch_tile_as(const ProdArgs& a, int shape, int smem, cudaStream_t s
         return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: block too large");
     const bool rows_first = (long long)a.M * a.n_in < a.stride * a.K;
     const auto kernel = spmm_tile_kernel<T, TRANS, VEC, QUADS>;
-    DIA_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static SmemRecord most;
+    DIA_TRY_CUDA(allow_smem(kernel, kTileSmem, most));
     kernel<<<(unsigned)(ngroups * ftiles), kTileWarps * 32, smem, stream>>>(a, shape, ftiles,
                                                                             ngroups, rows_first);
     DIA_TRY_CUDA(cudaGetLastError());
     return DIA_OK;
 }
-
-constexpr int kTileSmem = 112 * 1024;   /* two CTAs an SM */
 
 static int tile_smem(const SpmmDir& d, int shape, size_t elem)
 {
@@ -662,7 +679,7 @@ static int grad_part_rows(const DiaSpmmPlan* p, int dtype, long long M, int E, l
     /* a few CTAs an SM */
     const long long tiles = std::max<long long>(1, (stride + 127) / 128) * std::max(1, p->fwd.nwins);
     const long long want = std::max<long long>(1, 4ll * num_sms() / tiles - (E - 1));
-    const long long per = std::max<long long>(64, (M + want - 1) / want);
+    const long long per = std::max<long long>(32, (M + want - 1) / want);
     return (int)((per + 7) / 8 * 8);
 }
 
@@ -684,11 +701,24 @@ static int launch_grad(const GradArgs& a, int dtype, cudaStream_t stream)
     const long long parts = a.seg ? a.M / a.per + a.E : std::max(1, (a.M + a.per - 1) / a.per);
     const long long grid = parts * ftiles * nwins;
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
-    const int smem = kGradRows * ((a.dvals ? a.dir.wwidth : 0) + 128) * (int)sizeof(T);
-    const auto kernel = vec16(a.dz, a.lddz, dtype) && vec16(a.x, a.ldx, dtype)
-                            ? spmm_grad_kernel<T, true> : spmm_grad_kernel<T, false>;
-    DIA_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<(unsigned)grid, kTileWarps * 32, smem, stream>>>(a, ftiles, nwins);
+    /* rows a stage: two CTAs an SM where that leaves eight or more */
+    const int row_bytes = 2 * ((a.dvals ? a.dir.wwidth : 0) + 128) * (int)sizeof(T);
+    const int rows = std::min(32, std::max(8, 100 * 1024 / row_bytes / 8 * 8));
+    const int smem = rows * row_bytes;
+    const bool vec = vec16(a.dz, a.lddz, dtype) && vec16(a.x, a.ldx, dtype);
+    const int nd = a.dvals ? (a.dir.wdiags + kTileWarps - 1) / kTileWarps : 1;
+    const int pick = nd <= 1 ? 0 : nd <= 2 ? 1 : nd <= 3 ? 2 : nd <= 5 ? 3 : 4;
+    using Kernel = void (*)(GradArgs, int, int, int);
+    static const Kernel kernels[2][5] = {
+        {spmm_grad_kernel<T, false, 1>, spmm_grad_kernel<T, false, 2>,
+         spmm_grad_kernel<T, false, 3>, spmm_grad_kernel<T, false, 5>,
+         spmm_grad_kernel<T, false, 8>},
+        {spmm_grad_kernel<T, true, 1>, spmm_grad_kernel<T, true, 2>, spmm_grad_kernel<T, true, 3>,
+         spmm_grad_kernel<T, true, 5>, spmm_grad_kernel<T, true, 8>}};
+    const Kernel kernel = kernels[vec][pick];
+    static SmemRecord most[2][5];
+    DIA_TRY_CUDA(allow_smem(kernel, kGradSmem, most[vec][pick]));
+    kernel<<<(unsigned)grid, kTileWarps * 32, smem, stream>>>(a, ftiles, nwins, rows);
     DIA_TRY_CUDA(cudaGetLastError());
     return DIA_OK;
 }
@@ -834,9 +864,11 @@ static SpmmDir append_dir(std::vector<char>& blob, const std::vector<int>& off)
         wspans.insert(wspans.end(), spans.begin(), spans.end());
         wcols.insert(wcols.end(), cols.begin(), cols.end());
         d.wwidth = std::max(d.wwidth, width);
+        d.wdiags = std::max(d.wdiags, (int)(k1 - k0));
         k0 = k1;
     }
     d.nwins = (int)wins.size();
+    d.tile_span = append(blob, std::vector<InputSpan>{InputSpan{0, 128, 0, 0}});
     d.wins = append(blob, wins);
     d.wspans = append(blob, wspans);
     d.wcols = append(blob, wcols);
@@ -858,6 +890,7 @@ static SpmmDir dir_on_device(const void* blob, SpmmDir d)
         place(d.spans[shape], blob);
         place(d.cols[shape], blob);
     }
+    place(d.tile_span, blob);
     place(d.wins, blob);
     place(d.wspans, blob);
     place(d.wcols, blob);

@@ -11,6 +11,7 @@
 #include <math_constants.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <vector>
 
 #include "../../include/diagpu_b200.h"
@@ -66,6 +67,7 @@ struct SpmmDir {
     /* gradient of the diagonals, 128 features: windows over groups of diagonals */
     const GradWindow* wins;
     const InputSpan* wspans;
+    const InputSpan* tile_span;   /* the tile's own 128 features */
     const int* wcols;
     int nwins, wwidth, wdiags;
 };
@@ -121,14 +123,14 @@ __device__ __forceinline__ RowGroup row_group(const long long* seg, int E, int M
         return r;
     }
     const int lane = threadIdx.x & 31;
-    int slot0 = 0;
+    int slot0 = 0, nlo = 0, nhi = 0;
+    if (lane < E) expert_rows(seg, lane, M, nlo, nhi);
     for (int e0 = 0; e0 < E; e0 += 32) {
         const int e = e0 + lane;
-        int lo = 0, hi = 0, cnt = 0;
-        if (e < E) {
-            expert_rows(seg, e, M, lo, hi);
-            cnt = max((hi - lo + per - 1) / per, empties ? 1 : 0);
-        }
+        int lo = nlo, hi = nhi, cnt = 0;
+        /* the next experts' rows are on their way while these are counted */
+        if (e + 32 < E) expert_rows(seg, e + 32, M, nlo, nhi);
+        if (e < E) cnt = max((hi - lo + per - 1) / per, empties ? 1 : 0);
         int inc = cnt, sl = cnt > 1 ? cnt : 0;
         int sinc = sl;
 #pragma unroll
@@ -429,6 +431,26 @@ __device__ __forceinline__ void dependency_wait()
 __device__ __forceinline__ void dependents_begin()
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+/* Allows a kernel `smem` bytes of dynamic shared memory (always the same) on
+ * the current device; asks the driver once (`most`: the kernel's own record,
+ * one place a device). */
+struct SmemRecord {
+    std::atomic<int> bytes[64];
+};
+
+template <typename K>
+static cudaError_t allow_smem(K kernel, int smem, SmemRecord& most)
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::atomic<int>* rec = dev >= 0 && dev < 64 ? &most.bytes[dev] : nullptr;
+    if (rec && rec->load(std::memory_order_relaxed) >= smem) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && rec) rec->store(smem, std::memory_order_relaxed);
+    return e;
 }
 
 template <typename... P, typename... A>

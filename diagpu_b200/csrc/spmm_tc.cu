@@ -1104,8 +1104,8 @@ static int launch_tc(const CUtensorMap& map, const ProdArgs& a_, int K, cudaStre
     a.groups = (int)std::min<long long>(num_sms() / nfb, tiles);
     if (a.groups * nfb < std::min<long long>(items, num_sms() * 3 / 4)) a.groups = 0;
     if (a.groups > 0) grid = a.groups * nfb;
-    DIA_TRY_CUDA(cudaFuncSetAttribute(spmm_tc_kernel<T, TRANS, ACT>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem));
+    static SmemRecord most;
+    DIA_TRY_CUDA(allow_smem(spmm_tc_kernel<T, TRANS, ACT>, kTcSmem, most));
     DIA_TRY_CUDA(launch_dependent(spmm_tc_kernel<T, TRANS, ACT>, grid, kTcWarps * 32, kTcSmem,
                                   stream, map, a, K));
     return DIA_OK;
@@ -1129,8 +1129,8 @@ int spmm_tc_pack(const ProdArgs& a, cudaStream_t stream)
     const long long boxes = spmm_tc_pack_bytes(a.n_out, a.dir.nboxes, a.E) / kBoxBytes;
     if (boxes > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: operator too large");
     const auto pack = a.trans ? spmm_pack_kernel<true> : spmm_pack_kernel<false>;
-    DIA_TRY_CUDA(cudaFuncSetAttribute(pack, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kPackSmem));
+    static SmemRecord most[2];
+    DIA_TRY_CUDA(allow_smem(pack, kPackSmem, most[a.trans]));
     pack<<<(unsigned)boxes, 256, kPackSmem, stream>>>(a);
     DIA_TRY_CUDA(cudaGetLastError());
     return DIA_OK;
@@ -1154,8 +1154,8 @@ static int launch_grad_tc(const CUtensorMap& md, const CUtensorMap& mx, const Gr
     const long long parts = a.seg ? a.M / a.per + a.E : std::max(1, (a.M + a.per - 1) / a.per);
     const long long grid = parts * nfb * nch;
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
-    DIA_TRY_CUDA(cudaFuncSetAttribute(spmm_grad_tc_kernel<T>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kGSmem));
+    static SmemRecord most;
+    DIA_TRY_CUDA(allow_smem(spmm_grad_tc_kernel<T>, kGSmem, most));
     DIA_TRY_CUDA(launch_dependent(spmm_grad_tc_kernel<T>, (int)grid, kGWarps * 32, kGSmem, stream,
                                   md, mx, a, nfb, nch));
     return DIA_OK;
