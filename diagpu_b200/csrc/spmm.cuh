@@ -52,6 +52,8 @@ struct __align__(16) Box {
     int pad;
 };
 
+constexpr int kTileWarps = 8;                   /* of spmm_tile_kernel and spmm_grad_kernel */
+constexpr int kGradDiags = 8;                   /* most diagonals of a warp of the latter */
 constexpr int kTileF[3] = {256, 512, 1024};   /* feature tiles of spmm_tile_kernel */
 
 struct SpmmDir {
@@ -469,6 +471,17 @@ static cudaError_t launch_dependent(void (*kernel)(P...), int grid, int block, i
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
+
+/* CUDA-core forms (spmm_cores.cuh); join: sums of experts with several parts,
+ * for either form of the gradient */
+template <typename T>
+struct Cores {
+    static int product(const ProdArgs& a, cudaStream_t stream);
+    static int dz(int act, const void* dy, long long lddy, const void* z, long long ldz, void* dz,
+                  long long lddz, int M, int n, bool dependent, cudaStream_t stream);
+    static int gradient(const GradArgs& a, cudaStream_t stream);
+    static int join(const GradArgs& a, cudaStream_t stream);
+};
 
 /* Tensor-core forms for 16-bit blocks (spmm_tc.cu).  spmm_tc_block: address
  * and row stride are ones TMA takes. */
