@@ -499,6 +499,11 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
         a.part = (float*)((char*)d_work + g.dz_bytes);
         a.seg = p.seg;
         a.lddz = p.ldi;
+        a.dy = d_dy;
+        a.z = d_z;
+        a.lddy = lddy;
+        a.ldz = ldz;
+        a.act = act;
         a.ldx = ldx;
         a.stride = stride;
         a.estride = p.estride;
@@ -511,18 +516,19 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
         a.slots = grad_slots(M, g.per);
         a.dir = plan->fwd;
         const bool grad = (a.dvals || a.dbias) && stride > 0;
-        /* launches overlap where each is of the tensor-core form: operator
-         * packed, dz, gradient of the diagonals, dx, parts joined */
-        const bool tc = d_dx && product_on_tc(p, dtype);
+        /* launches of the tensor-core form overlap: operator packed, dz (made
+         * by the next one where it can be), gradient of the diagonals, dx,
+         * parts joined */
+        const bool tc = d_dx && product_on_tc(p, dtype), gtc = grad && grad_on_tc(a, dtype);
+        const bool makes = gtc && made && spmm_tc_makes_dz(a);
         int r = DIA_OK;
         if (tc) r = spmm_tc_pack(p, stream);
-        if (r == DIA_OK && made)
+        if (r == DIA_OK && made && !makes)
             r = Cores<T>::dz(act, d_dy, lddy, d_z, ldz, d_work, p.ldi, p.M, p.n_in, tc, stream);
-        if (r == DIA_OK && grad) {
-            const bool gtc = grad_on_tc(a, dtype);
-            r = gtc ? spmm_tc_gradient(a, dtype, stream) : Cores<T>::gradient(a, stream);
-            p.early = tc && gtc;
-        }
+        a.early = tc && makes;        /* what it reads is older than the packing */
+        p.early = tc && gtc && !makes;   /* what it reads is older than the gradient */
+        if (r == DIA_OK && grad)
+            r = gtc ? spmm_tc_gradient(a, dtype, makes, stream) : Cores<T>::gradient(a, stream);
         if (r == DIA_OK && d_dx) r = launch_product<T>(p, dtype, stream);
         if (r == DIA_OK && grad) r = Cores<T>::join(a, stream);
         return r;

@@ -405,14 +405,17 @@ struct ProdArgs {
 
 /* dvals[k, i] = sum_t dz[t, i] x[t, i + off_k], dbias[i] = sum_t dz[t, i] */
 struct GradArgs {
-    const void* dz;
+    const void* dz;       /* act other than none: the workspace's */
+    const void* dy;
+    const void* z;
     const void* x;
     void* dvals;          /* may be null */
     void* dbias;          /* may be null */
     float* part;          /* [slots][K + 1][stride] sums of experts with several parts */
     const long long* seg;
-    long long lddz, ldx, stride, estride;
-    int M, E, n_rows, n_cols, K;
+    long long lddz, lddy, ldz, ldx, stride, estride;
+    int M, E, n_rows, n_cols, K, act;
+    bool early;           /* tensor-core form: inputs are complete when the kernel may begin */
     int per;              /* rows a part */
     long long slots;      /* parts that `part` holds */
     SpmmDir dir;          /* forward */
@@ -489,7 +492,9 @@ bool spmm_tc_block(const void* p, long long ld);
 long long spmm_tc_pack_bytes(int n_out, int nboxes, int E);
 int spmm_tc_pack(const ProdArgs& a, cudaStream_t stream);   /* an ordinary launch */
 int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream);
-int spmm_tc_gradient(const GradArgs& a, int dtype, cudaStream_t stream);
+/* make: dz is made there from dy and z (spmm_tc_makes_dz says whether it can be) */
+bool spmm_tc_makes_dz(const GradArgs& a);
+int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, cudaStream_t stream);
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear);
 
 }  // namespace dia

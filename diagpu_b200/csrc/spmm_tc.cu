@@ -149,6 +149,11 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, ui
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};"
                  ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+__device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&v)[4])
+{
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
 __device__ __forceinline__ void sts16(uint32_t addr, uint16_t v)
 {
     asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
@@ -799,17 +804,14 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
  * D = dz^T x is a 128 x 256 product over the rows of one part of an expert,
  * both operands as TMA leaves them (rows of features: MN-major).  Of D the
  * diagonals are the result; it is copied to shared memory, where a diagonal
- * is a run of consecutive features.  A box of ones beside x makes dbias.
+ * is a run of consecutive features.
  * Rows of the last stage that are not the part's are cleared in both operands
  * before the MMAs read them. */
 constexpr int kGRows = 64;                     /* rows of a stage */
 constexpr int kGBoxBytes = kGRows * 128;
 constexpr int kGBoxes = 4;                     /* boxes of inputs of a CTA */
-constexpr int kGStageBytes = (2 + kGBoxes) * kGBoxBytes;
-constexpr int kGStages = 4;
-constexpr int kGOnes = 16;                      /* columns of ones */
-constexpr int kGOnesBytes = kGOnes * 16 * 2;
-constexpr int kGSmem = kGStages * kGStageBytes + kGOnesBytes + 1024;
+constexpr int kGDz = kGBoxes * kGBoxBytes;     /* in a stage: x, then dz (or dy), then z */
+constexpr int kGSmem = 192 * 1024 + 1024;
 constexpr int kGWarps = 18;                    /* TMA, MMA, sixteen for the results */
 constexpr int kGPitch = kGBoxes * kBoxCols + 1;
 
@@ -826,18 +828,6 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t addr)
     return d;
 }
 
-/* MN-major operand without swizzle, 8 x 8 cells of 128 bytes: for the ones,
- * of which any order is the same */
-__device__ __forceinline__ uint64_t ones_desc(uint32_t addr)
-{
-    uint64_t d = 0;
-    d |= (uint64_t)((addr >> 4) & 0x3FFF);
-    d |= (uint64_t)(128 >> 4) << 16;
-    d |= (uint64_t)(256 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    return d;
-}
-
 template <typename T>
 __device__ __noinline__ float gradient_terms(const GradArgs& a, int r0, int r1, int i, int j)
 {
@@ -847,14 +837,22 @@ __device__ __noinline__ float gradient_terms(const GradArgs& a, int r0, int r1, 
     return s;
 }
 
-template <typename T>
+/* ACT other than none: dz is made here, from dy and z, by the warps that wait
+ * for the results otherwise: into the stage, for the MMAs, and to a.dz, for
+ * the product that follows. */
+template <typename T, int ACT>
 __global__ void __launch_bounds__(kGWarps * 32, 1)
-spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmX,
-                    const __grid_constant__ GradArgs a, int nfb, int nch)
+spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmZ,
+                    const __grid_constant__ CUtensorMap tmX, const __grid_constant__ GradArgs a,
+                    int nfb, int nch)
 {
+    constexpr bool MAKE = ACT != DIA_ACT_NONE;
+    constexpr int STAGES = MAKE ? 3 : 4;
+    constexpr int STAGE = (kGBoxes + (MAKE ? 4 : 2)) * kGBoxBytes;
+    static_assert(STAGES * STAGE + 1024 <= kGSmem, "stages");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    __shared__ __align__(8) unsigned long long xfull[kGStages], xempty[kGStages], done;
+    __shared__ __align__(8) unsigned long long xfull[STAGES], xempty[STAGES], xready[STAGES], done;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ Box s_box[kGBoxes];
@@ -873,29 +871,24 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     const int b0 = (int)((long long)a.dir.nboxes * ch / nch);
     const int nb = (int)((long long)a.dir.nboxes * (ch + 1) / nch) - b0;
     const bool bias = a.dbias && ch == 0;
+    const bool conv = MAKE || bias;   /* the result warps look at every stage */
     const int nst = i0 < a.n_rows ? (rg.r1 - rg.r0 + kGRows - 1) / kGRows : 0;
-    unsigned char* ones = smem + kGStages * kGStageBytes;
 
     for (int k = tid; k < min(a.K, kOffs); k += kGWarps * 32) s_offs[k] = a.dir.offs[k];
     if (tid < nb) s_box[tid] = a.dir.boxes[b0 + tid];
     if (tid == 0) {
         s_abort = 0;
-        for (int s = 0; s < kGStages; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mbar_init(xfull[s], 1);
             mbar_init(xempty[s], 1);
+            mbar_init(xready[s], kGWarps - 2);
         }
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    {
-        const uint32_t one = pack2<T>(1.0f, 1.0f);
-        for (int o = tid; o < kGOnesBytes / 16; o += kGWarps * 32)
-            sts128(smem_u32(ones) + 16 * o, one);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&s_tmem)), "r"(512));
+                     ::"r"(smem_u32(&s_tmem)), "r"(256));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -903,15 +896,16 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
     bool ok = true;
-    /* dz is the launch before this one's; the product that follows needs
-     * nothing of this kernel's and may begin */
-    dependency_wait();
+    /* dz may be the launch before this one's */
+    if (!a.early) dependency_wait();
     dependents_begin();
 
     const uint32_t st0 = smem_u32(smem), full0 = smem_u32(xfull), empty0 = smem_u32(xempty);
+    const uint32_t ready0 = smem_u32(xready);
+    float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (warp == 0) {
         const bool leader = elect_one();
-        Ring<kGStages> x;
+        Ring<STAGES> x;
         int g = 0;
         for (; g < nst; ++g, x.next()) {
             ok = mm_wait(x.bar(empty0), x.round ^ 1, abort_flag);
@@ -919,68 +913,107 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
             if (!ok) break;
             if (leader) {
                 const int r = rg.r0 + g * kGRows;
-                const uint32_t st = st0 + x.s * kGStageBytes, bar = x.bar(full0);
+                const uint32_t st = st0 + x.s * STAGE, bar = x.bar(full0);
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                             ::"r"(bar), "r"((2 + nb) * kGBoxBytes) : "memory");
-                tma_box(st, &tmD, i0, r, bar);
-                tma_box(st + kGBoxBytes, &tmD, i0 + 64, r, bar);
+                             ::"r"(bar), "r"(((MAKE ? 4 : 2) + nb) * kGBoxBytes) : "memory");
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    tma_box(st + kGDz + h * kGBoxBytes, &tmD, i0 + 64 * h, r, bar);
+                    if (MAKE)
+                        tma_box(st + kGDz + (2 + h) * kGBoxBytes, &tmZ, i0 + 64 * h, r, bar);
+                }
                 for (int c = 0; c < nb; ++c)
-                    tma_box(st + (2 + c) * kGBoxBytes, &tmX, i0 + s_box[c].col, r, bar);
+                    tma_box(st + c * kGBoxBytes, &tmX, i0 + s_box[c].col, r, bar);
             }
         }
-        for (int n = min(g, kGStages); n < kGStages; ++n) x.next();
-        for (int n = 0; n < min(g, kGStages); ++n, x.next())
+        for (int n = min(g, STAGES); n < STAGES; ++n) x.next();
+        for (int n = 0; n < min(g, STAGES); ++n, x.next())
             mm_drain(x.bar(full0), x.round ^ 1);
     } else if (warp == 1) {
         const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-        const uint32_t id0 = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) |
-                             ((uint32_t)(128 >> 4) << 24);
-        const uint32_t idx = id0 | ((uint32_t)(nb * kBoxCols >> 3) << 17);
-        const uint32_t ido = id0 | ((uint32_t)(kGOnes >> 3) << 17);
+        const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) |
+                               ((uint32_t)(128 >> 4) << 24) |
+                               ((uint32_t)(nb * kBoxCols >> 3) << 17);
         const bool leader = elect_one();
-        const uint64_t desc0 = mn_desc(st0), odesc = ones_desc(smem_u32(ones));
-        Ring<kGStages> x;
+        const uint64_t desc0 = mn_desc(st0);
+        Ring<STAGES> x;
         for (int g = 0; g < nst; ++g, x.next()) {
             const int left = rg.r1 - rg.r0 - g * kGRows;
-            ok = mm_wait(x.bar(full0), x.round, abort_flag);
+            ok = mm_wait(x.bar(full0), x.round, abort_flag) &&
+                 (!conv || mm_wait(x.bar(ready0), x.round, abort_flag));
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (left < kGRows) {
                 /* rows past the part: another expert's, or nobody's */
-                const uint32_t st = st0 + x.s * kGStageBytes;
+                const uint32_t st = st0 + x.s * STAGE;
                 const int per = (kGRows - left) * 8;
-                for (int o = lane; o < per * (2 + nb); o += 32)
+                for (int o = lane; o < per * (kGBoxes + 2); o += 32)
                     sts128(st + o / per * kGBoxBytes + left * 128 + o % per * 16, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (leader) {
-                const uint64_t ad = desc0 + x.s * (kGStageBytes >> 4);
-                const uint64_t bd = ad + (2 * kGBoxBytes >> 4);
+                const uint64_t bd = desc0 + x.s * (STAGE >> 4);
+                const uint64_t ad = bd + (kGDz >> 4);
                 if (nb > 0) {
 #pragma unroll
                     for (int kk = 0; kk < kGRows / 16; ++kk)
-                        mma_f16(tmem, ad + 128 * kk, bd + 128 * kk, idx, g > 0 || kk > 0);
-                }
-                /* a loop of its own: alternating the two accumulators' MMAs in
-                 * one unrolled loop gave undefined sums in the second (nvcc 12.9) */
-                if (bias) {
-#pragma unroll
-                    for (int kk = 0; kk < kGRows / 16; ++kk)
-                        mma_f16(tmem + 256, ad + 128 * kk, odesc, ido, g > 0 || kk > 0);
+                        mma_f16(tmem, ad + 128 * kk, bd + 128 * kk, idesc, g > 0 || kk > 0);
                 }
                 mm_commit(x.bar(empty0));
             }
         }
         if (leader) mm_commit(smem_u32(&done));
         mm_drain(smem_u32(&done), 0);
+    } else if (conv) {
+        /* a thread looks at eight features of every 32nd row */
+        const int c = tid & 15, r0 = (tid - 64) >> 4, i = i0 + 8 * c;
+        Ring<STAGES> x;
+        for (int g = 0; g < nst; ++g, x.next()) {
+            ok = mm_wait(x.bar(full0), x.round, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int left = rg.r1 - rg.r0 - g * kGRows;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = r0 + 32 * h;
+                const uint32_t at = st0 + x.s * STAGE + kGDz + (c >> 3) * kGBoxBytes + r * 128 +
+                                    (((c ^ r) & 7) << 4);
+                uint32_t d[4];
+                lds128(at, d);
+                if (MAKE) {
+                    uint32_t z[4];
+                    lds128(at + 2 * kGBoxBytes, z);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float2 v = mul2(unpack2<T>(d[q]), dact2<ACT>(unpack2<T>(z[q])));
+                        d[q] = pack2<T>(v.x, v.y);
+                    }
+                    sts128(at, d[0], d[1], d[2], d[3]);
+                    if (r < left && i < a.n_rows)
+                        *(uint4*)((T*)a.dz + (long long)(rg.r0 + g * kGRows + r) * a.lddz + i) =
+                            make_uint4(d[0], d[1], d[2], d[3]);
+                }
+                if (bias && r < left)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float2 v = unpack2<T>(d[q]);
+                        sums[2 * q] += v.x;
+                        sums[2 * q + 1] += v.y;
+                    }
+            }
+            if (MAKE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(x.bar(ready0));
+        }
     }
     /* the results: every MMA has completed (the stages are free) */
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     ok = !__syncthreads_or(!ok);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     float* tile = (float*)smem;
+    float* colsum = tile + 128 * kGPitch;   /* [32 rows][128] */
     if (ok && warp >= 2 && nst > 0) {
         const uint32_t tq = (uint32_t)(warp & 3);
         const int grp = (warp - 2) >> 2, f = 32 * (int)tq + lane;
@@ -990,28 +1023,24 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
 #pragma unroll
             for (int c = 0; c < 16; ++c) tile[f * kGPitch + c0 + c] = v[c];
         }
-        if (bias && grp == 0) {
-            const float v = tmem_ld1(tmem + ((tq * 32) << 16) + 256u);
-            const int i = i0 + f;
-            if (i < a.n_rows) {
-                if (rg.nparts > 1)
-                    a.part[((long long)(rg.slot + rg.part) * (a.K + 1) + a.K) * a.stride + i] = v;
-                else
-                    ((T*)a.dbias)[(long long)rg.e * a.n_rows + i] = from_f<T>(v);
-            }
-        }
     }
+    if (bias && warp >= 2)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) colsum[((tid - 64) >> 4) * 128 + (tid & 15) * 8 + q] = sums[q];
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
+    if (a.early) dependency_wait();
     if (!ok) return;
-    if (nst == 0 && bias && tid < 128 && i0 + tid < a.n_rows) {
+    if (bias && tid < 128 && i0 + tid < a.n_rows) {
+        float v = 0.0f;
+        for (int r = 0; r < 32; ++r) v += colsum[r * 128 + tid];
         if (rg.nparts > 1)
-            a.part[((long long)(rg.slot + rg.part) * (a.K + 1) + a.K) * a.stride + i0 + tid] = 0.0f;
+            a.part[((long long)(rg.slot + rg.part) * (a.K + 1) + a.K) * a.stride + i0 + tid] = v;
         else
-            ((T*)a.dbias)[(long long)rg.e * a.n_rows + i0 + tid] = from_f<T>(0.0f);
+            ((T*)a.dbias)[(long long)rg.e * a.n_rows + i0 + tid] = from_f<T>(v);
     }
     if (!a.dvals) return;
     /* a diagonal's 128 entries: consecutive features, consecutive columns of
@@ -1020,6 +1049,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     int col[kGBoxes];
 #pragma unroll
     for (int c = 0; c < kGBoxes; ++c) col[c] = c < nb ? s_box[c].col : INT_MAX / 2;
+    const bool adjoin = nb > 0 && s_box[nb - 1].col == col[0] + kBoxCols * (nb - 1);
     const bool parts = rg.nparts > 1;
     const int f_end = (int)min(128ll, a.stride - i0);
     float* part0 = a.part + (long long)(rg.slot + rg.part) * (a.K + 1) * a.stride + i0 + lane;
@@ -1036,10 +1066,15 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int f = 32 * s + lane, p = o.x + f;
-            int at = -1;
+            int at = p - col[0];
+            if (adjoin) {   /* the boxes are one wide one */
+                if (at >= kBoxCols * nb) at = -1;
+            } else {
+                at = -1;
 #pragma unroll
-            for (int c = 0; c < kGBoxes; ++c)
-                if ((unsigned)(p - col[c]) < (unsigned)kBoxCols) at = c * kBoxCols + p - col[c];
+                for (int c = 0; c < kGBoxes; ++c)
+                    if ((unsigned)(p - col[c]) < (unsigned)kBoxCols) at = c * kBoxCols + p - col[c];
+            }
             on[s] = at >= 0 && f < f_end;
             v[s] = on[s] && f >= in_lo && f < in_hi ? row[32 * s * kGPitch + at] : 0.0f;
             bad |= !isfinite(v[s]);
@@ -1145,30 +1180,51 @@ int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream)
                             : launch_tc_type<__nv_bfloat16>(map, a, a.K, stream);
 }
 
-template <typename T>
-static int launch_grad_tc(const CUtensorMap& md, const CUtensorMap& mx, const GradArgs& a,
-                          cudaStream_t stream)
+bool spmm_tc_makes_dz(const GradArgs& a)
 {
+    /* an operator of several shares of boxes would make dz as many times */
+    return a.act != DIA_ACT_NONE && a.dir.nboxes <= kGBoxes && spmm_tc_block(a.dy, a.lddy) &&
+           spmm_tc_block(a.z, a.ldz);
+}
+
+template <typename T, int ACT>
+static int launch_grad_tc(const GradArgs& a, int dtype, cudaStream_t stream)
+{
+    CUtensorMap md, mz, mx;
+    const bool make = ACT != DIA_ACT_NONE;
+    if (!block_map(&md, make ? a.dy : a.dz, dtype, a.n_rows, a.M, make ? a.lddy : a.lddz, kGRows) ||
+        !block_map(&mx, a.x, dtype, a.n_cols, a.M, a.ldx, kGRows) ||
+        !block_map(&mz, make ? a.z : a.dz, dtype, a.n_rows, a.M, make ? a.ldz : a.lddz, kGRows))
+        return fail(DIA_ERR_CUDA, "dia_spmm_backward: cuTensorMapEncodeTiled failed");
     const int nfb = (int)((a.stride + 127) / 128);
     const int nch = std::max(1, (a.dir.nboxes + kGBoxes - 1) / kGBoxes);
     const long long parts = a.seg ? a.M / a.per + a.E : std::max(1, (a.M + a.per - 1) / a.per);
     const long long grid = parts * nfb * nch;
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
+    const auto kernel = spmm_grad_tc_kernel<T, ACT>;
     static SmemRecord most;
-    DIA_TRY_CUDA(allow_smem(spmm_grad_tc_kernel<T>, kGSmem, most));
-    DIA_TRY_CUDA(launch_dependent(spmm_grad_tc_kernel<T>, (int)grid, kGWarps * 32, kGSmem, stream,
-                                  md, mx, a, nfb, nch));
+    DIA_TRY_CUDA(allow_smem(kernel, kGSmem, most));
+    DIA_TRY_CUDA(launch_dependent(kernel, (int)grid, kGWarps * 32, kGSmem, stream, md, mz, mx, a,
+                                  nfb, nch));
     return DIA_OK;
 }
 
-int spmm_tc_gradient(const GradArgs& a, int dtype, cudaStream_t stream)
+template <typename T>
+static int launch_grad_act(const GradArgs& a, int dtype, bool make, cudaStream_t stream)
 {
-    CUtensorMap md, mx;
-    if (!block_map(&md, a.dz, dtype, a.n_rows, a.M, a.lddz, kGRows) ||
-        !block_map(&mx, a.x, dtype, a.n_cols, a.M, a.ldx, kGRows))
-        return fail(DIA_ERR_CUDA, "dia_spmm_backward: cuTensorMapEncodeTiled failed");
-    return dtype == DIA_F16 ? launch_grad_tc<__half>(md, mx, a, stream)
-                            : launch_grad_tc<__nv_bfloat16>(md, mx, a, stream);
+    switch (make ? a.act : DIA_ACT_NONE) {
+        case DIA_ACT_RELU: return launch_grad_tc<T, DIA_ACT_RELU>(a, dtype, stream);
+        case DIA_ACT_SILU: return launch_grad_tc<T, DIA_ACT_SILU>(a, dtype, stream);
+        case DIA_ACT_GELU: return launch_grad_tc<T, DIA_ACT_GELU>(a, dtype, stream);
+        case DIA_ACT_GELU_TANH: return launch_grad_tc<T, DIA_ACT_GELU_TANH>(a, dtype, stream);
+        default: return launch_grad_tc<T, DIA_ACT_NONE>(a, dtype, stream);
+    }
+}
+
+int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, cudaStream_t stream)
+{
+    return dtype == DIA_F16 ? launch_grad_act<__half>(a, dtype, make, stream)
+                            : launch_grad_act<__nv_bfloat16>(a, dtype, make, stream);
 }
 
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear)
