@@ -415,7 +415,6 @@ struct GradArgs {
     const long long* seg;
     long long lddz, lddy, ldz, ldx, stride, estride;
     int M, E, n_rows, n_cols, K, act;
-    bool early;           /* tensor-core form: inputs are complete when the kernel may begin */
     int per;              /* rows a part */
     long long slots;      /* parts that `part` holds */
     SpmmDir dir;          /* forward */
@@ -426,8 +425,10 @@ struct GradArgs {
  * The launches of one call overlap (programmatic dependent launch): a kernel
  * may begin once every CTA of the one before has said dependents_begin() or
  * ended, and dependency_wait() returns when that one has completed.  The
- * first launch of a call is an ordinary one, and every later one waits before
- * it ends, so that its own completion means that of all before. */
+ * first launch of a call is an ordinary one: it begins when all that was on
+ * the stream has completed, so arguments in device memory may be read before
+ * any wait.  Every later one waits before it ends, so that its own completion
+ * means that of all before. */
 __device__ __forceinline__ void dependency_wait()
 {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -458,9 +459,10 @@ static cudaError_t allow_smem(K kernel, int smem, SmemRecord& most)
     return e;
 }
 
+/* dependent: the launch may overlap the one before, which is of the same call */
 template <typename... P, typename... A>
-static cudaError_t launch_dependent(void (*kernel)(P...), int grid, int block, int smem,
-                                    cudaStream_t stream, A... args)
+static cudaError_t launch(bool dependent, void (*kernel)(P...), int grid, int block, int smem,
+                          cudaStream_t stream, A... args)
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
@@ -469,9 +471,9 @@ static cudaError_t launch_dependent(void (*kernel)(P...), int grid, int block, i
     cfg.stream = stream;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
+    at.val.programmaticStreamSerializationAllowed = dependent ? 1 : 0;
     cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = dependent ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -490,11 +492,11 @@ struct Cores {
  * and row stride are ones TMA takes. */
 bool spmm_tc_block(const void* p, long long ld);
 long long spmm_tc_pack_bytes(int n_out, int nboxes, int E);
-int spmm_tc_pack(const ProdArgs& a, cudaStream_t stream);   /* an ordinary launch */
+int spmm_tc_pack(const ProdArgs& a, bool dependent, cudaStream_t stream);
 int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream);
 /* make: dz is made there from dy and z (spmm_tc_makes_dz says whether it can be) */
 bool spmm_tc_makes_dz(const GradArgs& a);
-int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, cudaStream_t stream);
+int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, bool dependent, cudaStream_t stream);
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear);
 
 }  // namespace dia

@@ -602,11 +602,8 @@ static cudaError_t launch_dz_act(const void* dy, long long lddy, const void* z, 
     const auto kernel = vec16<T>(dy, lddy) && vec16<T>(z, ldz)
                             ? spmm_dz_kernel<T, ACT, true>
                             : spmm_dz_kernel<T, ACT, false>;
-    if (dependent)
-        return launch_dependent(kernel, grid, 256, 0, stream, (const T*)dy, lddy, (const T*)z, ldz,
-                                (T*)dz, lddz, M, n);
-    kernel<<<grid, 256, 0, stream>>>((const T*)dy, lddy, (const T*)z, ldz, (T*)dz, lddz, M, n);
-    return cudaGetLastError();
+    return launch(dependent, kernel, grid, 256, 0, stream, (const T*)dy, lddy, (const T*)z, ldz,
+                  (T*)dz, lddz, M, n);
 }
 
 template <typename T>
@@ -614,11 +611,11 @@ int Cores<T>::dz(int act, const void* dy, long long lddy, const void* z, long lo
                      void* dz, long long lddz, int M, int n, bool dependent, cudaStream_t stream)
 {
     if (M == 0 || n == 0) return DIA_OK;
-    const auto launch = act == DIA_ACT_RELU   ? launch_dz_act<T, DIA_ACT_RELU>
-                        : act == DIA_ACT_SILU ? launch_dz_act<T, DIA_ACT_SILU>
-                        : act == DIA_ACT_GELU ? launch_dz_act<T, DIA_ACT_GELU>
-                                              : launch_dz_act<T, DIA_ACT_GELU_TANH>;
-    DIA_TRY_CUDA(launch(dy, lddy, z, ldz, dz, lddz, M, n, dependent, stream));
+    const auto run = act == DIA_ACT_RELU   ? launch_dz_act<T, DIA_ACT_RELU>
+                     : act == DIA_ACT_SILU ? launch_dz_act<T, DIA_ACT_SILU>
+                     : act == DIA_ACT_GELU ? launch_dz_act<T, DIA_ACT_GELU>
+                                           : launch_dz_act<T, DIA_ACT_GELU_TANH>;
+    DIA_TRY_CUDA(run(dy, lddy, z, ldz, dz, lddz, M, n, dependent, stream));
     return DIA_OK;
 }
 
@@ -659,7 +656,7 @@ int Cores<T>::join(const GradArgs& a, cudaStream_t stream)
     const int cblocks = (int)((a.stride + 511) / 512);
     const long long grid = (long long)a.E * (a.K + 1) * cblocks;
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
-    DIA_TRY_CUDA(launch_dependent(spmm_join_kernel<T>, (int)grid, 128, 0, stream, a, cblocks));
+    DIA_TRY_CUDA(launch(true, spmm_join_kernel<T>, (int)grid, 128, 0, stream, a, cblocks));
     return DIA_OK;
 }
 

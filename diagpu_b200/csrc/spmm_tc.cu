@@ -275,7 +275,10 @@ __global__ void __launch_bounds__(256) spmm_pack_kernel(const __grid_constant__ 
     if (a.seg) {
         int lo, hi;
         expert_rows(a.seg, e, a.M, lo, hi);
-        if (lo == hi) return;   /* nobody reads them */
+        if (lo == hi) {   /* nobody reads them */
+            dependency_wait();
+            return;
+        }
     }
     const Box bx = a.dir.boxes[b];
     const int nk = bx.k1 - bx.k0, i0 = fb * kTN;
@@ -319,6 +322,7 @@ __global__ void __launch_bounds__(256) spmm_pack_kernel(const __grid_constant__ 
     uint4* dst = (uint4*)((char*)a.pack + (long long)blockIdx.x * kBoxBytes);
 #pragma unroll
     for (int o = 0; o < kBoxBytes / 16; o += 256) dst[o + tid] = ((const uint4*)box)[o + tid];
+    dependency_wait();
 }
 
 /* the sum of one output's own terms, in ascending order of the offsets */
@@ -813,6 +817,7 @@ constexpr int kGBoxes = 4;                     /* boxes of inputs of a CTA */
 constexpr int kGDz = kGBoxes * kGBoxBytes;     /* in a stage: x, then dz (or dy), then z */
 constexpr int kGSmem = 192 * 1024 + 1024;
 constexpr int kGWarps = 18;                    /* TMA, MMA, sixteen for the results */
+constexpr int kGConv = (kGWarps - 2) * 16;     /* threads that look at a stage */
 constexpr int kGPitch = kGBoxes * kBoxCols + 1;
 
 /* MN-major operand with the 128-byte swizzle: groups of 64 elements kGBoxBytes
@@ -881,7 +886,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(xfull[s], 1);
             mbar_init(xempty[s], 1);
-            mbar_init(xready[s], kGWarps - 2);
+            mbar_init(xready[s], kGConv / 32);
         }
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -897,7 +902,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     const uint32_t tmem = s_tmem;
     bool ok = true;
     /* dz may be the launch before this one's */
-    if (!a.early) dependency_wait();
+    dependency_wait();
     dependents_begin();
 
     const uint32_t st0 = smem_u32(smem), full0 = smem_u32(xfull), empty0 = smem_u32(xempty);
@@ -967,45 +972,60 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         if (leader) mm_commit(smem_u32(&done));
         mm_drain(smem_u32(&done), 0);
     } else if (conv) {
-        /* a thread looks at eight features of every 32nd row */
-        const int c = tid & 15, r0 = (tid - 64) >> 4, i = i0 + 8 * c;
+        /* half of the warps take the even stages, half the odd ones, so that
+         * one half's arithmetic runs while the other waits and stores; a
+         * thread looks at eight features of every 16th row */
+        const int half = (warp - 2) / (kGConv / 32);
+        const int c = tid & 15, r0 = ((tid - 64) % kGConv) >> 4, i = i0 + 8 * c;
         Ring<STAGES> x;
-        for (int g = 0; g < nst; ++g, x.next()) {
+        if (half) x.next();
+        for (int g = half; g < nst; g += 2, x.next(), x.next()) {
             ok = mm_wait(x.bar(full0), x.round, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int left = rg.r1 - rg.r0 - g * kGRows;
+            const uint32_t at0 = st0 + x.s * STAGE + kGDz + (c >> 3) * kGBoxBytes + r0 * 128 +
+                                 (((c ^ r0) & 7) << 4);
+            uint32_t d[4][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = r0 + 32 * h;
-                const uint32_t at = st0 + x.s * STAGE + kGDz + (c >> 3) * kGBoxBytes + r * 128 +
-                                    (((c ^ r) & 7) << 4);
-                uint32_t d[4];
-                lds128(at, d);
-                if (MAKE) {
-                    uint32_t z[4];
-                    lds128(at + 2 * kGBoxBytes, z);
+            for (int p = 0; p < 4; p += 2) {
+                const uint32_t at = at0 + p * 16 * 128;
+                lds128(at, d[p]);
+                lds128(at + 16 * 128, d[p + 1]);
+                if (!MAKE) continue;
+                uint32_t z[2][4];
+                lds128(at + 2 * kGBoxBytes, z[0]);
+                lds128(at + 2 * kGBoxBytes + 16 * 128, z[1]);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float2 v = mul2(unpack2<T>(d[q]), dact2<ACT>(unpack2<T>(z[q])));
-                        d[q] = pack2<T>(v.x, v.y);
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 v =
+                            mul2(unpack2<T>(d[p + h][q]), dact2<ACT>(unpack2<T>(z[h][q])));
+                        d[p + h][q] = pack2<T>(v.x, v.y);
                     }
-                    sts128(at, d[0], d[1], d[2], d[3]);
-                    if (r < left && i < a.n_rows)
-                        *(uint4*)((T*)a.dz + (long long)(rg.r0 + g * kGRows + r) * a.lddz + i) =
-                            make_uint4(d[0], d[1], d[2], d[3]);
-                }
-                if (bias && r < left)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float2 v = unpack2<T>(d[q]);
-                        sums[2 * q] += v.x;
-                        sums[2 * q + 1] += v.y;
-                    }
+                for (int h = 0; h < 2; ++h)
+                    sts128(at + h * 16 * 128, d[p + h][0], d[p + h][1], d[p + h][2], d[p + h][3]);
             }
             if (MAKE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(x.bar(ready0));
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const int r = r0 + 16 * h;
+                if (r >= left) continue;
+                if (MAKE && i < a.n_rows)
+                    *(uint4*)((T*)a.dz + (long long)(rg.r0 + g * kGRows + r) * a.lddz + i) =
+                        make_uint4(d[h][0], d[h][1], d[h][2], d[h][3]);
+                if (bias)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float2 v = unpack2<T>(d[h][q]);
+                        sums[2 * q] += v.x;
+                        sums[2 * q + 1] += v.y;
+                    }
+            }
         }
     }
     /* the results: every MMA has completed (the stages are free) */
@@ -1032,7 +1052,6 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
-    if (a.early) dependency_wait();
     if (!ok) return;
     if (bias && tid < 128 && i0 + tid < a.n_rows) {
         float v = 0.0f;
@@ -1055,7 +1074,33 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     float* part0 = a.part + (long long)(rg.slot + rg.part) * (a.K + 1) * a.stride + i0 + lane;
     T* out0 = (T*)a.dvals + rg.e * a.estride + i0 + lane;
     const float* row = tile + lane * kGPitch;
-    for (int k = k_lo + warp; k < k_hi; k += kGWarps) {
+    const int k_first = k_lo + warp;
+    /* the usual tile: every entry of every diagonal in the matrix and here */
+    if (nch == 1 && adjoin && nst > 0 && a.K <= kOffs && i0 + 128 <= a.n_rows &&
+        i0 + s_offs[0].x >= 0 && i0 + 127 + s_offs[a.K - 1].x < a.n_cols) {
+        const float* src = row - col[0] + lane;
+        bool bad = false;
+#pragma unroll 2
+        for (int k = k_first; k < k_hi; k += kGWarps) {
+            const int2 o = s_offs[k];
+            const long long at = (long long)o.y * a.stride;
+            float v[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                v[s] = src[32 * s * (kGPitch + 1) + o.x];
+                bad |= !isfinite(v[s]);
+            }
+            if (parts) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) part0[at + 32 * s] = v[s];
+            } else {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) out0[at + 32 * s] = from_f<T>(v[s]);
+            }
+        }
+        if (!__any_sync(0xffffffffu, bad)) return;   /* else once more, below */
+    }
+    for (int k = k_first; k < k_hi; k += kGWarps) {
         const int2 o = a.K <= kOffs ? s_offs[k] : a.dir.offs[k];
         /* features whose entry lies in the matrix; outside, and in the
          * padding, there is no gradient */
@@ -1141,8 +1186,7 @@ static int launch_tc(const CUtensorMap& map, const ProdArgs& a_, int K, cudaStre
     if (a.groups > 0) grid = a.groups * nfb;
     static SmemRecord most;
     DIA_TRY_CUDA(allow_smem(spmm_tc_kernel<T, TRANS, ACT>, kTcSmem, most));
-    DIA_TRY_CUDA(launch_dependent(spmm_tc_kernel<T, TRANS, ACT>, grid, kTcWarps * 32, kTcSmem,
-                                  stream, map, a, K));
+    DIA_TRY_CUDA(launch(true, spmm_tc_kernel<T, TRANS, ACT>, grid, kTcWarps * 32, kTcSmem, stream, map, a, K));
     return DIA_OK;
 }
 
@@ -1159,15 +1203,14 @@ static int launch_tc_type(const CUtensorMap& map, const ProdArgs& a, int K, cuda
     }
 }
 
-int spmm_tc_pack(const ProdArgs& a, cudaStream_t stream)
+int spmm_tc_pack(const ProdArgs& a, bool dependent, cudaStream_t stream)
 {
     const long long boxes = spmm_tc_pack_bytes(a.n_out, a.dir.nboxes, a.E) / kBoxBytes;
     if (boxes > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: operator too large");
     const auto pack = a.trans ? spmm_pack_kernel<true> : spmm_pack_kernel<false>;
     static SmemRecord most[2];
     DIA_TRY_CUDA(allow_smem(pack, kPackSmem, most[a.trans]));
-    pack<<<(unsigned)boxes, 256, kPackSmem, stream>>>(a);
-    DIA_TRY_CUDA(cudaGetLastError());
+    DIA_TRY_CUDA(launch(dependent, pack, (int)boxes, 256, kPackSmem, stream, a));
     return DIA_OK;
 }
 
@@ -1188,7 +1231,7 @@ bool spmm_tc_makes_dz(const GradArgs& a)
 }
 
 template <typename T, int ACT>
-static int launch_grad_tc(const GradArgs& a, int dtype, cudaStream_t stream)
+static int launch_grad_tc(const GradArgs& a, int dtype, bool dependent, cudaStream_t stream)
 {
     CUtensorMap md, mz, mx;
     const bool make = ACT != DIA_ACT_NONE;
@@ -1204,27 +1247,28 @@ static int launch_grad_tc(const GradArgs& a, int dtype, cudaStream_t stream)
     const auto kernel = spmm_grad_tc_kernel<T, ACT>;
     static SmemRecord most;
     DIA_TRY_CUDA(allow_smem(kernel, kGSmem, most));
-    DIA_TRY_CUDA(launch_dependent(kernel, (int)grid, kGWarps * 32, kGSmem, stream, md, mz, mx, a,
-                                  nfb, nch));
+    DIA_TRY_CUDA(launch(dependent, kernel, (int)grid, kGWarps * 32, kGSmem, stream, md, mz, mx, a,
+                        nfb, nch));
     return DIA_OK;
 }
 
 template <typename T>
-static int launch_grad_act(const GradArgs& a, int dtype, bool make, cudaStream_t stream)
+static int launch_grad_act(const GradArgs& a, int dtype, bool make, bool dependent,
+                           cudaStream_t stream)
 {
     switch (make ? a.act : DIA_ACT_NONE) {
-        case DIA_ACT_RELU: return launch_grad_tc<T, DIA_ACT_RELU>(a, dtype, stream);
-        case DIA_ACT_SILU: return launch_grad_tc<T, DIA_ACT_SILU>(a, dtype, stream);
-        case DIA_ACT_GELU: return launch_grad_tc<T, DIA_ACT_GELU>(a, dtype, stream);
-        case DIA_ACT_GELU_TANH: return launch_grad_tc<T, DIA_ACT_GELU_TANH>(a, dtype, stream);
-        default: return launch_grad_tc<T, DIA_ACT_NONE>(a, dtype, stream);
+        case DIA_ACT_RELU: return launch_grad_tc<T, DIA_ACT_RELU>(a, dtype, dependent, stream);
+        case DIA_ACT_SILU: return launch_grad_tc<T, DIA_ACT_SILU>(a, dtype, dependent, stream);
+        case DIA_ACT_GELU: return launch_grad_tc<T, DIA_ACT_GELU>(a, dtype, dependent, stream);
+        case DIA_ACT_GELU_TANH: return launch_grad_tc<T, DIA_ACT_GELU_TANH>(a, dtype, dependent, stream);
+        default: return launch_grad_tc<T, DIA_ACT_NONE>(a, dtype, dependent, stream);
     }
 }
 
-int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, cudaStream_t stream)
+int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, bool dependent, cudaStream_t stream)
 {
-    return dtype == DIA_F16 ? launch_grad_act<__half>(a, dtype, make, stream)
-                            : launch_grad_act<__nv_bfloat16>(a, dtype, make, stream);
+    return dtype == DIA_F16 ? launch_grad_act<__half>(a, dtype, make, dependent, stream)
+                            : launch_grad_act<__nv_bfloat16>(a, dtype, make, dependent, stream);
 }
 
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear)
