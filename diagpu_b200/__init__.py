@@ -96,11 +96,11 @@ def lib():
             getattr(L, name).restype = i
         L.dia_spmm_plan_create.argtypes = [i64, i64, i, p, p]
         L.dia_spmm_plan_destroy.argtypes = [p]
-        L.dia_spmm_workspace.argtypes = [p, i, i64, i]
+        L.dia_spmm_workspace.argtypes = [p, i, i64, i, i64]
         L.dia_spmm_workspace.restype = i64
         L.dia_spmm.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i, p, i64, p, i64, p, i64, p,
                                i64, p]
-        L.dia_spmm_backward_workspace.argtypes = [p, i, i64, i, i64, i]
+        L.dia_spmm_backward_workspace.argtypes = [p, i, i64, i, i64, i64, i64, i]
         L.dia_spmm_backward_workspace.restype = i64
         L.dia_spmm_backward.argtypes = [p, i, i64, i, p, p, i64, p, i64, p, i64, i, p, i64, p,
                                         i64, p, p, p, i64, p]
@@ -809,17 +809,17 @@ def _spmm_act(who, act):
     return code
 
 
-def _spmm_new(made, plan, shape, dtype):
-    made.append(torch.empty(shape, dtype=dtype, device=plan.device))
+def _spmm_new(made, like, shape, dtype=None):
+    made.append(like.new_empty(shape, dtype=dtype))
     return made[-1]
 
 
-def _spmm_work(who, made, work, need, plan):
+def _spmm_work(who, made, work, need, plan, like):
     """(pointer, bytes) of the workspace, made here if need be."""
     if work is None:
         if need <= 0:
             return None, 0
-        return _spmm_new(made, plan, (need,), torch.uint8).data_ptr(), need
+        return _spmm_new(made, like, (need,), torch.uint8).data_ptr(), need
     if work.dtype != torch.uint8 or work.device != plan.device or not work.is_contiguous():
         raise DiaError(DIA_ERR_INVALID, f"{who}: work must be a contiguous uint8 tensor on "
                                         f"{plan.device}")
@@ -869,13 +869,14 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
     bp = _spmm_vector(who, "bias", bias, plan, t, (n,) if seg is None else (E, n))
     rp, ldr = _spmm_block(who, "residual", residual, plan, t, M, n)
     if out is None:
-        out = _spmm_new(made, plan, (M, n), t)
+        out = _spmm_new(made, x, (M, n))
     yp, ldy = _spmm_block(who, "out", out, plan, t, M, n)
     if z is None and save_z:
-        z = _spmm_new(made, plan, (M, n), t)
+        z = _spmm_new(made, x, (M, n))
     zp, ldz = _spmm_block(who, "z", z, plan, t, M, n)
     L = lib()
-    wp, wbytes = _spmm_work(who, made, work, L.dia_spmm_workspace(plan._h, dt, M, E), plan)
+    wp, wbytes = _spmm_work(who, made, work, L.dia_spmm_workspace(plan._h, dt, M, E, ldx), plan,
+                            x)
     rc = L.dia_spmm(plan._h, dt, M, E, None if seg is None else seg.data_ptr(), xp, ldx,
                     vals.data_ptr(), stride, bp, code, rp, ldr, zp, ldz, yp, ldy, wp, wbytes,
                     _spmm_stream(plan, stream, made))
@@ -903,17 +904,17 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
     zp, ldz = _spmm_block(who, "z", z, plan, t, M, n) if code else (None, n)
     bshape = (n,) if seg is None else (E, n)
     if dx is None:
-        dx = _spmm_new(made, plan, (M, plan.n_cols), t)
+        dx = _spmm_new(made, x, (M, plan.n_cols))
     if dvals is None:
-        dvals = _spmm_new(made, plan, vals.shape, t)
+        dvals = _spmm_new(made, x, vals.shape)
     if dbias is None and bias_grad:
-        dbias = _spmm_new(made, plan, bshape, t)
+        dbias = _spmm_new(made, x, bshape)
     dxp, lddx = _spmm_block(who, "dx", dx, plan, t, M, plan.n_cols)
     dvp = _spmm_vector(who, "dvals", dvals, plan, t, vals.shape)
     dbp = _spmm_vector(who, "dbias", dbias, plan, t, bshape)
     L = lib()
-    need = L.dia_spmm_backward_workspace(plan._h, dt, M, E, stride, code)
-    wp, wbytes = _spmm_work(who, made, work, need, plan)
+    need = L.dia_spmm_backward_workspace(plan._h, dt, M, E, ldx, stride, lddy, code)
+    wp, wbytes = _spmm_work(who, made, work, need, plan, x)
     rc = L.dia_spmm_backward(plan._h, dt, M, E, None if seg is None else seg.data_ptr(), xp, ldx,
                              vals.data_ptr(), stride, gp, lddy, code, zp, ldz, dxp, lddx, dvp,
                              dbp, wp, wbytes, _spmm_stream(plan, stream, made))
@@ -922,23 +923,20 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
     return dx, dvals, dbias
 
 
-def spmm_workspace(plan: SpmmPlan, vals, M):
-    """Bytes of the work buffer of spmm for a block of M vectors."""
-    ws = lib().dia_spmm_workspace(plan._h, _SPMM_TYPES[vals.dtype], int(M),
-                                  vals.shape[0] if vals.dim() == 3 else 1)
-    if ws < 0:
-        raise DiaError(DIA_ERR_INVALID, "spmm_workspace: bad size")
-    return ws
+def spmm_workspace(plan: SpmmPlan, vals, x):
+    """Bytes of the work buffer of spmm for an operator and a block like these."""
+    E = vals.shape[0] if vals.dim() == 3 else 1
+    ldx = _spmm_block("spmm_workspace", "x", x, plan, vals.dtype, x.shape[0], plan.n_cols)[1]
+    return lib().dia_spmm_workspace(plan._h, _SPMM_TYPES[vals.dtype], x.shape[0], E, ldx)
 
 
-def spmm_backward_workspace(plan: SpmmPlan, vals, M, act="none"):
-    """Bytes of the work buffer of spmm_backward for a block of M vectors."""
-    ws = lib().dia_spmm_backward_workspace(plan._h, _SPMM_TYPES[vals.dtype], int(M),
-                                           vals.shape[0] if vals.dim() == 3 else 1,
-                                           vals.shape[-1], _spmm_act("spmm_backward", act))
-    if ws < 0:
-        raise DiaError(DIA_ERR_INVALID, "spmm_backward_workspace: bad size")
-    return ws
+def spmm_backward_workspace(plan: SpmmPlan, vals, x, dy, act="none"):
+    """Bytes of the work buffer of spmm_backward for operands like these."""
+    who, E, M = "spmm_backward_workspace", vals.shape[0] if vals.dim() == 3 else 1, x.shape[0]
+    ldx = _spmm_block(who, "x", x, plan, vals.dtype, M, plan.n_cols)[1]
+    lddy = _spmm_block(who, "dy", dy, plan, vals.dtype, M, plan.n_rows)[1]
+    return lib().dia_spmm_backward_workspace(plan._h, _SPMM_TYPES[vals.dtype], M, E, ldx,
+                                             vals.shape[-1], lddy, _spmm_act(who, act))
 
 
 # ---------------------------------------------------------------- gemm_diag

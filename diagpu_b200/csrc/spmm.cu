@@ -38,7 +38,11 @@ static bool tensor_form(int dtype, long long M, int E, const SpmmDir& d)
     const int form = g_form.load(std::memory_order_relaxed);
     if (dtype == DIA_F32 || d.nboxes == 0 || form == 1) return false;
     if (form == 2) return true;
-    return M / std::max(E, 1) >= 64;
+    /* Eight rows an expert pay for packing it and for a tile's way through the
+     * kernel (129 diagonals of 4096: 11 us against 51 on CUDA cores); with many
+     * experts, whose operators are packed for few rows each, more do (64 of
+     * 1024 x 33, 16 rows each: 28 against 26; 64 rows each: 38 against 48). */
+    return M >= (long long)E * std::max(8, E / 2);
 }
 
 static size_t elem_size(int dtype) { return dtype == DIA_F32 ? 4 : 2; }
@@ -299,28 +303,41 @@ static int by_type(int dtype, F f)
 static long long align256(long long b) { return (b + 255) / 256 * 256; }
 
 /* the operator in tensor-core form */
-static long long pack_bytes(const SpmmDir& d, int dtype, int64_t M, int E, int n_out)
+static long long pack_bytes(const SpmmDir& d, int K, int dtype, int64_t M, int E, int n_out)
 {
-    return M > 0 && tensor_form(dtype, M, E, d) ? spmm_tc_pack_bytes(n_out, d.nboxes, E) : 0;
+    return M > 0 && n_out > 0 && tensor_form(dtype, M, E, d)
+               ? align256(spmm_tc_pack_bytes(d, K, n_out, M, E)) : 0;
 }
 
-/* the gradient's workspace: dz (where the activation makes one), then sums
- * of parts (where there are several), then the operator's boxes */
+/* a copy of a block whose rows are not multiples of 16 bytes apart, which the
+ * tensor-core form reads instead */
+static long long copy_bytes(const SpmmDir& d, int dtype, int64_t M, int E, int n, int64_t ld)
+{
+    return M > 0 && ld % 8 != 0 && tensor_form(dtype, M, E, d)
+               ? align256(M * ((n + 7) / 8 * 8) * (long long)elem_size(dtype)) : 0;
+}
+
+/* the gradient's workspace: dz (where the activation makes one, or as a copy
+ * of dy), sums of parts (where there are several), the operator's boxes, a
+ * copy of x */
 struct GradPlan {
     int per;
-    long long lddz, dz_bytes, part_bytes, pack_bytes;
-    long long bytes() const { return dz_bytes + part_bytes + pack_bytes; }
+    bool made;
+    long long lddz, dz_bytes, part_bytes, pack_bytes, x_bytes;
+    long long bytes() const { return dz_bytes + part_bytes + pack_bytes + x_bytes; }
 };
 
-static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int E, int64_t stride,
-                          int act)
+static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int E, int64_t ldx,
+                          int64_t stride, int64_t lddy, int act)
 {
     GradPlan g;
     g.per = grad_part_rows(p, dtype, M, E, stride);
     g.lddz = (p->n_rows + 7) / 8 * 8;
-    g.dz_bytes = act == DIA_ACT_NONE ? 0 : align256(M * g.lddz * (long long)elem_size(dtype));
+    g.made = act != DIA_ACT_NONE || copy_bytes(p->fwd, dtype, M, E, p->n_rows, lddy) > 0;
+    g.dz_bytes = g.made ? align256(M * g.lddz * (long long)elem_size(dtype)) : 0;
     g.part_bytes = align256(grad_slots(M, g.per) * (p->K + 1) * stride * 4);
-    g.pack_bytes = pack_bytes(p->trn, dtype, M, E, p->n_cols);
+    g.pack_bytes = pack_bytes(p->trn, p->K, dtype, M, E, p->n_cols);
+    g.x_bytes = copy_bytes(p->fwd, dtype, M, E, p->n_cols, ldx);
     return g;
 }
 
@@ -399,7 +416,9 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
     if (rc == DIA_OK && d_res) rc = check_block(who, "residual", d_res, ldr, M, plan->n_rows, dtype);
     if (rc == DIA_OK && d_z) rc = check_block(who, "z", d_z, ldz, M, plan->n_rows, dtype);
     if (rc != DIA_OK) return rc;
-    const long long need = pack_bytes(plan->fwd, dtype, M, num_experts, plan->n_rows);
+    const long long pack = pack_bytes(plan->fwd, plan->K, dtype, M, num_experts, plan->n_rows);
+    const long long copy = copy_bytes(plan->fwd, dtype, M, num_experts, plan->n_cols, ldx);
+    const long long need = pack + copy;
     if (need > work_bytes) return fail(DIA_ERR_CAPACITY, "dia_spmm: workspace too small");
     if (need > 0 && (!d_work || (uintptr_t)d_work % 256))
         return fail(DIA_ERR_INVALID, "dia_spmm: workspace must be 256-byte aligned");
@@ -426,27 +445,37 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
     a.act = act;
     a.dir = plan->fwd;
     a.trans = false;
-    if (product_on_tc(a, dtype)) {
-        rc = spmm_tc_pack(a, false, stream);
-        if (rc != DIA_OK) return rc;
-    }
-    return by_type(dtype, [&](auto* t) {
-        return launch_product<std::remove_pointer_t<decltype(t)>>(a, dtype, stream);
+    return by_type(dtype, [&](auto* t) -> int {
+        using T = std::remove_pointer_t<decltype(t)>;
+        int r = DIA_OK;
+        if (copy > 0) {
+            a.in = (char*)d_work + pack;
+            a.ldi = (plan->n_cols + 7) / 8 * 8;
+            r = Cores<T>::dz(DIA_ACT_NONE, d_x, ldx, nullptr, 0, (char*)d_work + pack, a.ldi, a.M,
+                             a.n_in, false, stream);
+        }
+        if (r == DIA_OK && product_on_tc(a, dtype)) {
+            r = spmm_tc_pack(a, false, stream);
+            a.dependent = pack > 0;
+        }
+        return r == DIA_OK ? launch_product<T>(a, dtype, stream) : r;
     });
 }
 
 extern "C" int64_t dia_spmm_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
-                                      int num_experts)
+                                      int num_experts, int64_t ldx)
 {
     if (!plan || M < 0 || M > INT_MAX / 2 || num_experts < 1) return -1;
-    return pack_bytes(plan->fwd, dtype, M, num_experts, plan->n_rows);
+    return pack_bytes(plan->fwd, plan->K, dtype, M, num_experts, plan->n_rows) +
+           copy_bytes(plan->fwd, dtype, M, num_experts, plan->n_cols, ldx);
 }
 
 extern "C" int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
-                                               int num_experts, int64_t stride, int act)
+                                               int num_experts, int64_t ldx, int64_t stride,
+                                               int64_t lddy, int act)
 {
     if (!plan || M < 0 || M > INT_MAX / 2 || stride < 0 || num_experts < 1) return -1;
-    const GradPlan g = grad_plan(plan, dtype, M, num_experts, stride, act);
+    const GradPlan g = grad_plan(plan, dtype, M, num_experts, ldx, stride, lddy, act);
     return g.bytes();
 }
 
@@ -467,7 +496,7 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
         rc = check_block(who, "z", d_z, ldz, M, plan->n_rows, dtype);
     if (rc == DIA_OK && d_dx) rc = check_block(who, "dx", d_dx, lddx, M, plan->n_cols, dtype);
     if (rc != DIA_OK) return rc;
-    const GradPlan g = grad_plan(plan, dtype, M, num_experts, stride, act);
+    const GradPlan g = grad_plan(plan, dtype, M, num_experts, ldx, stride, lddy, act);
     if (g.bytes() > work_bytes)
         return fail(DIA_ERR_CAPACITY, "dia_spmm_backward: workspace too small");
     if (g.bytes() > 0 && (!d_work || (uintptr_t)d_work % 256))
@@ -475,7 +504,7 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
 
     return by_type(dtype, [&](auto* t) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        const bool made = act != DIA_ACT_NONE;
+        const bool made = g.made;
         ProdArgs p{};
         p.in = made ? d_work : d_dy;
         p.vals = d_vals;
@@ -518,23 +547,34 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
         a.slots = grad_slots(M, g.per);
         a.dir = plan->fwd;
         const bool grad = (a.dvals || a.dbias) && stride > 0;
+        int r = DIA_OK;
+        if (g.x_bytes > 0 && a.dvals) {
+            a.x = (char*)d_work + g.dz_bytes + g.part_bytes + g.pack_bytes;
+            a.ldx = (plan->n_cols + 7) / 8 * 8;
+            r = Cores<T>::dz(DIA_ACT_NONE, d_x, ldx, nullptr, 0, (void*)a.x, a.ldx, a.M, a.n_cols,
+                             false, stream);
+        }
         /* Launches of the tensor-core form overlap.  Where the diagonals'
          * gradient makes dz itself it goes first, the operator is packed on
          * the SMs that it leaves free; else the operator is packed under dz. */
         const bool tc = d_dx && product_on_tc(p, dtype), gtc = grad && grad_on_tc(a, dtype);
         const bool makes = gtc && made && spmm_tc_makes_dz(a);
-        int r = DIA_OK;
+        if (r != DIA_OK) return r;
         if (makes) {
             r = spmm_tc_gradient(a, dtype, true, false, stream);
             if (r == DIA_OK && tc) r = spmm_tc_pack(p, true, stream);
+            p.dependent = true;
         } else {
-            if (tc) r = spmm_tc_pack(p, false, stream);
+            const bool packed = tc && g.pack_bytes > 0;
+            if (packed) r = spmm_tc_pack(p, false, stream);
             if (r == DIA_OK && made)
-                r = Cores<T>::dz(act, d_dy, lddy, d_z, ldz, d_work, p.ldi, p.M, p.n_in, tc, stream);
+                r = Cores<T>::dz(act, d_dy, lddy, d_z, ldz, d_work, p.ldi, p.M, p.n_in, packed,
+                                 stream);
             if (r == DIA_OK && grad)
-                r = gtc ? spmm_tc_gradient(a, dtype, false, tc || made, stream)
+                r = gtc ? spmm_tc_gradient(a, dtype, false, packed || made, stream)
                         : Cores<T>::gradient(a, stream);
             p.early = tc && gtc;   /* what it reads is older than the gradient */
+            p.dependent = packed || made || grad;
         }
         if (r == DIA_OK && d_dx) r = launch_product<T>(p, dtype, stream);
         if (r == DIA_OK && grad) r = Cores<T>::join(a, stream);

@@ -399,7 +399,9 @@ struct ProdArgs {
     int act;
     SpmmDir dir;
     bool trans;
-    int groups;           /* set by the tensor-core launch */
+    int groups;           /* set by the tensor-core launch, */
+    bool build;           /* and this */
+    bool dependent;       /* tensor-core form: a launch of the same call is before it */
     bool early;           /* tensor-core form: inputs are complete when the kernel may begin */
 };
 
@@ -491,7 +493,9 @@ struct Cores {
 /* Tensor-core forms for 16-bit blocks (spmm_tc.cu).  spmm_tc_block: address
  * and row stride are ones TMA takes. */
 bool spmm_tc_block(const void* p, long long ld);
-long long spmm_tc_pack_bytes(int n_out, int nboxes, int E);
+/* 0 where the product makes the operator's boxes itself; spmm_tc_pack then
+ * launches nothing */
+long long spmm_tc_pack_bytes(const SpmmDir& d, int K, int n_out, long long M, int E);
 int spmm_tc_pack(const ProdArgs& a, bool dependent, cudaStream_t stream);
 int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream);
 /* make: dz is made there from dy and z (spmm_tc_makes_dz says whether it can be) */

@@ -188,31 +188,44 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
     const int f = f0 + (QUADS ? 4 * lane : lane), i = i0 + f;
     if (QUADS) {
         const Quad* quads = a.dir.quads[shape];
-        float carry[kTileRows][4];
-        int next = INT_MIN;   /* base of the quad whose first piece `carry` holds */
-        for (int q = 0; q < a.dir.nquads; ++q) {
+        /* a quad's values are read while the one before is worked on */
+        struct Weights {
+            float w[4][4];
+            int base, col, on;   /* on: bit s where slot s has a diagonal */
+        };
+        auto fetch = [&](int q, Weights& v) {
             const int4 h = __ldg((const int4*)&quads[q]);
             const int2 h2 = __ldg((const int2*)&quads[q].k[3]);
             const int kk[4] = {h.y, h.z, h.w, h2.x};
+            v.base = h.x;
+            v.col = h2.y;
+            v.on = 0;
             const int c = i + h.x;
-            float w[4][4];
+            const bool inside = c >= 0 && c + 7 <= a.n_in && i + 4 <= a.n_out;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 if (kk[s] < 0) continue;
-                const T* vp = vals + (long long)kk[s] * a.stride;
+                v.on |= 1 << s;
+                const T* vp = vals + (long long)kk[s] * a.stride + (TRANS ? c + s : i);
+                if (!TRANS && inside) {
+                    *(float4*)v.w[s] = load4<T>(vp);
+                } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = c + s + r;
-                    w[s][r] = i + r < a.n_out && (unsigned)j < (unsigned)a.n_in
-                                  ? to_f(vp[TRANS ? j : i + r]) : 0.0f;
+                    for (int r = 0; r < 4; ++r)
+                        v.w[s][r] = i + r < a.n_out && (unsigned)(c + s + r) < (unsigned)a.n_in
+                                        ? to_f(vp[r]) : 0.0f;
                 }
             }
-            const T* p = xw + h2.y + f;
-            if (h.x != next) {
+        };
+        float carry[kTileRows][4];
+        int next = INT_MIN;   /* base of the quad whose first piece `carry` holds */
+        auto work = [&](const Weights& v) {
+            const T* p = xw + v.col + f;
+            if (v.base != next) {
 #pragma unroll
                 for (int t = 0; t < kTileRows; ++t) *(float4*)carry[t] = load4<T>(p + t * pitch);
             }
-            next = h.x + 4;
+            next = v.base + 4;
 #pragma unroll
             for (int t = 0; t < kTileRows; ++t) {
                 float x[8];
@@ -221,41 +234,71 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
                 *(float4*)carry[t] = *(float4*)(x + 4);
 #pragma unroll
                 for (int s = 0; s < 4; ++s)
-                    if (kk[s] >= 0)
+                    if (v.on >> s & 1)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            acc[t][r] = fmaf(w[s][r], x[s + r], acc[t][r]);
+                            acc[t][r] = fmaf(v.w[s][r], x[s + r], acc[t][r]);
             }
+        };
+        Weights u, v;
+        fetch(0, u);
+        for (int q = 0; q < a.dir.nquads; q += 2) {
+            if (q + 1 < a.dir.nquads) fetch(q + 1, v);
+            work(u);
+            if (q + 1 >= a.dir.nquads) break;
+            if (q + 2 < a.dir.nquads) fetch(q + 2, u);
+            work(v);
         }
     } else {
         const int* cols = a.dir.cols[shape];
-        /* the next diagonal's values are on their way while one is worked on */
-        auto fetch = [&](int k, float (&w)[4], int& col) {
-            const int2 o = __ldg(&a.dir.offs[k]);
-            col = __ldg(cols + k);
-            const T* vp = vals + (long long)o.y * a.stride;
+        /* diagonals in fours; the next four's values are read while these are
+         * worked on */
+        constexpr int U = 4;
+        /* every entry of the warp's features is in the matrix */
+        const bool inside = i0 + f0 + 128 <= a.n_out && i0 + f0 + __ldg(&a.dir.offs[0].x) >= 0 &&
+                            i0 + f0 + 127 + __ldg(&a.dir.offs[a.K - 1].x) < a.n_in;
+        auto fetch = [&](int k0, float (&w)[U][4], int (&col)[U]) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int ir = i + 32 * r, j = ir + o.x;
-                w[r] = ir < a.n_out && (unsigned)j < (unsigned)a.n_in
-                           ? to_f(__ldg(vp + (TRANS ? j : ir))) : 0.0f;
+            for (int u = 0; u < U; ++u) {
+                const bool on = k0 + u < a.K;
+                const int k = on ? k0 + u : 0;
+                const int2 o = __ldg(&a.dir.offs[k]);
+                col[u] = __ldg(cols + k);
+                const T* vp = vals + (long long)o.y * a.stride + (TRANS ? o.x : 0) + i;
+                if (inside) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w[u][r] = to_f(__ldg(vp + 32 * r));
+                    continue;
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int ir = i + 32 * r;
+                    w[u][r] = on && ir < a.n_out && (unsigned)(ir + o.x) < (unsigned)a.n_in
+                                  ? to_f(vp[32 * r]) : 0.0f;
+                }
             }
         };
-        float w[4], wn[4];
-        int col = 0, cn = 0;
-        if (a.K > 0) fetch(0, w, col);
-#pragma unroll 2
-        for (int k = 0; k < a.K; ++k) {
-            if (k + 1 < a.K) fetch(k + 1, wn, cn);
-            const T* p = xw + col + f;
+        auto work = [&](const float (&w)[U][4], const int (&col)[U], int n) {
 #pragma unroll
-            for (int t = 0; t < kTileRows; ++t)
+            for (int u = 0; u < U; ++u) {
+                if (u >= n) break;
+                const T* p = xw + col[u] + f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    acc[t][r] = fmaf(w[r], to_f(p[t * pitch + 32 * r]), acc[t][r]);
+                for (int t = 0; t < kTileRows; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[r] = wn[r];
-            col = cn;
+                    for (int r = 0; r < 4; ++r)
+                        acc[t][r] = fmaf(w[u][r], to_f(p[t * pitch + 32 * r]), acc[t][r]);
+            }
+        };
+        float w[U][4], wn[U][4];
+        int col[U], cn[U];
+        fetch(0, w, col);
+        for (int k = 0; k < a.K; k += 2 * U) {
+            fetch(k + U, wn, cn);
+            work(w, col, a.K - k);
+            if (k + U >= a.K) break;
+            fetch(k + 2 * U, w, col);
+            work(wn, cn, a.K - k - U);
         }
     }
     float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -458,8 +501,9 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8])
 
 /* dz = dy * act'(z), rounded to the block's type: both gradients read it as
  * a matrix operand of that type, and one rounding of half a step is no more
- * than the ones dy and z already carry.  Eight elements a thread at a time,
- * two of them in flight. */
+ * than the ones dy and z already carry.  Without an activation it is a copy,
+ * for blocks whose rows TMA does not take.  Eight elements a thread at a time,
+ * two of them in flight; rows of dz are padded to eight. */
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256)
 spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z, long long ldz,
@@ -471,33 +515,36 @@ spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z
     for (long long p0 = blockIdx.x * 256ll + threadIdx.x; p0 < total; p0 += 2 * step) {
         float a[2][8], b[2][8];
         long long at[2];
-        bool wide[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const long long p = p0 + h * step;
             const long long t = p < total ? p / per : 0;
             const int i = (int)(p - t * per) * 8;
             at[h] = p < total ? t * lddz + i : -1;
-            wide[h] = VEC && i + 8 <= n;
             if (at[h] < 0) continue;
-            if (wide[h]) {
+            if (VEC && i + 8 <= n) {
                 load8<T>(dy + t * lddy + i, a[h]);
-                load8<T>(z + t * ldz + i, b[h]);
+                if (ACT != DIA_ACT_NONE) load8<T>(z + t * ldz + i, b[h]);
             } else {
-                for (int c = 0; c < 8 && i + c < n; ++c)
-                    dz[at[h] + c] = from_f<T>(to_f(dy[t * lddy + i + c]) *
-                                              dact_of<ACT>(to_f(z[t * ldz + i + c])));
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    a[h][c] = i + c < n ? to_f(dy[t * lddy + i + c]) : 0.0f;
+                    if (ACT != DIA_ACT_NONE)
+                        b[h][c] = i + c < n ? to_f(z[t * ldz + i + c]) : 0.0f;
+                }
             }
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (at[h] < 0 || !wide[h]) continue;
+            if (at[h] < 0) continue;
             __align__(16) T r[8];
 #pragma unroll
             for (int c = 0; c < 8; c += 2) {
-                const float2 d = sizeof(T) == 2
-                                     ? dact2<ACT>(make_float2(b[h][c], b[h][c + 1]))
-                                     : make_float2(dact_of<ACT>(b[h][c]), dact_of<ACT>(b[h][c + 1]));
+                float2 d = make_float2(1.0f, 1.0f);
+                if (ACT != DIA_ACT_NONE)
+                    d = sizeof(T) == 2
+                            ? dact2<ACT>(make_float2(b[h][c], b[h][c + 1]))
+                            : make_float2(dact_of<ACT>(b[h][c]), dact_of<ACT>(b[h][c + 1]));
                 r[c] = from_f<T>(a[h][c] * d.x);
                 r[c + 1] = from_f<T>(a[h][c + 1] * d.y);
             }
@@ -565,15 +612,23 @@ template <typename T, bool TRANS>
 static int launch_cores(const ProdArgs& a, cudaStream_t stream)
 {
     const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
-    if (per >= 8 && a.K > 0) {
+    /* below this there are too few warps of 128 features x 8 rows to hide the
+     * latency of the diagonals one after the other (4096 x 4096, 129 diagonals,
+     * fp32: 39 us at 32 rows, 32 us by few rows; 39 and 68 at 128) */
+    if (per >= 8 && a.K > 0 && (long long)a.M * a.n_out >= 196608) {
         /* the widest tile (an input is read again by fewer tiles) whose inputs
-         * fit and that leaves a CTA for every SM */
-        for (int shape = 2; shape >= 0; --shape) {
+         * fit and that leaves a CTA for every SM; else the narrowest that fits */
+        int shape = 2;
+        auto fits = [&](int s) { return tile_smem(a.dir, s, sizeof(T)) <= kTileSmem; };
+        auto ctas = [&](int s) {
+            const int rows = kTileWarps * kTileRows * 128 / kTileF[s];
+            return (long long)((a.n_out + kTileF[s] - 1) / kTileF[s]) * ((a.M + rows - 1) / rows);
+        };
+        while (shape >= 0 && !(fits(shape) && ctas(shape) >= num_sms())) --shape;
+        if (shape < 0)
+            for (shape = 0; shape < 3 && !fits(shape);) ++shape;
+        if (shape < 3) {
             const int smem = tile_smem(a.dir, shape, sizeof(T));
-            const int rows = kTileWarps * kTileRows * 128 / kTileF[shape];
-            const long long ctas = (long long)((a.n_out + kTileF[shape] - 1) / kTileF[shape]) *
-                                   ((a.M + rows - 1) / rows);
-            if (smem > kTileSmem || (shape > 0 && ctas < num_sms())) continue;
             const bool vec = vec16<T>(a.in, a.ldi), quads = 3 * a.dir.nquads <= a.K;
             if (vec)
                 return quads ? launch_tile_as<T, TRANS, true, true>(a, shape, smem, stream)
@@ -611,7 +666,8 @@ int Cores<T>::dz(int act, const void* dy, long long lddy, const void* z, long lo
                      void* dz, long long lddz, int M, int n, bool dependent, cudaStream_t stream)
 {
     if (M == 0 || n == 0) return DIA_OK;
-    const auto run = act == DIA_ACT_RELU   ? launch_dz_act<T, DIA_ACT_RELU>
+    const auto run = act == DIA_ACT_NONE   ? launch_dz_act<T, DIA_ACT_NONE>
+                     : act == DIA_ACT_RELU   ? launch_dz_act<T, DIA_ACT_RELU>
                      : act == DIA_ACT_SILU ? launch_dz_act<T, DIA_ACT_SILU>
                      : act == DIA_ACT_GELU ? launch_dz_act<T, DIA_ACT_GELU>
                                            : launch_dz_act<T, DIA_ACT_GELU_TANH>;

@@ -325,6 +325,86 @@ __global__ void __launch_bounds__(256) spmm_pack_kernel(const __grid_constant__ 
     dependency_wait();
 }
 
+/* The same by the epilogue's warps of spmm_tc_kernel, straight into its
+ * operator slots: for a CTA that keeps one feature tile and expert this takes
+ * less than a launch.  Boxes [b0, b1) of tile i0 go to slots 0, 1, ..; mem:
+ * the epilogue's buffers, not in use yet. */
+constexpr int kInlineDiags = 160;
+constexpr int kInlineOffs = kWSlots * 192 * 2;                 /* after the tables of rows */
+constexpr int kInlineSlab = kInlineOffs + kInlineDiags * 8;    /* after the offsets */
+static_assert(kInlineSlab % 16 == 0 &&
+              kInlineSlab + kInlineDiags * kPackPitch * 2 <= 2 * kEpiWarpsT * kEpiBuf, "slab");
+
+template <bool TRANS>
+__device__ __forceinline__ void build_operator(const ProdArgs& a, int K, int e, unsigned char* mem,
+                                               uint32_t slots, int i0, int b0, int b1, const int* cols,
+                                               int t)
+{
+    int16_t* s_row = (int16_t*)mem;
+    int2* s_off = (int2*)(mem + kInlineOffs);
+    uint16_t* slab = (uint16_t*)(mem + kInlineSlab);
+    for (int c = t; c < (b1 - b0) * 192; c += kEpiThreads) s_row[c] = -1;
+    if (t < K) s_off[t] = a.dir.offs[t];
+    asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+    for (int b = b0; b < b1; ++b) {
+        const Box bx = a.dir.boxes[b];
+        const int k = bx.k0 + t;
+        if (k < bx.k1) s_row[(b - b0) * 192 + s_off[k].x - (bx.col - 127)] = (int16_t)k;
+    }
+    const uint16_t* vals = (const uint16_t*)a.vals + e * a.estride;
+    /* four pieces a thread on their way at a time */
+    for (int o0 = t; o0 < K * 17; o0 += 4 * kEpiThreads) {
+        uint4 v[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const int o = min(o0 + h * kEpiThreads, K * 17 - 1), k = o / 17;
+            const int2 of = s_off[k];
+            const int x = ((TRANS ? i0 + of.x : i0) & ~7) + (o - k * 17) * 8;
+            v[h] = make_uint4(0, 0, 0, 0);
+            if (x >= 0 && x < a.stride) v[h] = __ldg((const uint4*)(vals + of.y * a.stride + x));
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const int o = o0 + h * kEpiThreads, k = o / 17;
+            if (o < K * 17) *(uint4*)(slab + k * kPackPitch + (o - k * 17) * 8) = v[h];
+        }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+    /* eight columns of a feature at a time; consecutive threads, consecutive
+     * features.  Consecutive offsets need no table, and entries of an inner
+     * tile no check. */
+    const int d0 = s_off[0].x, d1 = s_off[K - 1].x;
+    const bool band = d1 - d0 == K - 1;
+    const bool inner = i0 + 128 <= a.n_out && i0 + d0 >= 0 && i0 + 127 + d1 < a.n_in;
+    for (int c = t; c < (b1 - b0) * 1024; c += kEpiThreads) {
+        const int b = c >> 10, q = (c >> 7) & 7, f = c & 127, i = i0 + f;
+        const int d = cols[b0 + b] + 8 * q - f;      /* offset of the first column */
+        uint32_t u[4] = {0, 0, 0, 0};
+        if (band && inner) {
+            const uint16_t* p = slab + (d - d0) * kPackPitch + f;
+#pragma unroll
+            for (int h = 0; h < 8; ++h)
+                if ((unsigned)(d - d0 + h) < (unsigned)K) {
+                    const uint32_t v = p[h * kPackPitch + (TRANS ? (i0 + d + h) & 7 : 0)];
+                    u[h >> 1] |= h & 1 ? v << 16 : v;
+                }
+        } else if (i < a.n_out) {
+            const int16_t* rows = s_row + b * 192 + 8 * q - f + 127;
+#pragma unroll
+            for (int h = 0; h < 8; ++h) {
+                const int k = rows[h];
+                if (k >= 0 && (unsigned)(i + d + h) < (unsigned)a.n_in) {
+                    const uint32_t v = slab[k * kPackPitch + f + (TRANS ? (i0 + d + h) & 7 : 0)];
+                    u[h >> 1] |= h & 1 ? v << 16 : v;
+                }
+            }
+        }
+        sts128(slots + b * kBoxBytes + f * 128 + ((q ^ (f & 7)) << 4), u[0], u[1], u[2], u[3]);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+}
+
 /* the sum of one output's own terms, in ascending order of the offsets */
 template <typename T, bool TRANS>
 __device__ __noinline__ float product_terms(const ProdArgs& a, int K, int e, long long row, int i)
@@ -586,7 +666,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         int issued = 0;
         bool ok = true;
         const bool leader = elect_one();
-        while (ok && next_run(a, sh, r)) {
+        while (ok && !a.build && next_run(a, sh, r)) {
             int b0, b1;
             used_boxes(s_cols, a.dir, r.fb * kTN, a.n_in, b0, b1);
             const int used = b1 - b0;
@@ -697,6 +777,16 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             pcb += kEpiQuad;
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        if (a.build && sh.w < sh.w1) {
+            Share first = sh;
+            next_run(a, first, r);
+            int b0, b1;
+            used_boxes(s_cols, a.dir, r.fb * kTN, a.n_in, b0, b1);
+            build_operator<TRANS>(a, K, r.e, smem + (kWSlots + kXStages) * kBoxBytes, wst,
+                                  r.fb * kTN, b0, b1, s_cols, tid - kEpiWarp0t * 32);
+            if (tid < kEpiWarp0t * 32 + b1 - b0)
+                mbar_arrive(wfull + 8 * (tid - kEpiWarp0t * 32));
+        }
         if (has_res) next_fetch(0);
         int cb = turn;
         while (ok && next_run(a, sh, r)) {
@@ -1166,27 +1256,43 @@ static bool block_map(CUtensorMap* map, const void* base, int dtype, int width, 
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-long long spmm_tc_pack_bytes(int n_out, int nboxes, int E)
+/* CTAs a feature tile, each with every so-manieth tile of rows; 0: stretches
+ * of the list of tiles instead, where that would leave a quarter of the SMs
+ * idle (4096 x 4096 band, 2048 rows: 28.1 us against 30.6 by stretches) */
+static int row_groups_of(int n_out, long long M, int E, bool seg)
 {
-    return (long long)E * ((n_out + kTN - 1) / kTN) * nboxes * kBoxBytes;
+    const int nfb = (n_out + kTN - 1) / kTN;
+    const long long tiles = seg ? M / kTM + std::min<long long>(E, M) : (M + kTM - 1) / kTM;
+    const long long groups = std::min<long long>(num_sms() / nfb, tiles);
+    return groups * nfb < std::min<long long>(tiles * nfb, num_sms() * 3 / 4) ? 0 : (int)groups;
+}
+
+/* the product makes the operator's boxes itself */
+static bool builds(const SpmmDir& d, int K, int n_out, long long M, int E)
+{
+    return E == 1 && K <= kInlineDiags && d.nboxes <= kWSlots &&
+           row_groups_of(n_out, M, 1, false) > 0 && row_groups_of(n_out, M, 1, true) > 0;
+}
+
+long long spmm_tc_pack_bytes(const SpmmDir& d, int K, int n_out, long long M, int E)
+{
+    if (builds(d, K, n_out, M, E)) return 0;
+    return (long long)E * ((n_out + kTN - 1) / kTN) * d.nboxes * kBoxBytes;
 }
 
 template <typename T, bool TRANS, int ACT>
 static int launch_tc(const CUtensorMap& map, const ProdArgs& a_, int K, cudaStream_t stream)
 {
     const long long tiles = a_.seg ? a_.M / kTM + std::min(a_.E, a_.M) : (a_.M + kTM - 1) / kTM;
-    const long long items = tiles * ((a_.n_out + kTN - 1) / kTN);
     const int nfb = (a_.n_out + kTN - 1) / kTN;
     ProdArgs a = a_;
-    int grid = (int)std::min<long long>(items, num_sms());
-    /* whole rows at a time, unless that leaves a quarter of the SMs idle
-     * (4096 x 4096 band, 2048 rows: 28.1 us against 30.6 by stretches) */
-    a.groups = (int)std::min<long long>(num_sms() / nfb, tiles);
-    if (a.groups * nfb < std::min<long long>(items, num_sms() * 3 / 4)) a.groups = 0;
-    if (a.groups > 0) grid = a.groups * nfb;
+    a.groups = row_groups_of(a.n_out, a.M, a.E, a.seg != nullptr);
+    a.build = builds(a.dir, K, a.n_out, a.M, a.E);
+    const int grid = a.groups > 0 ? a.groups * nfb
+                                  : (int)std::min<long long>(tiles * nfb, num_sms());
     static SmemRecord most;
     DIA_TRY_CUDA(allow_smem(spmm_tc_kernel<T, TRANS, ACT>, kTcSmem, most));
-    DIA_TRY_CUDA(launch(true, spmm_tc_kernel<T, TRANS, ACT>, grid, kTcWarps * 32, kTcSmem, stream, map, a, K));
+    DIA_TRY_CUDA(launch(a.dependent, spmm_tc_kernel<T, TRANS, ACT>, grid, kTcWarps * 32, kTcSmem, stream, map, a, K));
     return DIA_OK;
 }
 
@@ -1205,7 +1311,8 @@ static int launch_tc_type(const CUtensorMap& map, const ProdArgs& a, int K, cuda
 
 int spmm_tc_pack(const ProdArgs& a, bool dependent, cudaStream_t stream)
 {
-    const long long boxes = spmm_tc_pack_bytes(a.n_out, a.dir.nboxes, a.E) / kBoxBytes;
+    const long long boxes = spmm_tc_pack_bytes(a.dir, a.K, a.n_out, a.M, a.E) / kBoxBytes;
+    if (boxes == 0) return DIA_OK;
     if (boxes > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: operator too large");
     const auto pack = a.trans ? spmm_pack_kernel<true> : spmm_pack_kernel<false>;
     static SmemRecord most[2];

@@ -176,7 +176,8 @@ int dia_spmspm_plan_destroy(DiaSpmspmPlan* plan);
  * off[k]], stride a multiple of 32 and >= n_rows, 16-byte aligned; entries
  * outside the matrix and the padding are not read as values (any bits).
  * Blocks whose address and row strides are multiples of 16 bytes are the
- * fastest; any element-aligned ones are taken.  Sums are fp32; results are
+ * fastest (others are copied first, or work on the CUDA cores); any
+ * element-aligned ones are taken.  Sums are fp32; results are
  * rounded once to the block's type, the same bits on every run. */
 enum { DIA_F32 = 0, DIA_F16 = 1, DIA_BF16 = 2 };
 enum {
@@ -208,7 +209,8 @@ int dia_spmm_plan_destroy(DiaSpmmPlan* plan);
  * stride).  Allocates nothing and does not synchronise.  work:
  * dia_spmm_workspace bytes (0 where the CUDA cores do the work), 256-byte
  * aligned, not shared by calls that may run at the same time. */
-int64_t dia_spmm_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts);
+int64_t dia_spmm_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
+                           int64_t ldx);
 int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
              const int64_t* d_seg, const void* d_x, int64_t ldx, const void* d_vals,
              int64_t stride, const void* d_bias, int act, const void* d_res, int64_t ldr,
@@ -226,7 +228,8 @@ int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
  * were.  work: dia_spmm_backward_workspace bytes, 256-byte aligned, not shared
  * by calls that may run at the same time. */
 int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
-                                    int num_experts, int64_t stride, int act);
+                                    int num_experts, int64_t ldx, int64_t stride, int64_t lddy,
+                                    int act);
 int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
                       const int64_t* d_seg, const void* d_x, int64_t ldx, const void* d_vals,
                       int64_t stride, const void* d_dy, int64_t lddy, int act, const void* d_z,

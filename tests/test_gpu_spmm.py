@@ -247,6 +247,7 @@ SHAPES = {
     "stencil": (257, 512, 512, [i + 8 * j + 64 * k for i in (-1, 0, 1) for j in (-1, 0, 1)
                                 for k in (-1, 0, 1)]),
     "long": (700, 264, 264, band(20)),
+    "odd widths": (300, 131, 203, [-40, -39, 0, 1, 2, 3, 70, 71, 90]),
 }
 
 
@@ -552,7 +553,7 @@ def test_refusals_on_the_device():
     refused(dg.DIA_ERR_INVALID, dg.spmm, plan, v, x[:1].expand(20, 64))
     refused(dg.DIA_ERR_INVALID, dg.spmm, plan, v, x, out=torch.zeros(20, 63, dtype=x.dtype,
                                                                       device="cuda"))
-    ws = dg.spmm_backward_workspace(plan, v, 20, "silu")
+    ws = dg.spmm_backward_workspace(plan, v, x, c.dy, "silu")
     assert ws > 0
     work = torch.empty(ws - 1, dtype=torch.uint8, device="cuda")
     refused(dg.DIA_ERR_CAPACITY, dg.spmm_backward, plan, v, x, c.dy, z=c.zin, act="silu",

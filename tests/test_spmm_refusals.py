@@ -103,6 +103,6 @@ def test_c_abi_before_cuda():
                           (dict(E=2), "seg"), (dict(), "null plan")):
             assert f(**bad) == dg.DIA_ERR_INVALID
             assert word in L.dia_last_error().decode(), bad
-    assert L.dia_spmm_workspace(None, 0, 4, 1) == -1
-    assert L.dia_spmm_backward_workspace(None, 0, 4, 1, 32, 0) == -1
+    assert L.dia_spmm_workspace(None, 0, 4, 1, 8) == -1
+    assert L.dia_spmm_backward_workspace(None, 0, 4, 1, 8, 32, 8, 0) == -1
     assert L.dia_test_spmm_form(3) == dg.DIA_ERR_INVALID
