@@ -303,6 +303,31 @@ def test_experts_long_and_short(t):
     c.gradient(act="gelu")
 
 
+# Long blocks: a CTA of the tensor-core form goes around its accumulators, keeps
+# an operator for many tiles or reads a large one again, takes a stretch of the
+# tiles or every so-manieth; parts of the gradient are joined.
+LONG = {
+    "band": (60000, 136, 136, band(4)),
+    "scattered": (30000, 264, 264, [-250, -201, -130, -64, -3, 0, 55, 120, 199, 260]),
+    "stretches": (600, 6400, 6400, [-2, -1, 0, 1, 700]),
+}
+
+
+@pytest.mark.parametrize("shape", LONG)
+def test_long_blocks(shape, t):
+    c = Case(t, *LONG[shape], seed=21)
+    c.product(act="silu", bias=True, res=True, z=True)
+    c.gradient(act="silu")
+    c.gradient(act="none")
+
+
+def test_long_blocks_of_experts(t):
+    c = Case(t, 20000, 136, 136, [-70, -8, 0, 1, 2, 65], seed=22,
+             seg=[0, 9000, 9000, 9001, 9700, 20000])
+    c.product(act="gelu", bias=True, res=True, z=True)
+    c.gradient(act="gelu")
+
+
 @pytest.mark.parametrize("M", [3, 140])
 def test_unread_values(M, t):
     """Bits outside the matrix, in the padding and in rows outside every expert
