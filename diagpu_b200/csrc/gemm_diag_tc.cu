@@ -1032,6 +1032,7 @@ extern "C" int dia_device_status(unsigned int* flags, int clear)
 
 extern "C" int dia_test_tc_wait(uint64_t wait_ns, int withhold)
 {
+    DIA_TRY_CUDA(dia::spmm_tc_test_wait(wait_ns, withhold ? 1 : 0));
     if (wait_ns == 0) wait_ns = dia::kWsWaitNs;
     const unsigned long long ns = wait_ns;
     const int w = withhold ? 1 : 0;

@@ -502,5 +502,6 @@ int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream);
 bool spmm_tc_makes_dz(const GradArgs& a);
 int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, bool dependent, cudaStream_t stream);
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear);
+cudaError_t spmm_tc_test_wait(unsigned long long wait_ns, int withhold);
 
 }  // namespace dia

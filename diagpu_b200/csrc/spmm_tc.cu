@@ -37,6 +37,10 @@ namespace dia {
 
 static __device__ unsigned int g_mm_status;
 constexpr unsigned long long kMmWaitNs = 2000000000ull;
+/* limit of every wait, and a test switch: CTA 0 withholds its first copy of
+ * the block, so that the MMA issuer's wait runs out (dia_test_tc_wait) */
+static __device__ unsigned long long g_mm_wait_ns = kMmWaitNs;
+static __device__ int g_mm_withhold;
 
 constexpr int kTM = 128;             /* rows of a tile */
 constexpr int kTN = 128;             /* features of a tile */
@@ -73,7 +77,7 @@ __device__ __noinline__ bool mm_wait_long(uint32_t bar, uint32_t parity, volatil
     for (;;) {
         if (mbar_try(bar, parity)) return true;
         if (*abort_flag) return false;
-        if (global_ns() - t0 > kMmWaitNs) {
+        if (global_ns() - t0 > g_mm_wait_ns) {
             *abort_flag = 1;
             atomicOr(&g_mm_status, (unsigned)DIA_TC_TIMEOUT);
             return false;
@@ -91,7 +95,7 @@ __device__ void mm_drain(uint32_t bar, uint32_t parity)
 {
     const unsigned long long t0 = global_ns();
     while (!mbar_try(bar, parity))
-        if (global_ns() - t0 > kMmWaitNs) {
+        if (global_ns() - t0 > g_mm_wait_ns) {
             atomicOr(&g_mm_status, (unsigned)DIA_TC_TIMEOUT);
             return;
         }
@@ -493,7 +497,6 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     __shared__ __align__(8) MmBars bars;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ __align__(16) float s_bias[kTN];
     __shared__ int s_cols[kSharedBoxes];
     volatile int* abort_flag = &s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -575,7 +578,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                         ok = mm_wait(x.bar(xempty), x.round ^ 1, abort_flag);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
-                        if (leader)
+                        if (leader && !(g_mm_withhold && blockIdx.x == 0 && issued == 0))
                             tma_load_2d(xst + x.s * kBoxBytes, &tmX, x0, r.r0 + j * row_step,
                                         x.bar(xfull), kBoxBytes);
                         x.next();
@@ -594,6 +597,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                                ((uint32_t)(kTN >> 3) << 17) | ((uint32_t)(kTM >> 4) << 24);
         const bool leader = elect_one();
         const uint64_t xdesc = smem_desc(xst), wdesc = smem_desc(wst);
+        if (!a.early) dependency_wait();   /* no wait below lasts as long as that launch */
         Ring<kXStages> x;
         Ring<kWSlots> wq;
         Ring<kAccs> ac;
@@ -787,18 +791,21 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             if (tid < kEpiWarp0t * 32 + b1 - b0)
                 mbar_arrive(wfull + 8 * (tid - kEpiWarp0t * 32));
         }
+        if (!a.early) dependency_wait();
         if (has_res) next_fetch(0);
         int cb = turn;
         while (ok && next_run(a, sh, r)) {
             const int i0 = r.fb * kTN, hi = r.hi, e = r.e;
-            if (!TRANS) {
-                asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
-                const int f = tid - kEpiWarp0t * 32;
-                if (f < kTN)
-                    s_bias[f] = a.bias && i0 + f < a.n_out
-                                    ? to_f(((const T*)a.bias)[(long long)e * a.n_out + i0 + f])
-                                    : 0.0f;
-                asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+            /* a lane keeps the bias of four features, the others ask it */
+            const bool has_bias = !TRANS && a.bias;
+            uint32_t mybias[2] = {0, 0};
+            if (has_bias) {
+                const int n = a.n_out - i0 - 4 * lane;
+                const uint16_t* p =
+                    (const uint16_t*)a.bias + (long long)e * a.n_out + i0 + 4 * lane;
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    if (h < n) mybias[h >> 1] |= (uint32_t)__ldg(p + h) << (16 * (h & 1));
             }
             int row0 = r.r0 + 32 * (int)tq;
             for (int j = r.ntiles; j > 0 && ok; --j, row0 += row_step, ac.next()) {
@@ -845,11 +852,12 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
 #pragma unroll
                     for (int h = 0; h < 4; ++h) u[h] = make_float2(v[8 * c + 2 * h], v[8 * c + 2 * h + 1]);
                     if (!TRANS) {
-                        const float4* b = (const float4*)&s_bias[fw + 8 * c];
-                        u[0] = add2(u[0], make_float2(b[0].x, b[0].y));
-                        u[1] = add2(u[1], make_float2(b[0].z, b[0].w));
-                        u[2] = add2(u[2], make_float2(b[1].x, b[1].y));
-                        u[3] = add2(u[3], make_float2(b[1].z, b[1].w));
+                        if (has_bias)
+#pragma unroll
+                            for (int h = 0; h < 4; ++h)
+                                u[h] = add2(u[h], unpack2<T>(__shfl_sync(
+                                                      0xffffffffu, mybias[h & 1],
+                                                      8 * cb + 2 * c + (h >> 1))));
                         /* the row's residual makes room for its z */
                         if (has_z)
                             sts128(at, pack2<T>(u[0].x, u[0].y), pack2<T>(u[1].x, u[1].y),
@@ -1006,7 +1014,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
             ok = mm_wait(x.bar(empty0), x.round ^ 1, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            if (leader) {
+            if (leader && !(g_mm_withhold && blockIdx.x == 0 && g == 0)) {
                 const int r = rg.r0 + g * kGRows;
                 const uint32_t st = st0 + x.s * STAGE, bar = x.bar(full0);
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
@@ -1376,6 +1384,13 @@ int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, bool dependent, cu
 {
     return dtype == DIA_F16 ? launch_grad_act<__half>(a, dtype, make, dependent, stream)
                             : launch_grad_act<__nv_bfloat16>(a, dtype, make, dependent, stream);
+}
+
+cudaError_t spmm_tc_test_wait(unsigned long long wait_ns, int withhold)
+{
+    if (wait_ns == 0) wait_ns = kMmWaitNs;
+    const cudaError_t e = cudaMemcpyToSymbol(g_mm_wait_ns, &wait_ns, sizeof(wait_ns));
+    return e != cudaSuccess ? e : cudaMemcpyToSymbol(g_mm_withhold, &withhold, sizeof(withhold));
 }
 
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear)

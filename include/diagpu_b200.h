@@ -487,15 +487,16 @@ int dia_dist_set_timeout(DiaDist* dist, int64_t ns);
 int dia_dist_status(DiaDist* dist, unsigned int* flags, int clear);
 
 /* Device status word shared by the library's kernels.  Kernels that wait on
- * the hardware (the tcgen05 dense-band kernel's mbarrier waits) never spin
+ * the hardware (the tcgen05 kernels' mbarrier waits) never spin
  * without bound: on giving up they set a bit here and return early.  Reads
  * the word into *flags (synchronous); clear != 0 resets it.  No counterpart
  * in the reference, whose kernels have no waits. */
 enum { DIA_TC_TIMEOUT = 1 };
 int dia_device_status(unsigned int* flags, int clear);
-/* Test hook of the tcgen05 dense-band kernel (current device): wait_ns sets
- * the limit of each of its waits (0: the default of 2 s); withhold != 0
- * makes one warp of its first CTA skip one arrival, so a wait is certain to
+/* Test hook of the tcgen05 kernels (current device): wait_ns sets
+ * the limit of each of their waits (0: the default of 2 s); withhold != 0
+ * makes the first CTA skip one arrival (dense band) or copy (block-vector
+ * product and gradient), so a wait is certain to
  * run out and the kernel's abort path (stop, drain issued copies and MMAs,
  * free tensor memory, set DIA_TC_TIMEOUT) runs.  Both persist until the
  * next call; reset with (0, 0).  Not for production use. */

@@ -586,3 +586,65 @@ def test_refusals_on_the_device():
     work = torch.empty(ws + 1, dtype=torch.uint8, device="cuda")[1:]
     refused(dg.DIA_ERR_INVALID, dg.spmm_backward, plan, v, x, c.dy, z=c.zin, act="silu",
             work=work)
+
+
+def test_a_wait_that_runs_out():
+    """Failure detection without a fault: with a limit of 1 ms and one copy
+    withheld, the tensor-core product and gradient stop, report DIA_TC_TIMEOUT
+    and leave the GPU usable: the next calls are right."""
+    L = dg.lib()
+    c = Case(torch.bfloat16, 600, 264, 264, band(6), seed=23)
+    dg.check(L.dia_test_spmm_form(2))
+    try:
+        dg.device_status(clear=True)
+        for f in (lambda: dg.spmm(c.plan, c.vals[0], c.x, act="silu"),
+                  lambda: dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=c.zin, act="silu"),
+                  lambda: dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy)):
+            dg.check(L.dia_test_tc_wait(1_000_000, 1))
+            try:
+                f()
+                torch.cuda.synchronize()
+            finally:
+                dg.check(L.dia_test_tc_wait(0, 0))
+            assert dg.device_status(clear=True) & dg.DIA_TC_TIMEOUT
+            c.product(act="silu", bias=True, res=True)
+            c.gradient(act="silu")
+            assert dg.device_status() == 0
+    finally:
+        dg.check(L.dia_test_spmm_form(0))
+
+
+@pytest.mark.parametrize("n,m,off", [(0, 8, [0, 1]), (8, 0, [0, -1]), (0, 0, []), (0, 0, [0])])
+@pytest.mark.parametrize("M", [0, 3, 200])
+def test_empty_sides(M, n, m, off, t):
+    c = Case(t, M, n, m, off, seed=24)
+    c.product(act="relu", bias=True, res=True, z=True)
+    c.gradient(act="relu")
+
+
+@pytest.mark.parametrize("M", [4, 300])
+def test_single_gradients(M, t):
+    """The C entry's outputs may each be left out: the others stay the same."""
+    c = Case(t, M, 136, 144, band(5), seed=25)
+    L, code = dg.lib(), {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[t]
+    dx, dv, db = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=c.zin, act="silu",
+                                  bias_grad=True)
+    st = c.vals.shape[-1]
+    ws = L.dia_spmm_backward_workspace(c.plan._h, code, M, 1, 144, st, 136, 2)
+    work = torch.empty(ws, dtype=torch.uint8, device="cuda")
+    for want in (dx, dv, db):
+        out = torch.full_like(want, 9.0)
+        p = [o.data_ptr() if w is want else None for w, o in ((dx, out), (dv, out), (db, out))]
+        for x in (c.x.data_ptr(),) if want is dv else (c.x.data_ptr(), None):
+            out.fill_(9.0)
+            dg.check(L.dia_spmm_backward(c.plan._h, code, M, 1, None, x, 144,
+                                         c.vals.data_ptr() if want is dx else None, st,
+                                         c.dy.data_ptr(), 136, 2, c.zin.data_ptr(), 136, p[0], 144,
+                                         p[1], p[2], work.data_ptr(), ws,
+                                         torch.cuda.current_stream().cuda_stream))
+            u = unit(t)
+            # dbias alone is summed on the CUDA cores, in another order
+            assert bool(((out.double() - want.double()).abs()
+                         <= 2 * u * want.double().abs() + (M + 4) * sum_unit(t) * 200).all())
+            if want is not db:
+                assert torch.equal(out, want)
