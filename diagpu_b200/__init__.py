@@ -809,31 +809,35 @@ def _spmm_act(who, act):
     return code
 
 
-def _spmm_new(made, like, shape, dtype=None):
-    made.append(like.new_empty(shape, dtype=dtype))
-    return made[-1]
+def _spmm_new(stream, like, shape, dtype=None):
+    """A tensor that a call on `stream` writes: out of that stream's memory
+    (the current stream's may still be in use there by earlier work), kept from
+    reuse until the current stream has passed the point where it is freed."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    current = torch.cuda.current_stream(like.device)
+    with torch.cuda.stream(stream):
+        t = like.new_empty(shape, dtype=dtype)
+    t.record_stream(current)
+    return t
 
 
-def _spmm_work(who, made, work, need, plan, like):
+def _spmm_work(who, stream, work, need, plan, like):
     """(pointer, bytes) of the workspace, made here if need be."""
     if work is None:
         if need <= 0:
             return None, 0
-        return _spmm_new(made, like, (need,), torch.uint8).data_ptr(), need
+        return _spmm_new(stream, like, (need,), torch.uint8).data_ptr(), need
     if work.dtype != torch.uint8 or work.device != plan.device or not work.is_contiguous():
         raise DiaError(DIA_ERR_INVALID, f"{who}: work must be a contiguous uint8 tensor on "
                                         f"{plan.device}")
     return work.data_ptr(), work.numel()
 
 
-def _spmm_stream(plan, stream, made):
-    """The raw stream of a call.  Tensors that the call allocated come from the
-    current stream: on another one they stay allocated until it has passed the
-    call."""
+def _spmm_stream(plan, stream):
+    """The raw stream of a call."""
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(plan.device.index)
-    for t in made:
-        t.record_stream(stream)
     return stream.cuda_stream
 
 
@@ -859,9 +863,10 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
     rows [seg[e], seg[e + 1]) of the block meet expert e; rows outside every
     expert are left as they were (unset in a new out).  act: "none", "relu",
     "silu", "gelu", "gelu_tanh".  Returns out [M, n_rows], or (out, z) with
-    save_z or a given z: the pre-activation that spmm_backward takes.  work:
+    save_z or a given z: the pre-activation that spmm_backward takes.  out and z
+    must not overlap the inputs, except that out may be residual.  work:
     uint8 buffer of spmm_workspace bytes, for callers that allocate nothing."""
-    who, made = "spmm", []
+    who = "spmm"
     code = _spmm_act(who, act)
     dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
     t, M, n = x.dtype, x.shape[0], plan.n_rows
@@ -869,17 +874,17 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
     bp = _spmm_vector(who, "bias", bias, plan, t, (n,) if seg is None else (E, n))
     rp, ldr = _spmm_block(who, "residual", residual, plan, t, M, n)
     if out is None:
-        out = _spmm_new(made, x, (M, n))
+        out = _spmm_new(stream, x, (M, n))
     yp, ldy = _spmm_block(who, "out", out, plan, t, M, n)
     if z is None and save_z:
-        z = _spmm_new(made, x, (M, n))
+        z = _spmm_new(stream, x, (M, n))
     zp, ldz = _spmm_block(who, "z", z, plan, t, M, n)
     L = lib()
-    wp, wbytes = _spmm_work(who, made, work, L.dia_spmm_workspace(plan._h, dt, M, E, ldx), plan,
+    wp, wbytes = _spmm_work(who, stream, work, L.dia_spmm_workspace(plan._h, dt, M, E, ldx), plan,
                             x)
     rc = L.dia_spmm(plan._h, dt, M, E, None if seg is None else seg.data_ptr(), xp, ldx,
                     vals.data_ptr(), stride, bp, code, rp, ldr, zp, ldz, yp, ldy, wp, wbytes,
-                    _spmm_stream(plan, stream, made))
+                    _spmm_stream(plan, stream))
     if rc:
         check(rc)
     return out if z is None else (out, z)
@@ -891,9 +896,10 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
     """Gradients (dx, dvals, dbias) of spmm for dy, the gradient of its result
     (dia_spmm_backward); that of the residual is dy.  z is what spmm saved, not
     wanted for act "none".  dvals has the shape of vals, with zeros outside the
-    matrix; dbias is None unless bias_grad or given.  work: uint8 buffer of
-    spmm_backward_workspace bytes, for callers that allocate nothing."""
-    who, made = "spmm_backward", []
+    matrix; dbias is None unless bias_grad or given.  Outputs must not overlap
+    inputs.  work: uint8 buffer of spmm_backward_workspace bytes, for callers
+    that allocate nothing."""
+    who = "spmm_backward"
     code = _spmm_act(who, act)
     dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
     t, M, n = x.dtype, x.shape[0], plan.n_rows
@@ -904,20 +910,20 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
     zp, ldz = _spmm_block(who, "z", z, plan, t, M, n) if code else (None, n)
     bshape = (n,) if seg is None else (E, n)
     if dx is None:
-        dx = _spmm_new(made, x, (M, plan.n_cols))
+        dx = _spmm_new(stream, x, (M, plan.n_cols))
     if dvals is None:
-        dvals = _spmm_new(made, x, vals.shape)
+        dvals = _spmm_new(stream, x, vals.shape)
     if dbias is None and bias_grad:
-        dbias = _spmm_new(made, x, bshape)
+        dbias = _spmm_new(stream, x, bshape)
     dxp, lddx = _spmm_block(who, "dx", dx, plan, t, M, plan.n_cols)
     dvp = _spmm_vector(who, "dvals", dvals, plan, t, vals.shape)
     dbp = _spmm_vector(who, "dbias", dbias, plan, t, bshape)
     L = lib()
     need = L.dia_spmm_backward_workspace(plan._h, dt, M, E, ldx, stride, lddy, code)
-    wp, wbytes = _spmm_work(who, made, work, need, plan, x)
+    wp, wbytes = _spmm_work(who, stream, work, need, plan, x)
     rc = L.dia_spmm_backward(plan._h, dt, M, E, None if seg is None else seg.data_ptr(), xp, ldx,
                              vals.data_ptr(), stride, gp, lddy, code, zp, ldz, dxp, lddx, dvp,
-                             dbp, wp, wbytes, _spmm_stream(plan, stream, made))
+                             dbp, wp, wbytes, _spmm_stream(plan, stream))
     if rc:
         check(rc)
     return dx, dvals, dbias

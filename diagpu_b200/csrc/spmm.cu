@@ -21,7 +21,6 @@
 #include <climits>
 #include <cstring>
 #include <new>
-#include <numeric>
 #include <vector>
 
 #include "dia_core.cuh"
@@ -33,40 +32,59 @@ namespace dia {
  * wherever they can run */
 static std::atomic<int> g_form{0};
 
-static bool tensor_form(int dtype, long long M, int E, const SpmmDir& d)
+/* Which form a call takes: the one whose time, by the measured costs of both,
+ * is shorter (16-bit types, one B200; over 176 calls of 8 to 4096 rows, 3 to
+ * 129 diagonals, 1 to 64 experts the form taken is 4 % slower than the better
+ * one on average).
+ *
+ * CUDA cores, us.  Few rows: 7 for every million (row, feature, group of four
+ * offsets).  Many: a wave of CTAs takes 15 + 0.4 K, then every million
+ * features 5.5 + 0.2 K.
+ * Tensor cores: the operator's boxes are packed and read (4 ns each, 10 where
+ * they no longer fit L2) and every tile has a way through the kernel; a packing
+ * launch of its own 2.5 us.
+ * 4096 x 129 diagonals: cores 63 us, tensor cores 12 at 64 rows; 27-point
+ * stencil on 262144: 31 and 323 at 8 rows, 387 and 374 at 128.  The gradients
+ * favour the cores a little more (65536, 33 scattered diagonals, 128 rows: 180
+ * and 214). */
+static bool tensor_form(const DiaSpmmPlan* p, int dtype, long long M, int E, bool backward)
 {
     const int form = g_form.load(std::memory_order_relaxed);
+    const SpmmDir& d = p->fwd;
     if (dtype == DIA_F32 || d.nboxes == 0 || form == 1) return false;
     if (form == 2) return true;
-    /* Eight rows an expert pay for packing it and for a tile's way through the
-     * kernel (129 diagonals of 4096: 11 us against 51 on CUDA cores); with many
-     * experts, whose operators are packed for few rows each, more do (64 of
-     * 1024 x 33, 16 rows each: 28 against 26; 64 rows each: 38 against 48). */
-    return M >= (long long)E * std::max(8, E / 2);
+    if (M < 8) return false;   /* the cores' time does not grow up to there */
+    const double nfb = (p->n_rows + 127) / 128, boxes = nfb * E * d.nboxes;
+    const double tiles = nfb * (M / 128.0 + (E > 1 ? (double)std::min<long long>(E, M) : 1.0));
+    const double mega = (double)M * p->n_rows * 1e-6;
+    const double cores = mega < 0.2 ? 6 + 7 * mega * d.nquads
+                                    : std::max(15 + 0.4 * p->K, (5.5 + 0.2 * p->K) * mega);
+    const double tensor = 8 + (E > 1 || d.nboxes > 6 ? 2.5 : 0.0) + 0.004 * boxes +
+                          0.006 * std::max(0.0, boxes - 2500) + 0.02 * tiles;
+    return (backward ? 0.8 : 1.0) * cores > tensor;
 }
 
 static size_t elem_size(int dtype) { return dtype == DIA_F32 ? 4 : 2; }
 
 /* the tensor-core form it is (its operator has to be packed first) */
-static bool product_on_tc(const ProdArgs& a, int dtype)
+static bool product_on_tc(const ProdArgs& a, bool tensor)
 {
-    return a.M > 0 && a.n_out > 0 && a.n_in > 0 && tensor_form(dtype, a.M, a.E, a.dir) &&
-           spmm_tc_block(a.in, a.ldi);
+    return a.M > 0 && a.n_out > 0 && a.n_in > 0 && tensor && spmm_tc_block(a.in, a.ldi);
 }
 
 template <typename T>
-static int launch_product(const ProdArgs& a, int dtype, cudaStream_t stream)
+static int launch_product(const ProdArgs& a, int dtype, bool tensor, cudaStream_t stream)
 {
     if (a.M == 0 || a.n_out == 0) return DIA_OK;
-    if (product_on_tc(a, dtype)) return spmm_tc_product(a, dtype, stream);
+    if (product_on_tc(a, tensor)) return spmm_tc_product(a, dtype, stream);
     return Cores<T>::product(a, stream);
 }
 
 /* rows of a part of the gradient's sum: enough parts to fill the GPU, none
  * so short that writing and joining its sums costs more than it saves */
-static int grad_part_rows(const DiaSpmmPlan* p, int dtype, long long M, int E, long long stride)
+static int grad_part_rows(const DiaSpmmPlan* p, bool tensor, long long M, int E, long long stride)
 {
-    if (tensor_form(dtype, M, E, p->fwd)) {
+    if (tensor) {
         /* one CTA an SM; an expert's last part is half full on average (8
          * experts, 4096 rows, 2048 features: 47 us at 704 rows a part, 53 at
          * 384, 61 at 2048) */
@@ -86,9 +104,9 @@ static int grad_part_rows(const DiaSpmmPlan* p, int dtype, long long M, int E, l
 /* parts of experts that have several: at most two a `per` rows */
 static long long grad_slots(long long M, long long per) { return M > per ? 2 * (M / per) + 1 : 0; }
 
-static bool grad_on_tc(const GradArgs& a, int dtype)
+static bool grad_on_tc(const GradArgs& a, bool tensor)
 {
-    return tensor_form(dtype, a.M, a.E, a.dir) && a.M > 0 && a.n_cols > 0 && a.n_rows > 0 &&
+    return tensor && a.M > 0 && a.n_cols > 0 && a.n_rows > 0 &&
            a.dvals && spmm_tc_block(a.dz, a.lddz) && spmm_tc_block(a.x, a.ldx);
 }
 
@@ -259,24 +277,24 @@ static SpmmDir dir_on_device(const void* blob, SpmmDir d)
 static int check_common(const char* who, const DiaSpmmPlan* p, int dtype, int64_t M, int E,
                         const int64_t* seg, int act, int64_t stride, const void* vals)
 {
-    const std::string w = std::string(who) + ": ";
-    if (dtype != DIA_F32 && dtype != DIA_F16 && dtype != DIA_BF16)
-        return fail(DIA_ERR_INVALID, w + "unknown dtype");
-    if (act < DIA_ACT_NONE || act > DIA_ACT_GELU_TANH)
-        return fail(DIA_ERR_INVALID, w + "unknown activation");
-    if (M < 0 || M > INT_MAX / 2) return fail(DIA_ERR_INVALID, w + "bad number of rows");
-    if (E < 1 || E > (1 << 20)) return fail(DIA_ERR_INVALID, w + "bad number of experts");
-    if (E > 1 && !seg) return fail(DIA_ERR_INVALID, w + "experts without seg");
-    if (!p) return fail(DIA_ERR_INVALID, w + "null plan");
+    auto bad = [&](const char* what) {
+        return fail(DIA_ERR_INVALID, std::string(who) + ": " + what);
+    };
+    if (dtype != DIA_F32 && dtype != DIA_F16 && dtype != DIA_BF16) return bad("unknown dtype");
+    if (act < DIA_ACT_NONE || act > DIA_ACT_GELU_TANH) return bad("unknown activation");
+    if (M < 0 || M > INT_MAX / 2) return bad("bad number of rows");
+    if (E < 1 || E > (1 << 20)) return bad("bad number of experts");
+    if (E > 1 && !seg) return bad("experts without seg");
+    if ((uintptr_t)seg % sizeof(int64_t)) return bad("seg is misaligned");
+    if (!p) return bad("null plan");
     int dev = -1;
     DIA_TRY_CUDA(cudaGetDevice(&dev));
-    if (dev != p->device)
-        return fail(DIA_ERR_INVALID, w + "the plan belongs to another device");
+    if (dev != p->device) return bad("the plan belongs to another device");
     if (stride < p->n_rows || stride % 32 != 0)
-        return fail(DIA_ERR_INVALID, w + "stride must be a multiple of 32, at least n_rows");
-    if (stride > INT_MAX / 2) return fail(DIA_ERR_UNSUPPORTED, w + "stride too large");
-    if (p->K > 0 && p->n_rows > 0 && !vals) return fail(DIA_ERR_INVALID, w + "null values");
-    if ((uintptr_t)vals % 16) return fail(DIA_ERR_INVALID, w + "values must be 16-byte aligned");
+        return bad("stride must be a multiple of 32, at least n_rows");
+    if (stride > INT_MAX / 2) return bad("stride too large");
+    if (p->K > 0 && p->n_rows > 0 && !vals) return bad("null values");
+    if ((uintptr_t)vals % 16) return bad("values must be 16-byte aligned");
     return DIA_OK;
 }
 
@@ -284,12 +302,21 @@ static int check_common(const char* who, const DiaSpmmPlan* p, int dtype, int64_
 static int check_block(const char* who, const char* name, const void* ptr, int64_t ld, int64_t M,
                        int n, int dtype)
 {
-    const std::string w = std::string(who) + ": " + name;
+    auto bad = [&](const char* what) {
+        return fail(DIA_ERR_INVALID, std::string(who) + ": " + name + what);
+    };
     if (M == 0 || n == 0) return DIA_OK;
-    if (!ptr) return fail(DIA_ERR_INVALID, w + " is null");
-    if (M > 1 && ld < n) return fail(DIA_ERR_INVALID, w + " has rows shorter than its width");
-    if ((uintptr_t)ptr % elem_size(dtype)) return fail(DIA_ERR_INVALID, w + " is misaligned");
+    if (!ptr) return bad(" is null");
+    if (M > 1 && ld < n) return bad(" has rows shorter than its width");
+    if ((uintptr_t)ptr % elem_size(dtype)) return bad(" is misaligned");
     return DIA_OK;
+}
+
+/* a vector for each expert, or NULL */
+static int check_vector(const char* who, const char* name, const void* ptr, int dtype)
+{
+    if ((uintptr_t)ptr % elem_size(dtype) == 0) return DIA_OK;
+    return fail(DIA_ERR_INVALID, std::string(who) + ": " + name + " is misaligned");
 }
 
 template <typename F>
@@ -303,18 +330,17 @@ static int by_type(int dtype, F f)
 static long long align256(long long b) { return (b + 255) / 256 * 256; }
 
 /* the operator in tensor-core form */
-static long long pack_bytes(const SpmmDir& d, int K, int dtype, int64_t M, int E, int n_out)
+static long long pack_bytes(const SpmmDir& d, int K, bool tensor, int64_t M, int E, int n_out)
 {
-    return M > 0 && n_out > 0 && tensor_form(dtype, M, E, d)
+    return M > 0 && n_out > 0 && tensor
                ? align256(spmm_tc_pack_bytes(d, K, n_out, M, E)) : 0;
 }
 
 /* a copy of a block whose rows are not multiples of 16 bytes apart, which the
  * tensor-core form reads instead */
-static long long copy_bytes(const SpmmDir& d, int dtype, int64_t M, int E, int n, int64_t ld)
+static long long copy_bytes(bool tensor, int64_t M, int n, int64_t ld)
 {
-    return M > 0 && ld % 8 != 0 && tensor_form(dtype, M, E, d)
-               ? align256(M * ((n + 7) / 8 * 8) * (long long)elem_size(dtype)) : 0;
+    return M > 0 && ld % 8 != 0 && tensor ? align256(M * ((n + 7) / 8 * 8) * 2ll) : 0;
 }
 
 /* the gradient's workspace: dz (where the activation makes one, or as a copy
@@ -322,7 +348,7 @@ static long long copy_bytes(const SpmmDir& d, int dtype, int64_t M, int E, int n
  * copy of x */
 struct GradPlan {
     int per;
-    bool made;
+    bool tensor, made;
     long long lddz, dz_bytes, part_bytes, pack_bytes, x_bytes;
     long long bytes() const { return dz_bytes + part_bytes + pack_bytes + x_bytes; }
 };
@@ -331,13 +357,14 @@ static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int E, int
                           int64_t stride, int64_t lddy, int act)
 {
     GradPlan g;
-    g.per = grad_part_rows(p, dtype, M, E, stride);
+    g.tensor = tensor_form(p, dtype, M, E, true);
+    g.per = grad_part_rows(p, g.tensor, M, E, stride);
     g.lddz = (p->n_rows + 7) / 8 * 8;
-    g.made = act != DIA_ACT_NONE || copy_bytes(p->fwd, dtype, M, E, p->n_rows, lddy) > 0;
+    g.made = act != DIA_ACT_NONE || copy_bytes(g.tensor, M, p->n_rows, lddy) > 0;
     g.dz_bytes = g.made ? align256(M * g.lddz * (long long)elem_size(dtype)) : 0;
     g.part_bytes = align256(grad_slots(M, g.per) * (p->K + 1) * stride * 4);
-    g.pack_bytes = pack_bytes(p->trn, p->K, dtype, M, E, p->n_cols);
-    g.x_bytes = copy_bytes(p->fwd, dtype, M, E, p->n_cols, ldx);
+    g.pack_bytes = pack_bytes(p->trn, p->K, g.tensor, M, E, p->n_cols);
+    g.x_bytes = copy_bytes(g.tensor, M, p->n_cols, ldx);
     return g;
 }
 
@@ -415,9 +442,11 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
     if (rc == DIA_OK) rc = check_block(who, "y", d_y, ldy, M, plan->n_rows, dtype);
     if (rc == DIA_OK && d_res) rc = check_block(who, "residual", d_res, ldr, M, plan->n_rows, dtype);
     if (rc == DIA_OK && d_z) rc = check_block(who, "z", d_z, ldz, M, plan->n_rows, dtype);
+    if (rc == DIA_OK) rc = check_vector(who, "bias", d_bias, dtype);
     if (rc != DIA_OK) return rc;
-    const long long pack = pack_bytes(plan->fwd, plan->K, dtype, M, num_experts, plan->n_rows);
-    const long long copy = copy_bytes(plan->fwd, dtype, M, num_experts, plan->n_cols, ldx);
+    const bool tensor = tensor_form(plan, dtype, M, num_experts, false);
+    const long long pack = pack_bytes(plan->fwd, plan->K, tensor, M, num_experts, plan->n_rows);
+    const long long copy = copy_bytes(tensor, M, plan->n_cols, ldx);
     const long long need = pack + copy;
     if (need > work_bytes) return fail(DIA_ERR_CAPACITY, "dia_spmm: workspace too small");
     if (need > 0 && (!d_work || (uintptr_t)d_work % 256))
@@ -454,11 +483,11 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
             r = Cores<T>::dz(DIA_ACT_NONE, d_x, ldx, nullptr, 0, (char*)d_work + pack, a.ldi, a.M,
                              a.n_in, false, stream);
         }
-        if (r == DIA_OK && product_on_tc(a, dtype)) {
+        if (r == DIA_OK && product_on_tc(a, tensor)) {
             r = spmm_tc_pack(a, false, stream);
             a.dependent = pack > 0;
         }
-        return r == DIA_OK ? launch_product<T>(a, dtype, stream) : r;
+        return r == DIA_OK ? launch_product<T>(a, dtype, tensor, stream) : r;
     });
 }
 
@@ -466,8 +495,9 @@ extern "C" int64_t dia_spmm_workspace(const DiaSpmmPlan* plan, int dtype, int64_
                                       int num_experts, int64_t ldx)
 {
     if (!plan || M < 0 || M > INT_MAX / 2 || num_experts < 1) return -1;
-    return pack_bytes(plan->fwd, plan->K, dtype, M, num_experts, plan->n_rows) +
-           copy_bytes(plan->fwd, dtype, M, num_experts, plan->n_cols, ldx);
+    const bool tensor = tensor_form(plan, dtype, M, num_experts, false);
+    return pack_bytes(plan->fwd, plan->K, tensor, M, num_experts, plan->n_rows) +
+           copy_bytes(tensor, M, plan->n_cols, ldx);
 }
 
 extern "C" int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
@@ -495,6 +525,9 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
     if (rc == DIA_OK && act != DIA_ACT_NONE)
         rc = check_block(who, "z", d_z, ldz, M, plan->n_rows, dtype);
     if (rc == DIA_OK && d_dx) rc = check_block(who, "dx", d_dx, lddx, M, plan->n_cols, dtype);
+    if (rc == DIA_OK) rc = check_vector(who, "dbias", d_dbias, dtype);
+    if (rc == DIA_OK && (uintptr_t)d_dvals % 16)
+        rc = fail(DIA_ERR_INVALID, "dia_spmm_backward: dvals must be 16-byte aligned");
     if (rc != DIA_OK) return rc;
     const GradPlan g = grad_plan(plan, dtype, M, num_experts, ldx, stride, lddy, act);
     if (g.bytes() > work_bytes)
@@ -557,7 +590,8 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
         /* Launches of the tensor-core form overlap.  Where the diagonals'
          * gradient makes dz itself it goes first, the operator is packed on
          * the SMs that it leaves free; else the operator is packed under dz. */
-        const bool tc = d_dx && product_on_tc(p, dtype), gtc = grad && grad_on_tc(a, dtype);
+        const bool tc = d_dx && product_on_tc(p, g.tensor);
+        const bool gtc = grad && grad_on_tc(a, g.tensor);
         const bool makes = gtc && made && spmm_tc_makes_dz(a);
         if (r != DIA_OK) return r;
         if (makes) {
@@ -576,7 +610,7 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
             p.early = tc && gtc;   /* what it reads is older than the gradient */
             p.dependent = packed || made || grad;
         }
-        if (r == DIA_OK && d_dx) r = launch_product<T>(p, dtype, stream);
+        if (r == DIA_OK && d_dx) r = launch_product<T>(p, dtype, g.tensor, stream);
         if (r == DIA_OK && grad) r = Cores<T>::join(a, stream);
         return r;
     });

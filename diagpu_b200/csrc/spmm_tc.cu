@@ -206,16 +206,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32])
         : "memory");
 }
 
-/* one column of them */
-__device__ __forceinline__ float tmem_ld1(uint32_t addr)
-{
-    float v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\t"
-                 "tcgen05.wait::ld.sync.aligned;"
-                 : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-
 /* ------------------------------------------------------ pairs of elements */
 
 template <typename T>

@@ -223,8 +223,9 @@ int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
  *   dvals[e,k,i] = sum_t dz[t,i] x[t,i+off[k]]  (whole stride: 0 outside the
  *   matrix and in the padding; 0 for an expert without rows),
  *   dbias[e,i] = sum_t dz[t,i].
- * dx, dvals and dbias may each be NULL; act DIA_ACT_NONE takes no z.  Outputs
- * are overwritten, rows of dx outside [seg[0], seg[num_experts]) left as they
+ * dx, dvals (16-byte aligned) and dbias may each be NULL; act DIA_ACT_NONE
+ * takes no z.  Outputs must not overlap inputs or one another; they are
+ * overwritten, rows of dx outside [seg[0], seg[num_experts]) left as they
  * were.  work: dia_spmm_backward_workspace bytes, 256-byte aligned, not shared
  * by calls that may run at the same time. */
 int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,

@@ -648,3 +648,54 @@ def test_single_gradients(M, t):
                          <= 2 * u * want.double().abs() + (M + 4) * sum_unit(t) * 200).all())
             if want is not db:
                 assert torch.equal(out, want)
+
+
+def test_refused_gradient_buffers():
+    c = Case(torch.bfloat16, 20, 64, 64, band(2), seed=17)
+    odd = torch.zeros(5 * 64 + 1, dtype=c.x.dtype, device="cuda")[1:].view(5, 64)
+    with pytest.raises(dg.DiaError) as e:
+        dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, dvals=odd)
+    assert e.value.code == dg.DIA_ERR_INVALID
+
+
+def test_results_on_another_stream_have_their_own_memory():
+    """What a call on a given stream allocates is not memory that the current
+    stream still writes."""
+    c = Case(torch.bfloat16, 256, 512, 512, band(3), seed=41)
+    want = dg.spmm(c.plan, c.vals[0], c.x)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        old = [torch.empty_like(want) for _ in range(4)]
+        torch.cuda._sleep(20_000_000)
+        for o in old:
+            o.fill_(float("nan"))
+        del old, o
+        got = dg.spmm(c.plan, c.vals[0], c.x, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M,tensor", [(8, False), (1024, True)])
+def test_wide_operators(M, tensor):
+    """Few rows under an operator of many boxes stay on the CUDA cores, which
+    want no workspace; either form's sums are the same to rounding."""
+    n, side = 32768, 32
+    off = [i + side * j + side * side * k
+           for i in (-1, 0, 1) for j in (-1, 0, 1) for k in (-1, 0, 1)]
+    c = Case(torch.bfloat16, M, n, n, off, seed=43)
+    assert (dg.spmm_workspace(c.plan, c.vals[0], c.x) > 0) == tensor
+    got = dg.spmm(c.plan, c.vals[0], c.x).double()
+    want = torch.zeros(M, n, dtype=torch.float64, device="cuda")
+    size = torch.zeros(M, n, dtype=torch.float64, device="cuda")
+    x, v = c.x.double(), c.vals[0].double()
+    for k, d in enumerate(off):
+        lo, hi = max(0, -d), min(n, n - d)
+        p = v[k, lo:hi] * x[:, lo + d:hi + d]
+        want[:, lo:hi] += p
+        size[:, lo:hi] += p.abs()
+    # the result's rounding to bf16, and 27 fp32 additions, each off by at most
+    # a step (the tensor cores may cut off instead of rounding)
+    u = unit(c.x.dtype)
+    limit = u * want.abs() + (1 + u) * 27 * 2.0 ** -23 * size
+    assert ((got - want).abs() <= limit).all()
