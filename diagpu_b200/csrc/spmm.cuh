@@ -197,6 +197,13 @@ __device__ __forceinline__ float act_of(float z)
     return z;
 }
 
+/* beyond +-16 the tanh form's derivative is 0 or 1, while its z^2 may overflow
+ * (NaN stays NaN) */
+__device__ __forceinline__ float within16(float z)
+{
+    return z > 16.0f ? 16.0f : (z < -16.0f ? -16.0f : z);
+}
+
 template <int ACT>
 __device__ __forceinline__ float dact_of(float z)
 {
@@ -208,6 +215,7 @@ __device__ __forceinline__ float dact_of(float z)
     if (ACT == DIA_ACT_GELU)
         return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
     if (ACT == DIA_ACT_GELU_TANH) {
+        z = within16(z);
         const float t = tanhf(0.79788456f * z * fmaf(0.044715f * z, z, 1.0f));
         return 0.5f * (1.0f + t) +
                0.5f * z * (1.0f - t * t) * 0.79788456f * fmaf(0.134145f * z, z, 1.0f);
@@ -329,6 +337,7 @@ __device__ __forceinline__ float2 dact2(float2 z)
         return fma2(mul2(z, both(0.39894228f)), e, c);
     }
     if (ACT == DIA_ACT_GELU_TANH) {
+        z = make_float2(within16(z.x), within16(z.y));
         const float2 w = mul2(z, both(0.044715f));
         const float2 u = mul2(z, fma2(w, z, both(1.0f)));
         const float2 s = logistic2(u, -2.0f * 0.79788456f * 1.44269504f);

@@ -699,3 +699,24 @@ def test_wide_operators(M, tensor):
     u = unit(c.x.dtype)
     limit = u * want.abs() + (1 + u) * 27 * 2.0 ** -23 * size
     assert ((got - want).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("act", ACTS[1:])
+def test_lowest_and_largest_values(act, t):
+    """Pre-activations of the type's lowest and largest value, as masks leave
+    them: the activation is 0 or z, its derivative 0 or 1, exactly."""
+    M, n = 40, 136
+    c = Case(t, M, n, n, [0], seed=47)
+    top = torch.finfo(t).max
+    z = c.block(torch.zeros(M, n))
+    z[:, ::2], z[:, 1::2] = -top, top
+    c.vals[0, 0].fill_(0.0)
+    c.vals[0, 0, :n] = 1.0
+    y, zz = dg.spmm(c.plan, c.vals[0], z, act=act, save_z=True)
+    assert torch.equal(zz, z)
+    assert bool((y[:, ::2] == 0).all()) and bool((y[:, 1::2] == top).all())
+    dx, dv, _ = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=z, act=act)
+    dz = c.dy.clone()
+    dz[:, ::2] = 0
+    assert torch.equal(dx, dz)
+    assert bool(dv.isfinite().all())
