@@ -1,7 +1,8 @@
 /*
- * spmm.cuh -- what the two translation units of the block-vector product
- * (spmm.cu: CUDA-core kernels, plan and C entry points; spmm_tc.cu: tcgen05
- * kernels) share: the plan, argument blocks, activations, expert lookup.
+ * spmm.cuh -- what the translation units of the block-vector product share
+ * (spmm.cu: plan, choice of form and C entry points; spmm_f32, spmm_f16,
+ * spmm_bf16.cu: CUDA-core kernels of a type; spmm_tc.cu: tcgen05 kernels): the
+ * plan, argument blocks, activations, expert lookup.
  */
 #pragma once
 

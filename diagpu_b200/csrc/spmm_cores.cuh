@@ -20,7 +20,10 @@ namespace dia {
  * memory latencies, so the CTA's warps split the diagonals `ks` ways (four at
  * a time in flight each) and add up in shared memory in a fixed order, and
  * what the epilogue reads is fetched first.  The other 16 / ks warps take
- * other features. */
+ * other features.  One row of 4096 under 129 diagonals, bf16: 5.5 us; eight
+ * rows under 33, fp32: 6.3 us; 64 rows of 64 experts (1024, 33 diagonals,
+ * fp16): 10.1 us, all a launch and three or four dependent reads (their bytes
+ * take 0.1 to 0.7 us). */
 constexpr int kFewWarps = 16;
 constexpr int kFewOffs = 512;   /* offsets staged at once */
 
@@ -114,7 +117,9 @@ spmm_few_kernel(const __grid_constant__ ProdArgs a, int ks, int ftiles, long lon
  * next quad's first: for runs of consecutive offsets shared memory gives a
  * piece per sixteen products.  Otherwise (fewer than three diagonals a quad)
  * a lane owns features 32 apart and reads an input per product, without bank
- * conflicts at any offset.  Shared memory's bandwidth bounds both. */
+ * conflicts at any offset.  Shared memory's bandwidth bounds both: 64 rows of
+ * 262144 under a 27-point stencil, fp32, 150 us (3.0 products a picosecond,
+ * 1.08 TB/s of the 163 MB that memory has to give; 25 us at its rate). */
 constexpr int kTileRows = 8;    /* rows of a warp */
 constexpr int kTileSmem = 112 * 1024;   /* two CTAs an SM */
 
@@ -333,7 +338,8 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
  * of an expert's rows, `rows` of them at a time by way of shared memory, the
  * next ones on their way meanwhile; a warp keeps the sums of its eight
  * diagonals at its lanes' four features.  Sums of an expert with one part go
- * out at once, others to `part`. */
+ * out at once, others to `part`.  A product costs a read of shared memory, which
+ * bounds it: 511 rows of 4096 under 33 diagonals, fp32, 27 us. */
 constexpr int kGradSmem = 160 * 1024;     /* two buffers of at least eight rows */
 
 template <typename T, bool VEC, int ND>
@@ -435,8 +441,9 @@ spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins, int 
         }
 }
 
-/* Sums the parts of experts that have several, in the parts' order; four
- * columns a thread. */
+/* Sums the parts of experts that have several, in the parts' order, so that
+ * the bits do not depend on which CTA was first; four columns a thread (129
+ * diagonals of 4096, four parts: 8.5 MB in 4 to 7 us). */
 template <typename T>
 __global__ void __launch_bounds__(128) spmm_join_kernel(GradArgs a, int cblocks)
 {

@@ -18,6 +18,11 @@
  * of the next.  An operator of more boxes than shared memory holds is read
  * again for every four tiles.
  *
+ * 4096 rows of 4096 under 129 diagonals, bf16, bias, GELU, residual, z kept:
+ * 41 us (135 MB: 3.3 TB/s; 21 us at the memory's rate).  The epilogue's
+ * instructions and the first tile's latency bound it: a CTA has eight tiles,
+ * DRAM is 22 % busy, the tensor cores 10 %.
+ *
  * Zeros of a box meet inputs that no diagonal joins to its features; where
  * such an input is infinite or undefined, so is the sum.  A sum that is not
  * finite is therefore computed again from its terms alone (finite ones had no
@@ -896,7 +901,10 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
  * D = dz^T x is a 128 x 256 product over the rows of one part of an expert,
  * both operands as TMA leaves them (rows of features: MN-major).  Of D the
  * diagonals are the result; it is copied to shared memory, where a diagonal
- * is a run of consecutive features.
+ * is a run of consecutive features.  dy, z and x are read once.  4096 rows of
+ * 4096, 129 diagonals, bf16, GELU: 35 us for 114 MB (3.3 TB/s; DRAM 41 % busy,
+ * tensor cores 16 %).  One CTA an SM does not overlap its start, the making of
+ * dz and the diagonals' way out with its neighbour's stream.
  * Rows of the last stage that are not the part's are cleared in both operands
  * before the MMAs read them. */
 constexpr int kGRows = 64;                     /* rows of a stage */
