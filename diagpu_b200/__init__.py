@@ -20,7 +20,6 @@ there: its products take one vector.
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import os
 from dataclasses import dataclass
 
@@ -757,8 +756,6 @@ class SpmmPlan:
 
 def _spmm_block(who, name, t, plan, dtype, rows, width):
     """(pointer, row stride) of a [rows, width] block with adjacent features."""
-    if t is None:
-        return None, width
     if t.dtype != dtype or t.device != plan.device or t.dim() != 2:
         raise DiaError(DIA_ERR_INVALID, f"{who}: {name} must be a 2-D {dtype} tensor on "
                                         f"{plan.device}")
@@ -814,7 +811,7 @@ def _spmm_new(stream, like, shape, dtype=None):
     (the current stream's may still be in use there by earlier work), kept from
     reuse until the current stream has passed the point where it is freed."""
     if stream is None:
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(*shape) if dtype is None else like.new_empty(shape, dtype=dtype)
     current = torch.cuda.current_stream(like.device)
     with torch.cuda.stream(stream):
         t = like.new_empty(shape, dtype=dtype)
@@ -841,18 +838,12 @@ def _spmm_stream(plan, stream):
     return stream.cuda_stream
 
 
-def _on_device(f):
-    """f(plan, ...) with the plan's device as the current one."""
-    @functools.wraps(f)
-    def call(plan, *args, **kwargs):
-        if plan.device.index is None or torch.cuda.current_device() == plan.device.index:
-            return f(plan, *args, **kwargs)
-        with torch.cuda.device(plan.device):
-            return f(plan, *args, **kwargs)
-    return call
+def _elsewhere(plan):
+    """Another device than the plan's is current."""
+    i = plan.device.index
+    return i is not None and torch._C._cuda_getDevice() != i
 
 
-@_on_device
 def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=None,
          save_z=False, out=None, z=None, work=None, stream=None):
     """act(x A^T + bias) + residual for a block x [M, n_cols] of vectors, one
@@ -866,19 +857,29 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
     save_z or a given z: the pre-activation that spmm_backward takes.  out and z
     must not overlap the inputs, except that out may be residual.  work:
     uint8 buffer of spmm_workspace bytes, for callers that allocate nothing."""
+    if _elsewhere(plan):
+        with torch.cuda.device(plan.device):
+            return spmm(plan, vals, x, bias=bias, act=act, residual=residual, seg=seg,
+                        save_z=save_z, out=out, z=z, work=work, stream=stream)
     who = "spmm"
     code = _spmm_act(who, act)
     dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
     t, M, n = x.dtype, x.shape[0], plan.n_rows
     xp, ldx = _spmm_block(who, "x", x, plan, t, M, plan.n_cols)
     bp = _spmm_vector(who, "bias", bias, plan, t, (n,) if seg is None else (E, n))
-    rp, ldr = _spmm_block(who, "residual", residual, plan, t, M, n)
+    rp, ldr = (_spmm_block(who, "residual", residual, plan, t, M, n) if residual is not None
+               else (None, n))
     if out is None:
         out = _spmm_new(stream, x, (M, n))
-    yp, ldy = _spmm_block(who, "out", out, plan, t, M, n)
-    if z is None and save_z:
+        yp, ldy = out.data_ptr(), n
+    else:
+        yp, ldy = _spmm_block(who, "out", out, plan, t, M, n)
+    zp, ldz = None, n
+    if z is not None:
+        zp, ldz = _spmm_block(who, "z", z, plan, t, M, n)
+    elif save_z:
         z = _spmm_new(stream, x, (M, n))
-    zp, ldz = _spmm_block(who, "z", z, plan, t, M, n)
+        zp = z.data_ptr()
     L = lib()
     wp, wbytes = _spmm_work(who, stream, work, L.dia_spmm_workspace(plan._h, dt, M, E, ldx), plan,
                             x)
@@ -890,7 +891,6 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
     return out if z is None else (out, z)
 
 
-@_on_device
 def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, bias_grad=False,
                   dx=None, dvals=None, dbias=None, work=None, stream=None):
     """Gradients (dx, dvals, dbias) of spmm for dy, the gradient of its result
@@ -899,6 +899,10 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
     matrix; dbias is None unless bias_grad or given.  Outputs must not overlap
     inputs.  work: uint8 buffer of spmm_backward_workspace bytes, for callers
     that allocate nothing."""
+    if _elsewhere(plan):
+        with torch.cuda.device(plan.device):
+            return spmm_backward(plan, vals, x, dy, z=z, act=act, seg=seg, bias_grad=bias_grad,
+                                 dx=dx, dvals=dvals, dbias=dbias, work=work, stream=stream)
     who = "spmm_backward"
     code = _spmm_act(who, act)
     dt, E, stride = _spmm_operator(who, plan, vals, x, seg)
@@ -911,12 +915,16 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
     bshape = (n,) if seg is None else (E, n)
     if dx is None:
         dx = _spmm_new(stream, x, (M, plan.n_cols))
+        dxp, lddx = dx.data_ptr(), plan.n_cols
+    else:
+        dxp, lddx = _spmm_block(who, "dx", dx, plan, t, M, plan.n_cols)
     if dvals is None:
         dvals = _spmm_new(stream, x, vals.shape)
+        dvp = dvals.data_ptr()
+    else:
+        dvp = _spmm_vector(who, "dvals", dvals, plan, t, vals.shape)
     if dbias is None and bias_grad:
         dbias = _spmm_new(stream, x, bshape)
-    dxp, lddx = _spmm_block(who, "dx", dx, plan, t, M, plan.n_cols)
-    dvp = _spmm_vector(who, "dvals", dvals, plan, t, vals.shape)
     dbp = _spmm_vector(who, "dbias", dbias, plan, t, bshape)
     L = lib()
     need = L.dia_spmm_backward_workspace(plan._h, dt, M, E, ldx, stride, lddy, code)
