@@ -12,6 +12,8 @@
 #include <math_constants.h>
 #include <stdint.h>
 
+#include <string.h>
+
 #include <atomic>
 #include <vector>
 
@@ -235,6 +237,13 @@ __device__ __forceinline__ float act_any(int act, float z)
     }
 }
 
+/* one copy of the functions for every row of a tile: inlined 32 times they
+ * did not fit the instruction cache */
+static __device__ __noinline__ float4 act4(int act, float4 z)
+{
+    return make_float4(act_any(act, z.x), act_any(act, z.y), act_any(act, z.z), act_any(act, z.w));
+}
+
 /* 16-bit blocks: two elements at a time, with the two-element fp32
  * instructions and the hardware's approximations of 2^x and 1/x (relative
  * errors of a few 2^-23).  They are within 2^-19 |z| of the function, far
@@ -390,6 +399,16 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p)
     const uint2 u = *(const uint2*)p;
     return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
                        __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+}
+
+__device__ __forceinline__ void store4(float* p, float4 v) { *(float4*)p = v; }
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 v)
+{
+    const T h[4] = {from_f<T>(v.x), from_f<T>(v.y), from_f<T>(v.z), from_f<T>(v.w)};
+    uint2 u;
+    memcpy(&u, h, 8);
+    *(uint2*)p = u;
 }
 
 /* ------------------------------------------------------------- arguments */

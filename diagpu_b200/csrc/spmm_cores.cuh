@@ -312,23 +312,49 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
         for (int r = 0; r < 4; ++r)
             if (i + STEP * r < a.n_out)
                 bias[r] = to_f(((const T*)a.bias)[(long long)rg.e * a.n_out + i + STEP * r]);
+    /* a lane's four features in one access, where they are adjacent and aligned */
+    auto quad = [&](const void* p, long long ld) {
+        return QUADS && i + 4 <= a.n_out && (uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0;
+    };
+    const bool vo = quad(a.out, a.ldo), vz = quad(a.z, a.ldz), vr = quad(a.res, a.ldr);
+    auto store = [&](void* base, long long at, float4 v, bool vec) {
+        T* p = (T*)base + at;
+        if (vec) {
+            store4(p, v);
+            return;
+        }
+        if (i < a.n_out) p[0] = from_f<T>(v.x);
+        if (i + STEP < a.n_out) p[STEP] = from_f<T>(v.y);
+        if (i + 2 * STEP < a.n_out) p[2 * STEP] = from_f<T>(v.z);
+        if (i + 3 * STEP < a.n_out) p[3 * STEP] = from_f<T>(v.w);
+    };
 #pragma unroll
     for (int t = 0; t < kTileRows; ++t) {
         if (t >= live) break;
         const long long row = (long long)rg.r0 + t0 + t;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int ir = i + STEP * r;
-            if (ir >= a.n_out) continue;
-            const float z = acc[t][r] + bias[r];
-            float y = z;
-            if (!TRANS) {
-                if (a.z) ((T*)a.z)[row * a.ldz + ir] = from_f<T>(z);
-                y = act_any(a.act, z);
-                if (a.res) y += to_f(((const T*)a.res)[row * a.ldr + ir]);
+        float4 y = make_float4(acc[t][0] + bias[0], acc[t][1] + bias[1], acc[t][2] + bias[2],
+                               acc[t][3] + bias[3]);
+        if (!TRANS) {
+            if (a.z) store(a.z, row * a.ldz + i, y, vz);
+            if (a.act != DIA_ACT_NONE) y = act4(a.act, y);
+            if (a.res) {
+                const T* p = (const T*)a.res + row * a.ldr + i;
+                float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (vr) {
+                    r = load4<T>(p);
+                } else {
+                    if (i < a.n_out) r.x = to_f(p[0]);
+                    if (i + STEP < a.n_out) r.y = to_f(p[STEP]);
+                    if (i + 2 * STEP < a.n_out) r.z = to_f(p[2 * STEP]);
+                    if (i + 3 * STEP < a.n_out) r.w = to_f(p[3 * STEP]);
+                }
+                y.x += r.x;
+                y.y += r.y;
+                y.z += r.z;
+                y.w += r.w;
             }
-            ((T*)a.out)[row * a.ldo + ir] = from_f<T>(y);
         }
+        store(a.out, row * a.ldo + i, y, vo);
     }
 }
 
