@@ -33,20 +33,20 @@ namespace dia {
 static std::atomic<int> g_form{0};
 
 /* Which form a call takes: the one whose time, by the measured costs of both,
- * is shorter (16-bit types, one B200; over 176 calls of 8 to 4096 rows, 3 to
- * 129 diagonals, 1 to 64 experts the form taken is 4 % slower than the better
- * one on average).
+ * is shorter (16-bit types, one B200; over 174 calls of 8 to 4096 rows, 3 to
+ * 129 diagonals, 1 to 64 experts the form taken is 1.5 % slower than the better
+ * one on average, 40 % at worst).
  *
- * CUDA cores, us.  Few rows: 7 for every million (row, feature, group of four
- * offsets).  Many: a wave of CTAs takes 15 + 0.4 K, then every million
- * features 5.5 + 0.2 K.
+ * CUDA cores, us.  Few rows: 6, and 4 for every million (row, feature, group of
+ * four offsets).  Many: a wave of CTAs takes 10 + 0.4 K, then every million
+ * features 4.5 + 0.2 K.
  * Tensor cores: the operator's boxes are packed and read (4 ns each, 10 where
  * they no longer fit L2) and every tile has a way through the kernel; a packing
  * launch of its own 2.5 us.
- * 4096 x 129 diagonals: cores 63 us, tensor cores 12 at 64 rows; 27-point
- * stencil on 262144: 31 and 323 at 8 rows, 387 and 374 at 128.  The gradients
- * favour the cores a little more (65536, 33 scattered diagonals, 128 rows: 180
- * and 214). */
+ * 4096 x 129 diagonals: cores 57 us, tensor cores 12 at 64 rows; 27-point
+ * stencil on 262144: 26 and 321 at 8 rows, 305 and 375 at 128.  The ratio of the
+ * gradients is nearly that of the products (65536, 33 scattered diagonals, 128
+ * rows: 97 and 107, gradients 180 and 214). */
 static bool tensor_form(const DiaSpmmPlan* p, int dtype, long long M, int E, bool backward)
 {
     const int form = g_form.load(std::memory_order_relaxed);
@@ -57,11 +57,11 @@ static bool tensor_form(const DiaSpmmPlan* p, int dtype, long long M, int E, boo
     const double nfb = (p->n_rows + 127) / 128, boxes = nfb * E * d.nboxes;
     const double tiles = nfb * (M / 128.0 + (E > 1 ? (double)std::min<long long>(E, M) : 1.0));
     const double mega = (double)M * p->n_rows * 1e-6;
-    const double cores = mega < 0.2 ? 6 + 7 * mega * d.nquads
-                                    : std::max(15 + 0.4 * p->K, (5.5 + 0.2 * p->K) * mega);
+    const double cores = mega < 0.2 ? 6 + 4 * mega * d.nquads
+                                    : std::max(10 + 0.4 * p->K, (4.5 + 0.2 * p->K) * mega);
     const double tensor = 8 + (E > 1 || d.nboxes > 6 ? 2.5 : 0.0) + 0.004 * boxes +
                           0.006 * std::max(0.0, boxes - 2500) + 0.02 * tiles;
-    return (backward ? 0.8 : 1.0) * cores > tensor;
+    return (backward ? 1.1 : 1.0) * cores > tensor;
 }
 
 static size_t elem_size(int dtype) { return dtype == DIA_F32 ? 4 : 2; }

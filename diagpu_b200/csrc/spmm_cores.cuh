@@ -118,8 +118,10 @@ spmm_few_kernel(const __grid_constant__ ProdArgs a, int ks, int ftiles, long lon
  * piece per sixteen products.  Otherwise (fewer than three diagonals a quad)
  * a lane owns features 32 apart and reads an input per product, without bank
  * conflicts at any offset.  Shared memory's bandwidth bounds both: 64 rows of
- * 262144 under a 27-point stencil, fp32, 150 us (3.0 products a picosecond,
- * 1.08 TB/s of the 163 MB that memory has to give; 25 us at its rate). */
+ * 262144 under a 27-point stencil, fp32, 115 us (3.9 products a picosecond,
+ * load and store unit two thirds busy; the 163 MB that memory has to give
+ * would take 25).  Twice the warps with half the features each took 128, two
+ * rows a packed multiplication changed nothing. */
 constexpr int kTileRows = 8;    /* rows of a warp */
 constexpr int kTileSmem = 112 * 1024;   /* two CTAs an SM */
 
@@ -602,10 +604,12 @@ static int launch_few(const ProdArgs& a, cudaStream_t stream)
 {
     const int ftiles = (a.n_out + 31) / 32;
     const long long ngroups = a.seg ? a.M / TT + std::min(a.E, a.M) : (a.M + TT - 1) / TT;
-    /* warps that share a tile: until every SM has 32, or a warp four diagonals */
+    /* warps that share a tile: until every SM has a CTA (two where a warp has
+     * one row), or a warp four diagonals (32 rows of 4096 under 129 diagonals,
+     * bf16: 27 us; with twice the CTAs 38) */
+    const long long warps = TT == 1 ? 2 * kFewWarps : kFewWarps;
     int ks = 1;
-    while (ks < kFewWarps && (long long)ftiles * ngroups * ks < 32ll * num_sms() && a.K > 4 * ks)
-        ks *= 2;
+    while (ks < kFewWarps && ftiles * ngroups * ks < warps * num_sms() && a.K > 4 * ks) ks *= 2;
     const int fper = kFewWarps / ks;
     const long long grid = ngroups * ((ftiles + fper - 1) / fper);
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: block too large");
@@ -647,7 +651,8 @@ static int launch_cores(const ProdArgs& a, cudaStream_t stream)
     const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
     /* below this there are too few warps of 128 features x 8 rows to hide the
      * latency of the diagonals one after the other (4096 x 4096, 129 diagonals,
-     * fp32: 39 us at 32 rows, 32 us by few rows; 39 and 68 at 128) */
+     * bf16: 57 us from 64 rows to 256; by few rows 27 at 32 rows, in proportion
+     * beyond) */
     if (per >= 8 && a.K > 0 && (long long)a.M * a.n_out >= 196608) {
         /* the widest tile (an input is read again by fewer tiles) whose inputs
          * fit and that leaves a CTA for every SM; else the narrowest that fits */
