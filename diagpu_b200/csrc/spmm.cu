@@ -385,7 +385,7 @@ extern "C" int dia_spmm_plan_create(int64_t n_rows, int64_t n_cols, int num_diag
     if (num_diags > 0 && !h_offsets)
         return fail(DIA_ERR_INVALID, "dia_spmm_plan_create: null offsets");
     /* every i + d of a stored entry, and a tile beyond, stays a 32-bit int */
-    if (n_rows + n_cols > INT_MAX / 2 || num_diags > (1 << 20))
+    if (n_rows > INT_MAX / 2 || n_cols > INT_MAX / 2 - n_rows || num_diags > (1 << 20))
         return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_plan_create: operator too large");
     try {
         std::vector<int> fwd(h_offsets, h_offsets + num_diags);

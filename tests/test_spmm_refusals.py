@@ -106,3 +106,12 @@ def test_c_abi_before_cuda():
     assert L.dia_spmm_workspace(None, 0, 4, 1, 8) == -1
     assert L.dia_spmm_backward_workspace(None, 0, 4, 1, 8, 32, 8, 0) == -1
     assert L.dia_test_spmm_form(3) == dg.DIA_ERR_INVALID
+
+
+@pytest.mark.parametrize("nr,nc", [((1 << 63) - 1, (1 << 63) - 1), (1 << 62, 1 << 62),
+                                   ((1 << 63) - 1, 1), (1, 1 << 40), (1 << 40, 0)])
+def test_plan_sizes_past_32_bits(nr, nc):
+    """No sum of two sizes wraps around into a size that is taken."""
+    L, h, off = dg.lib(), C.c_void_p(), np.zeros(1, np.int32)
+    rc = L.dia_spmm_plan_create(nr, nc, 1, off.ctypes.data_as(C.c_void_p), C.byref(h))
+    assert rc == dg.DIA_ERR_UNSUPPORTED and not h.value
