@@ -820,15 +820,18 @@ def _spmm_new(stream, like, shape, dtype=None):
 
 
 def _spmm_work(who, stream, work, need, plan, like):
-    """(pointer, bytes) of the workspace, made here if need be."""
+    """(tensor, pointer, bytes) of the workspace, made here if need be.  The
+    caller keeps the tensor until its kernels are on the stream: before that
+    another thread could be given its memory and write to it first."""
     if work is None:
         if need <= 0:
-            return None, 0
-        return _spmm_new(stream, like, (need,), torch.uint8).data_ptr(), need
+            return None, None, 0
+        work = _spmm_new(stream, like, (need,), torch.uint8)
+        return work, work.data_ptr(), need
     if work.dtype != torch.uint8 or work.device != plan.device or not work.is_contiguous():
         raise DiaError(DIA_ERR_INVALID, f"{who}: work must be a contiguous uint8 tensor on "
                                         f"{plan.device}")
-    return work.data_ptr(), work.numel()
+    return work, work.data_ptr(), work.numel()
 
 
 def _spmm_stream(plan, stream):
@@ -881,8 +884,8 @@ def spmm(plan: SpmmPlan, vals, x, *, bias=None, act="none", residual=None, seg=N
         z = _spmm_new(stream, x, (M, n))
         zp = z.data_ptr()
     L = lib()
-    wp, wbytes = _spmm_work(who, stream, work, L.dia_spmm_workspace(plan._h, dt, M, E, ldx), plan,
-                            x)
+    need = L.dia_spmm_workspace(plan._h, dt, M, E, ldx)
+    work, wp, wbytes = _spmm_work(who, stream, work, need, plan, x)
     rc = L.dia_spmm(plan._h, dt, M, E, None if seg is None else seg.data_ptr(), xp, ldx,
                     vals.data_ptr(), stride, bp, code, rp, ldr, zp, ldz, yp, ldy, wp, wbytes,
                     _spmm_stream(plan, stream))
@@ -928,7 +931,7 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
     dbp = _spmm_vector(who, "dbias", dbias, plan, t, bshape)
     L = lib()
     need = L.dia_spmm_backward_workspace(plan._h, dt, M, E, ldx, stride, lddy, code)
-    wp, wbytes = _spmm_work(who, stream, work, need, plan, x)
+    work, wp, wbytes = _spmm_work(who, stream, work, need, plan, x)
     rc = L.dia_spmm_backward(plan._h, dt, M, E, None if seg is None else seg.data_ptr(), xp, ldx,
                              vals.data_ptr(), stride, gp, lddy, code, zp, ldz, dxp, lddx, dvp,
                              dbp, wp, wbytes, _spmm_stream(plan, stream))

@@ -1,6 +1,7 @@
 """What the block-vector product refuses, on the host: Python checks of the
 tensors against the plan, and C-ABI checks that come before any CUDA call."""
 import ctypes as C
+import weakref
 
 import numpy as np
 import pytest
@@ -115,3 +116,39 @@ def test_plan_sizes_past_32_bits(nr, nc):
     L, h, off = dg.lib(), C.c_void_p(), np.zeros(1, np.int32)
     rc = L.dia_spmm_plan_create(nr, nc, 1, off.ctypes.data_as(C.c_void_p), C.byref(h))
     assert rc == dg.DIA_ERR_UNSUPPORTED and not h.value
+
+
+def test_workspace_lives_until_the_call_returns(monkeypatch):
+    """Another thread on the same stream must not be given the workspace before
+    the call has put its kernels on the stream: the tensor is alive in the C
+    entry."""
+    made, seen = [], []
+
+    class Entries:
+        @staticmethod
+        def dia_spmm_workspace(*a):
+            return 512
+
+        dia_spmm_backward_workspace = dia_spmm_workspace
+
+        @staticmethod
+        def entry(*a):
+            work, size = a[-3:-1]
+            seen.append((size, [r() for r in made if r() is not None
+                                and r().data_ptr() == work and r().numel() == size]))
+            return 0
+
+        dia_spmm = dia_spmm_backward = entry
+
+    def new(stream, like, shape, dtype=None):
+        t = torch.empty(shape, dtype=dtype or like.dtype)
+        made.append(weakref.ref(t))
+        return t
+
+    monkeypatch.setattr(dg, "lib", lambda: Entries)
+    monkeypatch.setattr(dg, "_spmm_new", new)
+    monkeypatch.setattr(dg, "_spmm_stream", lambda plan, stream: 0)
+    plan, vals, x = good()
+    dg.spmm(plan, vals, x)
+    dg.spmm_backward(plan, vals, x, torch.zeros(4, 8))
+    assert [(size, len(alive)) for size, alive in seen] == [(512, 1), (512, 1)]
