@@ -276,6 +276,26 @@ static SpmmDir dir_on_device(const void* blob, SpmmDir d)
     return d;
 }
 
+/* A device copy of the tables that any stream may read once this returns: a
+ * plain cudaMemcpy from pageable memory may return before the copy has reached
+ * the device, and streams that do not wait for the default one would read the
+ * tables half written. */
+static cudaError_t upload(void** dst, const std::vector<char>& blob)
+{
+    if (blob.empty()) return cudaSuccess;
+    cudaStream_t s = nullptr;
+    cudaError_t e = cudaMalloc(dst, blob.size());
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess)
+        e = cudaMemcpyAsync(*dst, blob.data(), blob.size(), cudaMemcpyHostToDevice, s);
+    if (s) {
+        const cudaError_t done = cudaStreamSynchronize(s);
+        if (e == cudaSuccess) e = done;
+        cudaStreamDestroy(s);
+    }
+    return e;
+}
+
 /* arguments both directions share; DIA_OK or the error */
 static int check_common(const char* who, const DiaSpmmPlan* p, int dtype, int64_t M, int E,
                         const int64_t* seg, int act, int64_t stride, const void* vals)
@@ -407,9 +427,7 @@ extern "C" int dia_spmm_plan_create(int64_t n_rows, int64_t n_cols, int num_diag
         p->n_cols = (int)n_cols;
         p->K = num_diags;
         cudaError_t e = cudaGetDevice(&p->device);
-        if (e == cudaSuccess && !blob.empty()) e = cudaMalloc(&p->blob, blob.size());
-        if (e == cudaSuccess && !blob.empty())
-            e = cudaMemcpy(p->blob, blob.data(), blob.size(), cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = upload(&p->blob, blob);
         if (e != cudaSuccess) {
             if (p->blob) cudaFree(p->blob);
             delete p;

@@ -720,3 +720,23 @@ def test_lowest_and_largest_values(act, t):
     dz[:, ::2] = 0
     assert torch.equal(dx, dz)
     assert bool(dv.isfinite().all())
+
+
+@pytest.mark.parametrize("M", [3, 300])
+def test_first_use_of_a_plan_on_another_stream(M, t):
+    """A new plan's tables are on the device when it is returned: its first
+    calls are on a stream that does not wait for the default one.  The offsets
+    are many, so that the tables are more than one staging buffer."""
+    n, off = 2000, list(range(-1900, 1900, 2))
+    c = Case(t, M, n, n, off, seed=51)
+    want = dg.spmm(c.plan, c.vals[0], c.x)
+    grads = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        plan = dg.SpmmPlan(n, n, np.array(off, np.int32))
+        got = dg.spmm(plan, c.vals[0], c.x, stream=side)
+        back = dg.spmm_backward(plan, c.vals[0], c.x, c.dy, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        assert all(torch.equal(p, q) for p, q in zip(back[:2], grads[:2]))
