@@ -276,6 +276,15 @@ static SpmmDir dir_on_device(const void* blob, SpmmDir d)
     return d;
 }
 
+/* Plans come and go while other work is captured into a graph (a collected
+ * plan of an earlier layer, say); their memory is no part of it.  Without this
+ * the runtime refuses cudaMalloc and cudaFree then, and the capture is lost. */
+struct BesideCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    BesideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~BesideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 /* A device copy of the tables that any stream may read once this returns: a
  * plain cudaMemcpy from pageable memory may return before the copy has reached
  * the device, and streams that do not wait for the default one would read the
@@ -283,6 +292,7 @@ static SpmmDir dir_on_device(const void* blob, SpmmDir d)
 static cudaError_t upload(void** dst, const std::vector<char>& blob)
 {
     if (blob.empty()) return cudaSuccess;
+    BesideCapture beside;
     cudaStream_t s = nullptr;
     cudaError_t e = cudaMalloc(dst, blob.size());
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
@@ -294,6 +304,13 @@ static cudaError_t upload(void** dst, const std::vector<char>& blob)
         cudaStreamDestroy(s);
     }
     return e;
+}
+
+static void release(DiaSpmmPlan* p)
+{
+    BesideCapture beside;
+    if (p->blob) cudaFree(p->blob);
+    delete p;
 }
 
 /* arguments both directions share; DIA_OK or the error */
@@ -429,8 +446,7 @@ extern "C" int dia_spmm_plan_create(int64_t n_rows, int64_t n_cols, int num_diag
         cudaError_t e = cudaGetDevice(&p->device);
         if (e == cudaSuccess) e = upload(&p->blob, blob);
         if (e != cudaSuccess) {
-            if (p->blob) cudaFree(p->blob);
-            delete p;
+            release(p);
             return cuda_fail(e, "dia_spmm_plan_create");
         }
         p->fwd = dir_on_device(p->blob, tf);
@@ -444,9 +460,7 @@ extern "C" int dia_spmm_plan_create(int64_t n_rows, int64_t n_cols, int num_diag
 
 extern "C" int dia_spmm_plan_destroy(DiaSpmmPlan* plan)
 {
-    if (!plan) return DIA_OK;
-    if (plan->blob) cudaFree(plan->blob);
-    delete plan;
+    if (plan) release(plan);
     return DIA_OK;
 }
 

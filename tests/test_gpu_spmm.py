@@ -740,3 +740,21 @@ def test_first_use_of_a_plan_on_another_stream(M, t):
         torch.cuda.synchronize()
         assert torch.equal(got, want)
         assert all(torch.equal(p, q) for p, q in zip(back[:2], grads[:2]))
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_plans_come_and_go_during_capture(t):
+    """A plan that is dropped, and one that is made, while a graph is captured
+    leave the capture alone."""
+    c = Case(t, 140, 136, 136, band(6), seed=52)
+    want = dg.spmm(c.plan, c.vals[0], c.x)
+    old = dg.SpmmPlan(64, 64, [0, 1])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        del old
+        plan = dg.SpmmPlan(136, 136, c.off)
+        got = dg.spmm(plan, c.vals[0], c.x)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
