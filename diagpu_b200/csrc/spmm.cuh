@@ -188,15 +188,17 @@ __device__ __forceinline__ long long row_groups(const long long* seg, int E, int
 
 /* ------------------------------------------------------------ activations */
 
-/* fp32 blocks: CUDA's functions. */
+/* fp32 blocks: CUDA's functions, in forms without a difference of nearly equal
+ * numbers, so that a small result (a negative z) is as exact as a large one:
+ * z Phi(z) by erfc, tanh by the logistic function. */
 template <int ACT>
 __device__ __forceinline__ float act_of(float z)
 {
     if (ACT == DIA_ACT_RELU) return z < 0.0f ? 0.0f : z;          /* NaN stays NaN */
     if (ACT == DIA_ACT_SILU) return z / (1.0f + expf(-z));
-    if (ACT == DIA_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    if (ACT == DIA_ACT_GELU) return 0.5f * z * erfcf(z * -0.70710678f);
     if (ACT == DIA_ACT_GELU_TANH)
-        return 0.5f * z * (1.0f + tanhf(0.79788456f * z * fmaf(0.044715f * z, z, 1.0f)));
+        return z / (1.0f + expf(-2.0f * 0.79788456f * z * fmaf(0.044715f * z, z, 1.0f)));
     return z;
 }
 
@@ -216,12 +218,12 @@ __device__ __forceinline__ float dact_of(float z)
         return s * fmaf(z, 1.0f - s, 1.0f);
     }
     if (ACT == DIA_ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
+        return 0.5f * erfcf(z * -0.70710678f) + z * 0.39894228f * expf(-0.5f * z * z);
     if (ACT == DIA_ACT_GELU_TANH) {
         z = within16(z);
-        const float t = tanhf(0.79788456f * z * fmaf(0.044715f * z, z, 1.0f));
-        return 0.5f * (1.0f + t) +
-               0.5f * z * (1.0f - t * t) * 0.79788456f * fmaf(0.134145f * z, z, 1.0f);
+        const float s =
+            1.0f / (1.0f + expf(-2.0f * 0.79788456f * z * fmaf(0.044715f * z, z, 1.0f)));
+        return s + 2.0f * 0.79788456f * z * fmaf(0.134145f * z, z, 1.0f) * s * (1.0f - s);
     }
     return 1.0f;
 }
@@ -246,11 +248,15 @@ static __device__ __noinline__ float4 act4(int act, float4 z)
 
 /* 16-bit blocks: two elements at a time, with the two-element fp32
  * instructions and the hardware's approximations of 2^x and 1/x (relative
- * errors of a few 2^-23).  They are within 2^-19 |z| of the function, far
- * below half a step of the result:
- *   z Phi(z) by Abramowitz and Stegun's 7.1.26 (their bound 1.5e-7 on erf):
- *     Phi(-x) = (a1 t + .. + a5 t^5) exp(-x^2 / 2) / 2, t = 1 / (1 + p x / sqrt 2);
- *   tanh u = 2 s - 1 with the logistic function s of 2 u. */
+ * errors of a few 2^-23).
+ *   Phi(-x) = (a1 t + .. + a6 t^6) exp(-x^2 / 2), t = 1 / (1 + p x), x >= 0: the
+ *     form of Abramowitz and Stegun's 7.1.26, p and a fitted here to the least
+ *     relative error up to x = 13.5 (iterated reweighted least squares, Lawson
+ *     1961): 3.7e-6, and 1e-5 with the rounding of x^2.  Theirs bounds the
+ *     absolute error, which passes half a step of the result below z = -4.
+ *   tanh u = 2 s - 1 with the logistic function s of 2 u.
+ * So values are within 2^-16 of themselves, a 32nd of half a step of fp16 or
+ * less; z Phi(z) underflows from z = -13 on. */
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 {
     float2 d;
@@ -305,12 +311,13 @@ __device__ __forceinline__ float2 logistic2(float2 z, float c)
 __device__ __forceinline__ float2 normal_cdf2(float2 z, float2& e)
 {
     const float2 x = make_float2(fabsf(z.x), fabsf(z.y));
-    const float2 t = rcp2(fma2(x, both(0.2316419f), both(1.0f)));
+    const float2 t = rcp2(fma2(x, both(0.3076393f), both(1.0f)));
     e = exp2_2(mul2(mul2(z, z), both(-0.72134752f)));
-    float2 p = fma2(t, both(0.5307027145f), both(-0.7265760135f));
-    p = fma2(p, t, both(0.7107068705f));
-    p = fma2(p, t, both(-0.142248368f));
-    p = fma2(p, t, both(0.127414796f));
+    float2 p = fma2(t, both(-0.07581779f), both(0.19163735f));
+    p = fma2(p, t, both(0.00532099f));
+    p = fma2(p, t, both(0.13731957f));
+    p = fma2(p, t, both(0.11854316f));
+    p = fma2(p, t, both(0.12299492f));
     p = mul2(p, mul2(t, e));
     const float2 q = fma2(p, both(-1.0f), both(1.0f));
     return make_float2(z.x < 0.0f ? p.x : q.x, z.y < 0.0f ? p.y : q.y);

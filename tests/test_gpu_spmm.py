@@ -758,3 +758,51 @@ def test_plans_come_and_go_during_capture(t):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("act", ACTS[2:])
+def test_activations_to_their_last_bits(act, M, t):
+    """Values and derivatives on [-6, 6] as an identity operator gives them,
+    bounded by the result itself, so that a negative z's small one counts too.
+
+    With a = 2^-23 (fp32) an argument z sqrt(1/2) is off by a of itself, which
+    erfc, whose logarithm's slope is below 2 x + 1 / x, makes (z^2 + 2) a; with
+    the function's own 4 a and three multiplications (8 + z^2) a.  Likewise
+    exp(-2 u) is off by 6 |u| a for u of the tanh form (six roundings), the
+    logistic function by (8 + 6 |u|) a.  16-bit types: 2^-16, the bound that the
+    polynomial of the normal distribution is fitted to, and for the logistic
+    functions the fp32 bounds once more for the hardware's functions.  A derivative's
+    terms carry these bounds each, and 1 - s is off by a."""
+    n = 700
+    c = Case(t, M, n, n, [0], seed=61)
+    c.vals[0, 0].fill_(0.0)
+    c.vals[0, 0, :n] = 1.0
+    z = torch.linspace(-6, 6, M * n, dtype=torch.float64).view(M, n)
+    c.x, c.zin = c.block(z), c.block(z)
+    c.dy = c.block(torch.ones(M, n))
+    z, u, a = c.v(c.zin), unit(t), 2.0 ** -23
+    half = math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+    if act == "gelu":
+        e = 2.0 ** -16 + torch.zeros_like(z) if t != torch.float32 else (8 + z * z) * a
+    else:
+        e = (8 + 6 * (half if act == "gelu_tanh" else z / 2).abs()) * a
+        e = e if t == torch.float32 else 2 * e
+    want = act64(z, act)
+    tol = (e + u * (1 + e)) * want.abs() + tiny(t)
+    near(dg.spmm(c.plan, c.vals[0], c.x, act=act), want, tol, "value")
+
+    want = dact64(z, act)
+    if act == "gelu":
+        slope = 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+        slope = slope + z.abs() * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+        err = e * slope
+    else:
+        s = torch.sigmoid(2 * half if act == "gelu_tanh" else z)
+        grow = torch.ones_like(z)
+        if act == "gelu_tanh":
+            grow = 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z * z)
+        # s + z grow s (1 - s): s twice, grow's three roundings, 1 - s
+        err = e * s + z.abs() * grow * s * ((1 - s) * (2 * e + 3 * a) + 2 * a)
+    dx = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=c.zin, act=act)[0]
+    near(dx, want, err + u * (want.abs() + err) + tiny(t), "derivative")
