@@ -906,7 +906,8 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
  * tensor cores 16 %).  One CTA an SM does not overlap its start, the making of
  * dz and the diagonals' way out with its neighbour's stream.
  * Rows of the last stage that are not the part's are cleared in both operands
- * before the MMAs read them. */
+ * before the MMAs read them, so that an entry of D sums its own terms alone:
+ * infinities and NaN reach the entries that they belong to and no others. */
 constexpr int kGRows = 64;                     /* rows of a stage */
 constexpr int kGBoxBytes = kGRows * 128;
 constexpr int kGBoxes = 4;                     /* boxes of inputs of a CTA */
@@ -927,15 +928,6 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t addr)
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
     return d;
-}
-
-template <typename T>
-__device__ __noinline__ float gradient_terms(const GradArgs& a, int r0, int r1, int i, int j)
-{
-    float s = 0.0f;
-    for (int t = r0; t < r1; ++t)
-        s = fmaf(to_f(((const T*)a.dz)[t * a.lddz + i]), to_f(((const T*)a.x)[t * a.ldx + j]), s);
-    return s;
 }
 
 /* ACT other than none: dz is made here, from dy and z, by the warps that wait
@@ -1175,17 +1167,13 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     if (nch == 1 && adjoin && nst > 0 && a.K <= kOffs && i0 + 128 <= a.n_rows &&
         i0 + s_offs[0].x >= 0 && i0 + 127 + s_offs[a.K - 1].x < a.n_cols) {
         const float* src = row - col[0] + lane;
-        bool bad = false;
 #pragma unroll 2
         for (int k = k_first; k < k_hi; k += kGWarps) {
             const int2 o = s_offs[k];
             const long long at = (long long)o.y * a.stride;
             float v[4];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                v[s] = src[32 * s * (kGPitch + 1) + o.x];
-                bad |= !isfinite(v[s]);
-            }
+            for (int s = 0; s < 4; ++s) v[s] = src[32 * s * (kGPitch + 1) + o.x];
             if (parts) {
 #pragma unroll
                 for (int s = 0; s < 4; ++s) part0[at + 32 * s] = v[s];
@@ -1194,7 +1182,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                 for (int s = 0; s < 4; ++s) out0[at + 32 * s] = from_f<T>(v[s]);
             }
         }
-        if (!__any_sync(0xffffffffu, bad)) return;   /* else once more, below */
+        return;
     }
     for (int k = k_first; k < k_hi; k += kGWarps) {
         const int2 o = a.K <= kOffs ? s_offs[k] : a.dir.offs[k];
@@ -1203,7 +1191,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         const int in_lo = max(0, -(i0 + o.x));
         const int in_hi = nst > 0 ? min(a.n_rows - i0, a.n_cols - i0 - o.x) : 0;
         float v[4];
-        bool on[4], bad = false;
+        bool on[4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int f = 32 * s + lane, p = o.x + f;
@@ -1218,13 +1206,6 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
             }
             on[s] = at >= 0 && f < f_end;
             v[s] = on[s] && f >= in_lo && f < in_hi ? row[32 * s * kGPitch + at] : 0.0f;
-            bad |= !isfinite(v[s]);
-        }
-        if (bad) {
-            for (int s = 0; s < 4; ++s) {
-                const int i = i0 + 32 * s + lane;
-                if (!isfinite(v[s])) v[s] = gradient_terms<T>(a, rg.r0, rg.r1, i, i + o.x);
-            }
         }
         const long long at = (long long)o.y * a.stride;
 #pragma unroll

@@ -806,3 +806,67 @@ def test_activations_to_their_last_bits(act, M, t):
         err = e * s + z.abs() * grow * s * ((1 - s) * (2 * e + 3 * a) + 2 * a)
     dx = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=c.zin, act=act)[0]
     near(dx, want, err + u * (want.abs() + err) + tiny(t), "derivative")
+
+
+def alike(got, want, what):
+    """Both NaN, or the same infinity, at every place."""
+    got, want = got.double().cpu(), want.double().cpu()
+    ok = (got == want) | (got.isnan() & want.isnan())
+    assert bool(ok.all()), (what, int((~ok).sum()), got[~ok][:4].tolist(), want[~ok][:4].tolist())
+
+
+def best_ms(f, n=4):
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    f()
+    best = math.inf
+    for _ in range(n):
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+def time_against_cores(f):
+    """Time of f in the tensor-core form over that in the CUDA-core form."""
+    L = dg.lib()
+    try:
+        dg.check(L.dia_test_spmm_form(1))
+        cores = best_ms(f)
+        dg.check(L.dia_test_spmm_form(2))
+        return best_ms(f) / cores
+    finally:
+        dg.check(L.dia_test_spmm_form(0))
+        assert dg.device_status() == 0
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_gradient_of_a_block_that_overflowed(value, t):
+    """dy as a step of too large a loss scale leaves it: every entry of the
+    diagonals' gradient is what its own terms give."""
+    M, n, off = 300, 264, band(20)
+    c = Case(t, M, n, n, off, seed=62)
+    c.dy.fill_(value)
+    dv = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy)[1]
+    want = gradient64(off, n, n, c.v(c.vals), c.v(c.x), c.v(c.dy), c.parts)[1][0]
+    alike(dv, want, "dvals")
+
+
+def test_time_of_a_gradient_that_overflowed():
+    """It costs no walk over the rows for each entry (with one, five times the
+    CUDA-core form's time, which does not look at its values)."""
+    M, n, off = 4096, 2048, band(64)
+    c = Case(torch.float16, M, n, n, off, seed=63)
+    c.dy.fill_(float("inf"))
+    dv = torch.zeros_like(c.vals[0])
+    L, st = dg.lib(), c.vals.shape[-1]
+    work = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+
+    def f():
+        dg.check(L.dia_spmm_backward(c.plan._h, 1, M, 1, None, c.x.data_ptr(), n, None, st,
+                                     c.dy.data_ptr(), n, 0, None, n, None, n, dv.data_ptr(), None,
+                                     work.data_ptr(), work.numel(),
+                                     torch.cuda.current_stream().cuda_stream))
+
+    assert time_against_cores(f) < 2
