@@ -24,9 +24,10 @@
  * DRAM is 22 % busy, the tensor cores 10 %.
  *
  * Zeros of a box meet inputs that no diagonal joins to its features; where
- * such an input is infinite or undefined, so is the sum.  A sum that is not
- * finite is therefore computed again from its terms alone (finite ones had no
- * such input), so results do not depend on the form chosen.
+ * such an input is infinite or undefined, so is the sum.  Sums that are not
+ * finite, and those beside them in the row, are therefore computed again from
+ * their terms alone (rows_again), so an infinity reaches the same outputs in
+ * either form.
  *
  * Every wait is bounded; when one runs out the kernel records DIA_TC_TIMEOUT
  * (dia_device_status), stops, lets its copies and MMAs land and returns.
@@ -75,27 +76,34 @@ __device__ __forceinline__ void mbar_init(unsigned long long& b, int count)
 }
 
 /* waits for the phase of `bar` with parity `parity`; false when the kernel
- * gives up (another role did, or this wait ran past its limit) */
-__device__ __noinline__ bool mm_wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag)
+ * gives up (another role did, or this wait ran past its limit).  state[0]: it
+ * gives up; state[1] counts the steps of rows_again, which takes its time: the
+ * limit runs from the last of them. */
+__device__ __noinline__ bool mm_wait_long(uint32_t bar, uint32_t parity, volatile int* state)
 {
-    const unsigned long long t0 = global_ns();
+    unsigned long long t0 = global_ns();
+    int step = state[1];
     for (;;) {
         if (mbar_try(bar, parity)) return true;
-        if (*abort_flag) return false;
+        if (state[0]) return false;
+        if (state[1] != step) {
+            step = state[1];
+            t0 = global_ns();
+        }
         if (global_ns() - t0 > g_mm_wait_ns) {
-            *abort_flag = 1;
+            state[0] = 1;
             atomicOr(&g_mm_status, (unsigned)DIA_TC_TIMEOUT);
             return false;
         }
     }
 }
 
-__device__ __forceinline__ bool mm_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag)
+__device__ __forceinline__ bool mm_wait(uint32_t bar, uint32_t parity, volatile int* state)
 {
-    return mbar_try(bar, parity) || mm_wait_long(bar, parity, abort_flag);
+    return mbar_try(bar, parity) || mm_wait_long(bar, parity, state);
 }
 
-/* without regard to the abort flag: copies and MMAs already issued land */
+/* without regard to the state: copies and MMAs already issued land */
 __device__ void mm_drain(uint32_t bar, uint32_t parity)
 {
     const unsigned long long t0 = global_ns();
@@ -404,39 +412,57 @@ __device__ __forceinline__ void build_operator(const ProdArgs& a, int K, int e, 
     asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
 }
 
-/* the sum of one output's own terms, in ascending order of the offsets */
-template <typename T, bool TRANS>
-__device__ __noinline__ float product_terms(const ProdArgs& a, int K, int e, long long row, int i)
-{
-    const T* in = (const T*)a.in + row * a.ldi;
-    const T* vals = (const T*)a.vals + e * a.estride;
-    float s = 0.0f;
-    for (int k = 0; k < K; ++k) {
-        const int2 ok = a.dir.offs[k];
-        const int j = i + ok.x;
-        if ((unsigned)j < (unsigned)a.n_in)
-            s = fmaf(to_f(vals[ok.y * a.stride + (TRANS ? j : i)]), to_f(in[j]), s);
-    }
-    return s;
-}
+/* Rows of a 32 x 32 block with sums that are not finite (bits of `rows`, from
+ * row0 on), computed from their own terms in ascending order of the offsets
+ * and stored.  Lanes are features, so that values and inputs are read side by
+ * side, and a value serves kAgainRows rows (eight would leave the caller too
+ * few registers: 41 -> 43 us for blocks that never come here).  4096 rows of
+ * 4096, 129 diagonals, fp16, no input finite: 3.7 ms, a tenth of what a lane
+ * for each row took and ten times the CUDA-core form; one infinity: 0.11 ms. */
+constexpr int kAgainRows = 4;
 
-/* The results of a row whose sums were not finite (bits of `which`, from
- * feature i on), from their own terms, into the row in shared memory (four
- * 16-byte pieces, piece c at c ^ spread). */
 template <typename T, bool TRANS, int ACT>
-__device__ __noinline__ void sum_again(const ProdArgs& a, int K, int e, long long row_, int i,
-                                       uint32_t which, uint32_t row, uint32_t spread, bool res)
+__device__ __noinline__ void rows_again(const ProdArgs& a, int K, int e, int row0, int i,
+                                        uint32_t rows, volatile int* state)
 {
-    for (; which; which &= which - 1) {
-        const int c = __ffs(which) - 1;
-        float v = product_terms<T, TRANS>(a, K, e, row_, i + c);
-        if (!TRANS) {
-            if (a.bias) v += to_f(((const T*)a.bias)[(long long)e * a.n_out + i + c]);
-            v = act_of<ACT>(v);
-            if (res && a.res) v += to_f(((const T*)a.res)[row_ * a.ldr + i + c]);
+    const bool on = i < a.n_out;
+    const T* vals = (const T*)a.vals + e * a.estride;
+    const float bias =
+        !TRANS && a.bias && on ? to_f(((const T*)a.bias)[(long long)e * a.n_out + i]) : 0.0f;
+    while (rows) {
+        int r[kAgainRows];
+        float sum[kAgainRows];
+        const T* in[kAgainRows];
+        const int n = min(kAgainRows, __popc(rows));
+#pragma unroll
+        for (int u = 0; u < kAgainRows; ++u) {   /* a row twice where there are fewer */
+            r[u] = row0 + (u < n ? __ffs(rows) - 1 : r[0] - row0);
+            rows &= rows - 1;
+            in[u] = (const T*)a.in + (long long)r[u] * a.ldi;
+            sum[u] = 0.0f;
         }
-        const T h = from_f<T>(v);
-        sts16(row + (((c >> 3) ^ spread) << 4) + (c & 7) * 2, *(const uint16_t*)&h);
+#pragma unroll 4
+        for (int k = 0; k < K; ++k) {
+            const int2 ok = __ldg(&a.dir.offs[k]);
+            const int j = i + ok.x;
+            if (on && (unsigned)j < (unsigned)a.n_in) {
+                const float w = to_f(vals[ok.y * a.stride + (TRANS ? j : i)]);
+#pragma unroll
+                for (int u = 0; u < kAgainRows; ++u) sum[u] = fmaf(w, to_f(in[u][j]), sum[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAgainRows; ++u) {
+            if (!on || u >= n) continue;
+            float y = sum[u] + bias;
+            if (!TRANS) {
+                if (a.z) ((T*)a.z)[r[u] * a.ldz + i] = from_f<T>(y);
+                y = act2<ACT>(both(y)).x;
+                if (a.res) y += to_f(((const T*)a.res)[r[u] * a.ldr + i]);
+            }
+            ((T*)a.out)[r[u] * a.ldo + i] = from_f<T>(y);
+        }
+        if ((threadIdx.x & 31) == 0) atomicAdd((int*)&state[1], 1);   /* waits wait on */
     }
 }
 
@@ -491,16 +517,15 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     __shared__ __align__(8) MmBars bars;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort;
+    __shared__ int s_state[2];   /* mm_wait_long */
     __shared__ int s_cols[kSharedBoxes];
-    volatile int* abort_flag = &s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t wst = smem_u32(smem), xst = wst + kWSlots * kBoxBytes;
 
     for (int b = tid; b < min(a.dir.nboxes, kSharedBoxes); b += kTcWarps * 32)
         s_cols[b] = a.dir.boxes[b].col;
     if (tid == 0) {
-        s_abort = 0;
+        s_state[0] = s_state[1] = 0;
         for (int s = 0; s < kXStages; ++s) {
             mbar_init(bars.xfull[s], 1);
             mbar_init(bars.xempty[s], 1);
@@ -570,7 +595,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 for (int b = b0; b < b1 && ok; ++b) {
                     const int x0 = i0 + (b < kSharedBoxes ? s_cols[b] : a.dir.boxes[b].col);
                     for (int j = j0; j < min(j0 + group, r.ntiles); ++j) {
-                        ok = mm_wait(x.bar(xempty), x.round ^ 1, abort_flag);
+                        ok = mm_wait(x.bar(xempty), x.round ^ 1, s_state);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         if (leader && !(g_mm_withhold && blockIdx.x == 0 && issued == 0))
@@ -599,7 +624,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         bool ok = true;
         /* one box of one tile; the stage goes back to the TMA */
         auto box = [&](uint32_t wslot, uint32_t acc, bool first) {
-            ok = mm_wait(x.bar(xfull), x.round, abort_flag);
+            ok = mm_wait(x.bar(xfull), x.round, s_state);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -615,7 +640,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             x.next();
         };
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            ok = mm_wait(bar, parity, abort_flag);
+            ok = mm_wait(bar, parity, s_state);
             ok = __all_sync(0xffffffffu, ok);
             return ok;
         };
@@ -674,7 +699,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                               ((long long)r.e * ((a.n_out + kTN - 1) / kTN) + r.fb) * NB * kBoxBytes;
             for (int rep = 0; rep < reps && ok; ++rep)
                 for (int b = b0; b < b1; ++b) {
-                    ok = mm_wait(q.bar(wempty), q.round ^ 1, abort_flag);
+                    ok = mm_wait(q.bar(wempty), q.round ^ 1, s_state);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (leader)
@@ -714,8 +739,8 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         const int cfeat = 8 * (lane & 3);
         uint32_t flip = 0;                        /* the buffer in use, 0 or kEpiBuf */
 
-        /* a 32 x 32 block out of the buffer; rows left of the expert */
-        auto copy_out = [&](T* p, long long ld, int i, int row0, int left, bool vec) {
+        /* the rows of a 32 x 32 block (a bit each) out of the buffer */
+        auto copy_out = [&](T* p, long long ld, int i, int row0, uint32_t rows, bool vec) {
             __syncwarp();
             const uint32_t src = buf0 + flip + mine;
             const int nc = a.n_out - i;           /* of this lane's eight features */
@@ -726,7 +751,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                 asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                              : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
                              : "r"(src + it * 512));
-                if (crow + 8 * it < left) {
+                if (rows >> (crow + 8 * it) & 1) {
                     if (vec && nc >= 8)
                         *(uint4*)q = make_uint4(x[0], x[1], x[2], x[3]);
                     else
@@ -805,7 +830,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             int row0 = r.r0 + 32 * (int)tq;
             for (int j = r.ntiles; j > 0 && ok; --j, row0 += row_step, ac.next()) {
                 const int left = hi - row0;
-                ok = mm_wait(ac.bar(afull), ac.round, abort_flag);
+                ok = mm_wait(ac.bar(afull), ac.round, s_state);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -822,13 +847,10 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
 #pragma unroll
                 for (int c = 0; c < 32; c += 2)
                     chk = fma2(make_float2(v[c], v[c + 1]), both(0.0f), chk);
-                uint32_t again = 0;
-                if (chk.x + chk.y != 0.0f && lane < left) {   /* some sum is not finite */
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (!isfinite(v[c]) && i0 + fw + c < a.n_out) again |= 1u << c;
-                }
-                __syncwarp();
+                /* rows of the expert; those with a sum that is not finite are
+                 * stored by rows_again (a result may lie over its residual) */
+                const uint32_t rows = left >= 32 ? ~0u : (1u << max(left, 0)) - 1;
+                const uint32_t again = rows & __ballot_sync(0xffffffffu, chk.x + chk.y != 0.0f);
                 if (has_res) {
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
                     __syncwarp();
@@ -866,19 +888,14 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
 #pragma unroll
                     for (int h = 0; h < 4; ++h) y[4 * c + h] = pack2<T>(u[h].x, u[h].y);
                 }
-                if (has_z) {
-                    if (again)
-                        sum_again<T, TRANS, DIA_ACT_NONE>(a, K, e, row0 + lane, i0 + fw, again, row,
-                                                          spread, false);
-                    copy_out((T*)a.z, a.ldz, i0 + cfeat + fw, row0, left, alz);
-                }
+                if (has_z) copy_out((T*)a.z, a.ldz, i0 + cfeat + fw, row0, rows & ~again, alz);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     sts128(row + ((c ^ spread) << 4), y[4 * c], y[4 * c + 1], y[4 * c + 2],
                            y[4 * c + 3]);
+                copy_out((T*)a.out, a.ldo, i0 + cfeat + fw, row0, rows & ~again, al);
                 if (again)
-                    sum_again<T, TRANS, ACT>(a, K, e, row0 + lane, i0 + fw, again, row, spread, true);
-                copy_out((T*)a.out, a.ldo, i0 + cfeat + fw, row0, left, al);
+                    rows_again<T, TRANS, ACT>(a, K, e, row0, i0 + fw + lane, again, s_state);
                 if (has_res) flip ^= kEpiBuf;
                 }
                 cb -= 4;
@@ -947,10 +964,9 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     __shared__ __align__(8) unsigned long long xfull[STAGES], xempty[STAGES], xready[STAGES], done;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort;
+    __shared__ int s_state[2];   /* mm_wait_long */
     __shared__ Box s_box[kGBoxes];
     __shared__ int2 s_offs[kOffs];
-    volatile int* abort_flag = &s_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long b = blockIdx.x;
     const int fb = (int)(b % nfb), ch = (int)(b / nfb % nch);
@@ -970,7 +986,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     for (int k = tid; k < min(a.K, kOffs); k += kGWarps * 32) s_offs[k] = a.dir.offs[k];
     if (tid < nb) s_box[tid] = a.dir.boxes[b0 + tid];
     if (tid == 0) {
-        s_abort = 0;
+        s_state[0] = s_state[1] = 0;
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(xfull[s], 1);
             mbar_init(xempty[s], 1);
@@ -1001,7 +1017,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         Ring<STAGES> x;
         int g = 0;
         for (; g < nst; ++g, x.next()) {
-            ok = mm_wait(x.bar(empty0), x.round ^ 1, abort_flag);
+            ok = mm_wait(x.bar(empty0), x.round ^ 1, s_state);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (leader && !(g_mm_withhold && blockIdx.x == 0 && g == 0)) {
@@ -1032,8 +1048,8 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         Ring<STAGES> x;
         for (int g = 0; g < nst; ++g, x.next()) {
             const int left = rg.r1 - rg.r0 - g * kGRows;
-            ok = mm_wait(x.bar(full0), x.round, abort_flag) &&
-                 (!conv || mm_wait(x.bar(ready0), x.round, abort_flag));
+            ok = mm_wait(x.bar(full0), x.round, s_state) &&
+                 (!conv || mm_wait(x.bar(ready0), x.round, s_state));
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (left < kGRows) {
@@ -1068,7 +1084,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         Ring<STAGES> x;
         if (half) x.next();
         for (int g = half; g < nst; g += 2, x.next(), x.next()) {
-            ok = mm_wait(x.bar(full0), x.round, abort_flag);
+            ok = mm_wait(x.bar(full0), x.round, s_state);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int left = rg.r1 - rg.r0 - g * kGRows;

@@ -870,3 +870,57 @@ def test_time_of_a_gradient_that_overflowed():
                                      torch.cuda.current_stream().cuda_stream))
 
     assert time_against_cores(f) < 2
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_product_of_a_block_that_overflowed(value, t):
+    """No input is finite: sums, z and results are what their own terms give,
+    gradients of the inputs likewise."""
+    M, n, off = 300, 264, [-250, -64, -1, 0, 1, 2, 3, 200]
+    c = Case(t, M, n, n, off, seed=64)
+    c.x.fill_(value)
+    c.dy.fill_(value)
+    v, x = c.v(c.vals), c.v(c.x)
+    y, z = dg.spmm(c.plan, c.vals[0], c.x, bias=c.bias[0], act="relu", residual=c.res, save_z=True)
+    want = product64(off, n, n, v, x, c.parts, c.v(c.bias))[0]
+    alike(z, want, "z")
+    finite = act64(want, "relu").isfinite()
+    alike(torch.where(finite.cuda(), 0, y), act64(want, "relu") + torch.where(finite, 0, c.v(c.res))
+          - torch.where(finite, act64(want, "relu"), 0), "y")
+    dx = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy)[0]
+    alike(dx, gradient64(off, n, n, v, x, c.v(c.dy), c.parts)[0], "dx")
+
+
+def test_time_of_a_product_that_overflowed():
+    """Sums over their own terms are shared out over the lanes (one lane a row
+    took 55 times the CUDA-core form's time and twice that with z kept, this nine
+    times)."""
+    c = Case(torch.float16, 4096, 2048, 2048, band(64), seed=65)
+    c.x.fill_(float("inf"))
+    y, z = torch.empty_like(c.x), torch.empty_like(c.x)
+    assert time_against_cores(lambda: dg.spmm(c.plan, c.vals[0], c.x, out=y)) < 25
+    assert time_against_cores(lambda: dg.spmm(c.plan, c.vals[0], c.x, out=y, z=z)) < 25
+
+
+def test_waits_outlast_sums_over_their_own_terms():
+    """A wait's limit does not run while the sums that it waits for are being
+    computed again: 2 ms, a block without a finite value, six tiles a CTA of
+    527 diagonals."""
+    M, n, off = 40000, 264, band(263)
+    c = Case(torch.bfloat16, M, n, n, off, seed=66)
+    c.x.fill_(float("inf"))
+    L = dg.lib()
+    want = product64(off, n, n, c.v(c.vals), c.v(c.x[:1]), [(0, 0, 1)])[0].expand(M, n)
+    dg.check(L.dia_test_spmm_form(2))
+    try:
+        dg.spmm(c.plan, c.vals[0], c.x)         # the kernel is loaded
+        torch.cuda.synchronize()
+        dg.device_status(clear=True)
+        dg.check(L.dia_test_tc_wait(2_000_000, 0))
+        y = dg.spmm(c.plan, c.vals[0], c.x)
+        torch.cuda.synchronize()
+        assert dg.device_status(clear=True) == 0
+    finally:
+        dg.check(L.dia_test_tc_wait(0, 0))
+        dg.check(L.dia_test_spmm_form(0))
+    alike(y, want, "y")
