@@ -240,7 +240,9 @@ __device__ __forceinline__ float act_any(int act, float z)
 }
 
 /* one copy of the functions for every row of a tile: inlined 32 times they
- * did not fit the instruction cache */
+ * did not fit the instruction cache, inlined eight times eight rows of 4096
+ * under 33 diagonals, without an activation, took 6.45 us in place of 5.2 */
+static __device__ __noinline__ float act1(int act, float z) { return act_any(act, z); }
 static __device__ __noinline__ float4 act4(int act, float4 z)
 {
     return make_float4(act_any(act, z.x), act_any(act, z.y), act_any(act, z.z), act_any(act, z.w));

@@ -21,7 +21,7 @@ namespace dia {
  * a time in flight each) and add up in shared memory in a fixed order, and
  * what the epilogue reads is fetched first.  The other 16 / ks warps take
  * other features.  One row of 4096 under 129 diagonals, bf16: 5.5 us; eight
- * rows under 33, fp32: 6.3 us; 64 rows of 64 experts (1024, 33 diagonals,
+ * rows under 33, fp32: 5.2 us; 64 rows of 64 experts (1024, 33 diagonals,
  * fp16): 10.1 us, all a launch and three or four dependent reads (their bytes
  * take 0.1 to 0.7 us). */
 constexpr int kFewWarps = 16;
@@ -102,9 +102,13 @@ spmm_few_kernel(const __grid_constant__ ProdArgs a, int ks, int ftiles, long lon
     for (int t = 0; t < TT; ++t) {
         if (t >= nt) break;
         const long long row = rg.r0 + t;
-        const float z = acc[t] + bias;
-        if (!TRANS && a.z) ((T*)a.z)[row * a.ldz + i] = from_f<T>(z);
-        ((T*)a.out)[row * a.ldo + i] = from_f<T>(TRANS ? z : act_any(a.act, z) + res[t]);
+        float y = acc[t] + bias;
+        if (!TRANS) {
+            if (a.z) ((T*)a.z)[row * a.ldz + i] = from_f<T>(y);
+            if (a.act != DIA_ACT_NONE) y = act1(a.act, y);
+            y += res[t];
+        }
+        ((T*)a.out)[row * a.ldo + i] = from_f<T>(y);
     }
 }
 
