@@ -54,6 +54,14 @@ static bool tensor_form(const DiaSpmmPlan* p, int dtype, long long M, int E, boo
     if (dtype == DIA_F32 || d.nboxes == 0 || form == 1) return false;
     if (form == 2) return true;
     if (M < 8) return false;   /* the cores' time does not grow up to there */
+    /* The packed operator takes 16 KB a box, for a few scattered diagonals up to
+     * fifty times the diagonals themselves (27-point stencil on 128^3: 5.6 GB),
+     * and a caller may lack the room: it takes no more than the block and its
+     * result do, or 2 GB. */
+    const double block = 2.0 * M * ((double)p->n_rows + p->n_cols);
+    const long long pack = backward ? spmm_tc_pack_bytes(p->trn, p->K, p->n_cols, M, E)
+                                    : spmm_tc_pack_bytes(d, p->K, p->n_rows, M, E);
+    if ((double)pack > std::max(block, 2147483648.0)) return false;
     const double nfb = (p->n_rows + 127) / 128, boxes = nfb * E * d.nboxes;
     const double tiles = nfb * (M / 128.0 + (E > 1 ? (double)std::min<long long>(E, M) : 1.0));
     const double mega = (double)M * p->n_rows * 1e-6;

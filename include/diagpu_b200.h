@@ -207,8 +207,11 @@ int dia_spmm_plan_destroy(DiaSpmmPlan* plan);
  * before seg[0] and from seg[num_experts] on are left as they were.  y and z
  * must not overlap inputs, except that y may be res itself (same address and
  * stride).  Allocates nothing and does not synchronise.  work:
- * dia_spmm_workspace bytes (0 where the CUDA cores do the work), 256-byte
- * aligned, not shared by calls that may run at the same time. */
+ * dia_spmm_workspace bytes (0 where the CUDA cores do the work; else the
+ * operator as the tensor cores read it, at most the larger of 2 GB and the
+ * bytes of x and y, and a copy of x where its row stride is not a multiple of
+ * 16 bytes), 256-byte aligned, not shared by calls that may run at the same
+ * time. */
 int64_t dia_spmm_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
                            int64_t ldx);
 int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
@@ -226,8 +229,9 @@ int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
  * dx, dvals (16-byte aligned) and dbias may each be NULL; act DIA_ACT_NONE
  * takes no z.  Outputs must not overlap inputs or one another; they are
  * overwritten, rows of dx outside [seg[0], seg[num_experts]) left as they
- * were.  work: dia_spmm_backward_workspace bytes, 256-byte aligned, not shared
- * by calls that may run at the same time. */
+ * were.  work: dia_spmm_backward_workspace bytes (dz, sums of parts, and as for
+ * dia_spmm), 256-byte aligned, not shared by calls that may run at the same
+ * time. */
 int64_t dia_spmm_backward_workspace(const DiaSpmmPlan* plan, int dtype, int64_t M,
                                     int num_experts, int64_t ldx, int64_t stride, int64_t lddy,
                                     int act);

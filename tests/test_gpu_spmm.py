@@ -924,3 +924,18 @@ def test_waits_outlast_sums_over_their_own_terms():
         dg.check(L.dia_test_tc_wait(0, 0))
         dg.check(L.dia_test_spmm_form(0))
     alike(y, want, "y")
+
+
+@pytest.mark.parametrize("side,M", [(128, 256), (256, 512), (256, 32), (64, 2048), (96, 8192)])
+def test_workspace_has_a_limit(side, M):
+    """An operator packed for the tensor cores takes no more room than the block
+    and its result, or 2 GB: scattered diagonals of large operators would take
+    fifty times their own.  Sizes only; nothing of them is allocated."""
+    n = side ** 3
+    plan = dg.SpmmPlan(n, n, [i + side * j + side * side * k for i in (-1, 0, 1)
+                              for j in (-1, 0, 1) for k in (-1, 0, 1)])
+    L, block = dg.lib(), 2 * 2 * M * n
+    most = max(block, 1 << 31)
+    assert 0 <= L.dia_spmm_workspace(plan._h, 2, M, 1, n) <= most
+    # and dz; features enough for every SM leave the rows in one part
+    assert 0 <= L.dia_spmm_backward_workspace(plan._h, 2, M, 1, n, n, n, 2) <= most + block // 2
