@@ -768,18 +768,25 @@ def _spmm_block(who, name, t, plan, dtype, rows, width):
     return t.data_ptr(), ld if rows > 1 else width
 
 
-def _spmm_operator(who, plan, vals, x, seg):
-    """(dtype code, number of experts, stride) after checking x, vals and seg."""
+def _spmm_vals(who, plan, vals, x, experts):
+    """The dtype code after checking vals against x and the plan."""
     code = _SPMM_TYPES.get(x.dtype)
     if code is None:
         raise DiaError(DIA_ERR_INVALID, f"{who}: {x.dtype} is not float32, float16 or bfloat16")
     shape = vals.shape
-    if len(shape) != (2 if seg is None else 3) or shape[-2] != plan.K:
+    if len(shape) != (3 if experts else 2) or shape[-2] != plan.K:
         raise DiaError(DIA_ERR_INVALID, f"{who}: vals must be "
-                       + ("[K, stride]" if seg is None else "[experts, K, stride]"))
+                       + ("[experts, K, stride]" if experts else "[K, stride]"))
     if vals.dtype != x.dtype or vals.device != plan.device or not vals.is_contiguous():
         raise DiaError(DIA_ERR_INVALID,
                        f"{who}: vals must be a contiguous {x.dtype} tensor on {plan.device}")
+    return code
+
+
+def _spmm_operator(who, plan, vals, x, seg):
+    """(dtype code, number of experts, stride) after checking x, vals and seg."""
+    code = _spmm_vals(who, plan, vals, x, seg is not None)
+    shape = vals.shape
     if seg is None:
         return code, 1, shape[1]
     E = shape[0]
@@ -942,18 +949,28 @@ def spmm_backward(plan: SpmmPlan, vals, x, dy, *, z=None, act="none", seg=None, 
 
 def spmm_workspace(plan: SpmmPlan, vals, x):
     """Bytes of the work buffer of spmm for an operator and a block like these."""
-    E = vals.shape[0] if vals.dim() == 3 else 1
-    ldx = _spmm_block("spmm_workspace", "x", x, plan, vals.dtype, x.shape[0], plan.n_cols)[1]
-    return lib().dia_spmm_workspace(plan._h, _SPMM_TYPES[vals.dtype], x.shape[0], E, ldx)
+    if _elsewhere(plan):
+        with torch.cuda.device(plan.device):
+            return spmm_workspace(plan, vals, x)
+    who = "spmm_workspace"
+    dt = _spmm_vals(who, plan, vals, x, vals.dim() == 3)
+    M, E = x.shape[0], vals.shape[0] if vals.dim() == 3 else 1
+    ldx = _spmm_block(who, "x", x, plan, x.dtype, M, plan.n_cols)[1]
+    return lib().dia_spmm_workspace(plan._h, dt, M, E, ldx)
 
 
 def spmm_backward_workspace(plan: SpmmPlan, vals, x, dy, act="none"):
     """Bytes of the work buffer of spmm_backward for operands like these."""
-    who, E, M = "spmm_backward_workspace", vals.shape[0] if vals.dim() == 3 else 1, x.shape[0]
-    ldx = _spmm_block(who, "x", x, plan, vals.dtype, M, plan.n_cols)[1]
-    lddy = _spmm_block(who, "dy", dy, plan, vals.dtype, M, plan.n_rows)[1]
-    return lib().dia_spmm_backward_workspace(plan._h, _SPMM_TYPES[vals.dtype], M, E, ldx,
-                                             vals.shape[-1], lddy, _spmm_act(who, act))
+    if _elsewhere(plan):
+        with torch.cuda.device(plan.device):
+            return spmm_backward_workspace(plan, vals, x, dy, act)
+    who = "spmm_backward_workspace"
+    code = _spmm_act(who, act)
+    dt = _spmm_vals(who, plan, vals, x, vals.dim() == 3)
+    M, E = x.shape[0], vals.shape[0] if vals.dim() == 3 else 1
+    ldx = _spmm_block(who, "x", x, plan, x.dtype, M, plan.n_cols)[1]
+    lddy = _spmm_block(who, "dy", dy, plan, x.dtype, M, plan.n_rows)[1]
+    return lib().dia_spmm_backward_workspace(plan._h, dt, M, E, ldx, vals.shape[-1], lddy, code)
 
 
 # ---------------------------------------------------------------- gemm_diag

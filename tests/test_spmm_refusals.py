@@ -152,3 +152,16 @@ def test_workspace_lives_until_the_call_returns(monkeypatch):
     dg.spmm(plan, vals, x)
     dg.spmm_backward(plan, vals, x, torch.zeros(4, 8))
     assert [(size, len(alive)) for size, alive in seen] == [(512, 1), (512, 1)]
+
+
+def test_workspace_queries():
+    """They refuse what the calls refuse."""
+    plan, vals, x = good()
+    dy = torch.zeros(4, 8)
+    for f, a in ((dg.spmm_workspace, ()), (dg.spmm_backward_workspace, (dy,))):
+        refused("not float32", f, plan, vals.double(), x.double(), *(t.double() for t in a))
+        refused("vals must be", f, plan, vals[:2], x, *a)
+        refused("vals must be", f, plan, vals[0], x, *a)
+        refused("contiguous", f, plan, vals.half(), x, *a)
+        refused("2-D", f, plan, vals, x[0], *a)
+    refused("act must be", dg.spmm_backward_workspace, plan, vals, x, dy, "swish")
