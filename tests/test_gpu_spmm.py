@@ -939,3 +939,64 @@ def test_workspace_has_a_limit(side, M):
     assert 0 <= L.dia_spmm_workspace(plan._h, 2, M, 1, n) <= most
     # and dz; features enough for every SM leave the rows in one part
     assert 0 <= L.dia_spmm_backward_workspace(plan._h, 2, M, 1, n, n, n, 2) <= most + block // 2
+
+
+# Sizes at which a kernel takes its other path: more diagonals than a CTA keeps
+# offsets of (512), more boxes than it keeps places of (64).
+LARGE = {
+    "diagonals, 1 row": (1, 700, 700, list(range(-550, 550))),
+    "diagonals, 2 rows": (2, 700, 700, list(range(-550, 550))),
+    "diagonals": (20, 700, 700, list(range(-550, 550))),
+    "diagonals, tiles": (300, 700, 700, list(range(-550, 550))),
+    "boxes": (200, 9200, 9200, list(range(-4550, 4550, 130))),
+}
+
+
+@pytest.mark.parametrize("shape", LARGE)
+def test_many_diagonals_and_boxes(shape, t):
+    c = Case(t, *LARGE[shape], seed=67)
+    c.product(act="silu", bias=True, res=True, z=True)
+    c.gradient(act="silu")
+
+
+def test_many_diagonals_of_experts(t):
+    c = Case(t, 150, 300, 300, list(range(-290, 290)), seed=68, seg=[0, 1, 40, 40, 149])
+    c.product(act="relu", bias=True)
+    c.gradient(act="relu")
+
+
+# The many-row CUDA-core kernel, which begins at 196608 results: rows and bases
+# that its vector accesses do not take, and each of its feature tiles (256, 512
+# and 1024: the widest that fits and leaves every SM a CTA).
+@pytest.mark.parametrize("off", [band(4), [-300, -40, 0, 1, 77, 400]], ids=["band", "scattered"])
+@pytest.mark.parametrize("M,n,ld,shift", [(300, 701, 1, 0), (300, 700, None, 1), (300, 702, 3, 2),
+                                          (600, 700, 4, 0), (8, 100000, None, 0),
+                                          (1200, 2100, None, 0), (1201, 2101, 1, 1)])
+def test_many_rows_on_the_cores(M, n, ld, shift, off, t):
+    c = Case(t, M, n, n, off, seed=69, ld=ld, shift=shift)
+    c.product(act="gelu", bias=True, res=True, z=True)
+    c.gradient(act="gelu")
+
+
+def test_offsets_past_32_bits_on_the_tensor_cores():
+    """As above, where TMA and the tensor cores' epilogue step from row to row."""
+    n, M, off = 64, 3, band(2)
+    ld = (1 << 30) + 8
+    buf = torch.empty(2 * ld + n, dtype=torch.bfloat16, device="cuda")
+    x = buf.as_strided((M, n), (ld, 1))
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x.copy_(torch.randn(M, n, generator=g, device="cuda"))
+    v = torch.randn(5, 64, generator=g, device="cuda").bfloat16()
+    plan, near = dg.SpmmPlan(n, n, off), x.contiguous()
+    dg.check(dg.lib().dia_test_spmm_form(2))
+    try:
+        want = dg.spmm(plan, v, near, act="silu", residual=near, save_z=True)
+        got = dg.spmm(plan, v, x, act="silu", residual=x, save_z=True)
+        a = dg.spmm_backward(plan, v, x, x, z=x, act="silu", bias_grad=True)
+        b = dg.spmm_backward(plan, v, near, near, z=near, act="silu", bias_grad=True)
+        dg.spmm(plan, v, near, out=x)
+        assert torch.equal(x, dg.spmm(plan, v, near))
+        assert dg.device_status() == 0
+    finally:
+        dg.check(dg.lib().dia_test_spmm_form(0))
+    assert all(torch.equal(p, q) for p, q in zip((*got, *a), (*want, *b)))
