@@ -317,7 +317,7 @@ static cudaError_t upload(void** dst, const std::vector<char>& blob)
 static void release(DiaSpmmPlan* p)
 {
     BesideCapture beside;
-    if (p->blob) cudaFree(p->blob);
+    if (p->blob && cudaFree(p->blob) != cudaSuccess) cudaGetLastError();
     delete p;
 }
 

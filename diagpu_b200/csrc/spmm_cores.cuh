@@ -619,9 +619,8 @@ static int launch_few(const ProdArgs& a, cudaStream_t stream)
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: block too large");
     /* the larger of block and operator is streamed once, the other stays in L2 */
     const bool rows_first = (long long)a.M * a.n_in < a.stride * a.K;
-    spmm_few_kernel<T, TRANS, TT><<<(unsigned)grid, kFewWarps * 32, 0, stream>>>(
-        a, ks, ftiles, ngroups, rows_first);
-    DIA_TRY_CUDA(cudaGetLastError());
+    DIA_TRY_CUDA(launch(false, spmm_few_kernel<T, TRANS, TT>, (int)grid, kFewWarps * 32, 0, stream,
+                        a, ks, ftiles, ngroups, rows_first));
     return DIA_OK;
 }
 
@@ -637,9 +636,8 @@ static int launch_tile_as(const ProdArgs& a, int shape, int smem, cudaStream_t s
     const auto kernel = spmm_tile_kernel<T, TRANS, VEC, QUADS>;
     static SmemRecord most;
     DIA_TRY_CUDA(allow_smem(kernel, kTileSmem, most));
-    kernel<<<(unsigned)(ngroups * ftiles), kTileWarps * 32, smem, stream>>>(a, shape, ftiles,
-                                                                            ngroups, rows_first);
-    DIA_TRY_CUDA(cudaGetLastError());
+    DIA_TRY_CUDA(launch(false, kernel, (int)(ngroups * ftiles), kTileWarps * 32, smem, stream, a,
+                        shape, ftiles, ngroups, rows_first));
     return DIA_OK;
 }
 
@@ -742,8 +740,8 @@ int Cores<T>::gradient(const GradArgs& a, cudaStream_t stream)
     const Kernel kernel = kernels[vec][pick];
     static SmemRecord most[2][5];
     DIA_TRY_CUDA(allow_smem(kernel, kGradSmem, most[vec][pick]));
-    kernel<<<(unsigned)grid, kTileWarps * 32, smem, stream>>>(a, ftiles, nwins, rows);
-    DIA_TRY_CUDA(cudaGetLastError());
+    DIA_TRY_CUDA(launch(false, kernel, (int)grid, kTileWarps * 32, smem, stream, a, ftiles, nwins,
+                        rows));
     return DIA_OK;
 }
 

@@ -26,6 +26,7 @@ int cuda_fail(cudaError_t e, const char* what)
 {
     g_last_error = std::string(what) + ": " + cudaGetErrorName(e) + " (" +
                    cudaGetErrorString(e) + ")";
+    cudaGetLastError();   /* reported here: the next launch does not find it again */
     return DIA_ERR_CUDA;
 }
 

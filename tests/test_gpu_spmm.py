@@ -1000,3 +1000,21 @@ def test_offsets_past_32_bits_on_the_tensor_cores():
     finally:
         dg.check(dg.lib().dia_test_spmm_form(0))
     assert all(torch.equal(p, q) for p, q in zip((*got, *a), (*want, *b)))
+
+
+@pytest.mark.parametrize("M", [1, 300])
+def test_an_error_is_reported_once(M, t):
+    """A call of the library that failed (here one that allocates, during a
+    capture) has reported its error; the next call, which is good, does not
+    report it again."""
+    c = Case(t, M, 700, 700, band(3), seed=70)
+    A = dg.DiaRows.synth(64, 64, np.array([0, 1], np.int32), seed=1)
+    calls = (lambda: (dg.spmm(c.plan, c.vals[0], c.x),),
+             lambda: dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy)[:2])
+    for f in calls:
+        want = f()
+        torch.cuda.synchronize()
+        with pytest.raises(Exception):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                dg.SpmspmPlan(A, A)
+        assert all(torch.equal(p, q) for p, q in zip(f(), want))
