@@ -51,7 +51,8 @@ static bool tensor_form(const DiaSpmmPlan* p, int dtype, long long M, int E, boo
 {
     const int form = g_form.load(std::memory_order_relaxed);
     const SpmmDir& d = p->fwd;
-    if (dtype == DIA_F32 || d.nboxes == 0 || form == 1) return false;
+    if (dtype == DIA_F32 || d.nboxes == 0 || p->n_rows == 0 || p->n_cols == 0 || form == 1)
+        return false;
     if (form == 2) return true;
     if (M < 8) return false;   /* the cores' time does not grow up to there */
     /* The packed operator takes 16 KB a box, for a few scattered diagonals up to
