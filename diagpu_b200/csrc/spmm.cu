@@ -392,8 +392,8 @@ static long long copy_bytes(bool tensor, int64_t M, int n, int64_t ld)
     return M > 0 && ld % 8 != 0 && tensor ? align256(M * ((n + 7) / 8 * 8) * 2ll) : 0;
 }
 
-/* the gradient's workspace: dz (where the activation makes one, or as a copy
- * of dy), sums of parts (where there are several), the operator's boxes, a
+/* the gradient's workspace: dz (32 bits, where there is an activation, or a
+ * copy of dy), sums of parts (where there are several), the operator's boxes, a
  * copy of x */
 struct GradPlan {
     int per;
@@ -410,7 +410,7 @@ static GradPlan grad_plan(const DiaSpmmPlan* p, int dtype, int64_t M, int E, int
     g.per = grad_part_rows(p, g.tensor, M, E, stride);
     g.lddz = (p->n_rows + 7) / 8 * 8;
     g.made = act != DIA_ACT_NONE || copy_bytes(g.tensor, M, p->n_rows, lddy) > 0;
-    g.dz_bytes = g.made ? align256(M * g.lddz * (long long)elem_size(dtype)) : 0;
+    g.dz_bytes = !g.made ? 0 : align256(M * g.lddz * (act != DIA_ACT_NONE ? 4ll : 2ll));
     g.part_bytes = align256(grad_slots(M, g.per) * (p->K + 1) * stride * 4);
     g.pack_bytes = pack_bytes(p->trn, p->K, g.tensor, M, E, p->n_cols);
     g.x_bytes = copy_bytes(g.tensor, M, p->n_cols, ldx);
@@ -524,8 +524,8 @@ extern "C" int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_e
         if (copy > 0) {
             a.in = (char*)d_work + pack;
             a.ldi = (plan->n_cols + 7) / 8 * 8;
-            r = Cores<T>::dz(DIA_ACT_NONE, d_x, ldx, nullptr, 0, (char*)d_work + pack, a.ldi, a.M,
-                             a.n_in, false, stream);
+            r = Cores<T>::dz(kDzSame, DIA_ACT_NONE, d_x, ldx, nullptr, 0, (char*)d_work + pack,
+                             nullptr, a.ldi, a.M, a.n_in, false, stream);
         }
         if (r == DIA_OK && product_on_tc(a, tensor)) {
             r = spmm_tc_pack(a, false, stream);
@@ -628,15 +628,34 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
         if (g.x_bytes > 0 && a.dvals) {
             a.x = (char*)d_work + g.dz_bytes + g.part_bytes + g.pack_bytes;
             a.ldx = (plan->n_cols + 7) / 8 * 8;
-            r = Cores<T>::dz(DIA_ACT_NONE, d_x, ldx, nullptr, 0, (void*)a.x, a.ldx, a.M, a.n_cols,
-                             false, stream);
+            r = Cores<T>::dz(kDzSame, DIA_ACT_NONE, d_x, ldx, nullptr, 0, (void*)a.x, nullptr, a.ldx,
+                             a.M, a.n_cols, false, stream);
+        }
+        /* Who reads dz on the CUDA cores has it in fp32, who does on the tensor
+         * cores as a pair.  Where the tensor cores take dx alone, the diagonals'
+         * or the bias's gradient goes first and dz is made twice. */
+        const bool tc = d_dx && product_on_tc(p, g.tensor);
+        const bool gtc = grad && grad_on_tc(a, g.tensor);
+        const bool acts = act != DIA_ACT_NONE;
+        const bool twice = acts && tc && grad && !gtc;
+        const bool makes = gtc && acts && spmm_tc_makes_dz(a);
+        const bool pair = acts && (tc || gtc);
+        char* const rest = (char*)d_work + (long long)p.M * p.ldi * 2;
+        auto make_dz = [&](DzForm form, bool dependent) {
+            return Cores<T>::dz(form, act, d_dy, lddy, d_z, ldz, d_work, rest, p.ldi, p.M, p.n_in,
+                                dependent, stream);
+        };
+        p.lo = pair && tc ? rest : nullptr;
+        a.lo = pair && gtc ? rest : nullptr;
+        p.in32 = acts && !tc;
+        a.dz32 = acts && !gtc;
+        if (r == DIA_OK && twice) {
+            r = make_dz(kDzF32, false);
+            if (r == DIA_OK) r = Cores<T>::gradient(a, stream);
         }
         /* Launches of the tensor-core form overlap.  Where the diagonals'
          * gradient makes dz itself it goes first, the operator is packed on
          * the SMs that it leaves free; else the operator is packed under dz. */
-        const bool tc = d_dx && product_on_tc(p, g.tensor);
-        const bool gtc = grad && grad_on_tc(a, g.tensor);
-        const bool makes = gtc && made && spmm_tc_makes_dz(a);
         if (r != DIA_OK) return r;
         if (makes) {
             r = spmm_tc_gradient(a, dtype, true, false, stream);
@@ -646,9 +665,8 @@ extern "C" int dia_spmm_backward(const DiaSpmmPlan* plan, int dtype, int64_t M, 
             const bool packed = tc && g.pack_bytes > 0;
             if (packed) r = spmm_tc_pack(p, false, stream);
             if (r == DIA_OK && made)
-                r = Cores<T>::dz(act, d_dy, lddy, d_z, ldz, d_work, p.ldi, p.M, p.n_in, packed,
-                                 stream);
-            if (r == DIA_OK && grad)
+                r = make_dz(!acts ? kDzSame : pair ? kDzPair : kDzF32, packed);
+            if (r == DIA_OK && grad && !twice)
                 r = gtc ? spmm_tc_gradient(a, dtype, false, packed || made, stream)
                         : Cores<T>::gradient(a, stream);
             p.early = tc && gtc;   /* what it reads is older than the gradient */

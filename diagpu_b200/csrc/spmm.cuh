@@ -425,6 +425,8 @@ __device__ __forceinline__ void store4(T* p, float4 v)
 /* out = act(in * A + bias) + res of one direction, z kept where given */
 struct ProdArgs {
     const void* in;
+    const void* lo;       /* tensor-core form of dx: the rest of dz (kDzPair), or null */
+    bool in32;            /* CUDA-core form of dx: dz is fp32 */
     const void* vals;
     const void* bias;
     const void* res;
@@ -446,6 +448,8 @@ struct ProdArgs {
 /* dvals[k, i] = sum_t dz[t, i] x[t, i + off_k], dbias[i] = sum_t dz[t, i] */
 struct GradArgs {
     const void* dz;       /* act other than none: the workspace's */
+    const void* lo;       /* tensor-core form: the rest of dz (kDzPair), or null */
+    bool dz32;            /* CUDA-core form: dz is fp32 */
     const void* dy;
     const void* z;
     const void* x;
@@ -517,13 +521,30 @@ static cudaError_t launch(bool dependent, void (*kernel)(P...), int grid, int bl
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+/* How dz = dy * act'(z) is kept for the gradients that read it.  Rounded to 16
+ * bits it would double the variance of their error (0.0024 of a bf16 gradient's
+ * size in place of 0.0017), so blocks of 16-bit types keep 32 bits: an fp32
+ * for the CUDA cores; for the tensor cores, whose operands are of the block's
+ * type, dz rounded and, in a second array, the rest of it rounded (2^-18 of dz
+ * for bf16; the rest of what is not finite is 0).  Where there is no activation
+ * dz is dy, and kDzSame a copy of a block whose rows TMA does not take. */
+enum DzForm { kDzSame, kDzF32, kDzPair };
+
+/* the rest of v that its rounding leaves */
+__device__ __forceinline__ float rest_of(float v, float rounded)
+{
+    const float r = v - rounded;
+    return fabsf(r) <= 3.4028235e38f ? r : 0.0f;
+}
+
 /* CUDA-core forms (spmm_cores.cuh); join: sums of experts with several parts,
  * for either form of the gradient */
 template <typename T>
 struct Cores {
     static int product(const ProdArgs& a, cudaStream_t stream);
-    static int dz(int act, const void* dy, long long lddy, const void* z, long long ldz, void* dz,
-                  long long lddz, int M, int n, bool dependent, cudaStream_t stream);
+    static int dz(DzForm form, int act, const void* dy, long long lddy, const void* z,
+                  long long ldz, void* dz, void* lo, long long lddz, int M, int n, bool dependent,
+                  cudaStream_t stream);
     static int gradient(const GradArgs& a, cudaStream_t stream);
     static int join(const GradArgs& a, cudaStream_t stream);
 };
@@ -536,7 +557,8 @@ bool spmm_tc_block(const void* p, long long ld);
 long long spmm_tc_pack_bytes(const SpmmDir& d, int K, int n_out, long long M, int E);
 int spmm_tc_pack(const ProdArgs& a, bool dependent, cudaStream_t stream);
 int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream);
-/* make: dz is made there from dy and z (spmm_tc_makes_dz says whether it can be) */
+/* make: dz (kDzPair) is made there from dy and z (spmm_tc_makes_dz says whether
+ * it can be) */
 bool spmm_tc_makes_dz(const GradArgs& a);
 int spmm_tc_gradient(const GradArgs& a, int dtype, bool make, bool dependent, cudaStream_t stream);
 cudaError_t spmm_tc_status(unsigned int* flags, bool clear);

@@ -27,7 +27,7 @@ namespace dia {
 constexpr int kFewWarps = 16;
 constexpr int kFewOffs = 512;   /* offsets staged at once */
 
-template <typename T, bool TRANS, int TT>
+template <typename T, typename IN, bool TRANS, int TT>
 __global__ void __launch_bounds__(kFewWarps * 32)
 spmm_few_kernel(const __grid_constant__ ProdArgs a, int ks, int ftiles, long long ngroups,
                 bool rows_first)
@@ -47,7 +47,7 @@ spmm_few_kernel(const __grid_constant__ ProdArgs a, int ks, int ftiles, long lon
     const bool on = i < a.n_out;
     const int nt = rg.r1 - rg.r0;
     const T* vals = (const T*)a.vals + rg.e * a.estride;
-    const T* in = (const T*)a.in + rg.r0 * a.ldi;
+    const IN* in = (const IN*)a.in + rg.r0 * a.ldi;
     float bias = 0.0f, res[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) res[t] = 0.0f;
@@ -164,13 +164,13 @@ __device__ __forceinline__ void stage_spans(T* dst, int pitch, const InputSpan* 
     }
 }
 
-template <typename T, bool TRANS, bool VEC, bool QUADS>
+template <typename T, typename IN, bool TRANS, bool VEC, bool QUADS>
 __global__ void __launch_bounds__(kTileWarps * 32)
 spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long long ngroups,
                  bool rows_first)
 {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    T* xs = (T*)smem_raw;
+    IN* xs = (IN*)smem_raw;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int F = kTileF[0] << shape, wf = F / 128;   /* warps side by side */
     const int rows = kTileWarps / wf * kTileRows;
@@ -180,15 +180,15 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
     const RowGroup rg = row_group(a.seg, a.E, a.M, rows, g, false);
     if (rg.e < 0) return;   /* whole CTA */
     const int nt = rg.r1 - rg.r0, pitch = a.dir.width[shape];
-    stage_spans<T, VEC>(xs, pitch, a.dir.spans[shape], 0, a.dir.nspans[shape],
-                        (const T*)a.in + rg.r0 * a.ldi, a.ldi, i0, a.n_in, rows, nt);
+    stage_spans<IN, VEC>(xs, pitch, a.dir.spans[shape], 0, a.dir.nspans[shape],
+                         (const IN*)a.in + rg.r0 * a.ldi, a.ldi, i0, a.n_in, rows, nt);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     const int t0 = warp / wf * kTileRows, f0 = warp % wf * 128;
     if (t0 >= nt || i0 + f0 >= a.n_out) return;
     const int live = min(nt - t0, kTileRows);
     const T* vals = (const T*)a.vals + rg.e * a.estride;
-    const T* xw = xs + t0 * pitch;
+    const IN* xw = xs + t0 * pitch;
     float acc[kTileRows][4];
 #pragma unroll
     for (int t = 0; t < kTileRows; ++t)
@@ -231,17 +231,17 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
         float carry[kTileRows][4];
         int next = INT_MIN;   /* base of the quad whose first piece `carry` holds */
         auto work = [&](const Weights& v) {
-            const T* p = xw + v.col + f;
+            const IN* p = xw + v.col + f;
             if (v.base != next) {
 #pragma unroll
-                for (int t = 0; t < kTileRows; ++t) *(float4*)carry[t] = load4<T>(p + t * pitch);
+                for (int t = 0; t < kTileRows; ++t) *(float4*)carry[t] = load4<IN>(p + t * pitch);
             }
             next = v.base + 4;
 #pragma unroll
             for (int t = 0; t < kTileRows; ++t) {
                 float x[8];
                 *(float4*)x = *(float4*)carry[t];
-                *(float4*)(x + 4) = load4<T>(p + t * pitch + 4);
+                *(float4*)(x + 4) = load4<IN>(p + t * pitch + 4);
                 *(float4*)carry[t] = *(float4*)(x + 4);
 #pragma unroll
                 for (int s = 0; s < 4; ++s)
@@ -293,7 +293,7 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (u >= n) break;
-                const T* p = xw + col[u] + f;
+                const IN* p = xw + col[u] + f;
 #pragma unroll
                 for (int t = 0; t < kTileRows; ++t)
 #pragma unroll
@@ -374,7 +374,7 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
  * bounds it: 511 rows of 4096 under 33 diagonals, fp32, 27 us. */
 constexpr int kGradSmem = 160 * 1024;     /* two buffers of at least eight rows */
 
-template <typename T, bool VEC, int ND>
+template <typename T, typename DZ, bool VEC, int ND>
 __global__ void __launch_bounds__(kTileWarps * 32)
 spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins, int rows)
 {
@@ -388,7 +388,8 @@ spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins, int 
     GradWindow win{};
     if (diags) win = a.dir.wins[wi];
     const int pitch = diags ? a.dir.wwidth : 0;
-    const int buf = rows * (pitch + 128);            /* x, then dz [row][128] */
+    /* a buffer: x, then dz [row][128] */
+    const int xbytes = rows * pitch * (int)sizeof(T), buf = xbytes + rows * 128 * (int)sizeof(DZ);
     const int per = (win.k1 - win.k0 + kTileWarps - 1) / kTileWarps;
     const int k0 = win.k0 + warp * per, nk = max(0, min(per, win.k1 - k0));
     /* a warp with fewer than ND repeats its last (or column 0) and drops it */
@@ -405,13 +406,13 @@ spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins, int 
     if (f0 < a.n_rows) {
         auto fetch = [&](int t0, int which) {
             const int nt = min(rg.r1 - t0, rows);
-            T* xs = (T*)smem_raw + which * buf;
+            unsigned char* xs = smem_raw + which * buf;
             if (nt > 0) {
                 if (diags)
-                    stage_spans<T, VEC>(xs, pitch, a.dir.wspans, win.s0, win.s1,
+                    stage_spans<T, VEC>((T*)xs, pitch, a.dir.wspans, win.s0, win.s1,
                                         (const T*)a.x + t0 * a.ldx, a.ldx, f0, a.n_cols, nt, nt);
-                stage_spans<T, VEC>(xs + rows * pitch, 128, a.dir.tile_span, 0, 1,
-                                    (const T*)a.dz + t0 * a.lddz, a.lddz, f0, a.n_rows, nt, nt);
+                stage_spans<DZ, VEC>((DZ*)(xs + xbytes), 128, a.dir.tile_span, 0, 1,
+                                     (const DZ*)a.dz + t0 * a.lddz, a.lddz, f0, a.n_rows, nt, nt);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -422,8 +423,8 @@ spmm_grad_kernel(const __grid_constant__ GradArgs a, int ftiles, int nwins, int 
             fetch(t0 + rows, which ^ 1);
             asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncthreads();
-            const T* xs = (const T*)smem_raw + which * buf;
-            const T* ds = xs + rows * pitch;
+            const T* xs = (const T*)(smem_raw + which * buf);
+            const DZ* ds = (const DZ*)(smem_raw + which * buf + xbytes);
             if (nk > 0 || bias) {
 #pragma unroll 4
                 for (int t = 0; t < nt; ++t) {
@@ -538,15 +539,24 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8])
     }
 }
 
-/* dz = dy * act'(z), rounded to the block's type: both gradients read it as
- * a matrix operand of that type, and one rounding of half a step is no more
- * than the ones dy and z already carry.  Without an activation it is a copy,
- * for blocks whose rows TMA does not take.  Eight elements a thread at a time,
- * two of them in flight; rows of dz are padded to eight. */
-template <typename T, int ACT, bool VEC>
+/* eight elements, p aligned to 16 bytes */
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8])
+{
+    __align__(16) T r[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) r[c] = from_f<T>(v[c]);
+#pragma unroll
+    for (int c = 0; c < (int)(8 * sizeof(T)); c += 16)
+        *(uint4*)((char*)p + c) = *(const uint4*)((const char*)r + c);
+}
+
+/* dz = dy * act'(z) in one of its forms (DzForm).  Eight elements a thread at a
+ * time, two of them in flight; rows of dz are padded to eight. */
+template <typename T, int ACT, DzForm FORM, bool VEC>
 __global__ void __launch_bounds__(256)
 spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z, long long ldz,
-               T* __restrict__ dz, long long lddz, int M, int n)
+               void* __restrict__ dz, void* __restrict__ lo, long long lddz, int M, int n)
 {
     dependents_begin();
     const int per = (n + 7) / 8;
@@ -576,7 +586,7 @@ spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (at[h] < 0) continue;
-            __align__(16) T r[8];
+            float v[8];
 #pragma unroll
             for (int c = 0; c < 8; c += 2) {
                 float2 d = make_float2(1.0f, 1.0f);
@@ -584,12 +594,19 @@ spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z
                     d = sizeof(T) == 2
                             ? dact2<ACT>(make_float2(b[h][c], b[h][c + 1]))
                             : make_float2(dact_of<ACT>(b[h][c]), dact_of<ACT>(b[h][c + 1]));
-                r[c] = from_f<T>(a[h][c] * d.x);
-                r[c + 1] = from_f<T>(a[h][c + 1] * d.y);
+                v[c] = a[h][c] * d.x;
+                v[c + 1] = a[h][c + 1] * d.y;
             }
+            if (FORM == kDzF32) {
+                store8<float>((float*)dz + at[h], v);
+            } else {
+                store8<T>((T*)dz + at[h], v);
+                if (FORM == kDzPair) {
 #pragma unroll
-            for (int c = 0; c < (int)(8 * sizeof(T)); c += 16)
-                *(uint4*)((char*)(dz + at[h]) + c) = *(const uint4*)((const char*)r + c);
+                    for (int c = 0; c < 8; ++c) v[c] = rest_of(v[c], to_f(from_f<T>(v[c])));
+                    store8<T>((T*)lo + at[h], v);
+                }
+            }
         }
     }
     dependency_wait();
@@ -603,7 +620,7 @@ static bool vec16(const void* p, long long ld)
     return (uintptr_t)p % 16 == 0 && ld * (long long)sizeof(T) % 16 == 0;
 }
 
-template <typename T, bool TRANS, int TT>
+template <typename T, typename IN, bool TRANS, int TT>
 static int launch_few(const ProdArgs& a, cudaStream_t stream)
 {
     const int ftiles = (a.n_out + 31) / 32;
@@ -619,12 +636,12 @@ static int launch_few(const ProdArgs& a, cudaStream_t stream)
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: block too large");
     /* the larger of block and operator is streamed once, the other stays in L2 */
     const bool rows_first = (long long)a.M * a.n_in < a.stride * a.K;
-    DIA_TRY_CUDA(launch(false, spmm_few_kernel<T, TRANS, TT>, (int)grid, kFewWarps * 32, 0, stream,
+    DIA_TRY_CUDA(launch(false, spmm_few_kernel<T, IN, TRANS, TT>, (int)grid, kFewWarps * 32, 0, stream,
                         a, ks, ftiles, ngroups, rows_first));
     return DIA_OK;
 }
 
-template <typename T, bool TRANS, bool VEC, bool QUADS>
+template <typename T, typename IN, bool TRANS, bool VEC, bool QUADS>
 static int launch_tile_as(const ProdArgs& a, int shape, int smem, cudaStream_t stream)
 {
     const int F = kTileF[shape], rows = kTileWarps * kTileRows * 128 / F;
@@ -633,7 +650,7 @@ static int launch_tile_as(const ProdArgs& a, int shape, int smem, cudaStream_t s
     if (ngroups * ftiles > INT_MAX)
         return fail(DIA_ERR_UNSUPPORTED, "dia_spmm: block too large");
     const bool rows_first = (long long)a.M * a.n_in < a.stride * a.K;
-    const auto kernel = spmm_tile_kernel<T, TRANS, VEC, QUADS>;
+    const auto kernel = spmm_tile_kernel<T, IN, TRANS, VEC, QUADS>;
     static SmemRecord most;
     DIA_TRY_CUDA(allow_smem(kernel, kTileSmem, most));
     DIA_TRY_CUDA(launch(false, kernel, (int)(ngroups * ftiles), kTileWarps * 32, smem, stream, a,
@@ -647,7 +664,7 @@ static int tile_smem(const SpmmDir& d, int shape, size_t elem)
                                                  kTileF[shape] * d.width[shape] * (long long)elem);
 }
 
-template <typename T, bool TRANS>
+template <typename T, typename IN, bool TRANS>
 static int launch_cores(const ProdArgs& a, cudaStream_t stream)
 {
     const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
@@ -659,7 +676,7 @@ static int launch_cores(const ProdArgs& a, cudaStream_t stream)
         /* the widest tile (an input is read again by fewer tiles) whose inputs
          * fit and that leaves a CTA for every SM; else the narrowest that fits */
         int shape = 2;
-        auto fits = [&](int s) { return tile_smem(a.dir, s, sizeof(T)) <= kTileSmem; };
+        auto fits = [&](int s) { return tile_smem(a.dir, s, sizeof(IN)) <= kTileSmem; };
         auto ctas = [&](int s) {
             const int rows = kTileWarps * kTileRows * 128 / kTileF[s];
             return (long long)((a.n_out + kTileF[s] - 1) / kTileF[s]) * ((a.M + rows - 1) / rows);
@@ -668,55 +685,65 @@ static int launch_cores(const ProdArgs& a, cudaStream_t stream)
         if (shape < 0)
             for (shape = 0; shape < 3 && !fits(shape);) ++shape;
         if (shape < 3) {
-            const int smem = tile_smem(a.dir, shape, sizeof(T));
-            const bool vec = vec16<T>(a.in, a.ldi), quads = 3 * a.dir.nquads <= a.K;
+            const int smem = tile_smem(a.dir, shape, sizeof(IN));
+            const bool vec = vec16<IN>(a.in, a.ldi), quads = 3 * a.dir.nquads <= a.K;
             if (vec)
-                return quads ? launch_tile_as<T, TRANS, true, true>(a, shape, smem, stream)
-                             : launch_tile_as<T, TRANS, true, false>(a, shape, smem, stream);
-            return quads ? launch_tile_as<T, TRANS, false, true>(a, shape, smem, stream)
-                         : launch_tile_as<T, TRANS, false, false>(a, shape, smem, stream);
+                return quads ? launch_tile_as<T, IN, TRANS, true, true>(a, shape, smem, stream)
+                             : launch_tile_as<T, IN, TRANS, true, false>(a, shape, smem, stream);
+            return quads ? launch_tile_as<T, IN, TRANS, false, true>(a, shape, smem, stream)
+                         : launch_tile_as<T, IN, TRANS, false, false>(a, shape, smem, stream);
         }
     }
-    if (per >= 5) return launch_few<T, TRANS, 8>(a, stream);
-    return per >= 2 ? launch_few<T, TRANS, 4>(a, stream) : launch_few<T, TRANS, 1>(a, stream);
+    if (per >= 5) return launch_few<T, IN, TRANS, 8>(a, stream);
+    return per >= 2 ? launch_few<T, IN, TRANS, 4>(a, stream)
+                    : launch_few<T, IN, TRANS, 1>(a, stream);
 }
 
 template <typename T>
 int Cores<T>::product(const ProdArgs& a, cudaStream_t stream)
 {
-    return a.trans ? launch_cores<T, true>(a, stream) : launch_cores<T, false>(a, stream);
+    if (!a.trans) return launch_cores<T, T, false>(a, stream);
+    return a.in32 ? launch_cores<T, float, true>(a, stream) : launch_cores<T, T, true>(a, stream);
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, DzForm FORM>
 static cudaError_t launch_dz_act(const void* dy, long long lddy, const void* z, long long ldz,
-                                 void* dz, long long lddz, int M, int n, bool dependent,
+                                 void* dz, void* lo, long long lddz, int M, int n, bool dependent,
                                  cudaStream_t stream)
 {
     const long long work = (long long)M * ((n + 7) / 8);
     const int grid = (int)std::min<long long>((work + 511) / 512, 8ll * num_sms());
     const auto kernel = vec16<T>(dy, lddy) && vec16<T>(z, ldz)
-                            ? spmm_dz_kernel<T, ACT, true>
-                            : spmm_dz_kernel<T, ACT, false>;
+                            ? spmm_dz_kernel<T, ACT, FORM, true>
+                            : spmm_dz_kernel<T, ACT, FORM, false>;
     return launch(dependent, kernel, grid, 256, 0, stream, (const T*)dy, lddy, (const T*)z, ldz,
-                  (T*)dz, lddz, M, n);
+                  dz, lo, lddz, M, n);
 }
 
 template <typename T>
-int Cores<T>::dz(int act, const void* dy, long long lddy, const void* z, long long ldz,
-                     void* dz, long long lddz, int M, int n, bool dependent, cudaStream_t stream)
+int Cores<T>::dz(DzForm form, int act, const void* dy, long long lddy, const void* z,
+                 long long ldz, void* dz, void* lo, long long lddz, int M, int n, bool dependent,
+                 cudaStream_t stream)
 {
     if (M == 0 || n == 0) return DIA_OK;
-    const auto run = act == DIA_ACT_NONE   ? launch_dz_act<T, DIA_ACT_NONE>
-                     : act == DIA_ACT_RELU   ? launch_dz_act<T, DIA_ACT_RELU>
-                     : act == DIA_ACT_SILU ? launch_dz_act<T, DIA_ACT_SILU>
-                     : act == DIA_ACT_GELU ? launch_dz_act<T, DIA_ACT_GELU>
-                                           : launch_dz_act<T, DIA_ACT_GELU_TANH>;
-    DIA_TRY_CUDA(run(dy, lddy, z, ldz, dz, lddz, M, n, dependent, stream));
+    constexpr DzForm F32 = kDzF32, PAIR = sizeof(T) == 2 ? kDzPair : kDzF32;
+    const bool pair = form == kDzPair;
+    const auto run =
+        act == DIA_ACT_NONE   ? launch_dz_act<T, DIA_ACT_NONE, kDzSame>
+        : act == DIA_ACT_RELU ? (pair ? launch_dz_act<T, DIA_ACT_RELU, PAIR>
+                                      : launch_dz_act<T, DIA_ACT_RELU, F32>)
+        : act == DIA_ACT_SILU ? (pair ? launch_dz_act<T, DIA_ACT_SILU, PAIR>
+                                      : launch_dz_act<T, DIA_ACT_SILU, F32>)
+        : act == DIA_ACT_GELU ? (pair ? launch_dz_act<T, DIA_ACT_GELU, PAIR>
+                                      : launch_dz_act<T, DIA_ACT_GELU, F32>)
+                              : (pair ? launch_dz_act<T, DIA_ACT_GELU_TANH, PAIR>
+                                      : launch_dz_act<T, DIA_ACT_GELU_TANH, F32>);
+    DIA_TRY_CUDA(run(dy, lddy, z, ldz, dz, lo, lddz, M, n, dependent, stream));
     return DIA_OK;
 }
 
-template <typename T>
-int Cores<T>::gradient(const GradArgs& a, cudaStream_t stream)
+template <typename T, typename DZ>
+static int launch_gradient(const GradArgs& a, cudaStream_t stream)
 {
     const int ftiles = (int)((a.stride + 127) / 128);
     const int nwins = a.dvals ? std::max(a.dir.nwins, 1) : 1;
@@ -724,25 +751,33 @@ int Cores<T>::gradient(const GradArgs& a, cudaStream_t stream)
     const long long grid = parts * ftiles * nwins;
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
     /* rows a stage: two CTAs an SM where that leaves eight or more */
-    const int row_bytes = 2 * ((a.dvals ? a.dir.wwidth : 0) + 128) * (int)sizeof(T);
+    const int row_bytes =
+        2 * ((a.dvals ? a.dir.wwidth : 0) * (int)sizeof(T) + 128 * (int)sizeof(DZ));
     const int rows = std::min(32, std::max(8, 100 * 1024 / row_bytes / 8 * 8));
     const int smem = rows * row_bytes;
-    const bool vec = vec16<T>(a.dz, a.lddz) && vec16<T>(a.x, a.ldx);
+    const bool vec = vec16<DZ>(a.dz, a.lddz) && vec16<T>(a.x, a.ldx);
     const int nd = a.dvals ? (a.dir.wdiags + kTileWarps - 1) / kTileWarps : 1;
     const int pick = nd <= 1 ? 0 : nd <= 2 ? 1 : nd <= 3 ? 2 : nd <= 5 ? 3 : 4;
     using Kernel = void (*)(GradArgs, int, int, int);
     static const Kernel kernels[2][5] = {
-        {spmm_grad_kernel<T, false, 1>, spmm_grad_kernel<T, false, 2>,
-         spmm_grad_kernel<T, false, 3>, spmm_grad_kernel<T, false, 5>,
-         spmm_grad_kernel<T, false, 8>},
-        {spmm_grad_kernel<T, true, 1>, spmm_grad_kernel<T, true, 2>, spmm_grad_kernel<T, true, 3>,
-         spmm_grad_kernel<T, true, 5>, spmm_grad_kernel<T, true, 8>}};
+        {spmm_grad_kernel<T, DZ, false, 1>, spmm_grad_kernel<T, DZ, false, 2>,
+         spmm_grad_kernel<T, DZ, false, 3>, spmm_grad_kernel<T, DZ, false, 5>,
+         spmm_grad_kernel<T, DZ, false, 8>},
+        {spmm_grad_kernel<T, DZ, true, 1>, spmm_grad_kernel<T, DZ, true, 2>,
+         spmm_grad_kernel<T, DZ, true, 3>, spmm_grad_kernel<T, DZ, true, 5>,
+         spmm_grad_kernel<T, DZ, true, 8>}};
     const Kernel kernel = kernels[vec][pick];
     static SmemRecord most[2][5];
     DIA_TRY_CUDA(allow_smem(kernel, kGradSmem, most[vec][pick]));
     DIA_TRY_CUDA(launch(false, kernel, (int)grid, kTileWarps * 32, smem, stream, a, ftiles, nwins,
                         rows));
     return DIA_OK;
+}
+
+template <typename T>
+int Cores<T>::gradient(const GradArgs& a, cudaStream_t stream)
+{
+    return a.dz32 ? launch_gradient<T, float>(a, stream) : launch_gradient<T, T>(a, stream);
 }
 
 template <typename T>

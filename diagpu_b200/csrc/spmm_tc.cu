@@ -434,6 +434,7 @@ __device__ __noinline__ void rows_again(const ProdArgs& a, int K, int e, int row
         float sum[kAgainRows];
         const T* in[kAgainRows];
         const int n = min(kAgainRows, __popc(rows));
+        const long long rest = TRANS && a.lo ? (const T*)a.lo - (const T*)a.in : 0;
 #pragma unroll
         for (int u = 0; u < kAgainRows; ++u) {   /* a row twice where there are fewer */
             r[u] = row0 + (u < n ? __ffs(rows) - 1 : r[0] - row0);
@@ -448,7 +449,11 @@ __device__ __noinline__ void rows_again(const ProdArgs& a, int K, int e, int row
             if (on && (unsigned)j < (unsigned)a.n_in) {
                 const float w = to_f(vals[ok.y * a.stride + (TRANS ? j : i)]);
 #pragma unroll
-                for (int u = 0; u < kAgainRows; ++u) sum[u] = fmaf(w, to_f(in[u][j]), sum[u]);
+                for (int u = 0; u < kAgainRows; ++u) {
+                    float x = to_f(in[u][j]);
+                    if (TRANS && rest) x += to_f(in[u][j + rest]);
+                    sum[u] = fmaf(w, x, sum[u]);
+                }
             }
         }
 #pragma unroll
@@ -511,7 +516,8 @@ __device__ __forceinline__ void used_boxes(const int* cols, const SpmmDir& d, in
 
 template <typename T, bool TRANS, int ACT>
 __global__ void __launch_bounds__(kTcWarps * 32, 1)
-spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ ProdArgs a, int K)
+spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmL,
+               const __grid_constant__ ProdArgs a, int K)
 {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -572,6 +578,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     }
     const int row_step = sh.step * kTM;
     const int NB = a.dir.nboxes;
+    const int halves = TRANS && a.lo ? 2 : 1;   /* of dz: each box of it, then of the rest */
     Run r;
 
     const uint32_t xfull = smem_u32(bars.xfull), xempty = smem_u32(bars.xempty);
@@ -594,13 +601,16 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             for (int j0 = 0; j0 < r.ntiles && ok; j0 += group)
                 for (int b = b0; b < b1 && ok; ++b) {
                     const int x0 = i0 + (b < kSharedBoxes ? s_cols[b] : a.dir.boxes[b].col);
-                    for (int j = j0; j < min(j0 + group, r.ntiles); ++j) {
+                    const int n = min(group, r.ntiles - j0) * halves;
+                    for (int j = 0; j < n; ++j) {
                         ok = mm_wait(x.bar(xempty), x.round ^ 1, s_state);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
+                        const bool rest = TRANS && halves == 2 && (j & 1);
+                        const int tile = j0 + (TRANS && halves == 2 ? j >> 1 : j);
                         if (leader && !(g_mm_withhold && blockIdx.x == 0 && issued == 0))
-                            tma_load_2d(xst + x.s * kBoxBytes, &tmX, x0, r.r0 + j * row_step,
-                                        x.bar(xfull), kBoxBytes);
+                            tma_load_2d(xst + x.s * kBoxBytes, rest ? &tmL : &tmX, x0,
+                                        r.r0 + tile * row_step, x.bar(xfull), kBoxBytes);
                         x.next();
                         ++issued;
                     }
@@ -656,6 +666,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                     for (int u = 0; u < used && ok; ++u, q.next()) {
                         if (j == 0 && !wait(q.bar(wfull), q.round)) break;
                         box(q.s, ac.s, u == 0);
+                        if (TRANS && halves == 2 && ok) box(q.s, ac.s, false);
                         if (ok && j == r.ntiles - 1 && leader) mm_commit(q.bar(wempty));
                     }
                     if (ok && leader) mm_commit(ac.bar(afull));
@@ -672,6 +683,7 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
                         t = ac;
                         for (int j = 0; j < n && ok; ++j, t.next()) {
                             box(wq.s, t.s, u == 0);
+                            if (TRANS && halves == 2 && ok) box(wq.s, t.s, false);
                             if (ok && u == used - 1 && leader) mm_commit(t.bar(afull));
                         }
                         if (ok && leader) mm_commit(wq.bar(wempty));
@@ -928,7 +940,8 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
 constexpr int kGRows = 64;                     /* rows of a stage */
 constexpr int kGBoxBytes = kGRows * 128;
 constexpr int kGBoxes = 4;                     /* boxes of inputs of a CTA */
-constexpr int kGDz = kGBoxes * kGBoxBytes;     /* in a stage: x, then dz (or dy), then z */
+constexpr int kGDz = kGBoxes * kGBoxBytes;     /* in a stage: x, then dz (or dy), then its
+                                                * rest (or z) */
 constexpr int kGSmem = 192 * 1024 + 1024;
 constexpr int kGWarps = 18;                    /* TMA, MMA, sixteen for the results */
 constexpr int kGConv = (kGWarps - 2) * 16;     /* threads that look at a stage */
@@ -947,18 +960,21 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t addr)
     return d;
 }
 
-/* ACT other than none: dz is made here, from dy and z, by the warps that wait
- * for the results otherwise: into the stage, for the MMAs, and to a.dz, for
- * the product that follows. */
-template <typename T, int ACT>
+/* PAIR: dz comes as a rounded part and the rest of it (kDzPair), and the sum
+ * over both is two MMAs.  ACT other than none: the pair is made here, from dy
+ * and z, by the warps that wait for the results otherwise: into the stage, for
+ * the MMAs, and to a.dz and a.lo, for the product that follows. */
+template <typename T, int ACT, bool PAIR>
 __global__ void __launch_bounds__(kGWarps * 32, 1)
 spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmZ,
                     const __grid_constant__ CUtensorMap tmX, const __grid_constant__ GradArgs a,
                     int nfb, int nch)
 {
     constexpr bool MAKE = ACT != DIA_ACT_NONE;
-    constexpr int STAGES = MAKE ? 3 : 4;
-    constexpr int STAGE = (kGBoxes + (MAKE ? 4 : 2)) * kGBoxBytes;
+    static_assert(PAIR || !MAKE, "made in pairs");
+    constexpr int ROWS = PAIR ? 4 : 2;             /* boxes of dz, or of dy and z */
+    constexpr int STAGES = PAIR ? 3 : 4;
+    constexpr int STAGE = (kGBoxes + ROWS) * kGBoxBytes;
     static_assert(STAGES * STAGE + 1024 <= kGSmem, "stages");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -1024,11 +1040,11 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                 const int r = rg.r0 + g * kGRows;
                 const uint32_t st = st0 + x.s * STAGE, bar = x.bar(full0);
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                             ::"r"(bar), "r"(((MAKE ? 4 : 2) + nb) * kGBoxBytes) : "memory");
+                             ::"r"(bar), "r"((ROWS + nb) * kGBoxBytes) : "memory");
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     tma_box(st + kGDz + h * kGBoxBytes, &tmD, i0 + 64 * h, r, bar);
-                    if (MAKE)
+                    if (PAIR)
                         tma_box(st + kGDz + (2 + h) * kGBoxBytes, &tmZ, i0 + 64 * h, r, bar);
                 }
                 for (int c = 0; c < nb; ++c)
@@ -1056,7 +1072,7 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                 /* rows past the part: another expert's, or nobody's */
                 const uint32_t st = st0 + x.s * STAGE;
                 const int per = (kGRows - left) * 8;
-                for (int o = lane; o < per * (kGBoxes + 2); o += 32)
+                for (int o = lane; o < per * (kGBoxes + ROWS); o += 32)
                     sts128(st + o / per * kGBoxBytes + left * 128 + o % per * 16, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -1067,8 +1083,12 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                 const uint64_t ad = bd + (kGDz >> 4);
                 if (nb > 0) {
 #pragma unroll
-                    for (int kk = 0; kk < kGRows / 16; ++kk)
+                    for (int kk = 0; kk < kGRows / 16; ++kk) {
                         mma_f16(tmem, ad + 128 * kk, bd + 128 * kk, idesc, g > 0 || kk > 0);
+                        if (PAIR)
+                            mma_f16(tmem, ad + (2 * kGBoxBytes >> 4) + 128 * kk, bd + 128 * kk,
+                                    idesc, true);
+                    }
                 }
                 mm_commit(x.bar(empty0));
             }
@@ -1094,23 +1114,41 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
 #pragma unroll
             for (int p = 0; p < 4; p += 2) {
                 const uint32_t at = at0 + p * 16 * 128;
+                uint32_t z[2][4];   /* then the rest of dz */
                 lds128(at, d[p]);
                 lds128(at + 16 * 128, d[p + 1]);
-                if (!MAKE) continue;
-                uint32_t z[2][4];
-                lds128(at + 2 * kGBoxBytes, z[0]);
-                lds128(at + 2 * kGBoxBytes + 16 * 128, z[1]);
+                if (PAIR) {
+                    lds128(at + 2 * kGBoxBytes, z[0]);
+                    lds128(at + 2 * kGBoxBytes + 16 * 128, z[1]);
+                }
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int h = 0; h < 2; ++h) {
+                    const int r = r0 + 16 * (p + h);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float2 v =
-                            mul2(unpack2<T>(d[p + h][q]), dact2<ACT>(unpack2<T>(z[h][q])));
-                        d[p + h][q] = pack2<T>(v.x, v.y);
+                    for (int q = 0; q < 4; ++q) {
+                        float2 v = unpack2<T>(d[p + h][q]);
+                        if (MAKE) {
+                            v = mul2(v, dact2<ACT>(unpack2<T>(z[h][q])));
+                            d[p + h][q] = pack2<T>(v.x, v.y);
+                            const float2 w = unpack2<T>(d[p + h][q]);
+                            z[h][q] = pack2<T>(rest_of(v.x, w.x), rest_of(v.y, w.y));
+                        } else if (PAIR) {
+                            v = add2(v, unpack2<T>(z[h][q]));
+                        }
+                        if (bias && r < left) {
+                            sums[2 * q] += v.x;
+                            sums[2 * q + 1] += v.y;
+                        }
                     }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    sts128(at + h * 16 * 128, d[p + h][0], d[p + h][1], d[p + h][2], d[p + h][3]);
+                    if (MAKE) {
+                        const uint32_t to = at + h * 16 * 128;
+                        sts128(to, d[p + h][0], d[p + h][1], d[p + h][2], d[p + h][3]);
+                        sts128(to + 2 * kGBoxBytes, z[h][0], z[h][1], z[h][2], z[h][3]);
+                        if (r < left && i < a.n_rows)
+                            *(uint4*)((T*)a.lo + (long long)(rg.r0 + g * kGRows + r) * a.lddz + i) =
+                                make_uint4(z[h][0], z[h][1], z[h][2], z[h][3]);
+                    }
+                }
             }
             if (MAKE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -1118,17 +1156,9 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
                 const int r = r0 + 16 * h;
-                if (r >= left) continue;
-                if (MAKE && i < a.n_rows)
+                if (MAKE && r < left && i < a.n_rows)
                     *(uint4*)((T*)a.dz + (long long)(rg.r0 + g * kGRows + r) * a.lddz + i) =
                         make_uint4(d[h][0], d[h][1], d[h][2], d[h][3]);
-                if (bias)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float2 v = unpack2<T>(d[h][q]);
-                        sums[2 * q] += v.x;
-                        sums[2 * q + 1] += v.y;
-                    }
             }
         }
     }
@@ -1284,7 +1314,7 @@ long long spmm_tc_pack_bytes(const SpmmDir& d, int K, int n_out, long long M, in
 }
 
 template <typename T, bool TRANS, int ACT>
-static int launch_tc(const CUtensorMap& map, const ProdArgs& a_, int K, cudaStream_t stream)
+static int launch_tc(const CUtensorMap (&map)[2], const ProdArgs& a_, int K, cudaStream_t stream)
 {
     const long long tiles = a_.seg ? a_.M / kTM + std::min(a_.E, a_.M) : (a_.M + kTM - 1) / kTM;
     const int nfb = (a_.n_out + kTN - 1) / kTN;
@@ -1295,12 +1325,14 @@ static int launch_tc(const CUtensorMap& map, const ProdArgs& a_, int K, cudaStre
                                   : (int)std::min<long long>(tiles * nfb, num_sms());
     static SmemRecord most;
     DIA_TRY_CUDA(allow_smem(spmm_tc_kernel<T, TRANS, ACT>, kTcSmem, most));
-    DIA_TRY_CUDA(launch(a.dependent, spmm_tc_kernel<T, TRANS, ACT>, grid, kTcWarps * 32, kTcSmem, stream, map, a, K));
+    DIA_TRY_CUDA(launch(a.dependent, spmm_tc_kernel<T, TRANS, ACT>, grid, kTcWarps * 32, kTcSmem, stream,
+                        map[0], map[1], a, K));
     return DIA_OK;
 }
 
 template <typename T>
-static int launch_tc_type(const CUtensorMap& map, const ProdArgs& a, int K, cudaStream_t stream)
+static int launch_tc_type(const CUtensorMap (&map)[2], const ProdArgs& a, int K,
+                          cudaStream_t stream)
 {
     if (a.trans) return launch_tc<T, true, DIA_ACT_NONE>(map, a, K, stream);
     switch (a.act) {
@@ -1326,8 +1358,9 @@ int spmm_tc_pack(const ProdArgs& a, bool dependent, cudaStream_t stream)
 
 int spmm_tc_product(const ProdArgs& a, int dtype, cudaStream_t stream)
 {
-    CUtensorMap map;
-    if (!block_map(&map, a.in, dtype, a.n_in, a.M, a.ldi, kTM))
+    CUtensorMap map[2];
+    if (!block_map(&map[0], a.in, dtype, a.n_in, a.M, a.ldi, kTM) ||
+        !block_map(&map[1], a.lo ? a.lo : a.in, dtype, a.n_in, a.M, a.ldi, kTM))
         return fail(DIA_ERR_CUDA, "dia_spmm: cuTensorMapEncodeTiled failed");
     return dtype == DIA_F16 ? launch_tc_type<__half>(map, a, a.K, stream)
                             : launch_tc_type<__nv_bfloat16>(map, a, a.K, stream);
@@ -1340,21 +1373,22 @@ bool spmm_tc_makes_dz(const GradArgs& a)
            spmm_tc_block(a.z, a.ldz);
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool PAIR>
 static int launch_grad_tc(const GradArgs& a, int dtype, bool dependent, cudaStream_t stream)
 {
     CUtensorMap md, mz, mx;
     const bool make = ACT != DIA_ACT_NONE;
+    const void* second = make ? a.z : (PAIR ? a.lo : a.dz);
     if (!block_map(&md, make ? a.dy : a.dz, dtype, a.n_rows, a.M, make ? a.lddy : a.lddz, kGRows) ||
         !block_map(&mx, a.x, dtype, a.n_cols, a.M, a.ldx, kGRows) ||
-        !block_map(&mz, make ? a.z : a.dz, dtype, a.n_rows, a.M, make ? a.ldz : a.lddz, kGRows))
+        !block_map(&mz, second, dtype, a.n_rows, a.M, make ? a.ldz : a.lddz, kGRows))
         return fail(DIA_ERR_CUDA, "dia_spmm_backward: cuTensorMapEncodeTiled failed");
     const int nfb = (int)((a.stride + 127) / 128);
     const int nch = std::max(1, (a.dir.nboxes + kGBoxes - 1) / kGBoxes);
     const long long parts = a.seg ? a.M / a.per + a.E : std::max(1, (a.M + a.per - 1) / a.per);
     const long long grid = parts * nfb * nch;
     if (grid > INT_MAX) return fail(DIA_ERR_UNSUPPORTED, "dia_spmm_backward: block too large");
-    const auto kernel = spmm_grad_tc_kernel<T, ACT>;
+    const auto kernel = spmm_grad_tc_kernel<T, ACT, PAIR>;
     static SmemRecord most;
     DIA_TRY_CUDA(allow_smem(kernel, kGSmem, most));
     DIA_TRY_CUDA(launch(dependent, kernel, (int)grid, kGWarps * 32, kGSmem, stream, md, mz, mx, a,
@@ -1367,11 +1401,14 @@ static int launch_grad_act(const GradArgs& a, int dtype, bool make, bool depende
                            cudaStream_t stream)
 {
     switch (make ? a.act : DIA_ACT_NONE) {
-        case DIA_ACT_RELU: return launch_grad_tc<T, DIA_ACT_RELU>(a, dtype, dependent, stream);
-        case DIA_ACT_SILU: return launch_grad_tc<T, DIA_ACT_SILU>(a, dtype, dependent, stream);
-        case DIA_ACT_GELU: return launch_grad_tc<T, DIA_ACT_GELU>(a, dtype, dependent, stream);
-        case DIA_ACT_GELU_TANH: return launch_grad_tc<T, DIA_ACT_GELU_TANH>(a, dtype, dependent, stream);
-        default: return launch_grad_tc<T, DIA_ACT_NONE>(a, dtype, dependent, stream);
+        case DIA_ACT_RELU: return launch_grad_tc<T, DIA_ACT_RELU, true>(a, dtype, dependent, stream);
+        case DIA_ACT_SILU: return launch_grad_tc<T, DIA_ACT_SILU, true>(a, dtype, dependent, stream);
+        case DIA_ACT_GELU: return launch_grad_tc<T, DIA_ACT_GELU, true>(a, dtype, dependent, stream);
+        case DIA_ACT_GELU_TANH:
+            return launch_grad_tc<T, DIA_ACT_GELU_TANH, true>(a, dtype, dependent, stream);
+        default:
+            return a.lo ? launch_grad_tc<T, DIA_ACT_NONE, true>(a, dtype, dependent, stream)
+                        : launch_grad_tc<T, DIA_ACT_NONE, false>(a, dtype, dependent, stream);
     }
 }
 

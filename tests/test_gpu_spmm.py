@@ -937,8 +937,8 @@ def test_workspace_has_a_limit(side, M):
     L, block = dg.lib(), 2 * 2 * M * n
     most = max(block, 1 << 31)
     assert 0 <= L.dia_spmm_workspace(plan._h, 2, M, 1, n) <= most
-    # and dz; features enough for every SM leave the rows in one part
-    assert 0 <= L.dia_spmm_backward_workspace(plan._h, 2, M, 1, n, n, n, 2) <= most + block // 2
+    # and dz in 32 bits; features enough for every SM leave the rows in one part
+    assert 0 <= L.dia_spmm_backward_workspace(plan._h, 2, M, 1, n, n, n, 2) <= most + block
 
 
 # Sizes at which a kernel takes its other path: more diagonals than a CTA keeps
@@ -1018,3 +1018,39 @@ def test_an_error_is_reported_once(M, t):
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
                 dg.SpmspmPlan(A, A)
         assert all(torch.equal(p, q) for p, q in zip(f(), want))
+
+
+WIDE = [-250, -201, -130, -64, -3, 0, 55, 120, 199, 260]
+
+
+@pytest.mark.parametrize("M,off,seg,shift", [
+    (3, band(2), None, 0), (300, band(2), None, 0), (300, WIDE, None, 0),
+    (300, band(2), None, 1), (300, WIDE, None, 1), (1500, band(2), None, 0),
+    (300, band(2), [3, 70, 70, 71, 290], 0), (300, WIDE, [0, 1, 200, 300], 0)])
+def test_gradients_keep_dz_in_32_bits(M, off, seg, shift, t):
+    """The gradients' error is the sums' and one rounding: dz = dy silu'(z) is not
+    rounded to the block's type before them.  silu' is off by less than 2^-16 (1 +
+    |z|) (the logistic function by 2^-19 of itself), a dz of two halves by 2^-18,
+    and where fp16's second half underflows by half a step of 2^-24.  Operators of
+    a few boxes and of many, parts, experts, blocks that TMA does not take."""
+    n = 264
+    c = Case(t, M, n, n, off, seed=71, seg=seg, shift=shift)
+    sq = (lambda a: a) if seg is not None else (lambda a: a[0])
+    dx, dv = c.block(torch.full((M, n), 3.0)), torch.full_like(c.vals, 9.0)
+    db = torch.full_like(c.bias, 9.0)
+    dg.spmm_backward(c.plan, c.pv(), c.x, c.dy, z=c.zin, act="silu", seg=c.dseg, dx=dx,
+                     dvals=sq(dv), dbias=sq(db))
+    dy, x, vals, z, u = c.v(c.dy), c.v(c.x), c.v(c.vals), c.v(c.zin), unit(t)
+    dz = dy * dact64(z, "silu")
+    ed = 2.0 ** -16 * (1 + z.abs()) * dy.abs() + 2.0 ** -18 * dz.abs()
+    ed = ed + (2.0 ** -25 if t == torch.float16 else 0)
+    want = gradient64(off, n, n, vals, x, dz, c.parts)
+    S = gradient64(off, n, n, vals.abs(), x.abs(), dz.abs(), c.parts)
+    T = gradient64(off, n, n, vals.abs(), x.abs(), ed, c.parts)
+    on, rows = c.rows(), max(b - a for _, a, b in c.parts)
+    for got, w, s, e, terms, what in ((dx[on], want[0][on], S[0][on], T[0][on], len(off), "dx"),
+                                      (dv, want[1], S[1], T[1], rows, "dvals"),
+                                      (db, want[2], S[2], T[2], rows, "dbias")):
+        e = e + (2 * terms + 4) * sum_unit(t) * (s + e)     # two halves: twice the terms
+        near(got, w, e + u * (w.abs() + e) + tiny(t), what)
+    assert bool((dx[~on].cpu() == 3).all())
