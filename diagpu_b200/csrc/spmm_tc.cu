@@ -944,7 +944,7 @@ constexpr int kGDz = kGBoxes * kGBoxBytes;     /* in a stage: x, then dz (or dy)
                                                 * rest (or z) */
 constexpr int kGSmem = 192 * 1024 + 1024;
 constexpr int kGWarps = 18;                    /* TMA, MMA, sixteen for the results */
-constexpr int kGConv = (kGWarps - 2) * 16;     /* threads that look at a stage */
+constexpr int kGConv = (kGWarps - 2) * 32;     /* threads that look at every stage */
 constexpr int kGPitch = kGBoxes * kBoxCols + 1;
 
 /* MN-major operand with the 128-byte swizzle: groups of 64 elements kGBoxBytes
@@ -1096,69 +1096,61 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         if (leader) mm_commit(smem_u32(&done));
         mm_drain(smem_u32(&done), 0);
     } else if (conv) {
-        /* half of the warps take the even stages, half the odd ones, so that
-         * one half's arithmetic runs while the other waits and stores; a
-         * thread looks at eight features of every 16th row */
-        const int half = (warp - 2) / (kGConv / 32);
-        const int c = tid & 15, r0 = ((tid - 64) % kGConv) >> 4, i = i0 + 8 * c;
+        /* a thread looks at eight features of two rows of every stage.  Every
+         * warp takes part in every stage, so that it has seen every phase of a
+         * barrier before the next can end.  (Halves of the warps in turn did not:
+         * with three stages a half came back to one whose round before it had
+         * not waited for, and the parity of the round before that let it pass:
+         * stale rows, or a wait that ran out.) */
+        const int c = tid & 15, r0 = (tid - 64) >> 4, i = i0 + 8 * c;
         Ring<STAGES> x;
-        if (half) x.next();
-        for (int g = half; g < nst; g += 2, x.next(), x.next()) {
+        for (int g = 0; g < nst; ++g, x.next()) {
             ok = mm_wait(x.bar(full0), x.round, s_state);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int left = rg.r1 - rg.r0 - g * kGRows;
-            const uint32_t at0 = st0 + x.s * STAGE + kGDz + (c >> 3) * kGBoxBytes + r0 * 128 +
-                                 (((c ^ r0) & 7) << 4);
-            uint32_t d[4][4];
+            const uint32_t at = st0 + x.s * STAGE + kGDz + (c >> 3) * kGBoxBytes + r0 * 128 +
+                                (((c ^ r0) & 7) << 4);
+            uint32_t d[2][4], z[2][4];   /* z, then the rest of dz */
 #pragma unroll
-            for (int p = 0; p < 4; p += 2) {
-                const uint32_t at = at0 + p * 16 * 128;
-                uint32_t z[2][4];   /* then the rest of dz */
-                lds128(at, d[p]);
-                lds128(at + 16 * 128, d[p + 1]);
-                if (PAIR) {
-                    lds128(at + 2 * kGBoxBytes, z[0]);
-                    lds128(at + 2 * kGBoxBytes + 16 * 128, z[1]);
-                }
+            for (int h = 0; h < 2; ++h) {
+                lds128(at + h * 32 * 128, d[h]);
+                if (PAIR) lds128(at + h * 32 * 128 + 2 * kGBoxBytes, z[h]);
+            }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = r0 + 16 * (p + h);
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float2 v = unpack2<T>(d[p + h][q]);
-                        if (MAKE) {
-                            v = mul2(v, dact2<ACT>(unpack2<T>(z[h][q])));
-                            d[p + h][q] = pack2<T>(v.x, v.y);
-                            const float2 w = unpack2<T>(d[p + h][q]);
-                            z[h][q] = pack2<T>(rest_of(v.x, w.x), rest_of(v.y, w.y));
-                        } else if (PAIR) {
-                            v = add2(v, unpack2<T>(z[h][q]));
-                        }
-                        if (bias && r < left) {
-                            sums[2 * q] += v.x;
-                            sums[2 * q + 1] += v.y;
-                        }
-                    }
+                for (int q = 0; q < 4; ++q) {
+                    float2 v = unpack2<T>(d[h][q]);
                     if (MAKE) {
-                        const uint32_t to = at + h * 16 * 128;
-                        sts128(to, d[p + h][0], d[p + h][1], d[p + h][2], d[p + h][3]);
-                        sts128(to + 2 * kGBoxBytes, z[h][0], z[h][1], z[h][2], z[h][3]);
-                        if (r < left && i < a.n_rows)
-                            *(uint4*)((T*)a.lo + (long long)(rg.r0 + g * kGRows + r) * a.lddz + i) =
-                                make_uint4(z[h][0], z[h][1], z[h][2], z[h][3]);
+                        v = mul2(v, dact2<ACT>(unpack2<T>(z[h][q])));
+                        d[h][q] = pack2<T>(v.x, v.y);
+                        const float2 w = unpack2<T>(d[h][q]);
+                        z[h][q] = pack2<T>(rest_of(v.x, w.x), rest_of(v.y, w.y));
+                    } else if (PAIR) {
+                        v = add2(v, unpack2<T>(z[h][q]));
                     }
+                    if (bias && r0 + 32 * h < left) {
+                        sums[2 * q] += v.x;
+                        sums[2 * q + 1] += v.y;
+                    }
+                }
+                if (MAKE) {
+                    const uint32_t to = at + h * 32 * 128;
+                    sts128(to, d[h][0], d[h][1], d[h][2], d[h][3]);
+                    sts128(to + 2 * kGBoxBytes, z[h][0], z[h][1], z[h][2], z[h][3]);
                 }
             }
             if (MAKE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(x.bar(ready0));
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                const int r = r0 + 16 * h;
-                if (MAKE && r < left && i < a.n_rows)
-                    *(uint4*)((T*)a.dz + (long long)(rg.r0 + g * kGRows + r) * a.lddz + i) =
-                        make_uint4(d[h][0], d[h][1], d[h][2], d[h][3]);
+            for (int h = 0; h < 2; ++h) {
+                const int r = r0 + 32 * h;
+                if (!MAKE || r >= left || i >= a.n_rows) continue;
+                const long long to = (long long)(rg.r0 + g * kGRows + r) * a.lddz + i;
+                *(uint4*)((T*)a.dz + to) = make_uint4(d[h][0], d[h][1], d[h][2], d[h][3]);
+                *(uint4*)((T*)a.lo + to) = make_uint4(z[h][0], z[h][1], z[h][2], z[h][3]);
             }
         }
     }

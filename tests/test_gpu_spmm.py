@@ -1054,3 +1054,36 @@ def test_gradients_keep_dz_in_32_bits(M, off, seg, shift, t):
         e = e + (2 * terms + 4) * sum_unit(t) * (s + e)     # two halves: twice the terms
         near(got, w, e + u * (w.abs() + e) + tiny(t), what)
     assert bool((dx[~on].cpu() == 3).all())
+
+
+@pytest.mark.parametrize("n,M,off,act", [
+    (65536, 512, [-500, -377, -200, -64, 0, 13, 90, 255, 500], "silu"),
+    (65536, 512, [-500, -377, -200, -64, 0, 13, 90, 255, 500], "none"),
+    (65536, 512, band(16), "relu"), (4096, 4096, band(64), "gelu"), (2048, 4096, band(64), "relu")])
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+def test_gradient_stages_are_read_when_they_are_full(n, M, off, act, t):
+    """Thousands of CTAs whose warps make or sum dz from a ring of three stages: no
+    warp takes an earlier round of a stage for the one that it waits for.  The
+    same bits every time and no wait that runs out; for dz = dy or 0 the CUDA-core
+    form's bits, since sums of small whole numbers are exact in any order."""
+    g = torch.Generator(device="cuda").manual_seed(72)
+    plan, K = dg.SpmmPlan(n, n, off), len(off)
+    r = lambda *s: torch.randint(-3, 4, s, generator=g, device="cuda").to(t)
+    v, x, dy, z = r(K, n), r(M, n), r(M, n), r(M, n)
+    L = dg.lib()
+
+    def run():
+        return dg.spmm_backward(plan, v, x, dy, z=z, act=act, bias_grad=True)
+
+    try:
+        dg.check(L.dia_test_spmm_form(1))
+        cores = run()
+        dg.check(L.dia_test_spmm_form(2))
+        first = run()
+        for _ in range(20):
+            assert all(torch.equal(p, q) for p, q in zip(run(), first))
+        assert dg.device_status() == 0
+    finally:
+        dg.check(L.dia_test_spmm_form(0))
+    if act in ("none", "relu"):
+        assert all(torch.equal(p, q) for p, q in zip(first, cores))
