@@ -69,7 +69,8 @@ static bool tensor_form(const DiaSpmmPlan* p, int dtype, long long M, int E, boo
     const double cores = mega < 0.2 ? 6 + 4 * mega * d.nquads
                                     : std::max(10 + 0.4 * p->K, (4.5 + 0.2 * p->K) * mega);
     const double tensor = 8 + (E > 1 || d.nboxes > 6 ? 2.5 : 0.0) + 0.004 * boxes +
-                          0.006 * std::max(0.0, boxes - 2500) + 0.02 * tiles;
+                          0.006 * std::max(0.0, boxes - 2500) + 0.02 * tiles +
+                          (backward && d.nboxes > 4 ? 8.0 : 0.0);
     return (backward ? 1.1 : 1.0) * cores > tensor;
 }
 
