@@ -12,8 +12,9 @@
  * The block holds one vector per row, so neighbouring lanes read neighbouring
  * features and every diagonal value is read once for several vectors instead
  * of once per vector, which is what a loop of SpMVs would do.  All sums are
- * held in fp32, in ascending order of the offsets, and rounded once to the
- * block's type.  Grouped: the rows are sorted by expert, rows [seg[e],
+ * held in fp32, in an order that the sizes and the form fix (the same bits on
+ * every run), and rounded once to the block's type; dz is held in 32 bits.
+ * Grouped: the rows are sorted by expert, rows [seg[e],
  * seg[e+1]) use the diagonals vals[e].
  */
 #include <algorithm>
@@ -34,19 +35,19 @@ static std::atomic<int> g_form{0};
 
 /* Which form a call takes: the one whose time, by the measured costs of both,
  * is shorter (16-bit types, one B200; over 174 calls of 8 to 4096 rows, 3 to
- * 129 diagonals, 1 to 64 experts the form taken is 1.5 % slower than the better
- * one on average, 40 % at worst).
+ * 129 diagonals, 1 to 64 experts the form taken is 1.4 % slower than the better
+ * one on average, 43 % at worst).
  *
  * CUDA cores, us.  Few rows: 6, and 4 for every million (row, feature, group of
  * four offsets).  Many: a wave of CTAs takes 10 + 0.4 K, then every million
  * features 4.5 + 0.2 K.
  * Tensor cores: the operator's boxes are packed and read (4 ns each, 10 where
  * they no longer fit L2) and every tile has a way through the kernel; a packing
- * launch of its own 2.5 us.
+ * launch of its own 2.5 us, one that makes dz 8.
  * 4096 x 129 diagonals: cores 57 us, tensor cores 12 at 64 rows; 27-point
- * stencil on 262144: 26 and 321 at 8 rows, 305 and 375 at 128.  The ratio of the
- * gradients is nearly that of the products (65536, 33 scattered diagonals, 128
- * rows: 97 and 107, gradients 180 and 214). */
+ * stencil on 262144: 26 and 324 at 8 rows, 306 and 374 at 128.  The ratio of the
+ * gradients is near that of the products (65536, 33 scattered diagonals, 128
+ * rows: 97 and 107, gradients 179 and 237). */
 static bool tensor_form(const DiaSpmmPlan* p, int dtype, long long M, int E, bool backward)
 {
     const int form = g_form.load(std::memory_order_relaxed);

@@ -371,7 +371,8 @@ spmm_tile_kernel(const __grid_constant__ ProdArgs a, int shape, int ftiles, long
  * next ones on their way meanwhile; a warp keeps the sums of its eight
  * diagonals at its lanes' four features.  Sums of an expert with one part go
  * out at once, others to `part`.  A product costs a read of shared memory, which
- * bounds it: 511 rows of 4096 under 33 diagonals, fp32, 27 us. */
+ * bounds it (load and store unit 58 % busy, instructions issued in 51 % of the
+ * cycles): 511 rows of 4096 under 33 diagonals, fp32, 30 us. */
 constexpr int kGradSmem = 160 * 1024;     /* two buffers of at least eight rows */
 
 template <typename T, typename DZ, bool VEC, int ND>
@@ -627,7 +628,8 @@ static int launch_few(const ProdArgs& a, cudaStream_t stream)
     const long long ngroups = a.seg ? a.M / TT + std::min(a.E, a.M) : (a.M + TT - 1) / TT;
     /* warps that share a tile: until every SM has a CTA (two where a warp has
      * one row), or a warp four diagonals (32 rows of 4096 under 129 diagonals,
-     * bf16: 27 us; with twice the CTAs 38) */
+     * bf16: 28 us; with twice the CTAs 38; the rule gives that call to the
+     * tensor cores, 11 us) */
     const long long warps = TT == 1 ? 2 * kFewWarps : kFewWarps;
     int ks = 1;
     while (ks < kFewWarps && ftiles * ngroups * ks < warps * num_sms() && a.K > 4 * ks) ks *= 2;
@@ -670,8 +672,10 @@ static int launch_cores(const ProdArgs& a, cudaStream_t stream)
     const int per = a.M / std::max(a.E, 1);   /* rows of a usual expert */
     /* below this there are too few warps of 128 features x 8 rows to hide the
      * latency of the diagonals one after the other (4096 x 4096, 129 diagonals,
-     * bf16: 57 us from 64 rows to 256; by few rows 27 at 32 rows, in proportion
-     * beyond) */
+     * bf16 in this form: 57 us from 64 rows to 256; by few rows 28 at 32 rows, in
+     * proportion beyond).  Operators whose inputs fit no tile have no other
+     * kernel than the few rows' (fp32 27-point stencil, 64 rows: 0.25 us a
+     * million products on 64^3 and 76^3, 0.77 on 80^3 to 128^3) */
     if (per >= 8 && a.K > 0 && (long long)a.M * a.n_out >= 196608) {
         /* the widest tile (an input is read again by fewer tiles) whose inputs
          * fit and that leaves a CTA for every SM; else the narrowest that fits */

@@ -19,9 +19,10 @@
  * again for every four tiles.
  *
  * 4096 rows of 4096 under 129 diagonals, bf16, bias, GELU, residual, z kept:
- * 41 us (135 MB: 3.3 TB/s; 21 us at the memory's rate).  The epilogue's
- * instructions and the first tile's latency bound it: a CTA has eight tiles,
- * DRAM is 22 % busy, the tensor cores 10 %.
+ * 40 us (135 MB: 3.4 TB/s; 21 us at the memory's rate).  The epilogue's
+ * instructions and the first tile's latency make it up: a CTA has eight tiles,
+ * DRAM is 26 % busy, the tensor cores 11 %, instructions issue in 43 % of the
+ * cycles.
  *
  * Zeros of a box meet inputs that no diagonal joins to its features; where
  * such an input is infinite or undefined, so is the sum.  Sums that are not
@@ -931,8 +932,8 @@ spmm_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
  * both operands as TMA leaves them (rows of features: MN-major).  Of D the
  * diagonals are the result; it is copied to shared memory, where a diagonal
  * is a run of consecutive features.  dy, z and x are read once.  4096 rows of
- * 4096, 129 diagonals, bf16, GELU: 35 us for 114 MB (3.3 TB/s; DRAM 41 % busy,
- * tensor cores 16 %).  One CTA an SM does not overlap its start, the making of
+ * 4096, 129 diagonals, bf16, GELU: 41 us for 168 MB with both halves of dz
+ * written (4.1 TB/s; DRAM 45 % busy, tensor cores 27 %).  One CTA an SM does not overlap its start, the making of
  * dz and the diagonals' way out with its neighbour's stream.
  * Rows of the last stage that are not the part's are cleared in both operands
  * before the MMAs read them, so that an entry of D sums its own terms alone:
