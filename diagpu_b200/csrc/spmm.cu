@@ -97,8 +97,8 @@ static int grad_part_rows(const DiaSpmmPlan* p, bool tensor, long long M, int E,
 {
     if (tensor) {
         /* one CTA an SM; an expert's last part is half full on average (8
-         * experts, 4096 rows, 2048 features: 47 us at 704 rows a part, 53 at
-         * 384, 61 at 2048) */
+         * experts, 4096 rows, 2048 features: 56 us at 704 rows a part, 61 at
+         * 384, 74 at 2048) */
         const long long tiles = std::max<long long>(1, (stride + 127) / 128) *
                                 ((p->fwd.nboxes + 3) / 4);
         const long long want = std::max<long long>(1, num_sms() / tiles - (E - 1) / 2);
@@ -106,7 +106,7 @@ static int grad_part_rows(const DiaSpmmPlan* p, bool tensor, long long M, int E,
         return (int)((per + 63) / 64 * 64);
     }
     /* two CTAs an SM, all at once (511 rows of 4096, 33 scattered diagonals,
-     * fp32: 51 us against 54 with four); uneven experts want four to share out
+     * fp32: 53 us against 56 with four); uneven experts want four to share out
      * (16 experts, 4096 rows: 80 against 90) */
     const long long tiles = std::max<long long>(1, (stride + 127) / 128) * std::max(1, p->fwd.nwins);
     const long long want =
