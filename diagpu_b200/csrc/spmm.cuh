@@ -15,6 +15,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/diagpu_b200.h"
@@ -386,6 +387,46 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v)
     return __float2bfloat16_rn(v);
 }
 
+/* pairs of elements in a word */
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&h;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&h;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u)
+{
+    return __half22float2(*(const __half2*)&u);
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u)
+{
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+/* an infinity, or what would round to one, is the type's largest number (NaN
+ * stays NaN) */
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_finite(float a, float b)
+{
+    uint32_t d;
+    if (std::is_same<T, __half>::value)
+        asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+    else
+        asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+    return d;
+}
+
 /* four consecutive elements, p aligned to four elements (global or shared) */
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p);
@@ -525,17 +566,11 @@ static cudaError_t launch(bool dependent, void (*kernel)(P...), int grid, int bl
  * bits it would double the variance of their error (0.0024 of a bf16 gradient's
  * size in place of 0.0017), so blocks of 16-bit types keep 32 bits: an fp32
  * for the CUDA cores; for the tensor cores, whose operands are of the block's
- * type, dz rounded and, in a second array, the rest of it rounded (2^-18 of dz
- * for bf16; the rest of what is not finite is 0).  Where there is no activation
- * dz is dy, and kDzSame a copy of a block whose rows TMA does not take. */
+ * type, dz rounded to a finite number and, in a second array, the rest of it
+ * rounded (2^-18 of dz for bf16; infinite where dz is).  Where there is no
+ * activation dz is dy, and kDzSame a copy of a block whose rows TMA does not
+ * take. */
 enum DzForm { kDzSame, kDzF32, kDzPair };
-
-/* the rest of v that its rounding leaves */
-__device__ __forceinline__ float rest_of(float v, float rounded)
-{
-    const float r = v - rounded;
-    return fabsf(r) <= 3.4028235e38f ? r : 0.0f;
-}
 
 /* CUDA-core forms (spmm_cores.cuh); join: sums of experts with several parts,
  * for either form of the gradient */

@@ -598,15 +598,20 @@ spmm_dz_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ z
                 v[c] = a[h][c] * d.x;
                 v[c + 1] = a[h][c + 1] * d.y;
             }
-            if (FORM == kDzF32) {
+            if constexpr (FORM == kDzF32) {
                 store8<float>((float*)dz + at[h], v);
-            } else {
+            } else if constexpr (FORM == kDzSame) {
                 store8<T>((T*)dz + at[h], v);
-                if (FORM == kDzPair) {
+            } else {
+                uint32_t hi[4], rest[4];
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) v[c] = rest_of(v[c], to_f(from_f<T>(v[c])));
-                    store8<T>((T*)lo + at[h], v);
+                for (int c = 0; c < 4; ++c) {
+                    hi[c] = pack2_finite<T>(v[2 * c], v[2 * c + 1]);
+                    const float2 w = unpack2<T>(hi[c]);
+                    rest[c] = pack2<T>(v[2 * c] - w.x, v[2 * c + 1] - w.y);
                 }
+                *(uint4*)((T*)dz + at[h]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *(uint4*)((T*)lo + at[h]) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
             }
         }
     }

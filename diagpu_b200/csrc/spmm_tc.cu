@@ -220,35 +220,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32])
         : "memory");
 }
 
-/* ------------------------------------------------------ pairs of elements */
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    return *(const uint32_t*)&h;
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b)
-{
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *(const uint32_t*)&h;
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t u);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t u)
-{
-    return __half22float2(*(const __half2*)&u);
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u)
-{
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint32_t bar)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
@@ -1125,9 +1096,9 @@ spmm_grad_tc_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                     float2 v = unpack2<T>(d[h][q]);
                     if (MAKE) {
                         v = mul2(v, dact2<ACT>(unpack2<T>(z[h][q])));
-                        d[h][q] = pack2<T>(v.x, v.y);
-                        const float2 w = unpack2<T>(d[h][q]);
-                        z[h][q] = pack2<T>(rest_of(v.x, w.x), rest_of(v.y, w.y));
+                        d[h][q] = pack2_finite<T>(v.x, v.y);
+                        const float2 w = fma2(unpack2<T>(d[h][q]), both(-1.0f), v);
+                        z[h][q] = pack2<T>(w.x, w.y);
                     } else if (PAIR) {
                         v = add2(v, unpack2<T>(z[h][q]));
                     }

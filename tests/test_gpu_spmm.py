@@ -1087,3 +1087,65 @@ def test_gradient_stages_are_read_when_they_are_full(n, M, off, act, t):
         dg.check(L.dia_test_spmm_form(0))
     if act in ("none", "relu"):
         assert all(torch.equal(p, q) for p, q in zip(first, cores))
+
+
+@pytest.mark.parametrize("off", [band(2), WIDE], ids=["made in the gradient", "made before"])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan"), "large"])
+def test_dz_past_the_type(value, off, t):
+    """dz that is not finite reaches the results that its terms reach; finite dz
+    past the largest number of fp16 (dy times a derivative up to 1.1) stays
+    finite, in either form."""
+    M, n = 300, 264
+    c = Case(t, M, n, n, off, seed=73)
+    c.zin[:, ::3] = 2.4
+    if value == "large":
+        top = torch.finfo(t).max if t == torch.float16 else 65504.0
+        c.dy[:, ::3] = top
+        c.vals.mul_(2.0 ** -10)
+        c.x.mul_(2.0 ** -14)
+    else:
+        c.dy[::7, ::5] = value
+    dx, dv, db = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=c.zin, act="silu", bias_grad=True)
+    dz = c.v(c.dy) * dact64(c.v(c.zin), "silu")
+    want = gradient64(off, n, n, c.v(c.vals), c.v(c.x), dz, c.parts)
+    for got, w, what in ((dx, want[0], "dx"), (dv, want[1][0], "dvals"), (db, want[2][0], "dbias")):
+        got = got.double().cpu()
+        if value == "large":
+            # sums of dbias pass the type; the others are finite and near
+            fits = w.abs() < 0.9 * torch.finfo(t).max
+            assert what == "dbias" or bool(fits.all())
+            err = (got - w)[fits].norm() / w[fits].norm()
+            assert bool(got[fits].isfinite().all()) and float(err) <= 2 * unit(t) + 2.0 ** -14
+        else:
+            bad = ~w.isfinite()
+            alike(torch.where(bad, got, 0), torch.where(bad, w, 0), what)
+            assert bool(got[~bad].isfinite().all())
+
+
+@pytest.mark.parametrize("M", [4, 300])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_pairs_of_gradients(M, shift, t):
+    """Two of the C entry's outputs without the third: the same as all three,
+    but for the order of the sums where another form takes the rest."""
+    n, m = 136, 144
+    c = Case(t, M, n, m, band(5), seed=74, shift=shift)
+    L, code = dg.lib(), {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[t]
+    want = dg.spmm_backward(c.plan, c.vals[0], c.x, c.dy, z=c.zin, act="silu", bias_grad=True)
+    st = c.vals.shape[-1]
+    ws = L.dia_spmm_backward_workspace(c.plan._h, code, M, 1, m, st, n, 2)
+    work = torch.empty(ws, dtype=torch.uint8, device="cuda")
+    for left in range(3):
+        out = [torch.full_like(w, 9.0) for w in want]
+        p = [None if k == left else o.data_ptr() for k, o in enumerate(out)]
+        dg.check(L.dia_spmm_backward(c.plan._h, code, M, 1, None, c.x.data_ptr(), m,
+                                     c.vals.data_ptr(), st, c.dy.data_ptr(), n, 2,
+                                     c.zin.data_ptr(), n, p[0], m, p[1], p[2], work.data_ptr(), ws,
+                                     torch.cuda.current_stream().cuda_stream))
+        for k, (o, w) in enumerate(zip(out, want)):
+            if k == left:
+                assert bool((o == 9).all())
+                continue
+            S = (11, M, M)[k] * (float(c.vals.abs().max()), float(c.x.abs().max()), 1.0)[k]
+            S *= 1.2 * float(c.dy.abs().max())
+            lim = 2 * unit(t) * w.double().abs() + (M + 15) * sum_unit(t) * S + 2.0 ** -16 * S
+            assert bool(((o.double() - w.double()).abs() <= lim + tiny(t)).all())
