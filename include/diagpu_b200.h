@@ -222,7 +222,8 @@ int dia_spmm(const DiaSpmmPlan* plan, int dtype, int64_t M, int num_experts,
 
 /* Gradients of dia_spmm for dy = the gradient of y (that of the residual is
  * dy itself).  With dz = dy act'(z), held in 32 bits (for the tensor cores as
- * the sum of two numbers of the block's type, to 2^-18 of it):
+ * the sum of two numbers of the block's type, to 2^-18 of it, in fp16 to no less
+ * than 2^-25):
  *   dx[t,j] = sum_k vals[e,k,j-off[k]] dz[t,j-off[k]],
  *   dvals[e,k,i] = sum_t dz[t,i] x[t,i+off[k]]  (whole stride: 0 outside the
  *   matrix and in the padding; 0 for an expert without rows),
